@@ -13,6 +13,9 @@ Modules
     ce_reduce        drop-in for the owner-sum kernel of yoco/models/decoder/ce_reduce.py (_sum_slots, _sum)
     embedding        drop-in for the owner's token-embedding gradient (aten embedding_dense_backward + 1/world)
     trainer_glue     the optimizer part of trainer_nosync.train_step: one-launch scalar chain + deferred checks
+    norm             layer norm and RMS norm, forward and backward, with 8-bit results and checkpoints
+    act8             8-bit activations: rows in blocks of 128 with power-of-two scales
+    linear8          products of 8-bit rows and weights, and the weight's gradient from 8-bit rows
     exchange         the BF16 exchange pipelined with the step (row ranges, side-stream sends)
     configs          the benchmark/parity workloads (tensor lists and synthetic inputs)
     standins         stand-ins of the fairseq / fairscale objects the drop-in surfaces are driven through where
@@ -21,4 +24,4 @@ Modules
 from . import _lib, library, ops  # noqa: F401
 
 __all__ = ['library', 'ops', 'kernels', 'shard', 'fused_adam_cast', 'zero1_fast', 'ce_reduce', 'configs', 'layout',
-           'trainer_glue', 'embedding', 'exchange', 'standins']
+           'trainer_glue', 'embedding', 'exchange', 'norm', 'act8', 'linear8', 'standins']

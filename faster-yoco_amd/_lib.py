@@ -16,6 +16,7 @@ LIB_PATH = os.environ.get('YOCO_Z1_LIB') or os.path.join(_HERE, LIB_NAME)
 
 Z1_F32 = 0
 Z1_BF16 = 1
+Z1_F16 = 2
 Z1_MAX_WORLD = 16
 Z1_NORM_PARTIALS = 2048
 Z1_NOALLOC_MAX_N = 1 << 29
@@ -67,6 +68,17 @@ SIGNATURES = {
     'z1_cast_bf16': ([_P, _P, _I64, _P], _I),
     'z1_embedding_backward': ([_P, _P, _I64, _I64, _I64, _I64, _F, _I, _P, _P, _I64, _P], _I),
     'z1_embedding_backward_workspace': ([_I64, _I64, _I64], _I64),
+    'z1_norm_forward': ([_P, _I64, _I64, _I64, _I, _P, _P, _I, _F, _I, _P, _P, _P, _P, _P, _P, _P, _P], _I),
+    'z1_norm_backward': ([_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I64,
+                          _P], _I),
+    'z1_norm_backward_workspace': ([_I64, _I64], _I64),
+    'z1_act8_columns': ([_I64], _I64),
+    'z1_act8_scales': ([_I64], _I64),
+    'z1_act8_pack': ([_P, _I64, _I64, _I64, _I, _P, _P, _P], _I),
+    'z1_act8_unpack': ([_P, _P, _I64, _I64, _P, _I, _P], _I),
+    'z1_weight8_pack': ([_P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P], _I),
+    'z1_product8': ([_P, _P, _I64, _P, _P, _I64, _I64, _P, _I, _P], _I),
+    'z1_weight_grad8': ([_P, _I64, _P, _P, _I64, _I64, _I64, _P, _I, _P], _I),
     'z1_strerror': ([_I], ctypes.c_char_p),
 }
 

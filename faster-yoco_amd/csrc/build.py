@@ -6,15 +6,18 @@ disabled."""
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 CSRC = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(CSRC)
 ROOT = os.path.dirname(PKG)
 INCLUDE = os.path.join(ROOT, 'include')
-SOURCES = [os.path.join(CSRC, 'z1_kernels.hip'), os.path.join(CSRC, 'z1_embedding.hip')]
+SOURCES = [os.path.join(CSRC, f) for f in ('z1_kernels.hip', 'z1_embedding.hip', 'z1_norm.hip', 'z1_act8.hip',
+                                           'z1_linear8.hip')]
 OUTPUT = os.path.join(PKG, 'libyoco_z1.so')
 ARCH = os.environ.get('YOCO_Z1_ARCH', 'gfx950')
-OPS_SOURCE = os.path.join(CSRC, 'z1_torch_ops.cpp')
+OPS_SOURCES = [os.path.join(CSRC, f) for f in ('z1_torch_ops.cpp', 'z1_torch_block_ops.cpp')]
 OPS_OUTPUT = os.path.join(PKG, 'libyoco_z1_torch.so')
 
 FLAGS = [
@@ -31,18 +34,25 @@ def hipcc():
 
 
 def build(output=OUTPUT, extra=(), verbose=False):
-    """Compile every source into `output` (written to a temporary name first, then renamed)."""
+    """Compile every source, side by side, and link them into `output` (written to a temporary name first, then
+    renamed)."""
+    def run(cmd):
+        if verbose:
+            print(' '.join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        # hipcc's host pass reports the device-only feature flag as unknown; that line is expected
+        noise = [l for l in res.stderr.splitlines() if l.strip() and 'packed-fp32-ops' not in l]
+        if res.returncode != 0:
+            raise RuntimeError('yoco_z1: hipcc failed:\n' + res.stderr)
+        if noise and verbose:
+            print('\n'.join(noise), file=sys.stderr)
+
     tmp = output + '.tmp'
-    cmd = [hipcc()] + FLAGS + list(extra) + ['-I', INCLUDE, '-o', tmp] + SOURCES
-    if verbose:
-        print(' '.join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    # hipcc's host pass reports the device-only feature flag as unknown; that line is expected
-    noise = [l for l in res.stderr.splitlines() if l.strip() and 'packed-fp32-ops' not in l]
-    if res.returncode != 0:
-        raise RuntimeError('yoco_z1: hipcc failed:\n' + res.stderr)
-    if noise and verbose:
-        print('\n'.join(noise), file=sys.stderr)
+    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(4) as pool:
+        objects = [os.path.join(d, os.path.basename(s) + '.o') for s in SOURCES]
+        compile_ = [f for f in FLAGS if f != '-shared'] + list(extra) + ['-I', INCLUDE, '-c']
+        list(pool.map(lambda so: run([hipcc()] + compile_ + ['-o', so[1], so[0]]), zip(SOURCES, objects)))
+        run([hipcc()] + FLAGS + list(extra) + ['-o', tmp] + objects)
     os.replace(tmp, output)
     return output
 
@@ -58,9 +68,8 @@ def build_ops(output=OPS_OUTPUT, verbose=False):
     tmp = output + '.tmp'
     cmd = (['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall', '-Werror',
             f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-D__HIP_PLATFORM_AMD__=1',
-            '-DUSE_ROCM=1'] + inc + ['-I', os.path.join(rocm, 'include'), '-I', INCLUDE, OPS_SOURCE,
-                                     '-L', tlib, '-lc10', '-lc10_hip', '-ltorch_cpu', '-ldl',
-                                     f'-Wl,-rpath,{tlib}', '-o', tmp])
+            '-DUSE_ROCM=1'] + inc + ['-I', os.path.join(rocm, 'include'), '-I', INCLUDE] + OPS_SOURCES +
+           ['-L', tlib, '-lc10', '-lc10_hip', '-ltorch_cpu', '-ldl', f'-Wl,-rpath,{tlib}', '-o', tmp])
     if verbose:
         print(' '.join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

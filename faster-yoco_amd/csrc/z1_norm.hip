@@ -1,0 +1,563 @@
+// Layer norm and RMS norm over rows, forward and backward (declarations: include/yoco_z1.h).
+//
+//   forward   mu = mean(x) (0 for RMS), r = 1/sqrt(mean((x-mu)^2) + eps), y = (x-mu) r w + b
+//   backward  xh = (x-mu) r, g = dy w:  dx = r (g - mean(g) - xh mean(g xh)) (no mean(g) for RMS),
+//             dw = sum over rows of dy xh, db = sum over rows of dy
+//
+// All of it is bound by memory: a row is read once, held in registers (kLane = 8 columns of a lane at a time), and the
+// variance is taken about the mean in a second pass over the registers, so that a large common offset costs no digits.
+// Statistics and sums are fp32.
+#include "z1_block.h"
+
+#pragma clang fp contract(off)
+
+namespace {
+
+using namespace z1blk;
+
+constexpr int kFwdThreads = 256;
+constexpr int kBwdThreads = 512;
+constexpr int kUnit = 64 * kLane;                      // columns of one wave's access
+constexpr int kLongThreads = 1024;
+
+struct Forward {
+    const void* x;
+    int64_t stride;                                    // elements between rows
+    const void* w;
+    const void* b;
+    void* y;                                           // y in x's type, or
+    uint8_t* yq;                                       // its 8-bit form
+    uint8_t* ys;
+    uint8_t* cq;                                       // the 8-bit form of x
+    uint8_t* cs;
+    float* mean;
+    float* rstd;
+    int64_t row0, rows;                                // this launch's first row, and the end of all rows
+    int dim, wide, pitch;
+    int wpr;                                           // waves of a row: 1, 2 or 4
+    int w32;                                           // w and b are fp32 (else x's type)
+    float eps;
+};
+
+template <typename T>
+__device__ __forceinline__ void load_weight(const void* p, int w32, int64_t c, int n, float* v) {
+    if (w32) load_row<F32>(p, c, n, v);
+    else load_row<T>(p, c, n, v);
+}
+
+// Sum over a row's wpr waves (red: one slot per wave of the workgroup).  Every wave of the workgroup is here.
+__device__ __forceinline__ float row_sum(float s, float* red, int wave, int wpr) {
+    s = wave_sum(s);
+    if (wpr == 1) return s;
+    red[wave] = s;                                     // every lane writes the same value
+    __syncthreads();
+    const int first = wave & ~(wpr - 1);
+    s = red[first];
+    for (int i = 1; i < wpr; ++i) s += red[first + i];
+    return s;
+}
+
+// The 8-bit form of eight columns from c on, of which n are in the row (the rest are zeros): bytes, scale, padding.
+__device__ __forceinline__ void put8(uint8_t* q, uint8_t* s, int64_t row, int c, const Forward& a, const float* v) {
+    uint32_t byte;
+    const u2 w = quantize8(v, byte);
+    if (c < a.wide) {
+        *(Z1B_GLOBAL u2*)(q + row * a.wide + c) = w;
+        if ((c & (kBlock - 1)) == 0) s[row * a.pitch + c / kBlock] = (uint8_t)byte;
+    }
+}
+__device__ __forceinline__ void pad_scales(uint8_t* s, int64_t row, int lane, int wide, int pitch) {
+    if (lane < pitch - wide / kBlock) s[row * pitch + wide / kBlock + lane] = 127;
+}
+
+template <typename T, bool CENTER>
+__device__ __forceinline__ void finish8(const Forward& a, int64_t row, int c, int n, float mu, float r, const float* v) {
+    float y[kLane];
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) y[j] = (CENTER ? v[j] - mu : v[j]) * r;
+    if (a.w) {
+        float w[kLane];
+        load_weight<T>(a.w, a.w32, c, n, w);
+        if (CENTER && a.b) {
+            float b[kLane];
+            load_weight<T>(a.b, a.w32, c, n, b);
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) y[j] = __builtin_fmaf(y[j], w[j], b[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) y[j] *= w[j];
+        }
+    } else if (CENTER && a.b) {
+        float b[kLane];
+        load_weight<T>(a.b, a.w32, c, n, b);
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) y[j] += b[j];
+    }
+    if (a.y) {
+        store_row<T>(a.y, row * a.dim + c, n, y);
+    } else {
+        if (n < kLane) {
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) y[j] = j < n ? y[j] : 0.0f;
+        }
+        put8(a.yq, a.ys, row, c, a, y);
+    }
+    if (a.cq) put8(a.cq, a.cs, row, c, a, v);
+}
+
+// Rows of up to 4 * NV * 512 columns: a row's wpr waves hold it in registers.
+template <typename T, int NV, bool CENTER>
+__global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
+    __shared__ float red[2][kFwdThreads / 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wpr = a.wpr, group = wave / wpr, wi = wave - group * wpr;
+    int64_t row = a.row0 + (int64_t)blockIdx.x * (kFwdThreads / 64 / wpr) + group;
+    const bool live = row < a.rows;                    // every wave stays for the barriers
+    if (!live) row = a.rows - 1;
+    float v[NV][kLane];
+    float s = 0.0f;
+    int c0 = (wi * 64 + lane) * kLane;
+    const int step = wpr * kUnit;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) load_row<T>(a.x, row * a.stride + c0 + k * step, a.dim - c0 - k * step, v[k]);
+    float mu = 0.0f;
+    if (CENTER) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) s += v[k][j];
+        mu = row_sum(s, red[0], wave, wpr) / (float)a.dim;
+    }
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int n = a.dim - c0 - k * step;
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            const float d = CENTER ? (j < n ? v[k][j] - mu : 0.0f) : v[k][j];
+            s = __builtin_fmaf(d, d, s);
+        }
+    }
+    s = row_sum(s, red[1], wave, wpr);
+    const float r = 1.0f / sqrtf(s / (float)a.dim + a.eps);
+    if (!live) return;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = c0 + k * step;
+        // all 64 lanes or none take part in an 8-bit form; a lane of no columns writes nothing
+        if (c - lane * kLane < a.wide) finish8<T, CENTER>(a, row, c, a.dim - c, mu, r, v[k]);
+    }
+    if (wi == 0) {
+        if (lane == 0) {
+            if (CENTER) a.mean[row] = mu;
+            a.rstd[row] = r;
+        }
+        if (a.yq) pad_scales(a.ys, row, lane, a.wide, a.pitch);
+        if (a.cq) pad_scales(a.cs, row, lane, a.wide, a.pitch);
+    }
+}
+
+__device__ __forceinline__ float block_sum(float s, float* red, int wave, int waves) {
+    s = wave_sum(s);
+    __syncthreads();
+    red[wave] = s;
+    __syncthreads();
+    s = red[0];
+    for (int i = 1; i < waves; ++i) s += red[i];
+    return s;
+}
+
+// Longer rows: one workgroup reads its row again for each pass.
+template <typename T, bool CENTER>
+__global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(Forward a) {
+    __shared__ float red[kLongThreads / 64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = a.row0 + blockIdx.x, at = row * a.stride;
+    const int step = kLongThreads * kLane;
+    float mu = 0.0f, s = 0.0f, v[kLane];
+    if (CENTER) {
+        for (int c = threadIdx.x * kLane; c < a.dim; c += step) {
+            load_row<T>(a.x, at + c, a.dim - c, v);
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) s += v[j];
+        }
+        mu = block_sum(s, red, wave, kLongThreads / 64) / (float)a.dim;
+    }
+    s = 0.0f;
+    for (int c = threadIdx.x * kLane; c < a.dim; c += step) {
+        load_row<T>(a.x, at + c, a.dim - c, v);
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            const float d = j < a.dim - c ? v[j] - mu : 0.0f;
+            s = __builtin_fmaf(d, d, s);
+        }
+    }
+    s = block_sum(s, red, wave, kLongThreads / 64);
+    const float r = 1.0f / sqrtf(s / (float)a.dim + a.eps);
+    for (int base = wave * kUnit; base < a.wide; base += step) {        // whole waves: the 8-bit forms need 16 lanes
+        const int c = base + lane * kLane;
+        load_row<T>(a.x, at + c, a.dim - c, v);
+        finish8<T, CENTER>(a, row, c, a.dim - c, mu, r, v);
+    }
+    if (wave == 0) {
+        if (lane == 0) {
+            if (CENTER) a.mean[row] = mu;
+            a.rstd[row] = r;
+        }
+        if (a.yq) pad_scales(a.ys, row, lane, a.wide, a.pitch);
+        if (a.cq) pad_scales(a.cs, row, lane, a.wide, a.pitch);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ backward
+struct Backward {
+    const void* dy;
+    int64_t dy_stride;
+    const void* x;                                     // x in dy's type, or
+    int64_t x_stride;
+    const uint8_t* q;                                  // its 8-bit form
+    const uint8_t* s;
+    const float* mean;
+    const float* rstd;
+    const void* w;
+    void* dx;
+    float* part;                                       // [blocks][2][dim]: sums of dy xh and of dy; NULL: none
+    int64_t row0, rows;                                // a launch's first row (long rows only), and the end of all rows
+    int dim, wide, pitch;
+    int wpr;                                           // waves of a row: 1, 2, 4 or 8
+    int w32;
+};
+
+// xh of eight columns (zeros past the row's end).
+template <typename T, bool Q, bool CENTER>
+__device__ __forceinline__ void load_xh(const Backward& a, int64_t row, int c, int n, float mu, float r, float* xh) {
+    if (Q) {
+        if (n > 0) {
+            const float f = scale_value(a.s[row * a.pitch + c / kBlock]);
+            open8(*(const Z1B_GLOBAL u2*)(a.q + row * a.wide + c), xh);
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) xh[j] *= f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) xh[j] = 0.0f;
+        }
+    } else {
+        load_row<T>(a.x, row * a.x_stride + c, n, xh);
+    }
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) xh[j] = (CENTER ? (j < n ? xh[j] - mu : 0.0f) : xh[j]) * r;
+}
+
+// Both sums of a row over its wpr waves.
+__device__ __forceinline__ void row_sums(float& s1, float& s2, float (*red)[2], int wave, int wpr) {
+    s1 = wave_sum(s1);
+    s2 = wave_sum(s2);
+    if (wpr == 1) return;
+    red[wave][0] = s1;
+    red[wave][1] = s2;
+    __syncthreads();
+    const int first = wave & ~(wpr - 1);
+    s1 = red[first][0];
+    s2 = red[first][1];
+    for (int i = 1; i < wpr; ++i) s1 += red[first + i][0], s2 += red[first + i][1];
+}
+
+// Rows of up to 8 * NV * 512 columns.  A workgroup's groups of wpr waves take rows in turn; a lane keeps its columns'
+// dw and db sums in registers over all of them, the groups' sums meet in LDS at the end, and the workgroup writes one
+// partial row of each, which norm_reduce_kernel adds in order.
+template <typename T, int NV, bool Q, bool CENTER>
+__global__ __launch_bounds__(kBwdThreads) void norm_backward_kernel(Backward a) {
+    __shared__ float red[2][kBwdThreads / 64][2];
+    __shared__ float sums[kBwdThreads * NV * kLane];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wpr = a.wpr, groups = kBwdThreads / 64 / wpr, group = wave / wpr, wi = wave - group * wpr;
+    const int c0 = (wi * 64 + lane) * kLane, step = wpr * kUnit;
+    float dw[NV][kLane] = {}, db[NV][kLane] = {};
+    const float inv = 1.0f / (float)a.dim;
+    int turn = 0;
+    for (int64_t first = (int64_t)blockIdx.x * groups; first < a.rows; first += (int64_t)gridDim.x * groups) {
+        const int64_t row = first + group;
+        const bool live = row < a.rows;                // every wave stays for the barriers
+        float xh[NV][kLane], g[NV][kLane], s1 = 0.0f, s2 = 0.0f, r = 0.0f;
+        if (live) {
+            r = a.rstd[row];
+            const float mu = CENTER ? a.mean[row] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = c0 + k * step, n = a.dim - c;
+                load_xh<T, Q, CENTER>(a, row, c, n, mu, r, xh[k]);
+                load_row<T>(a.dy, row * a.dy_stride + c, n, g[k]);
+#pragma unroll
+                for (int j = 0; j < kLane; ++j) {
+                    dw[k][j] = __builtin_fmaf(g[k][j], xh[k][j], dw[k][j]);
+                    if (CENTER) db[k][j] += g[k][j];
+                }
+                if (a.w) {
+                    float w[kLane];
+                    load_weight<T>(a.w, a.w32, c, n, w);
+#pragma unroll
+                    for (int j = 0; j < kLane; ++j) g[k][j] *= w[j];
+                }
+#pragma unroll
+                for (int j = 0; j < kLane; ++j) {
+                    if (CENTER) s1 += g[k][j];
+                    s2 = __builtin_fmaf(g[k][j], xh[k][j], s2);
+                }
+            }
+        }
+        row_sums(s1, s2, red[turn], wave, wpr);
+        turn ^= 1;                                     // the next row's sums need no barrier before they are written
+        if (live) {
+            const float m1 = s1 * inv, m2 = s2 * inv;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                const int c = c0 + k * step, n = a.dim - c;
+                float dx[kLane];
+#pragma unroll
+                for (int j = 0; j < kLane; ++j) {
+                    const float t = CENTER ? g[k][j] - m1 : g[k][j];
+                    dx[j] = __builtin_fmaf(-xh[k][j], m2, t) * r;
+                }
+                if (n > 0) store_row<T>(a.dx, row * a.dim + c, n, dx);
+            }
+        }
+    }
+    if (!a.part) return;
+    float* out = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+    const int columns = step * NV;                     // of a group, in column order below
+#pragma unroll
+    for (int which = 0; which < (CENTER ? 2 : 1); ++which) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) sums[group * columns + c0 + k * step + j] = which ? db[k][j] : dw[k][j];
+        __syncthreads();
+        for (int c = threadIdx.x; c < a.dim; c += kBwdThreads) {
+            float t = sums[c];
+            for (int i = 1; i < groups; ++i) t += sums[i * columns + c];
+            out[which * a.dim + c] = t;
+        }
+    }
+}
+
+// Longer rows: dx by one workgroup a row, which reads it twice; the columns' sums apart (norm_columns_kernel).
+template <typename T, bool Q, bool CENTER>
+__global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(Backward a) {
+    __shared__ float red[kLongThreads / 64];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = a.row0 + blockIdx.x;
+    const int step = kLongThreads * kLane;
+    const float r = a.rstd[row], mu = CENTER ? a.mean[row] : 0.0f;
+    float s1 = 0.0f, s2 = 0.0f, xh[kLane], g[kLane];
+    for (int pass = 0; pass < 2; ++pass) {
+        const float m1 = s1 / (float)a.dim, m2 = s2 / (float)a.dim;
+        for (int c = threadIdx.x * kLane; c < a.dim; c += step) {
+            const int n = a.dim - c;
+            load_xh<T, Q, CENTER>(a, row, c, n, mu, r, xh);
+            load_row<T>(a.dy, row * a.dy_stride + c, n, g);
+            if (a.w) {
+                float w[kLane];
+                load_weight<T>(a.w, a.w32, c, n, w);
+#pragma unroll
+                for (int j = 0; j < kLane; ++j) g[j] *= w[j];
+            }
+            if (pass == 0) {
+#pragma unroll
+                for (int j = 0; j < kLane; ++j) s1 += g[j], s2 = __builtin_fmaf(g[j], xh[j], s2);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kLane; ++j)
+                    g[j] = __builtin_fmaf(-xh[j], m2, CENTER ? g[j] - m1 : g[j]) * r;
+                store_row<T>(a.dx, row * a.dim + c, n, g);
+            }
+        }
+        if (pass == 0) {
+            s1 = block_sum(s1, red, wave, kLongThreads / 64);
+            s2 = block_sum(s2, red, wave, kLongThreads / 64);
+        }
+    }
+}
+
+constexpr int kColumnThreads = 256;
+// dw and db partials of kColumnThreads * 8 columns (blockIdx.x) over the blockIdx.y-th of gridDim.y shares of the rows.
+template <typename T, bool Q, bool CENTER>
+__global__ __launch_bounds__(kColumnThreads) void norm_columns_kernel(Backward a) {
+    const int c = (blockIdx.x * kColumnThreads + threadIdx.x) * kLane, n = a.dim - c;
+    if (n <= 0) return;
+    float dw[kLane] = {}, db[kLane] = {}, xh[kLane], g[kLane];
+    for (int64_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        load_xh<T, Q, CENTER>(a, row, c, n, CENTER ? a.mean[row] : 0.0f, a.rstd[row], xh);
+        load_row<T>(a.dy, row * a.dy_stride + c, n, g);
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            dw[j] = __builtin_fmaf(g[j], xh[j], dw[j]);
+            if (CENTER) db[j] += g[j];
+        }
+    }
+    float* out = a.part + (int64_t)blockIdx.y * 2 * a.dim;
+    store_row<F32>(out, c, n, dw);
+    if (CENTER) store_row<F32>(out, (int64_t)a.dim + c, n, db);
+}
+
+// dw and db from `parts` partial rows, added in order: 64 columns and 4 shares of the partials to a workgroup.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_reduce_kernel(const float* part, int parts, int dim, void* dw, void* db) {
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6;
+    const int blocks = (dim + 63) / 64;
+    const int which = blockIdx.x >= blocks;
+    const int c = (blockIdx.x - which * blocks) * 64 + lane;
+    float t = 0.0f;
+    if (c < dim)
+        for (int i = share; i < parts; i += 4) t += part[((int64_t)i * 2 + which) * dim + c];
+    sums[share][lane] = t;
+    __syncthreads();
+    void* out = which ? db : dw;
+    if (share == 0 && c < dim && out) T::put(out, c, ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]);
+}
+
+// ------------------------------------------------------------------------------------------------------ host
+constexpr int kMaxVectors = 4;
+constexpr int kMaxBlocks = 256;                        // workgroups of the backward pass: one partial row each
+
+// A launch counts its threads in 32 bits: at most this many rows (a multiple of every workgroup's rows) to one.
+constexpr int64_t kLaunchRows = 1 << 21;
+unsigned launch_rows(int64_t left) { return (unsigned)(left < kLaunchRows ? left : kLaunchRows); }
+
+template <typename T, bool CENTER>
+int forward(Forward& a, hipStream_t st) {
+    const int units = (a.dim + kUnit - 1) / kUnit;
+    if (units > 4 * kMaxVectors) {
+        for (; a.row0 < a.rows; a.row0 += kLaunchRows)
+            norm_forward_long_kernel<T, CENTER><<<launch_rows(a.rows - a.row0), kLongThreads, 0, st>>>(a);
+        return (int)hipGetLastError();
+    }
+    a.wpr = units <= kMaxVectors ? 1 : units <= 2 * kMaxVectors ? 2 : 4;
+    const int nv = (units + a.wpr - 1) / a.wpr, per = kFwdThreads / 64 / a.wpr;
+    for (; a.row0 < a.rows; a.row0 += kLaunchRows) {
+        const dim3 grid((launch_rows(a.rows - a.row0) + per - 1) / per);
+        switch (nv) {
+            case 1: norm_forward_kernel<T, 1, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 2: norm_forward_kernel<T, 2, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 3: norm_forward_kernel<T, 3, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            default: norm_forward_kernel<T, 4, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+        }
+    }
+    return (int)hipGetLastError();
+}
+
+struct Shape { int wpr, nv, blocks; };                 // wpr 0: the long rows' kernels, `blocks` shares of the rows
+
+Shape backward_shape(int64_t rows, int dim) {
+    const int units = (dim + kUnit - 1) / kUnit;
+    if (units > 8 * kMaxVectors) return {0, 0, (int)(rows < 64 ? rows : 64)};
+    const int wpr = units <= 3 ? 1 : units <= 6 ? 2 : units <= 12 ? 4 : 8;
+    const int groups = kBwdThreads / 64 / wpr;
+    const int64_t need = (rows + groups - 1) / groups;
+    return {wpr, (units + wpr - 1) / wpr, (int)(need < kMaxBlocks ? need : kMaxBlocks)};
+}
+
+template <typename T, bool Q, bool CENTER>
+int backward(Backward& a, const Shape& s, hipStream_t st) {
+    if (s.wpr == 0) {
+        for (; a.row0 < a.rows; a.row0 += kLaunchRows)
+            norm_backward_long_kernel<T, Q, CENTER><<<launch_rows(a.rows - a.row0), kLongThreads, 0, st>>>(a);
+        if (a.part) {
+            const dim3 grid((unsigned)((a.dim + kColumnThreads * kLane - 1) / (kColumnThreads * kLane)), s.blocks);
+            norm_columns_kernel<T, Q, CENTER><<<grid, kColumnThreads, 0, st>>>(a);
+        }
+        return (int)hipGetLastError();
+    }
+    a.wpr = s.wpr;
+    switch (s.nv) {
+        case 1: norm_backward_kernel<T, 1, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
+        case 2: norm_backward_kernel<T, 2, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
+        case 3: norm_backward_kernel<T, 3, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
+        default: norm_backward_kernel<T, 4, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
+    }
+    return (int)hipGetLastError();
+}
+
+template <typename T>
+int backward_of(Backward& a, bool center, const Shape& s, hipStream_t st) {
+    if (a.q) return center ? backward<T, true, true>(a, s, st) : backward<T, true, false>(a, s, st);
+    return center ? backward<T, false, true>(a, s, st) : backward<T, false, false>(a, s, st);
+}
+
+bool bad_dtype(int d) { return d != Z1_F32 && d != Z1_BF16 && d != Z1_F16; }
+
+constexpr int64_t kMaxRows = 1ll << 38;                // rows times columns fit 63 bits
+constexpr int64_t kMaxDim = 1 << 24;                   // a whole number in fp32, and columns fit an int
+
+int bad_shape(int64_t rows, int64_t dim, int64_t stride) {
+    if (rows < 0 || rows > kMaxRows || dim < 1 || dim > kMaxDim || stride < 0) return Z1_E_SIZE;
+    return Z1_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int z1_norm_forward(const void* x, int64_t rows, int64_t dim, int64_t stride, int dtype, const void* w, const void* b,
+                    int w_dtype, float eps, int center, void* y, void* yq, void* ys, void* cq, void* cs, float* mean,
+                    float* rstd, void* stream) {
+    if (const int rc = bad_shape(rows, dim, stride)) return rc;
+    if (bad_dtype(dtype) || (w_dtype != dtype && w_dtype != Z1_F32)) return Z1_E_DTYPE;
+    if (center != 0 && center != 1) return Z1_E_MODE;
+    if (rows == 0) return Z1_OK;
+    if (!x || !rstd || (center && !mean) || !y == !yq || !yq != !ys || !cq != !cs || (b && !center)) return Z1_E_NULL;
+    Forward a{x, stride, w, b, y, (uint8_t*)yq, (uint8_t*)ys, (uint8_t*)cq, (uint8_t*)cs, mean, rstd, 0, rows, (int)dim,
+              wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32, eps};
+    const hipStream_t st = (hipStream_t)stream;
+    switch (dtype) {
+        case Z1_F32: return center ? forward<F32, true>(a, st) : forward<F32, false>(a, st);
+        case Z1_BF16: return center ? forward<BF16, true>(a, st) : forward<BF16, false>(a, st);
+        default: return center ? forward<F16, true>(a, st) : forward<F16, false>(a, st);
+    }
+}
+
+int64_t z1_norm_backward_workspace(int64_t rows, int64_t dim) {
+    if (bad_shape(rows, dim, 0)) return Z1_E_SIZE;
+    return (int64_t)backward_shape(rows, (int)dim).blocks * 2 * dim;
+}
+
+int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* q, const void* s,
+                     int64_t rows, int64_t dim, int dtype, const float* mean, const float* rstd, const void* w,
+                     int w_dtype, int center, void* dx, void* dw, void* db, int grad_dtype, float* workspace,
+                     int64_t workspace_floats, void* stream) {
+    if (const int rc = bad_shape(rows, dim, dy_stride)) return rc;
+    if (x && x_stride < 0) return Z1_E_SIZE;
+    if (bad_dtype(dtype) || (w_dtype != dtype && w_dtype != Z1_F32) || bad_dtype(grad_dtype)) return Z1_E_DTYPE;
+    if (center != 0 && center != 1) return Z1_E_MODE;
+    if (db && !center) return Z1_E_NULL;
+    const hipStream_t st = (hipStream_t)stream;
+    const Shape sh = backward_shape(rows, (int)dim);
+    if (rows > 0) {
+        if (!dy || !x == !q || !q != !s || !rstd || (center && !mean) || !dx) return Z1_E_NULL;
+        if (dw || db) {
+            if (!workspace) return Z1_E_NULL;
+            if (workspace_floats < (int64_t)sh.blocks * 2 * dim) return Z1_E_WORKSPACE;
+        }
+        Backward a{dy, dy_stride, x, x_stride, (const uint8_t*)q, (const uint8_t*)s, mean, rstd, w, dx,
+                   dw || db ? workspace : nullptr, 0, rows, (int)dim, wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32};
+        int rc;
+        switch (dtype) {
+            case Z1_F32: rc = backward_of<F32>(a, center, sh, st); break;
+            case Z1_BF16: rc = backward_of<BF16>(a, center, sh, st); break;
+            default: rc = backward_of<F16>(a, center, sh, st); break;
+        }
+        if (rc) return rc;
+    }
+    if (!dw && !db) return Z1_OK;
+    const dim3 grid((unsigned)((dim + 63) / 64 * (center ? 2 : 1)));
+    const int parts = rows > 0 ? sh.blocks : 0;
+    switch (grad_dtype) {
+        case Z1_F32: norm_reduce_kernel<F32><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, dw, db); break;
+        case Z1_BF16: norm_reduce_kernel<BF16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, dw, db); break;
+        default: norm_reduce_kernel<F16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, dw, db); break;
+    }
+    return (int)hipGetLastError();
+}
+
+}  // extern "C"

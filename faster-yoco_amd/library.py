@@ -52,6 +52,10 @@ def _load():
     rc = L.z1t_init(abi._name.encode())
     if rc != 0:
         raise RuntimeError(f'yoco_z1: the operator library could not bind to {abi._name} (code {rc})')
+    L.z1t_init_block.argtypes, L.z1t_init_block.restype = [ctypes.c_char_p], ctypes.c_int
+    rc = L.z1t_init_block(abi._name.encode())
+    if rc not in (0, -2):                   # -2: another build of the ABI without them; the operators say so when called
+        raise RuntimeError(f'yoco_z1: the block-side operators could not bind to {abi._name} (code {rc})')
     return L
 
 
@@ -76,3 +80,44 @@ OPS = ('grad_sumsq_', 'norm_clip_', 'grad_norm_clip_', 'update_scalars_', 'grad_
 for _name in OPS:
     torch.library.register_fake(f'{NS}::{_name}',
                                 _embedding_fake if _name == 'embedding_dense_backward' else _none)
+
+
+# ------------------------------------------------------------------------------------------------ block-side operators
+# (norms, 8-bit rows and weights, 8-bit products: csrc/z1_torch_block_ops.cpp).  They return new tensors and write none.
+F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _empty8(like, rows, dim, scale_rows):
+    return [like.new_empty((rows, -(-dim // 128) * 128), dtype=F8),
+            like.new_empty((scale_rows, -(-dim // 512) * 4), dtype=E8)]
+
+
+def _norm_forward_fake(x, weight, bias, eps, center, y8, checkpoint):
+    n, d = x.shape
+    out = _empty8(x, n, d, n) if y8 else [x.new_empty((n, d))]
+    out += [x.new_empty((n,), dtype=torch.float32) for _ in range(2 if center else 1)]
+    return out + (_empty8(x, n, d, n) if checkpoint else [])
+
+
+def _norm_backward_fake(dy, x, q, s, mean, rstd, weight, center, need_dw, need_db):
+    gt = dy.dtype if weight is None else weight.dtype
+    return [dy.new_empty(dy.shape)] + [dy.new_empty((dy.shape[1],), dtype=gt) for _ in range(need_dw + need_db)]
+
+
+def _weight8_pack_fake(w, transposed):
+    n, k = w.shape
+    return _empty8(w, n, k, -(-n // 128)) + (_empty8(w, k, n, -(-k // 128)) if transposed else [])
+
+
+BLOCK_OPS = {
+    'norm_forward': _norm_forward_fake,
+    'norm_backward': _norm_backward_fake,
+    'act8_pack': lambda x: tuple(_empty8(x, x.shape[0], x.shape[1], x.shape[0])),
+    'act8_unpack': lambda q, s, dim, dtype: q.new_empty((q.shape[0], dim), dtype=dtype),
+    'weight8_pack': _weight8_pack_fake,
+    'product8': lambda q, s, wq, ws, inner, dtype: q.new_empty((q.shape[0], wq.shape[0]), dtype=dtype),
+    'weight_grad8': lambda dy, q, s, inner, dtype: dy.new_empty((dy.shape[1], inner), dtype=dtype),
+}
+
+for _name, _fake in BLOCK_OPS.items():
+    torch.library.register_fake(f'{NS}::{_name}', _fake)

@@ -1,0 +1,88 @@
+"""Linear maps on 8-bit operands: the forward product, the input's gradient and the weight's gradient.
+
+    a = act8.pack(x)                          # or norm.layer_norm(..., y8=True): the operand, and the checkpoint
+    w = linear8.pack_weight(weight)           # after each optimizer update
+    y = linear8.matmul(a, w)                  # x @ weight.T
+    dx = linear8.matmul(act8.pack(dy), w, transposed=True)        # dy @ weight
+    dw = linear8.weight_grad(dy, a)           # dy.T @ x, from the checkpoint
+
+``linear`` is the three of them as one differentiable function.  Products read e4m3 values and their scales and sum in
+fp32; the weight's gradient reads dy in bf16 and the checkpoint's values, which bf16 holds exactly.
+"""
+from dataclasses import dataclass
+
+import torch
+
+from . import act8, library  # noqa: F401  (library registers the operators)
+from .act8 import Act8
+
+_OPS = torch.ops.yoco_z1
+
+
+@dataclass(frozen=True, slots=True)
+class Weight8:
+    """A weight [N, K] in 128 x 128 blocks of one power-of-two scale each, in both orders: ``q`` float8_e4m3fn [N, K
+    rounded up to 128] with ``s`` float8_e8m0fnu [ceil(N / 128), blocks of K rounded up to 4], and ``qt`` [K, N rounded up
+    to 128] with ``st`` for the input's gradient (None: forward only)."""
+    q: torch.Tensor
+    s: torch.Tensor
+    qt: torch.Tensor
+    st: torch.Tensor
+    shape: tuple
+
+    def nbytes(self):
+        return sum(t.numel() for t in (self.q, self.s, self.qt, self.st) if t is not None)
+
+
+def pack_weight(w, transposed=True):
+    """The 8-bit form of a weight [N, K] (fp32, bf16 or fp16), with its other order unless transposed is False."""
+    if w.dim() != 2:
+        raise RuntimeError('linear8.pack_weight: expected a weight [N, K]')
+    out = _OPS.weight8_pack(act8.rows_of(w), transposed)
+    return Weight8(*(out if transposed else (*out, None, None)), tuple(w.shape))
+
+
+def matmul(a, w, dtype=torch.bfloat16, transposed=False):
+    """8-bit rows a [M, K] times the transpose of w [N, K]: [M, N] in `dtype`; transposed: a [M, N] times w: [M, K]."""
+    N, K = w.shape
+    if a.dim != (N if transposed else K):
+        raise RuntimeError(f'linear8.matmul: rows of {a.dim} columns do not fit a weight {N} x {K}'
+                           f'{" from the left" if transposed else ""}')
+    if transposed:
+        if w.qt is None:
+            raise RuntimeError('linear8.matmul: the weight was packed without its other order')
+        return _OPS.product8(a.q, a.s, w.qt, w.st, N, dtype)
+    return _OPS.product8(a.q, a.s, w.q, w.s, K, dtype)
+
+
+def weight_grad(dy, a, dtype=torch.bfloat16):
+    """dy^T x, [N, K] in `dtype`, from bf16 gradient rows dy [..., N] and the 8-bit rows a of x [..., K]."""
+    return _OPS.weight_grad8(act8.rows_of(dy), a.q, a.s, a.dim, dtype)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, w8):
+        a = act8.pack(x)
+        ctx.save_for_backward(a.q, a.s)
+        ctx.w8, ctx.dim, ctx.x_shape, ctx.dtype, ctx.w_dtype = w8, a.dim, x.shape, x.dtype, weight.dtype
+        return matmul(a, w8, x.dtype).view(*x.shape[:-1], w8.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = matmul(act8.pack(dy), ctx.w8, ctx.dtype, transposed=True).view(ctx.x_shape)
+        if ctx.needs_input_grad[1]:
+            dw = weight_grad(dy, Act8(*ctx.saved_tensors, ctx.dim), ctx.w_dtype)
+        return dx, dw, None
+
+
+def linear(x, weight, w8):
+    """x @ weight.T for bf16 x [..., K], differentiable: w8 is pack_weight(weight), packed again whenever the weight
+    changes.  What is kept for the backward pass is the 8-bit rows of x."""
+    if x.dtype != torch.bfloat16:
+        raise RuntimeError('linear8.linear: expected bf16 rows')
+    if tuple(weight.shape) != tuple(w8.shape):
+        raise RuntimeError(f'linear8.linear: a weight of {tuple(weight.shape)} and 8-bit blocks of {tuple(w8.shape)}')
+    return _Linear.apply(x, weight, w8)

@@ -42,7 +42,7 @@ enum {
                               FP32 gradient outputs by z1_table_set_grad_out */
 };
 
-enum { Z1_F32 = 0, Z1_BF16 = 1 };           /* gradient dtype codes */
+enum { Z1_F32 = 0, Z1_BF16 = 1, Z1_F16 = 2 }; /* dtype codes; gradients of the update: the first two */
 
 #define Z1_MAX_WORLD 16                      /* most contributions one owner-sum call takes */
 #define Z1_NORM_PARTIALS 2048                /* doubles in the norm workspace (fixed: the reduction order) */
@@ -252,6 +252,59 @@ int z1_embedding_backward(const int64_t* ids, const uint16_t* grad, int64_t R, i
                           int64_t workspace_bytes, void* stream);
 int64_t z1_embedding_backward_workspace(int64_t R, int64_t D, int64_t V);
 /* (z1_embedding_backward records no memset into a graph being captured: it orders the ids without one then.) */
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * Around the update: the blocks' norms, 8-bit activations and the linear maps that multiply them.
+ *
+ * 8-bit rows.  x[rows][dim] is held as bytes q[rows][wide] (e4m3) and s[rows][pitch] (E8M0), wide = dim rounded up to
+ * 128, pitch = wide / 128 rounded up to 4 (z1_act8_columns, z1_act8_scales).  Block j = columns 128 j .. 128 j + 127:
+ * e = the least integer >= -127 with max |x| <= 448 * 2^e over the block's finite elements, s = e + 127,
+ * q = e4m3(x * 2^-e) (nearest, ties to even), so x stands as q * 2^e.  Infinities and NaN become e4m3's NaN.  Padding:
+ * q is 0, s is 127 (a scale of 1).  q needs 16-byte alignment, s 4-byte.
+ *
+ * 8-bit weights.  w[N][K] is held in 128 x 128 blocks of one scale each, by the same rule: q[N][wide(K)] with
+ * s[ceil(N / 128)][pitch(K)], and in the other order qt[K][wide(N)] with st[ceil(K / 128)][pitch(N)] (the same bytes and
+ * scales transposed).
+ *
+ * Rows of x, dy and w start `stride` elements apart, at any element; results are contiguous.  Shapes without elements
+ * are no-ops.  dtype: Z1_F32, Z1_BF16 or Z1_F16.  Statistics and sums are fp32, and no sum's order depends on timing.
+ */
+
+/* Layer norm (center 1) or RMS norm (center 0) of each row: mean = sum(x) / dim (center 0: none), rstd =
+ * 1 / sqrt(sum((x - mean)^2) / dim + eps), y = (x - mean) rstd w + b.  w, b: [dim] in x's dtype or Z1_F32, or NULL (b
+ * only with center 1).  y (x's dtype) or its 8-bit rows yq, ys: one of the two.  cq, cs: NULL, or the 8-bit rows of x
+ * itself, a checkpoint that z1_norm_backward reads in x's place. */
+int z1_norm_forward(const void* x, int64_t rows, int64_t dim, int64_t stride, int dtype, const void* w, const void* b,
+                    int w_dtype, float eps, int center, void* y, void* yq, void* ys, void* cq, void* cs, float* mean,
+                    float* rstd, void* stream);
+
+/* Its gradients, from dy and x (dtype) or x's 8-bit rows q, s: dx (dtype), dw = sum over rows of dy (x - mean) rstd, db =
+ * sum over rows of dy (grad_dtype; NULL: not wanted, db only with center 1).  workspace: device floats,
+ * z1_norm_backward_workspace(rows, dim) of them; NULL where neither dw nor db is wanted. */
+int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* q, const void* s,
+                     int64_t rows, int64_t dim, int dtype, const float* mean, const float* rstd, const void* w,
+                     int w_dtype, int center, void* dx, void* dw, void* db, int grad_dtype, float* workspace,
+                     int64_t workspace_floats, void* stream);
+int64_t z1_norm_backward_workspace(int64_t rows, int64_t dim);
+
+/* Rows to 8 bits and back.  Unpacked, a finite value stays finite: one past dtype's largest becomes the largest. */
+int64_t z1_act8_columns(int64_t dim);
+int64_t z1_act8_scales(int64_t dim);
+int z1_act8_pack(const void* x, int64_t rows, int64_t dim, int64_t stride, int dtype, void* q, void* s, void* stream);
+int z1_act8_unpack(const void* q, const void* s, int64_t rows, int64_t dim, void* out, int dtype, void* stream);
+
+/* A weight to 8 bits, in both orders (qt, st NULL: the first only). */
+int z1_weight8_pack(const void* w, int64_t N, int64_t K, int64_t stride, int dtype, void* q, void* s, void* qt, void* st,
+                    void* stream);
+
+/* y[M][N] (dtype) = 8-bit rows a, as [M][K] times the transpose of 8-bit weight w, ws [N][K].  The input gradient is the
+ * same product with the rows of dy and the weight's other order. */
+int z1_product8(const void* a, const void* as, int64_t M, const void* w, const void* ws, int64_t N, int64_t K, void* y,
+                int dtype, void* stream);
+
+/* dw[N][K] (dtype) = sum over T tokens of dy[t][n] (bf16) times the 8-bit rows q, s [T][K]; zeros for T = 0. */
+int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const void* s, int64_t T, int64_t N, int64_t K,
+                    void* dw, int dtype, void* stream);
 
 /* Text for a return code (negative: argument errors; positive: hipError_t). */
 const char* z1_strerror(int code);
