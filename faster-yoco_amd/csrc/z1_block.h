@@ -55,6 +55,18 @@ struct F32 {
         q[1] = b;
     }
     static __device__ __forceinline__ void put(void* p, int64_t i, float v) { ((Z1B_GLOBAL float*)p)[i] = v; }
+    // eight elements to a row in LDS from element i (a multiple of 8) on, and from there to memory
+    static __device__ __forceinline__ void store_local(uint8_t* row, int i, const float* v) {
+        f4* q = (f4*)(row + i * 4);
+        q[0] = f4{v[0], v[1], v[2], v[3]};
+        q[1] = f4{v[4], v[5], v[6], v[7]};
+    }
+    static __device__ __forceinline__ void copy_local(void* p, int64_t at, const uint8_t* row, int i) {
+        const f4* q = (const f4*)(row + i * 4);
+        Z1B_GLOBAL f4_any4* to = (Z1B_GLOBAL f4_any4*)((float*)p + at);
+        to[0] = q[0];
+        to[1] = q[1];
+    }
     static constexpr float kMax = 3.402823466e38f;
 };
 
@@ -71,14 +83,21 @@ struct BF16 {
     static __device__ __forceinline__ float one(const void* p, int64_t i) {
         return as_f32((uint32_t)((const Z1B_GLOBAL uint16_t*)p)[i] << 16);
     }
-    static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
+    static __device__ __forceinline__ u4 close(const float* v) {
         u4 w;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const f2 x = {v[2 * j], v[2 * j + 1]};
             w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, b2));
         }
-        *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + i) = w;
+        return w;
+    }
+    static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
+        *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + i) = close(v);
+    }
+    static __device__ __forceinline__ void store_local(uint8_t* row, int i, const float* v) { *(u4*)(row + i * 2) = close(v); }
+    static __device__ __forceinline__ void copy_local(void* p, int64_t at, const uint8_t* row, int i) {
+        *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + at) = *(const u4*)(row + i * 2);
     }
     static __device__ __forceinline__ void put(void* p, int64_t i, float v) { ((Z1B_GLOBAL __bf16*)p)[i] = (__bf16)v; }
     static constexpr float kMax = 3.3895313893e38f;
@@ -99,14 +118,21 @@ struct F16 {
     static __device__ __forceinline__ float one(const void* p, int64_t i) {
         return (float)((const Z1B_GLOBAL _Float16*)p)[i];
     }
-    static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
+    static __device__ __forceinline__ u4 close(const float* v) {
         u4 w;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const f2 x = {v[2 * j], v[2 * j + 1]};
             w[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, h2));
         }
-        *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + i) = w;
+        return w;
+    }
+    static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
+        *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + i) = close(v);
+    }
+    static __device__ __forceinline__ void store_local(uint8_t* row, int i, const float* v) { *(u4*)(row + i * 2) = close(v); }
+    static __device__ __forceinline__ void copy_local(void* p, int64_t at, const uint8_t* row, int i) {
+        BF16::copy_local(p, at, row, i);
     }
     static __device__ __forceinline__ void put(void* p, int64_t i, float v) {
         ((Z1B_GLOBAL _Float16*)p)[i] = (_Float16)v;

@@ -44,20 +44,14 @@ __device__ __forceinline__ u4 open_bf16(u2 q, float f) {
 // Adds the products of two 32-row fragments of 64 columns.  The 8-bit instructions sum 8 products at a time on a common
 // exponent and cut what is more than 13 bits below the largest (probed: 256 + 2^-5 arrives, 256 + 2^-6 does not, while
 // sums across groups keep 24 bits), an error of 1.5e-5 of the result on activations: far below a 16-bit result's own
-// rounding, not below an fp32 one's.  PRECISE opens both operands to bf16 (exact) for the bf16 instructions, whose sums
-// are fp32 throughout, at half the rate.
-template <bool PRECISE, int NO, int NT>
-__device__ __forceinline__ void multiply(f16 (&acc)[NO][NT], const i8 (&fo)[NO], const i8 (&ft)[NT], uint32_t so,
-                                         const uint32_t (&st)[NT]) {
-    if (!PRECISE) {
-#pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fo[i], ft[j], acc[i][j], kE4M3, kE4M3, 0, (int)so,
-                                                                            0, (int)st[j]);
-        return;
-    }
+// rounding, not below an fp32 one's.  The precise form opens both operands to bf16 (exact) for the bf16 instructions, whose
+// sums are fp32 throughout, at half the rate.
+__device__ __forceinline__ f16 multiply(f16 acc, i8 fo, i8 ft, uint32_t so, uint32_t st) {
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fo, ft, acc, kE4M3, kE4M3, 0, (int)so, 0, (int)st);
+}
+template <int NO, int NT>
+__device__ __forceinline__ void multiply_precise(f16 (&acc)[NO][NT], const i8 (&fo)[NO], const i8 (&ft)[NT], uint32_t so,
+                                                 const uint32_t (&st)[NT]) {
     const float go = scale_value(so & 0xffu);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {                      // 8 bytes of a lane: 16 columns of the wave
@@ -76,15 +70,70 @@ __device__ __forceinline__ void multiply(f16 (&acc)[NO][NT], const i8 (&fo)[NO],
     }
 }
 
-// A lane's 16 consecutive outputs of one row; n of them are in the row.
-template <typename T>
-__device__ __forceinline__ void put16(void* out, int64_t at, int64_t n, const f16& v) {
-    float x[16];
+// A wave's 32 rows of C columns of a result, out of the matrix instructions' layout by way of its own ROOM bytes of LDS: a
+// lane holds 16 columns of one row, whose pieces of 16 bytes would go out as requests of their own (64 to an instruction),
+// while the rows read back go out as whole lines.  row0, col0: the first of them in out[rows][cols].
+template <typename T, int C, int ROOM>
+struct Flush {
+    static constexpr int kElem = (int)sizeof(typename T::elem);
+    static constexpr int pitch(int c) { return c * kElem + 16; }               // 16 neighbouring rows in different banks
+    static constexpr int kC = 32 * pitch(C) <= ROOM ? C : 32 * pitch(C / 2) <= ROOM ? C / 2 : 32;      // at a time
+    static constexpr int kPitch = pitch(kC);
+    static_assert(32 * kPitch <= ROOM, "room for a wave's rows");
+    static __device__ __forceinline__ void run(uint8_t* own, int lane, const f16 (&acc)[C / 32], void* out, int64_t row0,
+                                               int64_t rows, int col0, int cols) {
+        const int r32 = lane & 31, half = lane >> 5;
+        constexpr int kGroups = kC / kLane, kRows = 64 / kGroups;              // rows of one access
+        const int c = lane % kGroups * kLane, r = lane / kGroups;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = v[i];
+        for (int c0 = 0; c0 < C; c0 += kC) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-        if (n > 8 * h) store_row<T>(out, at + 8 * h, n - 8 * h < kLane ? (int)(n - 8 * h) : kLane, x + 8 * h);
+            for (int i = 0; i < kC / 32; ++i) {
+                float x[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[k] = acc[c0 / 32 + i][k];
+                uint8_t* to = own + r32 * kPitch;
+                T::store_local(to, i * 32 + half * 16, x);
+                T::store_local(to, i * 32 + half * 16 + 8, x + 8);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // a wave's own bytes: nobody to meet
+            const int n = cols - col0 - c0 - c;
+#pragma unroll
+            for (int k = 0; k < 32 / kRows; ++k) {
+                const int row = k * kRows + r;
+                if (row0 + row >= rows || n <= 0) continue;
+                const uint8_t* from = own + row * kPitch;
+                const int64_t at = (row0 + row) * cols + col0 + c0 + c;
+                if (n >= kLane) {
+                    T::copy_local(out, at, from, c);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kLane; ++j)
+                        if (j < n) ((Z1B_GLOBAL typename T::elem*)out)[at + j] = ((const typename T::elem*)from)[c + j];
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // before the next rows overwrite them
+        }
+    }
+};
+
+// All waves of the workgroup are here, their direct loads into LDS have arrived and their reads from it are done.
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A raw buffer of `bytes` (none where negative) from p: loads past it give zeros (word 3: the raw 32-bit data format).
+// Without a branch: a loop around it keeps its loads on their way.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64_t bytes) {
+    const uint32_t low = (uint32_t)bytes, high = (uint32_t)(bytes >> 32);
+    const uint32_t n = (low | (uint32_t)-(int)(high != 0)) & ~(uint32_t)((int)high >> 31);
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n, 0x00020000);
+}
+// 16 bytes a lane, straight into LDS at `to` + 16 * lane.
+__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, void* to, int lane_at, int at) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Z1B_LDS void*)to, 16, lane_at, at, 0, 0);
 }
 
 struct Product {
@@ -99,15 +148,11 @@ struct Product {
 };
 
 // Staging keeps rows of 128 bytes (one block of K).  A lane of a direct load writes 16 bytes at its own place in a run of
-// 1024, so the order of a row's eight 16-byte pieces is changed at the source: piece p of a row lies at p ^ key(row), and
-// the eight rows that neighbouring lanes read together have eight different keys.
-__device__ __forceinline__ int key_plain(int row) { return row & 7; }
-__device__ __forceinline__ int key_spread(int row) { return (row & 3) | ((row >> 4 & 1) << 2); }
-
-__device__ __forceinline__ i8 piece_pair(const uint8_t* row, int p, int key) {
-    const i4 lo = *(const i4*)(row + ((p ^ key) << 4)), hi = *(const i4*)(row + (((p + 1) ^ key) << 4));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+// 1024, so the order of a row's eight 16-byte pieces is changed at the source: piece p of a row lies at p ^ key(row).  LDS
+// has 64 banks of 4 bytes, two rows: the 16 rows that neighbouring lanes read together are eight of either parity, with
+// eight different keys.
+__device__ __forceinline__ int key_plain(int row) { return row >> 1 & 7; }
+__device__ __forceinline__ int key_spread(int row) { return (row >> 1 & 3) | (row >> 4 & 1) << 2; }
 
 // BT x BO outputs (tokens x outputs) of a workgroup, WT x WO of a wave.
 template <typename T, bool PRECISE, int BT, int BO, int WT, int WO>
@@ -122,46 +167,32 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     const int o0 = (int)(blockIdx.x % tiles_o) * BO;
     const int wt = wave / (BO / WO) * WT, wo = wave % (BO / WO) * WO;          // the wave's part of the tile
 
-    const uint8_t* src_t[kPT];
-    const uint8_t* src_o[kPO];
+    // Rows past the end lie past their buffer's range, which a load turns to zeros.
+    const __amdgpu_buffer_rsrc_t buf_t = buffer_of(a.a + t0 * a.wide, (a.M - t0) * a.wide);
+    const __amdgpu_buffer_rsrc_t buf_o = buffer_of(a.w + o0 * a.wide, (a.N - o0) * a.wide);
+    const int wide = (int)a.wide;
     const int sub = lane >> 3, piece = lane & 7;
-#pragma unroll
-    for (int i = 0; i < kPT; ++i) {
-        const int row = (wave * kPT + i) * 8 + sub;
-        int64_t t = t0 + row;
-        t = t < a.M ? t : a.M - 1;                     // rows past the end repeat the last; their results are dropped
-        src_t[i] = a.a + t * a.wide + ((piece ^ key_plain(row)) << 4);
-    }
-#pragma unroll
-    for (int i = 0; i < kPO; ++i) {
-        const int row = (wave * kPO + i) * 8 + sub;
-        int o = o0 + row;
-        o = o < a.N ? o : a.N - 1;
-        src_o[i] = a.w + o * a.wide + ((piece ^ key_spread(row)) << 4);
-    }
-    auto stage = [&](int kb, uint8_t* buf) {
-#pragma unroll
-        for (int i = 0; i < kPT; ++i)
-            __builtin_amdgcn_global_load_lds((const Z1B_GLOBAL void*)(src_t[i] + (int64_t)kb * kBlock),
-                                             (Z1B_LDS void*)(buf + (wave * kPT + i) * 8 * kBlock), 16, 0, 0);
-#pragma unroll
-        for (int i = 0; i < kPO; ++i)
-            __builtin_amdgcn_global_load_lds((const Z1B_GLOBAL void*)(src_o[i] + (int64_t)kb * kBlock),
-                                             (Z1B_LDS void*)(buf + (BT + (wave * kPO + i) * 8) * kBlock), 16, 0, 0);
+    const int from = sub * wide + ((piece ^ (sub >> 1)) << 4);                 // in 8 rows whose keys' third bit is 0
+    auto stage = [&](int kb, int i) {                  // the i-th direct load of this wave's part of a block
+        uint8_t* buf = lds[kb & 1];
+        const int g = i < kPT ? wave * kPT + i : wave * kPO + i - kPT;
+        const int at = g * 8 * wide + kb * kBlock;
+        if (i < kPT) load_lds(buf_t, buf + g * 8 * kBlock, g & 1 ? from ^ 64 : from, at);
+        else load_lds(buf_o, buf + (BT + g * 8) * kBlock, g & 2 ? from ^ 64 : from, at);
     };
     // scales: four blocks' bytes at a time, the next four loaded ahead
-    const uint8_t* sa[NT];
-    uint32_t now[NT], next[NT];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        int64_t t = t0 + wt + j * 32 + (lane & 31);
-        t = t < a.M ? t : a.M - 1;
-        sa[j] = a.as + t * a.pitch;
-        next[j] = *(const Z1B_GLOBAL uint32_t*)sa[j];
-    }
+    const __amdgpu_buffer_rsrc_t buf_s = buffer_of(a.as + t0 * a.pitch, (a.M - t0) * a.pitch);
+    const int r32 = lane & 31, half = lane >> 5, rs = spread(r32);
     const int ob = (o0 + wo) / kBlock, ob_last = (a.N - 1) / kBlock;
-    const uint8_t* sw = a.ws + (int64_t)(ob < ob_last ? ob : ob_last) * a.pitch;
-    uint32_t now_w = 0, next_w = *(const Z1B_GLOBAL uint32_t*)sw;
+    const uint32_t* sw = (const uint32_t*)(a.ws + (int64_t)(ob < ob_last ? ob : ob_last) * a.pitch);
+    uint32_t now[NT] = {}, next[NT], now_w = 0, next_w;
+    auto scales = [&](int kb) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            next[j] = __builtin_amdgcn_raw_buffer_load_b32(buf_s, r32 * a.pitch, (wt + j * 32) * a.pitch + kb, 0);
+        next_w = sw[kb / 4];
+    };
+    scales(0);
 
     f16 acc[NO][NT];
 #pragma unroll
@@ -169,46 +200,77 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f16{};
 
-    const int r32 = lane & 31, half = lane >> 5, rs = spread(r32);
-    stage(0, lds[0]);
+    // A block's two halves of 64 columns are read ahead by one half, and the workgroup meets between them: what follows
+    // the meeting -- the next block's first reads, the direct loads into the buffer that has just been read -- runs beside
+    // the second half's products, one read or load after each, and what it waits for was issued a whole block before.
+    // (All loads at once after the meeting hold up the products until the address unit has taken them: 64 loads of 16
+    // cycles.)  Past the last block the reads and loads are of no use, and in bounds.
+    constexpr int kReads = 2 * (NT + NO), kLoads = kPT + kPO, kProducts = NT * NO;
+    i4 f[2][NT + NO][2];
+    auto read = [&](int kb, int h, int q) {
+        const int i = q >> 1, p = 4 * h + 2 * half + (q & 1);
+        const uint8_t* row = i < NT ? lds[kb & 1] + (wt + i * 32 + r32) * kBlock
+                                    : lds[kb & 1] + (BT + wo + (i - NT) * 32 + rs) * kBlock;
+        f[h][i][q & 1] = *(const i4*)(row + ((p ^ (i < NT ? key_plain(r32) : key_spread(rs))) << 4));
+    };
+    // products of half h; beside them, the reads of half 1 - h of block kb_read and the loads of block kb_load (< 0: none)
+    auto products = [&](int h, int kb_read, int kb_load) {
+        auto beside = [&](int m, int of) {
+#pragma unroll
+            for (int q = 0; q < kReads; ++q)
+                if (q * of / kReads == m) read(kb_read, 1 - h, q);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                if (kb_load >= 0 && i * of / kLoads == m) stage(kb_load, i);
+        };
+        auto pair = [&](int i) { return __builtin_shufflevector(f[h][i][0], f[h][i][1], 0, 1, 2, 3, 4, 5, 6, 7); };
+        if constexpr (PRECISE) {
+            beside(0, 1);
+            i8 ft[NT], fo[NO];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) ft[j] = pair(j);
+#pragma unroll
+            for (int i = 0; i < NO; ++i) fo[i] = pair(NT + i);
+            multiply_precise(acc, fo, ft, now_w, now);
+        } else {
+#pragma unroll
+            for (int m = 0; m < kProducts; ++m) {
+                const int i = m / NT, j = m % NT;
+                acc[i][j] = multiply(acc[i][j], pair(NT + i), pair(j), now_w, now[j]);
+                beside(m, kProducts);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) stage(0, i);
+    meet();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) stage(1, i);
+#pragma unroll
+    for (int q = 0; q < kReads; ++q) read(0, 0, q);
     for (int kb = 0; kb < a.blocks; ++kb) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");                       // this wave's direct loads of block kb
-        __syncthreads();                               // every wave's, and block kb - 1 has been read
-        if (kb + 1 < a.blocks) stage(kb + 1, lds[(kb + 1) & 1]);
         if ((kb & 3) == 0) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) now[j] = next[j];
             now_w = next_w;
-            if (kb + 4 < a.blocks) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) next[j] = *(const Z1B_GLOBAL uint32_t*)(sa[j] + kb + 4);
-                next_w = *(const Z1B_GLOBAL uint32_t*)(sw + kb + 4);
-            }
+            scales(kb + 4 < a.blocks ? kb + 4 : 0);
         }
-        const uint8_t* bt = lds[kb & 1] + (wt + r32) * kBlock;
-        const uint8_t* bo = lds[kb & 1] + (BT + wo + rs) * kBlock;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            i8 ft[NT], fo[NO];
-#pragma unroll
-            for (int j = 0; j < NT; ++j) ft[j] = piece_pair(bt + j * 32 * kBlock, 4 * h + 2 * half, key_plain(r32));
-#pragma unroll
-            for (int i = 0; i < NO; ++i) fo[i] = piece_pair(bo + i * 32 * kBlock, 4 * h + 2 * half, key_spread(rs));
-            multiply<PRECISE>(acc, fo, ft, now_w, now);
-        }
+        products(0, kb, -1);
+        meet();                                        // block kb has been read, block kb + 1 has arrived
+        products(1, kb + 1, kb + 2);
 #pragma unroll
         for (int j = 0; j < NT; ++j) now[j] >>= 8;
         now_w >>= 8;
     }
+    meet();                                            // the staging buffers are free
+    constexpr int kRoom = (int)sizeof(lds) / kWaves;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-        const int64_t t = t0 + wt + j * 32 + r32;
-        if (t >= a.M) continue;
+        f16 part[NO];
 #pragma unroll
-        for (int i = 0; i < NO; ++i) {
-            const int o = o0 + wo + i * 32 + half * 16;
-            put16<T>(a.y, t * a.N + o, a.N - o, acc[i][j]);
-        }
+        for (int i = 0; i < NO; ++i) part[i] = acc[i][j];
+        Flush<T, WO, kRoom>::run(&lds[0][0] + wave * kRoom, lane, part, a.y, t0 + wt + j * 32, a.M, o0 + wo, a.N);
     }
 }
 
@@ -236,7 +298,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(Product a) 
             const i8 fx[1] = {__builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7)};
             const i8 fw[1] = {__builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7)};
             const uint32_t sx[1] = {sa[kb]};
-            multiply<PRECISE>(acc, fw, fx, sw[kb], sx);
+            if constexpr (PRECISE) multiply_precise(acc, fw, fx, sw[kb], sx);
+            else acc[0][0] = multiply(acc[0][0], fw[0], fx[0], sw[kb], sx[0]);
         }
     }
 #pragma unroll
@@ -270,13 +333,28 @@ __device__ __forceinline__ s8 column_pair(const uint16_t* lo, const uint16_t* hi
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// BN x BK of dw to a workgroup, WN x WK to a wave, TS tokens staged at a time.
-template <typename T, int BN, int BK, int WN, int WK, int TS>
+// Eight 16-bit values moved down by n (0..7) places.
+__device__ __forceinline__ u4 shift_pieces(u4 v, int n) {
+    v = n & 4 ? u4{v[2], v[3], 0, 0} : v;
+    v = n & 2 ? u4{v[1], v[2], v[3], 0} : v;
+    const u4 w = {v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    return n & 1 ? w : v;
+}
+
+// BN x BK of dw to a workgroup, WN x WK to a wave, TS tokens staged at a time, twice buffered.  While a step's products
+// run, the next step's pieces go from registers into the other buffer, and the pieces of the step after that are loaded
+// into those registers: a load has a whole step to arrive, and neither staging nor opening stands between two steps.  The
+// loop has no branch (a branch around a load makes the waits for all of them complete): the first step has the rows that
+// do not fill one, every other is full, and past the last one the same rows are loaded again and not used.
+enum Edge { kWhole, kCut, kFew };                      // N a multiple of 8; not, but at least 8; less than 8
+template <typename T, Edge EDGE, int BN, int BK, int WN, int WK, int TS>
 __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(Gradient a) {
     constexpr int kThreads = BN / WN * (BK / WK) * 64;
     constexpr int kPitchN = BN + 32, kPitchK = BK + 32;                        // elements: rows 64 bytes apart in the banks
     constexpr int kDy = TS * BN / 8 / kThreads, kX = TS * BK / 8 / kThreads;   // 8-element pieces of a thread
-    constexpr int NN = WN / 32, NK = WK / 32;
+    constexpr int kDyRows = kThreads / (BN / 8), kXRows = kThreads / (BK / 8); // rows between a thread's pieces
+    constexpr int NN = WN / 32, NK = WK / 32, KK = TS / 16;
+    static_assert(kThreads % (BN / 8) == 0 && kThreads % (BK / 8) == 0, "a thread keeps its columns");
     __shared__ __align__(16) uint16_t lds_n[2][TS * kPitchN];
     __shared__ __align__(16) uint16_t lds_k[2][TS * kPitchK];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -284,43 +362,71 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     const int n0 = (int)(blockIdx.x / tiles_k) * BN, k0 = (int)(blockIdx.x % tiles_k) * BK;
     const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
 
+    // Loads ask nothing: rows past the end repeat the last one (zeroed when kept), columns past it repeat columns whose
+    // results are dropped.  A piece that the row's end cuts starts 8 columns before the end and is shifted when kept.
+    const int last_n = a.N - 8, cut = a.N & 7;
+    const int row_n = threadIdx.x / (BN / 8), row_k = threadIdx.x / (BK / 8);
+    const int my_n = threadIdx.x % (BN / 8) * 8, my_k = threadIdx.x % (BK / 8) * 8;
+    const int from_n = n0 + my_n < last_n ? n0 + my_n : last_n;
+    const int from_k = k0 + my_k < a.wide ? k0 + my_k : a.wide - 8;
+    const bool shifted = EDGE == kCut && n0 + my_n > last_n;
     u4 dy[kDy];
     u2 x[kX];
     uint32_t xs[kX];
-    auto fetch = [&](int64_t t0) {
+    uint32_t at_n[kDy], at_k[kX], at_s[kX];            // offsets of the pieces from a step's first row
+    auto place = [&](int rows) {                       // of a step with that many rows
 #pragma unroll
         for (int i = 0; i < kDy; ++i) {
-            const int e = i * kThreads + threadIdx.x, c = e % (BN / 8) * 8;
-            const int64_t t = t0 + e / (BN / 8);
-            const int n = t < a.T ? a.N - n0 - c : 0;
-            if (n >= 8) {
-                dy[i] = *(const Z1B_GLOBAL u4_any2*)(a.dy + t * a.stride + n0 + c);
-            } else {
+            const int t = row_n + i * kDyRows < rows ? row_n + i * kDyRows : rows - 1;
+            at_n[i] = (uint32_t)t * (uint32_t)a.stride + (EDGE == kFew ? 0u : (uint32_t)from_n);
+        }
+#pragma unroll
+        for (int i = 0; i < kX; ++i) {
+            const int t = row_k + i * kXRows < rows ? row_k + i * kXRows : rows - 1;
+            at_k[i] = (uint32_t)t * (uint32_t)a.wide + (uint32_t)from_k;
+            at_s[i] = (uint32_t)t * (uint32_t)a.pitch + (uint32_t)from_k / kBlock;
+        }
+    };
+    auto fetch = [&](int64_t t0, int part, int parts) {
+        const uint16_t* dy0 = a.dy + t0 * a.stride;
+        const uint8_t* q0 = a.q + t0 * a.wide;
+        const uint8_t* s0 = a.s + t0 * a.pitch;
+#pragma unroll
+        for (int i = 0; i < kDy; ++i) {
+            if (i * parts / kDy != part) continue;
+            if (EDGE == kFew) {
                 dy[i] = u4{};
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (j < n) dy[i][j / 2] |= (uint32_t)((const Z1B_GLOBAL uint16_t*)a.dy)[t * a.stride + n0 + c + j] << (16 * (j % 2));
+                    if (j < a.N) dy[i][j / 2] |= (uint32_t)((const Z1B_GLOBAL uint16_t*)dy0)[at_n[i] + j] << (16 * (j % 2));
+            } else {
+                dy[i] = *(const Z1B_GLOBAL u4_any2*)(dy0 + at_n[i]);
             }
         }
 #pragma unroll
         for (int i = 0; i < kX; ++i) {
-            const int e = i * kThreads + threadIdx.x, c = e % (BK / 8) * 8;
-            const int64_t t = t0 + e / (BK / 8);
-            const bool in = t < a.T && k0 + c < a.wide;
-            x[i] = in ? *(const Z1B_GLOBAL u2*)(a.q + t * a.wide + k0 + c) : u2{0, 0};
-            xs[i] = in ? a.s[t * a.pitch + (k0 + c) / kBlock] : 127u;
+            if (i * parts / kX != part) continue;
+            x[i] = *(const Z1B_GLOBAL u2*)(q0 + at_k[i]);
+            xs[i] = s0[at_s[i]];
         }
     };
-    auto keep = [&](int buf) {
+    auto keep = [&](int rows, int buf, int part, int parts) {
 #pragma unroll
         for (int i = 0; i < kDy; ++i) {
-            const int e = i * kThreads + threadIdx.x;
-            *(u4*)(lds_n[buf] + e / (BN / 8) * kPitchN + e % (BN / 8) * 8) = dy[i];
+            if (i * parts / kDy != part) continue;
+            const int t = row_n + i * kDyRows;
+            u4 v = dy[i];
+            if (EDGE == kCut) v = shift_pieces(v, shifted ? 8 - cut : 0);
+            if (rows < TS && t >= rows) v = u4{};
+            *(u4*)(lds_n[buf] + t * kPitchN + my_n) = v;
         }
 #pragma unroll
         for (int i = 0; i < kX; ++i) {
-            const int e = i * kThreads + threadIdx.x;
-            *(u4*)(lds_k[buf] + e / (BK / 8) * kPitchK + e % (BK / 8) * 8) = open_bf16(x[i], scale_value(xs[i]));
+            if (i * parts / kX != part) continue;
+            const int t = row_k + i * kXRows;
+            u4 v = open_bf16(x[i], scale_value(xs[i]));
+            if (rows < TS && t >= rows) v = u4{};
+            *(u4*)(lds_k[buf] + t * kPitchK + my_k) = v;
         }
     };
 
@@ -335,44 +441,199 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     const int row = (group >> 1) * 8 + (p >> 2);
     const int col_n = (group & 1) * 16 + (p & 3) * 4;
     const int col_k = spread((group & 1) * 16 + (p & 3) * 4);                  // rows of the result in spread order
-    fetch(0);
-    keep(0);
-    int buf = 0;
-    for (int64_t t0 = 0; t0 < a.T; t0 += TS) {
+    const int64_t steps = (a.T + TS - 1) / TS;
+    const int first = (int)(a.T - (steps - 1) * TS);   // rows of the first step
+    if (steps > 0) {
+        place(first);
+        fetch(0, 0, 1);
+        keep(first, 0, 0, 1);
+        if (steps > 1) {
+            place(TS);
+            fetch(first, 0, 1);
+        }
+    }
+    const int64_t end = steps > 1 ? a.T - TS : 0;      // first row of the last step
+    int64_t next = end < first + TS ? end : first + TS;
+    for (int64_t step = 0; step < steps; ++step) {
+        const int buf = (int)(step & 1);
         __syncthreads();
-        if (t0 + TS < a.T) fetch(t0 + TS);
         const uint16_t* bn = lds_n[buf] + row * kPitchN + wn + col_n;
         const uint16_t* bk = lds_k[buf] + row * kPitchK + wk + col_k;
-#pragma unroll
-        for (int kk = 0; kk < TS / 16; ++kk) {
-            s8 fn[NN], fk[NK];
+        s8 fn[2][NN], fk[2][NK];
+        auto read = [&](int kk) {
 #pragma unroll
             for (int j = 0; j < NN; ++j)
-                fn[j] = column_pair(bn + kk * 16 * kPitchN + j * 32, bn + (kk * 16 + 4) * kPitchN + j * 32);
+                fn[kk & 1][j] = column_pair(bn + kk * 16 * kPitchN + j * 32, bn + (kk * 16 + 4) * kPitchN + j * 32);
 #pragma unroll
             for (int i = 0; i < NK; ++i)
-                fk[i] = column_pair(bk + kk * 16 * kPitchK + i * 32, bk + (kk * 16 + 4) * kPitchK + i * 32);
+                fk[kk & 1][i] = column_pair(bk + kk * 16 * kPitchK + i * 32, bk + (kk * 16 + 4) * kPitchK + i * 32);
+        };
+        read(0);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            if (kk + 1 < KK) read(kk + 1);
+            keep(TS, buf ^ 1, kk, KK);
+            fetch(next, kk, KK);
+            __builtin_amdgcn_sched_barrier(0);         // the compiler would gather the loads at the step's end
 #pragma unroll
             for (int i = 0; i < NK; ++i)
 #pragma unroll
                 for (int j = 0; j < NN; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, fk[i]),
-                                                                        __builtin_bit_cast(b8, fn[j]), acc[i][j], 0, 0, 0);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, fk[kk & 1][i]),
+                                                                        __builtin_bit_cast(b8, fn[kk & 1][j]), acc[i][j],
+                                                                        0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (t0 + TS < a.T) keep(buf ^ 1);
-        buf ^= 1;
+        next = next + TS < end ? next + TS : end;
     }
-    const int half = lane >> 5;
+    __syncthreads();                                   // the staging buffers are free
+    constexpr int kRoom = (int)sizeof(lds_n) / (kThreads / 64) & ~15;
 #pragma unroll
     for (int j = 0; j < NN; ++j) {
-        const int n = n0 + wn + j * 32 + (lane & 31);
-        if (n >= a.N) continue;
+        f16 part[NK];
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const int k = k0 + wk + i * 32 + half * 16;
-            put16<T>(a.dw, (int64_t)n * a.K + k, a.K - k, acc[i][j]);
-        }
+        for (int i = 0; i < NK; ++i) part[i] = acc[i][j];
+        Flush<T, WK, kRoom>::run((uint8_t*)lds_n + wave * kRoom, lane, part, a.dw, n0 + wn + j * 32, a.N, k0 + wk, a.K);
     }
+}
+
+// The same where dy's rows start at whole dwords: dy goes straight into LDS, and both operands are staged the way the
+// product's are.  Rows of both lie whole in LDS; a transposing read takes 64 bytes of four tokens at a time, so a row's
+// 64-byte runs are placed at run ^ (token & 3), which puts the four in different banks.  What lies past the last token or
+// past a tensor's end is zero (the buffers' ranges).
+//
+// A step of TS tokens is TS / 16 parts.  Each part's operands are read a part ahead, and the workgroup meets before the
+// last part: all of the step has been read by then.  From one meeting to the next (`between`) everything is read from one
+// buffer, the next step's, while the direct loads of dy and the opened rows of a two steps on (loaded into registers a
+// step before) go into the other.  It is one function of four restricted pointers because the compiler else takes every
+// transposing read for one of the bytes on their way and waits for them.
+template <typename T, int BN, int BK, int WN, int WK, int TS>
+__global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_kernel(Gradient a) {
+    constexpr int kThreads = BN / WN * (BK / WK) * 64, kWaves = kThreads / 64;
+    constexpr int NN = WN / 32, NK = WK / 32, KK = TS / 16;
+    constexpr int kRowN = BN * 2, kRowK = BK * 2;                              // bytes of a row in LDS
+    constexpr int kLoadRows = 1024 / kRowN;                                    // rows of a wave's direct load
+    constexpr int kLoads = TS / kLoadRows / kWaves;
+    constexpr int kX = TS * BK / 16 / kThreads, kXRows = kThreads / (BK / 16); // 16-column pieces of a thread
+    static_assert(kLoadRows == 2 || kLoadRows == 4, "rows of 256 or 512 bytes");
+    __shared__ __align__(1024) uint8_t lds[2 * TS * (kRowN + kRowK)];
+    auto lds_n = [&](int64_t step) { return lds + (step & 1) * TS * kRowN; };
+    auto lds_k = [&](int64_t step) { return lds + (2 * kRowN + (step & 1) * kRowK) * TS; };
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tiles_k = (a.K + BK - 1) / BK;
+    const int n0 = (int)(blockIdx.x / tiles_k) * BN, k0 = (int)(blockIdx.x % tiles_k) * BK;
+    const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
+    const int64_t steps = (a.T + TS - 1) / TS;
+
+    // direct loads: a lane's row and piece of 16 bytes within a load's rows
+    const int sub = lane / (64 / kLoadRows), piece = lane % (64 / kLoadRows);
+    const int row_bytes = (int)a.stride * 2;
+    int from[kLoadRows == 2 ? 2 : 1];                  // by the parity of the load: two rows are half of four
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(from) / sizeof(int)); ++i)
+        from[i] = sub * row_bytes + ((piece ^ (((i * kLoadRows + sub) & 3) << 2)) << 4);
+    const int64_t bytes_n = (a.T - 1) * row_bytes + (a.N - n0) * 2;            // from the tile's first column to dy's end
+    auto stage = [&](int64_t step, int i, uint8_t* to) {
+        const int64_t t0 = step * TS;
+        const int g = wave * kLoads + i;
+        const __amdgpu_buffer_rsrc_t rows = buffer_of(a.dy + t0 * a.stride + n0, bytes_n - t0 * row_bytes);
+        load_lds(rows, to + g * 1024, from[kLoadRows == 2 ? g & 1 : 0], g * kLoadRows * row_bytes);
+    };
+    u4 x[kX];
+    uint32_t xs[kX];
+    const int row_x = threadIdx.x / (BK / 16), col_x = threadIdx.x % (BK / 16) * 16;
+    const int from_q = row_x * a.wide + k0 + col_x, from_s = row_x * a.pitch + (k0 + col_x) / kBlock;
+    auto fetch = [&](int64_t step, int i) {
+        const int64_t t0 = step * TS, left = a.T - t0;
+        x[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.q + t0 * a.wide, left * a.wide), from_q,
+                                                     i * kXRows * a.wide, 0);
+        xs[i] = __builtin_amdgcn_raw_buffer_load_b8(buffer_of(a.s + t0 * a.pitch, left * a.pitch), from_s,
+                                                    i * kXRows * a.pitch, 0);
+    };
+    auto keep = [&](int i, uint8_t* rows) {
+        const int t = row_x + i * kXRows;
+        const float f = scale_value(xs[i]);
+        // half of the lanes write their second half first: neighbours' pieces, 32 bytes apart, then differ in their banks
+        const bool flip = (threadIdx.x >> 2 ^ threadIdx.x >> 3) & 1;
+        u4* to = (u4*)(rows + t * kRowK + (((col_x >> 3) ^ ((t & 3) << 2)) << 4));
+        to[flip ? 1 : 0] = open_bf16(flip ? u2{x[i][2], x[i][3]} : u2{x[i][0], x[i][1]}, f);
+        to[flip ? 0 : 1] = open_bf16(flip ? u2{x[i][0], x[i][1]} : u2{x[i][2], x[i][3]}, f);
+    };
+
+    // lane -> the token and the four columns whose address it gives to a transposing read
+    const int group = lane >> 4, p = lane & 15;
+    const int token = (group >> 1) * 8 + (p >> 2);
+    const int col_n = (group & 1) * 16 + (p & 3) * 4;
+    const int col_k = spread((group & 1) * 16 + (p & 3) * 4);                  // rows of the result in spread order
+    s4 f[2][NK + NN][2] = {};                          // in the order in which the products want them
+    constexpr int kReads = 2 * (NN + NK), kProducts = NN * NK;
+    f16 acc[NN][NK];
+#pragma unroll
+    for (int i = 0; i < NN; ++i)
+#pragma unroll
+        for (int j = 0; j < NK; ++j) acc[i][j] = f16{};
+    auto product = [&](int h, int m) {
+        const int i = m / NK, j = m % NK;
+        auto pair = [&](int k) {
+            return __builtin_bit_cast(b8, __builtin_shufflevector(f[h][k][0], f[h][k][1], 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(pair(j), pair(NK + i), acc[i][j], 0, 0, 0);
+    };
+    // the last part of step - 1, and all parts but the last of `step`, which lies in from_n and from_k
+    auto between = [&](int64_t step, const uint8_t* __restrict__ from_n, const uint8_t* __restrict__ from_k,
+                       uint8_t* __restrict__ to_n, uint8_t* __restrict__ to_k) {
+#pragma unroll
+        for (int kk = -1; kk < KK - 1; ++kk) {
+#pragma unroll
+            for (int m = 0; m < kProducts; ++m) {
+                product((kk + KK) & 1, m);
+#pragma unroll
+                for (int q = 0; q < kReads; ++q) {
+                    if (q * kProducts / kReads != m) continue;
+                    const int i = q >> 1, t = token + (kk + 1) * 16 + (q & 1) * 4;
+                    const int run = i < NK ? wk / 32 + i : wn / 32 + i - NK;
+                    const uint8_t* at = (i < NK ? from_k + t * kRowK : from_n + t * kRowN) + ((run ^ (p >> 2)) << 6) +
+                                        (i < NK ? col_k : col_n) * 2;
+                    f[(kk + 1) & 1][i][q & 1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Z1B_LDS s4*)at);
+                }
+                if (kk < 0) {
+#pragma unroll
+                    for (int l = 0; l < kLoads; ++l)
+                        if (l * kProducts / kLoads == m) stage(step + 1, l, to_n);
+                }
+                if (kk == 0) {
+#pragma unroll
+                    for (int l = 0; l < kX; ++l)
+                        if (l * kProducts / kX == m) {
+                            keep(l, to_k);
+                            fetch(step + 2, l);
+                        }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    static_assert(KK % 2 == 0, "the parts' registers alternate");
+
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) stage(0, i, lds_n(0));
+#pragma unroll
+    for (int i = 0; i < kX; ++i) fetch(0, i);
+#pragma unroll
+    for (int i = 0; i < kX; ++i) keep(i, lds_k(0));
+#pragma unroll
+    for (int i = 0; i < kX; ++i) fetch(1, i);
+    for (int64_t step = 0; step < steps; ++step) {
+        meet();                                        // step - 1 has been read, `step` has arrived
+        between(step, lds_n(step), lds_k(step), lds_n(step + 1), lds_k(step + 1));
+    }
+#pragma unroll
+    for (int m = 0; m < kProducts; ++m) product(1, m);
+    meet();                                            // the staging buffers are free
+    constexpr int kRoom = (int)sizeof(lds) / kWaves & ~15;
+#pragma unroll
+    for (int i = 0; i < NN; ++i)
+        Flush<T, WK, kRoom>::run(lds + wave * kRoom, lane, acc[i], a.dw, n0 + wn + i * 32, a.N, k0 + wk, a.K);
 }
 
 constexpr int64_t kMaxRows = 1ll << 40;
@@ -381,17 +642,29 @@ constexpr int64_t kMaxTiles = 1ll << 22;               // of a launch: its threa
 
 bool bad_dtype(int d) { return d != Z1_F32 && d != Z1_BF16 && d != Z1_F16; }
 
+constexpr int kCus = 256;
+
+template <typename T, bool PRECISE, int BT, int BO, int WT, int WO>
+int launch_tiles(const Product& a, hipStream_t st) {
+    const int64_t tiles = (a.M + BT - 1) / BT * ((a.N + BO - 1) / BO);
+    if (tiles > kMaxTiles) return Z1_E_SIZE;
+    product_kernel<T, PRECISE, BT, BO, WT, WO><<<dim3((unsigned)tiles), BT / WT * (BO / WO) * 64, 0, st>>>(a);
+    return (int)hipGetLastError();
+}
+
 template <typename T, bool PRECISE>
 int launch_product(const Product& a, hipStream_t st) {
     if (a.M <= 32) {
         product_few_kernel<T, PRECISE><<<dim3((unsigned)((a.N + 31) / 32)), kFewWaves * 64, 0, st>>>(a);
         return (int)hipGetLastError();
     }
-    constexpr int B = 128;
-    const int64_t tiles = (a.M + B - 1) / B * ((a.N + B - 1) / B);
-    if (tiles > kMaxTiles) return Z1_E_SIZE;
-    product_kernel<T, PRECISE, B, B, 64, 64><<<dim3((unsigned)tiles), 256, 0, st>>>(a);
-    return (int)hipGetLastError();
+    if (PRECISE) return launch_tiles<T, PRECISE, 128, 128, 64, 64>(a, st);
+    // Large tiles move fewer bytes per product (8192 x 8192 x 8192: 422 us against 553), small ones leave fewer CUs without
+    // work.  A CU takes one large tile at a time, or two small ones in 0.65 of its time; the fewer rounds win.
+    const int64_t large = (a.M + 255) / 256 * ((a.N + 255) / 256), small = (a.M + 127) / 128 * ((a.N + 127) / 128);
+    const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
+    if (100 * large_rounds <= 65 * small_rounds) return launch_tiles<T, PRECISE, 256, 256, 64, 128>(a, st);
+    return launch_tiles<T, PRECISE, 128, 128, 64, 64>(a, st);
 }
 
 // fp32 results are always precise; 16-bit ones where K is short, since a short sum has few groups over which the cuts
@@ -406,13 +679,31 @@ int product<F32>(const Product& a, hipStream_t st) {
     return launch_product<F32, true>(a, st);
 }
 
+#ifndef WG
+#define WG 128, 128, 64, 64, 32
+#endif
+template <typename T, Edge EDGE, int BN, int BK, int WN, int WK, int TS>
+int launch_gradient(const Gradient& a, hipStream_t st) {
+    const int64_t tiles = (int64_t)((a.N + BN - 1) / BN) * ((a.K + BK - 1) / BK);
+    if (tiles > kMaxTiles) return Z1_E_SIZE;
+    weight_grad_kernel<T, EDGE, BN, BK, WN, WK, TS><<<dim3((unsigned)tiles), BN / WN * (BK / WK) * 64, 0, st>>>(a);
+    return (int)hipGetLastError();
+}
+#ifndef WD
+#define WD 256, 256, 128, 64, 64
+#endif
+template <typename T, int BN, int BK, int WN, int WK, int TS>
+int launch_direct(const Gradient& a, hipStream_t st) {
+    const int64_t tiles = (int64_t)((a.N + BN - 1) / BN) * ((a.K + BK - 1) / BK);
+    if (tiles > kMaxTiles) return Z1_E_SIZE;
+    weight_grad_direct_kernel<T, BN, BK, WN, WK, TS><<<dim3((unsigned)tiles), BN / WN * (BK / WK) * 64, 0, st>>>(a);
+    return (int)hipGetLastError();
+}
 template <typename T>
 int gradient(const Gradient& a, hipStream_t st) {
-    constexpr int B = 128;
-    const int64_t tiles = (int64_t)((a.N + B - 1) / B) * ((a.K + B - 1) / B);
-    if (tiles > kMaxTiles) return Z1_E_SIZE;
-    weight_grad_kernel<T, B, B, 64, 64, 32><<<dim3((unsigned)tiles), 256, 0, st>>>(a);
-    return (int)hipGetLastError();
+    if (a.stride % 2 == 0 && reinterpret_cast<uintptr_t>(a.dy) % 4 == 0) return launch_direct<T, WD>(a, st);
+    if (a.N < 8) return launch_gradient<T, kFew, 128, 128, 64, 64, 32>(a, st);
+    return launch_gradient<T, kCut, 128, 128, 64, 64, 32>(a, st);
 }
 
 }  // namespace
