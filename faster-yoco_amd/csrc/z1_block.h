@@ -165,6 +165,20 @@ __device__ __forceinline__ void store_row(void* p, int64_t i, int n, const float
     }
 }
 
+// A lane's eight elements of a row of `dim` >= 8 from column c on without a branch: it loads eight that are there, from
+// column min(c, dim - 8) on, and what the row's end cuts off is moved down and filled with zeros (`settle`) afterwards.
+// `by`: c - (dim - 8) where positive; 8 and more: no element is the lane's.
+template <typename T>
+__device__ __forceinline__ void settle(float* v, int by) {
+#pragma unroll
+    for (int s = 4; s; s >>= 1) {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) v[j] = by & s ? (j + s < kLane ? v[j + s] : 0.0f) : v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) v[j] = by >= kLane ? 0.0f : v[j];
+}
+
 // The largest of 16 neighbouring lanes (one DPP row), in every lane of them.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
@@ -236,15 +250,18 @@ __device__ __forceinline__ void open8(u2 q, float* v) {
     }
 }
 
-// Sum over the 64 lanes of a wave, in every lane; the same tree for every call.
+// Sum over the 64 lanes of a wave, in every lane; the same tree for every call.  All lanes are active.
 __device__ __forceinline__ float wave_sum(float x) {
     x += dpp<0x128>(x);
     x += dpp<0x124>(x);
     x += dpp<0x122>(x);
     x += dpp<0x121>(x);
-    x += __shfl_xor(x, 16);
-    x += __shfl_xor(x, 32);
-    return x;
+    const int i = __builtin_bit_cast(int, x);
+    const float a = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 0));
+    const float b = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 16));
+    const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 32));
+    const float d = __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, 48));
+    return (a + b) + (c + d);
 }
 
 inline int wide_of(int64_t dim) { return (int)((dim + kBlock - 1) / kBlock * kBlock); }

@@ -262,9 +262,40 @@ __device__ __forceinline__ void row_sums(float& s1, float& s2, float (*red)[2], 
     for (int i = 1; i < wpr; ++i) s1 += red[first + i][0], s2 += red[first + i][1];
 }
 
-// Rows of up to 8 * NV * 512 columns.  A workgroup's groups of wpr waves take rows in turn; a lane keeps its columns'
-// dw and db sums in registers over all of them, the groups' sums meet in LDS at the end, and the workgroup writes one
-// partial row of each, which norm_reduce_kernel adds in order.
+// Eight columns of a row as they are loaded: x in T, or its 8-bit rows' bytes and scale.
+template <typename T, bool Q>
+struct Input {
+    typename T::raw r;
+    static __device__ __forceinline__ Input load(const Backward& a, int64_t row, int c, int from) {
+        return {T::load((const typename T::elem*)a.x + row * a.x_stride, from)};
+    }
+    __device__ __forceinline__ void open(float* v, bool edge, int by) const {
+        T::open(r, v);
+        if (edge) settle<T>(v, by);
+    }
+};
+template <typename T>
+struct Input<T, true> {
+    u2 q;
+    uint32_t s;
+    static __device__ __forceinline__ Input load(const Backward& a, int64_t row, int c, int from) {
+        c = c < a.wide ? c : a.wide - kLane;           // past the row's end: zeros, or not used
+        const uint8_t* q = a.q + row * a.wide;
+        const uint8_t* s = a.s + row * a.pitch;
+        return {*(const Z1B_GLOBAL u2*)(q + (uint32_t)c), ((const Z1B_GLOBAL uint8_t*)s)[(uint32_t)c / kBlock]};
+    }
+    __device__ __forceinline__ void open(float* v, bool edge, int by) const {
+        const float f = scale_value(s);
+        open8(q, v);
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) v[j] = edge && j + by >= kLane ? 0.0f : v[j] * f;
+    }
+};
+
+// Rows of 8 to 8 * NV * 512 columns.  A workgroup's groups of wpr waves take rows in turn; a lane keeps its columns' dw and
+// db sums in registers over all of them, the groups' sums meet in LDS at the end, and the workgroup writes one partial row
+// of each, which norm_reduce_kernel adds in order.  The next rows are loaded while the present ones are computed, and no
+// load stands behind a branch.
 template <typename T, int NV, bool Q, bool CENTER>
 __global__ __launch_bounds__(kBwdThreads) void norm_backward_kernel(Backward a) {
     __shared__ float red[2][kBwdThreads / 64][2];
@@ -272,54 +303,90 @@ __global__ __launch_bounds__(kBwdThreads) void norm_backward_kernel(Backward a) 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wpr = a.wpr, groups = kBwdThreads / 64 / wpr, group = wave / wpr, wi = wave - group * wpr;
     const int c0 = (wi * 64 + lane) * kLane, step = wpr * kUnit;
+    int from[NV], by[NV];
+    bool edge[NV];                                     // the row ends in this wave's k-th part, or before it
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = c0 + k * step, last = a.dim - kLane;
+        from[k] = c < last ? c : last;
+        by[k] = c - from[k];
+        edge[k] = (wi + 1) * kUnit + k * step > a.dim;
+    }
+    float w[NV][kLane];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) w[k][j] = 1.0f;
+        if (a.w) {
+            if (a.w32) F32::open(F32::load(a.w, from[k]), w[k]);
+            else T::open(T::load(a.w, from[k]), w[k]);
+            settle<T>(w[k], by[k]);
+        }
+    }
     float dw[NV][kLane] = {}, db[NV][kLane] = {};
     const float inv = 1.0f / (float)a.dim;
+    typename T::raw dy[NV];
+    Input<T, Q> x[NV];
+    float r_next = 0.0f, mu_next = 0.0f;
+    auto fetch = [&](int64_t row) {                    // past the last row: the last, not used
+        row = row < a.rows ? row : a.rows - 1;
+        r_next = a.rstd[row];
+        mu_next = CENTER ? a.mean[row] : 0.0f;
+        const void* d = (const typename T::elem*)a.dy + row * a.dy_stride;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            dy[k] = T::load(d, from[k]);
+            x[k] = Input<T, Q>::load(a, row, c0 + k * step, from[k]);
+        }
+    };
+    const int64_t stride = (int64_t)gridDim.x * groups;
+    int64_t row = (int64_t)blockIdx.x * groups + group;
+    const int64_t end = a.rows + group;                // every wave stays for the barriers: the group's last turn
     int turn = 0;
-    for (int64_t first = (int64_t)blockIdx.x * groups; first < a.rows; first += (int64_t)gridDim.x * groups) {
-        const int64_t row = first + group;
-        const bool live = row < a.rows;                // every wave stays for the barriers
-        float xh[NV][kLane], g[NV][kLane], s1 = 0.0f, s2 = 0.0f, r = 0.0f;
-        if (live) {
-            r = a.rstd[row];
-            const float mu = CENTER ? a.mean[row] : 0.0f;
+    fetch(row);
+    for (; row < end; row += stride) {
+        const bool live = row < a.rows;
+        const float r = r_next, mu = mu_next;
+        float xh[NV][kLane], g[NV][kLane], s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c = c0 + k * step, n = a.dim - c;
-                load_xh<T, Q, CENTER>(a, row, c, n, mu, r, xh[k]);
-                load_row<T>(a.dy, row * a.dy_stride + c, n, g[k]);
+        for (int k = 0; k < NV; ++k) {
+            T::open(dy[k], g[k]);
+            if (edge[k]) settle<T>(g[k], by[k]);
+            x[k].open(xh[k], edge[k], by[k]);
+        }
+        fetch(row + stride);
+        if (!live) {
 #pragma unroll
-                for (int j = 0; j < kLane; ++j) {
-                    dw[k][j] = __builtin_fmaf(g[k][j], xh[k][j], dw[k][j]);
-                    if (CENTER) db[k][j] += g[k][j];
-                }
-                if (a.w) {
-                    float w[kLane];
-                    load_weight<T>(a.w, a.w32, c, n, w);
+            for (int k = 0; k < NV; ++k)
 #pragma unroll
-                    for (int j = 0; j < kLane; ++j) g[k][j] *= w[j];
-                }
+                for (int j = 0; j < kLane; ++j) g[k][j] = 0.0f, xh[k][j] = 0.0f;
+        }
 #pragma unroll
-                for (int j = 0; j < kLane; ++j) {
-                    if (CENTER) s1 += g[k][j];
-                    s2 = __builtin_fmaf(g[k][j], xh[k][j], s2);
-                }
+        for (int k = 0; k < NV; ++k) {
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) {
+                // past the row's end dy and w are zeros, and so is all that xh enters
+                xh[k][j] = (CENTER ? xh[k][j] - mu : xh[k][j]) * r;
+                dw[k][j] = __builtin_fmaf(g[k][j], xh[k][j], dw[k][j]);
+                if (CENTER) db[k][j] += g[k][j];
+                g[k][j] *= w[k][j];
+                if (CENTER) s1 += g[k][j];
+                s2 = __builtin_fmaf(g[k][j], xh[k][j], s2);
             }
         }
         row_sums(s1, s2, red[turn], wave, wpr);
         turn ^= 1;                                     // the next row's sums need no barrier before they are written
-        if (live) {
-            const float m1 = s1 * inv, m2 = s2 * inv;
+        if (!live) continue;
+        const float m1 = s1 * inv, m2 = s2 * inv;
+        void* out = (typename T::elem*)a.dx + row * a.dim;
 #pragma unroll
-            for (int k = 0; k < NV; ++k) {
-                const int c = c0 + k * step, n = a.dim - c;
-                float dx[kLane];
+        for (int k = 0; k < NV; ++k) {
+            float dx[kLane];
 #pragma unroll
-                for (int j = 0; j < kLane; ++j) {
-                    const float t = CENTER ? g[k][j] - m1 : g[k][j];
-                    dx[j] = __builtin_fmaf(-xh[k][j], m2, t) * r;
-                }
-                if (n > 0) store_row<T>(a.dx, row * a.dim + c, n, dx);
-            }
+            for (int j = 0; j < kLane; ++j)
+                dx[j] = __builtin_fmaf(-xh[k][j], m2, CENTER ? g[k][j] - m1 : g[k][j]) * r;
+            if (edge[k]) store_row<T>(out, c0 + k * step, a.dim - c0 - k * step, dx);
+            else T::store(out, c0 + k * step, dx);
         }
     }
     if (!a.part) return;
@@ -400,21 +467,47 @@ __global__ __launch_bounds__(kColumnThreads) void norm_columns_kernel(Backward a
     if (CENTER) store_row<F32>(out, (int64_t)a.dim + c, n, db);
 }
 
-// dw and db from `parts` partial rows, added in order: 64 columns and 4 shares of the partials to a workgroup.
+// dw and db from `parts` partial rows of `columns` sums (dw's, then db's): 64 columns to a workgroup, four to a lane, and
+// the partial rows in 16 shares, each added in order and the shares in order after that.
+constexpr int kReduceShares = 16;
 template <typename T>
-__global__ __launch_bounds__(256) void norm_reduce_kernel(const float* part, int parts, int dim, void* dw, void* db) {
-    __shared__ float sums[4][64];
-    const int lane = threadIdx.x & 63, share = threadIdx.x >> 6;
-    const int blocks = (dim + 63) / 64;
-    const int which = blockIdx.x >= blocks;
-    const int c = (blockIdx.x - which * blocks) * 64 + lane;
-    float t = 0.0f;
-    if (c < dim)
-        for (int i = share; i < parts; i += 4) t += part[((int64_t)i * 2 + which) * dim + c];
-    sums[share][lane] = t;
+__global__ __launch_bounds__(256) void norm_reduce_kernel(const float* part, int parts, int dim, int columns, void* dw,
+                                                          void* db) {
+    __shared__ float sums[kReduceShares][64];
+    const int lane = threadIdx.x & 15, share = threadIdx.x >> 4;
+    const int c = blockIdx.x * 64 + lane * 4;
+    const int64_t row = 2 * (int64_t)dim;
+    f4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c + 4 <= columns) {
+        const float* p = part + c;
+        int i = share;
+        for (; i + 7 * kReduceShares < parts; i += 8 * kReduceShares) {
+            f4 v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = *(const Z1B_GLOBAL f4_any4*)(p + (i + k * kReduceShares) * row);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) t += v[k];
+        }
+        for (; i < parts; i += kReduceShares) t += *(const Z1B_GLOBAL f4_any4*)(p + i * row);
+    } else {
+        for (int i = share; i < parts; i += kReduceShares)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (c + j < columns) t[j] += part[i * row + c + j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sums[share][lane * 4 + j] = t[j];
     __syncthreads();
-    void* out = which ? db : dw;
-    if (share == 0 && c < dim && out) T::put(out, c, ((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]);
+    const int at = blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x >= 64 || at >= columns) return;
+    float s = sums[0][threadIdx.x];
+#pragma unroll
+    for (int i = 1; i < kReduceShares; ++i) s += sums[i][threadIdx.x];
+    if (at < dim) {
+        if (dw) T::put(dw, at, s);
+    } else if (db) {
+        T::put(db, at - dim, s);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------ host
@@ -451,7 +544,7 @@ struct Shape { int wpr, nv, blocks; };                 // wpr 0: the long rows' 
 
 Shape backward_shape(int64_t rows, int dim) {
     const int units = (dim + kUnit - 1) / kUnit;
-    if (units > 8 * kMaxVectors) return {0, 0, (int)(rows < 64 ? rows : 64)};
+    if (units > 8 * kMaxVectors || dim < kLane) return {0, 0, (int)(rows < 64 ? rows : 64)};
     const int wpr = units <= 3 ? 1 : units <= 6 ? 2 : units <= 12 ? 4 : 8;
     const int groups = kBwdThreads / 64 / wpr;
     const int64_t need = (rows + groups - 1) / groups;
@@ -550,12 +643,13 @@ int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x
         if (rc) return rc;
     }
     if (!dw && !db) return Z1_OK;
-    const dim3 grid((unsigned)((dim + 63) / 64 * (center ? 2 : 1)));
+    const int columns = (int)dim * (center ? 2 : 1);
+    const dim3 grid((unsigned)((columns + 63) / 64));
     const int parts = rows > 0 ? sh.blocks : 0;
     switch (grad_dtype) {
-        case Z1_F32: norm_reduce_kernel<F32><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, dw, db); break;
-        case Z1_BF16: norm_reduce_kernel<BF16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, dw, db); break;
-        default: norm_reduce_kernel<F16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, dw, db); break;
+        case Z1_F32: norm_reduce_kernel<F32><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
+        case Z1_BF16: norm_reduce_kernel<BF16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
+        default: norm_reduce_kernel<F16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
     }
     return (int)hipGetLastError();
 }
