@@ -69,7 +69,7 @@ def build_ops(output=OPS_OUTPUT, verbose=False):
     cmd = (['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-Wall', '-Werror',
             f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}', '-D__HIP_PLATFORM_AMD__=1',
             '-DUSE_ROCM=1'] + inc + ['-I', os.path.join(rocm, 'include'), '-I', INCLUDE] + OPS_SOURCES +
-           ['-L', tlib, '-lc10', '-lc10_hip', '-ltorch_cpu', '-ldl', f'-Wl,-rpath,{tlib}', '-o', tmp])
+           ['-L', tlib, '-lc10', '-lc10_hip', '-ltorch_cpu', '-ltorch_hip', '-ldl', f'-Wl,-rpath,{tlib}', '-o', tmp])
     if verbose:
         print(' '.join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

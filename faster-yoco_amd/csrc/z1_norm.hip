@@ -16,9 +16,9 @@ namespace {
 using namespace z1blk;
 
 constexpr int kFwdThreads = 256;
-constexpr int kBwdThreads = 512;
+constexpr int kRowThreads = 512;
 constexpr int kUnit = 64 * kLane;                      // columns of one wave's access
-constexpr int kLongThreads = 1024;
+constexpr int kLongThreads = 1024;                     // of those that read them again
 
 struct Forward {
     const void* x;
@@ -32,9 +32,9 @@ struct Forward {
     uint8_t* cs;
     float* mean;
     float* rstd;
-    int64_t row0, rows;                                // this launch's first row, and the end of all rows
+    int64_t row0, rows;                                // a launch's first row (long rows only), and the end of all rows
     int dim, wide, pitch;
-    int wpr;                                           // waves of a row: 1, 2 or 4
+    int wpr;                                           // waves of a row: 1, 2, 4 or 8
     int w32;                                           // w and b are fp32 (else x's type)
     float eps;
 };
@@ -105,8 +105,11 @@ __device__ __forceinline__ void finish8(const Forward& a, int64_t row, int c, in
     if (a.cq) put8(a.cq, a.cs, row, c, a, v);
 }
 
-// Rows of up to 4 * NV * 512 columns: a row's wpr waves hold it in registers.
-template <typename T, int NV, bool CENTER>
+// Rows of 8 to 4 * NV * 512 columns: a row's wpr waves hold it in registers.  One row to them: a grid of rows, which the
+// hardware hands out, is faster here than one that takes rows in turn and loads ahead (layer norm of 16384 x 3072 BF16 37.6
+// us against 48-65).
+// All loads are under way before the first sum, and none stands behind a branch (settle).
+template <typename T, typename W, int NV, bool CENTER>
 __global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
     __shared__ float red[2][kFwdThreads / 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -114,38 +117,80 @@ __global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
     int64_t row = a.row0 + (int64_t)blockIdx.x * (kFwdThreads / 64 / wpr) + group;
     const bool live = row < a.rows;                    // every wave stays for the barriers
     if (!live) row = a.rows - 1;
-    float v[NV][kLane];
-    float s = 0.0f;
-    int c0 = (wi * 64 + lane) * kLane;
-    const int step = wpr * kUnit;
+    const int c0 = (wi * 64 + lane) * kLane, step = wpr * kUnit, last = a.dim - kLane;
+    typename T::raw x[NV];
+    typename W::raw w[NV], b[NV];
+    const void* p = (const typename T::elem*)a.x + row * a.stride;
+    const void* pw = a.w ? a.w : a.b ? a.b : a.x;      // something to load, where there is no weight
+    const void* pb = a.b ? a.b : pw;
 #pragma unroll
-    for (int k = 0; k < NV; ++k) load_row<T>(a.x, row * a.stride + c0 + k * step, a.dim - c0 - k * step, v[k]);
-    float mu = 0.0f;
+    for (int k = 0; k < NV; ++k) x[k] = T::load(p, c0 + k * step < last ? c0 + k * step : last);
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int c = c0 + k * step < last ? c0 + k * step : last;
+        w[k] = W::load(pw, c);
+        if (CENTER) b[k] = W::load(pb, c);
+    }
+    float v[NV][kLane], s = 0.0f, mu = 0.0f;
+    const float inv = 1.0f / (float)a.dim;
+    // whether the row ends in this wave's k-th part, or before it; what then is the lane's
+    auto edge = [&](int k) { return (wi + 1) * kUnit + k * step > a.dim; };
+    auto by = [&](int k) { return c0 + k * step < last ? 0 : c0 + k * step - last; };
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        T::open(x[k], v[k]);
+        if (edge(k)) settle<T>(v[k], by(k));
+    }
     if (CENTER) {
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < kLane; ++j) s += v[k][j];
-        mu = row_sum(s, red[0], wave, wpr) / (float)a.dim;
+        mu = row_sum(s, red[0], wave, wpr) * inv;
     }
     s = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        const int n = a.dim - c0 - k * step;
+        const bool cut = CENTER && edge(k);
 #pragma unroll
         for (int j = 0; j < kLane; ++j) {
-            const float d = CENTER ? (j < n ? v[k][j] - mu : 0.0f) : v[k][j];
+            float d = v[k][j] - mu;
+            if (cut) d = j + by(k) < kLane ? d : 0.0f;
             s = __builtin_fmaf(d, d, s);
         }
     }
     s = row_sum(s, red[1], wave, wpr);
-    const float r = 1.0f / sqrtf(s / (float)a.dim + a.eps);
+    const float r = 1.0f / sqrtf(s * inv + a.eps);
     if (!live) return;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = c0 + k * step;
-        // all 64 lanes or none take part in an 8-bit form; a lane of no columns writes nothing
-        if (c - lane * kLane < a.wide) finish8<T, CENTER>(a, row, c, a.dim - c, mu, r, v[k]);
+        if (c - lane * kLane >= a.wide) continue;      // no lane of the wave has a column here
+        float y[kLane], f[kLane], g[kLane];
+        W::open(w[k], f);
+        if (CENTER) W::open(b[k], g);
+        if (edge(k)) {
+            settle<W>(f, by(k));
+            if (CENTER) settle<W>(g, by(k));
+        }
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            y[j] = (CENTER ? v[k][j] - mu : v[k][j]) * r;
+            if (!CENTER) y[j] = a.w ? y[j] * f[j] : y[j];
+            else y[j] = __builtin_fmaf(y[j], a.w ? f[j] : 1.0f, a.b ? g[j] : 0.0f);
+        }
+        if (edge(k)) {                                 // y's padding
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) y[j] = j + by(k) < kLane ? y[j] : 0.0f;
+        }
+        if (a.y) {
+            void* out = (typename T::elem*)a.y + row * a.dim;
+            if (edge(k)) store_row<T>(out, c, a.dim - c, y);
+            else T::store(out, c, y);
+        } else {
+            put8(a.yq, a.ys, row, c, a, y);
+        }
+        if (a.cq) put8(a.cq, a.cs, row, c, a, v[k]);
     }
     if (wi == 0) {
         if (lane == 0) {
@@ -297,11 +342,11 @@ struct Input<T, true> {
 // of each, which norm_reduce_kernel adds in order.  The next rows are loaded while the present ones are computed, and no
 // load stands behind a branch.
 template <typename T, int NV, bool Q, bool CENTER>
-__global__ __launch_bounds__(kBwdThreads) void norm_backward_kernel(Backward a) {
-    __shared__ float red[2][kBwdThreads / 64][2];
-    __shared__ float sums[kBwdThreads * NV * kLane];
+__global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) {
+    __shared__ float red[2][kRowThreads / 64][2];
+    __shared__ float sums[kRowThreads * NV * kLane];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wpr = a.wpr, groups = kBwdThreads / 64 / wpr, group = wave / wpr, wi = wave - group * wpr;
+    const int wpr = a.wpr, groups = kRowThreads / 64 / wpr, group = wave / wpr, wi = wave - group * wpr;
     const int c0 = (wi * 64 + lane) * kLane, step = wpr * kUnit;
     int from[NV], by[NV];
     bool edge[NV];                                     // the row ends in this wave's k-th part, or before it
@@ -400,7 +445,7 @@ __global__ __launch_bounds__(kBwdThreads) void norm_backward_kernel(Backward a) 
 #pragma unroll
             for (int j = 0; j < kLane; ++j) sums[group * columns + c0 + k * step + j] = which ? db[k][j] : dw[k][j];
         __syncthreads();
-        for (int c = threadIdx.x; c < a.dim; c += kBwdThreads) {
+        for (int c = threadIdx.x; c < a.dim; c += kRowThreads) {
             float t = sums[c];
             for (int i = 1; i < groups; ++i) t += sums[i * columns + c];
             out[which * a.dim + c] = t;
@@ -467,22 +512,22 @@ __global__ __launch_bounds__(kColumnThreads) void norm_columns_kernel(Backward a
     if (CENTER) store_row<F32>(out, (int64_t)a.dim + c, n, db);
 }
 
-// dw and db from `parts` partial rows of `columns` sums (dw's, then db's): 64 columns to a workgroup, four to a lane, and
-// the partial rows in 16 shares, each added in order and the shares in order after that.
-constexpr int kReduceShares = 16;
+// dw and db from `parts` partial rows of `columns` sums (dw's, then db's): a few columns to a workgroup, four to a lane, and
+// the partial rows in shares, each added in order and the shares in order after that.
+constexpr int kReduceShares = 32, kReduceColumns = 1024 / kReduceShares;
 template <typename T>
 __global__ __launch_bounds__(256) void norm_reduce_kernel(const float* part, int parts, int dim, int columns, void* dw,
                                                           void* db) {
-    __shared__ float sums[kReduceShares][64];
-    const int lane = threadIdx.x & 15, share = threadIdx.x >> 4;
-    const int c = blockIdx.x * 64 + lane * 4;
+    __shared__ float sums[kReduceShares][kReduceColumns];
+    const int lane = threadIdx.x % (kReduceColumns / 4), share = threadIdx.x / (kReduceColumns / 4);
+    const int c = blockIdx.x * kReduceColumns + lane * 4;
     const int64_t row = 2 * (int64_t)dim;
     f4 t = {0.0f, 0.0f, 0.0f, 0.0f};
     if (c + 4 <= columns) {
         const float* p = part + c;
         int i = share;
         for (; i + 7 * kReduceShares < parts; i += 8 * kReduceShares) {
-            f4 v[8];
+            f4 v[8];                                   // loads side by side
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = *(const Z1B_GLOBAL f4_any4*)(p + (i + k * kReduceShares) * row);
 #pragma unroll
@@ -498,8 +543,8 @@ __global__ __launch_bounds__(256) void norm_reduce_kernel(const float* part, int
 #pragma unroll
     for (int j = 0; j < 4; ++j) sums[share][lane * 4 + j] = t[j];
     __syncthreads();
-    const int at = blockIdx.x * 64 + threadIdx.x;
-    if (threadIdx.x >= 64 || at >= columns) return;
+    const int at = blockIdx.x * kReduceColumns + threadIdx.x;
+    if (threadIdx.x >= kReduceColumns || at >= columns) return;
     float s = sums[0][threadIdx.x];
 #pragma unroll
     for (int i = 1; i < kReduceShares; ++i) s += sums[i][threadIdx.x];
@@ -518,26 +563,39 @@ constexpr int kMaxBlocks = 256;                        // workgroups of the back
 constexpr int64_t kLaunchRows = 1 << 21;
 unsigned launch_rows(int64_t left) { return (unsigned)(left < kLaunchRows ? left : kLaunchRows); }
 
+// Waves of a row of `units` * 512 columns: up to three 8-column groups to a lane while that is enough.
+int waves_of(int units) { return units <= 3 ? 1 : units <= 6 ? 2 : units <= 12 ? 4 : 8; }
+
+template <typename T, typename W, bool CENTER>
+int forward_rows(Forward& a, int nv, hipStream_t st) {
+    const int per = kFwdThreads / 64 / a.wpr;
+    for (; a.row0 < a.rows; a.row0 += kLaunchRows) {
+        const dim3 grid((launch_rows(a.rows - a.row0) + per - 1) / per);
+        switch (nv) {
+            case 1: norm_forward_kernel<T, W, 1, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 2: norm_forward_kernel<T, W, 2, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 3: norm_forward_kernel<T, W, 3, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 4: norm_forward_kernel<T, W, 4, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            default: norm_forward_kernel<T, W, 6, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+        }
+    }
+    return (int)hipGetLastError();
+}
+
 template <typename T, bool CENTER>
 int forward(Forward& a, hipStream_t st) {
     const int units = (a.dim + kUnit - 1) / kUnit;
-    if (units > 4 * kMaxVectors) {
+    if (units > 4 * 6 || a.dim < kLane) {
         for (; a.row0 < a.rows; a.row0 += kLaunchRows)
             norm_forward_long_kernel<T, CENTER><<<launch_rows(a.rows - a.row0), kLongThreads, 0, st>>>(a);
         return (int)hipGetLastError();
     }
-    a.wpr = units <= kMaxVectors ? 1 : units <= 2 * kMaxVectors ? 2 : 4;
-    const int nv = (units + a.wpr - 1) / a.wpr, per = kFwdThreads / 64 / a.wpr;
-    for (; a.row0 < a.rows; a.row0 += kLaunchRows) {
-        const dim3 grid((launch_rows(a.rows - a.row0) + per - 1) / per);
-        switch (nv) {
-            case 1: norm_forward_kernel<T, 1, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-            case 2: norm_forward_kernel<T, 2, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-            case 3: norm_forward_kernel<T, 3, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-            default: norm_forward_kernel<T, 4, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-        }
+    a.wpr = units <= 3 ? 1 : units <= 6 ? 2 : 4;       // two to a lane: 43.4 us, four the same as three, six 47.3
+    const int nv = (units + a.wpr - 1) / a.wpr;
+    if constexpr (sizeof(typename T::elem) == 2) {
+        if (a.w32 && (a.w || a.b)) return forward_rows<T, F32, CENTER>(a, nv, st);
     }
-    return (int)hipGetLastError();
+    return forward_rows<T, T, CENTER>(a, nv, st);
 }
 
 struct Shape { int wpr, nv, blocks; };                 // wpr 0: the long rows' kernels, `blocks` shares of the rows
@@ -545,8 +603,8 @@ struct Shape { int wpr, nv, blocks; };                 // wpr 0: the long rows' 
 Shape backward_shape(int64_t rows, int dim) {
     const int units = (dim + kUnit - 1) / kUnit;
     if (units > 8 * kMaxVectors || dim < kLane) return {0, 0, (int)(rows < 64 ? rows : 64)};
-    const int wpr = units <= 3 ? 1 : units <= 6 ? 2 : units <= 12 ? 4 : 8;
-    const int groups = kBwdThreads / 64 / wpr;
+    const int wpr = waves_of(units);
+    const int groups = kRowThreads / 64 / wpr;
     const int64_t need = (rows + groups - 1) / groups;
     return {wpr, (units + wpr - 1) / wpr, (int)(need < kMaxBlocks ? need : kMaxBlocks)};
 }
@@ -564,10 +622,10 @@ int backward(Backward& a, const Shape& s, hipStream_t st) {
     }
     a.wpr = s.wpr;
     switch (s.nv) {
-        case 1: norm_backward_kernel<T, 1, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
-        case 2: norm_backward_kernel<T, 2, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
-        case 3: norm_backward_kernel<T, 3, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
-        default: norm_backward_kernel<T, 4, Q, CENTER><<<s.blocks, kBwdThreads, 0, st>>>(a); break;
+        case 1: norm_backward_kernel<T, 1, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
+        case 2: norm_backward_kernel<T, 2, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
+        case 3: norm_backward_kernel<T, 3, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
+        default: norm_backward_kernel<T, 4, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
     }
     return (int)hipGetLastError();
 }
@@ -644,7 +702,7 @@ int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x
     }
     if (!dw && !db) return Z1_OK;
     const int columns = (int)dim * (center ? 2 : 1);
-    const dim3 grid((unsigned)((columns + 63) / 64));
+    const dim3 grid((unsigned)((columns + kReduceColumns - 1) / kReduceColumns));
     const int parts = rows > 0 ? sh.blocks : 0;
     switch (grad_dtype) {
         case Z1_F32: norm_reduce_kernel<F32><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;

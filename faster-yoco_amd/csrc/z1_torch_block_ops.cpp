@@ -6,7 +6,7 @@
  * z1t_init does for the update's operators.
  */
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -130,13 +130,18 @@ void check8(const Tensor& q, const Tensor& s, int64_t rows, int64_t dim, int64_t
                 what, ": ", name, ": values must be 16-byte aligned and scales 4-byte aligned");
 }
 
+// A new tensor on the current device, from torch's allocator.  (at::empty goes through the dispatcher again: a norm's four
+// to six results then cost 2 us more.)
+Tensor fresh(at::IntArrayRef size, at::ScalarType dtype) {
+    return Tensor(at::detail::empty_cuda(size, dtype, c10::Device(c10::DeviceType::CUDA), std::nullopt));
+}
+
 struct Pair {
     Tensor q, s;
 };
-Pair empty8(int64_t rows, int64_t dim, int64_t scale_rows, const at::TensorOptions& o, const char* what) {
+Pair empty8(int64_t rows, int64_t dim, int64_t scale_rows, const char* what) {
     const int64_t wide = wide_of(dim, what);
-    return {at::empty({rows, wide}, o.dtype(at::kFloat8_e4m3fn)),
-            at::empty({scale_rows, api().act8_scales(dim)}, o.dtype(at::kFloat8_e8m0fnu))};
+    return {fresh({rows, wide}, at::kFloat8_e4m3fn), fresh({scale_rows, api().act8_scales(dim)}, at::kFloat8_e8m0fnu)};
 }
 
 struct OnDevice {
@@ -162,29 +167,28 @@ std::vector<Tensor> norm_forward(const Tensor& x, const OptTensor& weight, const
     TORCH_CHECK(eps >= 0, what, ": eps must not be negative");
     const int w_dtype = w || b ? dtype_code((w ? *weight : *bias).scalar_type(), what) : Z1_F32;
     OnDevice on(x);
-    const auto o = x.options();
     std::vector<Tensor> out;
     void *y = nullptr, *yq = nullptr, *ys = nullptr, *cq = nullptr, *cs = nullptr;
     float* mean = nullptr;
     out.reserve(6);
     if (y8) {
-        Pair p = empty8(r.rows, r.dim, r.rows, o, what);
+        Pair p = empty8(r.rows, r.dim, r.rows, what);
         yq = p.q.data_ptr();
         ys = p.s.data_ptr();
         out.push_back(std::move(p.q));
         out.push_back(std::move(p.s));
     } else {
-        out.push_back(at::empty({r.rows, r.dim}, o));
+        out.push_back(fresh({r.rows, r.dim}, x.scalar_type()));
         y = out.back().data_ptr();
     }
     if (center) {
-        out.push_back(at::empty({r.rows}, o.dtype(at::kFloat)));
+        out.push_back(fresh({r.rows}, at::kFloat));
         mean = static_cast<float*>(out.back().data_ptr());
     }
-    out.push_back(at::empty({r.rows}, o.dtype(at::kFloat)));
+    out.push_back(fresh({r.rows}, at::kFloat));
     float* rstd = static_cast<float*>(out.back().data_ptr());
     if (checkpoint) {
-        Pair p = empty8(r.rows, r.dim, r.rows, o, what);
+        Pair p = empty8(r.rows, r.dim, r.rows, what);
         cq = p.q.data_ptr();
         cs = p.s.data_ptr();
         out.push_back(std::move(p.q));
@@ -226,16 +230,17 @@ std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const Op
     const void* w = weight_of(weight, dy, r.dim, what, "weight");
     const at::ScalarType gt = w ? weight->scalar_type() : dy.scalar_type();
     OnDevice on(dy);
-    const auto o = dy.options();
-    std::vector<Tensor> out{at::empty({r.rows, r.dim}, o)};
-    if (need_dw) out.push_back(at::empty({r.dim}, o.dtype(gt)));
-    if (need_db) out.push_back(at::empty({r.dim}, o.dtype(gt)));
+    std::vector<Tensor> out;
+    out.reserve(3);
+    out.push_back(fresh({r.rows, r.dim}, dy.scalar_type()));
+    if (need_dw) out.push_back(fresh({r.dim}, gt));
+    if (need_db) out.push_back(fresh({r.dim}, gt));
     Tensor ws;
     int64_t floats = 0;
     if (need_dw || need_db) {
         floats = api().norm_backward_workspace(r.rows, r.dim);
         if (floats < 0) check_rc(floats, "z1_norm_backward_workspace");
-        ws = at::empty({floats}, o.dtype(at::kFloat));
+        ws = fresh({floats}, at::kFloat);
     }
     check_rc(api().norm_backward(r.p, r.stride, plain ? xr.p : nullptr, xr.stride, packed ? q->const_data_ptr() : nullptr,
                                  packed ? s->const_data_ptr() : nullptr, r.rows, r.dim, r.dtype, mp, rp, w,
@@ -252,7 +257,7 @@ std::tuple<Tensor, Tensor> act8_pack(const Tensor& x) {
     require_gpu(x, what, "x");
     const Rows r = rows_of(x, what, "x");
     OnDevice on(x);
-    Pair p = empty8(r.rows, r.dim, r.rows, x.options(), what);
+    Pair p = empty8(r.rows, r.dim, r.rows, what);
     check_rc(api().act8_pack(r.p, r.rows, r.dim, r.stride, r.dtype, p.q.data_ptr(), p.s.data_ptr(), on.stream),
              "z1_act8_pack");
     return {std::move(p.q), std::move(p.s)};
@@ -265,7 +270,7 @@ Tensor act8_unpack(const Tensor& q, const Tensor& s, int64_t dim, at::ScalarType
     check8(q, s, q.size(0), dim, q.size(0), what, "a");
     const int code = dtype_code(dtype, what);
     OnDevice on(q);
-    Tensor out = at::empty({q.size(0), dim}, q.options().dtype(dtype));
+    Tensor out = fresh({q.size(0), dim}, dtype);
     check_rc(api().act8_unpack(q.const_data_ptr(), s.const_data_ptr(), q.size(0), dim, out.data_ptr(), code, on.stream),
              "z1_act8_unpack");
     return out;
@@ -278,8 +283,8 @@ std::vector<Tensor> weight8_pack(const Tensor& w, bool transposed) {
     const Rows r = rows_of(w, what, "w");
     TORCH_CHECK(r.rows >= 1, what, ": expected at least one row");
     OnDevice on(w);
-    Pair p = empty8(r.rows, r.dim, blocks_of(r.rows), w.options(), what), t;
-    if (transposed) t = empty8(r.dim, r.rows, blocks_of(r.dim), w.options(), what);
+    Pair p = empty8(r.rows, r.dim, blocks_of(r.rows), what), t;
+    if (transposed) t = empty8(r.dim, r.rows, blocks_of(r.dim), what);
     check_rc(api().weight8_pack(r.p, r.rows, r.dim, r.stride, r.dtype, p.q.data_ptr(), p.s.data_ptr(),
                                 transposed ? t.q.data_ptr() : nullptr, transposed ? t.s.data_ptr() : nullptr, on.stream),
              "z1_weight8_pack");
@@ -302,7 +307,7 @@ Tensor product8(const Tensor& q, const Tensor& s, const Tensor& wq, const Tensor
     check8(wq, ws, N, inner, blocks_of(N), what, "w");
     const int code = dtype_code(dtype, what);
     OnDevice on(q);
-    Tensor y = at::empty({M, N}, q.options().dtype(dtype));
+    Tensor y = fresh({M, N}, dtype);
     check_rc(api().product8(q.const_data_ptr(), s.const_data_ptr(), M, wq.const_data_ptr(), ws.const_data_ptr(), N, inner,
                             y.data_ptr(), code, on.stream), "z1_product8");
     return y;
@@ -317,7 +322,7 @@ Tensor weight_grad8(const Tensor& dy, const Tensor& q, const Tensor& s, int64_t 
     check8(q, s, r.rows, inner, r.rows, what, "a");
     const int code = dtype_code(dtype, what);
     OnDevice on(dy);
-    Tensor dw = at::empty({r.dim, inner}, dy.options().dtype(dtype));
+    Tensor dw = fresh({r.dim, inner}, dtype);
     check_rc(api().weight_grad8(static_cast<const uint16_t*>(r.p), r.stride, q.const_data_ptr(), s.const_data_ptr(),
                                 r.rows, r.dim, inner, dw.data_ptr(), code, on.stream), "z1_weight_grad8");
     return dw;

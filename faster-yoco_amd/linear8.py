@@ -9,26 +9,24 @@
 ``linear`` is the three of them as one differentiable function.  Products read e4m3 values and their scales and sum in
 fp32; the weight's gradient reads dy in bf16 and the checkpoint's values, which bf16 holds exactly.
 """
-from dataclasses import dataclass
-
 import torch
 
 from . import act8, library  # noqa: F401  (library registers the operators)
 from .act8 import Act8
 
-_OPS = torch.ops.yoco_z1
+_pack = torch.ops.yoco_z1.weight8_pack.default
+_product = torch.ops.yoco_z1.product8.default
+_weight_grad = torch.ops.yoco_z1.weight_grad8.default
 
 
-@dataclass(frozen=True, slots=True)
 class Weight8:
     """A weight [N, K] in 128 x 128 blocks of one power-of-two scale each, in both orders: ``q`` float8_e4m3fn [N, K
     rounded up to 128] with ``s`` float8_e8m0fnu [ceil(N / 128), blocks of K rounded up to 4], and ``qt`` [K, N rounded up
-    to 128] with ``st`` for the input's gradient (None: forward only)."""
-    q: torch.Tensor
-    s: torch.Tensor
-    qt: torch.Tensor
-    st: torch.Tensor
-    shape: tuple
+    to 128] with ``st`` for the input's gradient (None: forward only).  ``shape`` is (N, K)."""
+    __slots__ = ('q', 's', 'qt', 'st', 'shape')
+
+    def __init__(self, q, s, qt, st, shape):
+        self.q, self.s, self.qt, self.st, self.shape = q, s, qt, st, shape
 
     def nbytes(self):
         return sum(t.numel() for t in (self.q, self.s, self.qt, self.st) if t is not None)
@@ -38,7 +36,7 @@ def pack_weight(w, transposed=True):
     """The 8-bit form of a weight [N, K] (fp32, bf16 or fp16), with its other order unless transposed is False."""
     if w.dim() != 2:
         raise RuntimeError('linear8.pack_weight: expected a weight [N, K]')
-    out = _OPS.weight8_pack(act8.rows_of(w), transposed)
+    out = _pack(act8.rows_of(w), transposed)
     return Weight8(*(out if transposed else (*out, None, None)), tuple(w.shape))
 
 
@@ -51,13 +49,13 @@ def matmul(a, w, dtype=torch.bfloat16, transposed=False):
     if transposed:
         if w.qt is None:
             raise RuntimeError('linear8.matmul: the weight was packed without its other order')
-        return _OPS.product8(a.q, a.s, w.qt, w.st, N, dtype)
-    return _OPS.product8(a.q, a.s, w.q, w.s, K, dtype)
+        return _product(a.q, a.s, w.qt, w.st, N, dtype)
+    return _product(a.q, a.s, w.q, w.s, K, dtype)
 
 
 def weight_grad(dy, a, dtype=torch.bfloat16):
     """dy^T x, [N, K] in `dtype`, from bf16 gradient rows dy [..., N] and the 8-bit rows a of x [..., K]."""
-    return _OPS.weight_grad8(act8.rows_of(dy), a.q, a.s, a.dim, dtype)
+    return _weight_grad(act8.rows_of(dy), a.q, a.s, a.dim, dtype)
 
 
 class _Linear(torch.autograd.Function):

@@ -9,12 +9,13 @@ import torch
 from . import act8, library  # noqa: F401  (library registers the operators)
 from .act8 import Act8
 
-_OPS = torch.ops.yoco_z1
+_norm_forward = torch.ops.yoco_z1.norm_forward.default
+_norm_backward = torch.ops.yoco_z1.norm_backward.default
 
 
 def _forward(x, weight, bias, eps, center, y8, checkpoint):
     r = act8.rows_of(x)
-    out = _OPS.norm_forward(r, weight, bias, eps, center, y8, checkpoint)
+    out = _norm_forward(r, weight, bias, eps, center, y8, checkpoint)
     d = x.shape[-1]
     if y8:
         out[0:2] = [Act8(out[0], out[1], d)]
@@ -43,9 +44,9 @@ def _backward(dy, x, mean, rstd, weight, center, need_weight, need_bias):
     if isinstance(x, Act8):
         if x.dim != dy.shape[-1]:
             raise RuntimeError(f'norm_backward: a checkpoint of {x.dim} columns, gradient rows of {dy.shape[-1]}')
-        out = _OPS.norm_backward(r, None, x.q, x.s, mean, rstd, weight, center, need_weight, need_bias)
+        out = _norm_backward(r, None, x.q, x.s, mean, rstd, weight, center, need_weight, need_bias)
     else:
-        out = _OPS.norm_backward(r, act8.rows_of(x), None, None, mean, rstd, weight, center, need_weight, need_bias)
+        out = _norm_backward(r, act8.rows_of(x), None, None, mean, rstd, weight, center, need_weight, need_bias)
     if dy.dim() != 2:
         out[0] = out[0].view(dy.shape)
     return tuple(out)
