@@ -77,8 +77,10 @@ SIGNATURES = {
     'z1_act8_pack': ([_P, _I64, _I64, _I64, _I, _P, _P, _P], _I),
     'z1_act8_unpack': ([_P, _P, _I64, _I64, _P, _I, _P], _I),
     'z1_weight8_pack': ([_P, _I64, _I64, _I64, _I, _P, _P, _P, _P, _P], _I),
-    'z1_product8': ([_P, _P, _I64, _P, _P, _I64, _I64, _P, _I, _P], _I),
-    'z1_weight_grad8': ([_P, _I64, _P, _P, _I64, _I64, _I64, _P, _I, _P], _I),
+    'z1_product8': ([_P, _P, _I64, _P, _P, _I64, _I64, _P, _I, _P, _I64, _P], _I),
+    'z1_product8_workspace': ([_I64, _I64, _I64, _I], _I64),
+    'z1_weight_grad8': ([_P, _I64, _P, _P, _I64, _I64, _I64, _P, _I, _P, _I64, _P], _I),
+    'z1_weight_grad8_workspace': ([_I64, _I64, _I64], _I64),
     'z1_strerror': ([_I], ctypes.c_char_p),
 }
 

@@ -141,7 +141,8 @@ struct Product {
     const uint8_t* as;                                 // [M, pitch]
     const uint8_t* w;                                  // [N, wide]
     const uint8_t* ws;                                 // [ceil(N / 128), pitch]
-    void* y;                                           // [M, N]
+    void* y;                                           // [M, N], or [parts, M, N] fp32
+    int per;                                           // blocks of K to a part: all, or a multiple of four
     int64_t M;
     int N, blocks, pitch;                              // blocks of 128 along K
     int64_t wide;
@@ -167,9 +168,16 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     const int o0 = (int)(blockIdx.x % tiles_o) * BO;
     const int wt = wave / (BO / WO) * WT, wo = wave % (BO / WO) * WO;          // the wave's part of the tile
 
+    const int kb0 = blockIdx.y * a.per;                // this part's blocks of K
+    const int blocks = a.blocks - kb0 < a.per ? a.blocks - kb0 : a.per;
+    a.a += (int64_t)kb0 * kBlock;
+    a.w += (int64_t)kb0 * kBlock;
+    a.as += kb0;
+    a.ws += kb0;
+    const int64_t before = (int64_t)kb0 * kBlock;
     // Rows past the end lie past their buffer's range, which a load turns to zeros.
-    const __amdgpu_buffer_rsrc_t buf_t = buffer_of(a.a + t0 * a.wide, (a.M - t0) * a.wide);
-    const __amdgpu_buffer_rsrc_t buf_o = buffer_of(a.w + o0 * a.wide, (a.N - o0) * a.wide);
+    const __amdgpu_buffer_rsrc_t buf_t = buffer_of(a.a + t0 * a.wide, (a.M - t0) * a.wide - before);
+    const __amdgpu_buffer_rsrc_t buf_o = buffer_of(a.w + o0 * a.wide, (a.N - o0) * a.wide - before);
     const int wide = (int)a.wide;
     const int sub = lane >> 3, piece = lane & 7;
     const int from = sub * wide + ((piece ^ (sub >> 1)) << 4);                 // in 8 rows whose keys' third bit is 0
@@ -181,7 +189,7 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
         else load_lds(buf_o, buf + (BT + g * 8) * kBlock, g & 2 ? from ^ 64 : from, at);
     };
     // scales: four blocks' bytes at a time, the next four loaded ahead
-    const __amdgpu_buffer_rsrc_t buf_s = buffer_of(a.as + t0 * a.pitch, (a.M - t0) * a.pitch);
+    const __amdgpu_buffer_rsrc_t buf_s = buffer_of(a.as + t0 * a.pitch, (a.M - t0) * a.pitch - kb0);
     const int r32 = lane & 31, half = lane >> 5, rs = spread(r32);
     const int ob = (o0 + wo) / kBlock, ob_last = (a.N - 1) / kBlock;
     const uint32_t* sw = (const uint32_t*)(a.ws + (int64_t)(ob < ob_last ? ob : ob_last) * a.pitch);
@@ -249,12 +257,12 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     for (int i = 0; i < kLoads; ++i) stage(1, i);
 #pragma unroll
     for (int q = 0; q < kReads; ++q) read(0, 0, q);
-    for (int kb = 0; kb < a.blocks; ++kb) {
+    for (int kb = 0; kb < blocks; ++kb) {
         if ((kb & 3) == 0) {
 #pragma unroll
             for (int j = 0; j < NT; ++j) now[j] = next[j];
             now_w = next_w;
-            scales(kb + 4 < a.blocks ? kb + 4 : 0);
+            scales(kb + 4 < blocks ? kb + 4 : 0);
         }
         products(0, kb, -1);
         meet();                                        // block kb has been read, block kb + 1 has arrived
@@ -265,53 +273,83 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     }
     meet();                                            // the staging buffers are free
     constexpr int kRoom = (int)sizeof(lds) / kWaves;
+    void* y = (typename T::elem*)a.y + blockIdx.y * a.M * a.N;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         f16 part[NO];
 #pragma unroll
         for (int i = 0; i < NO; ++i) part[i] = acc[i][j];
-        Flush<T, WO, kRoom>::run(&lds[0][0] + wave * kRoom, lane, part, a.y, t0 + wt + j * 32, a.M, o0 + wo, a.N);
+        Flush<T, WO, kRoom>::run(&lds[0][0] + wave * kRoom, lane, part, y, t0 + wt + j * 32, a.M, o0 + wo, a.N);
     }
 }
 
-// Up to 32 rows: the weight is read once, straight into the matrix instructions' registers, 32 outputs to a workgroup and
-// K shared by its waves, whose sums meet in LDS.
+// Few rows: the weight is read once, straight into the matrix instructions' registers, by workgroups of OB outputs whose
+// waves share K and whose sums meet in LDS; OB rows at most.  With OB 8 or 16 the instruction's 32 rows and columns
+// are 32 / OB groups, each of the same outputs and rows with a block of K of its own: the results on its diagonal are that
+// many partial sums, so that an output range of 8 keeps all lanes loading and there are workgroups for all CUs (8192 x
+// 3072, one row: 1024 of 8 outputs).  A wave has the loads of U steps under way together.
 constexpr int kFewWaves = 8;
-template <typename T, bool PRECISE>
+template <typename T, bool PRECISE, int OB, int U>
 __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(Product a) {
+    constexpr int G = 32 / OB;                         // blocks of K to an instruction
     __shared__ float sums[kFewWaves][32 * 33];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int o0 = blockIdx.x * 32, r32 = lane & 31, half = lane >> 5;
-    int o = o0 + spread(r32);
+    const int o0 = blockIdx.x * OB, r32 = lane & 31, half = lane >> 5, g = r32 / OB;
+    int o = o0 + r32 % OB;
     o = o < a.N ? o : a.N - 1;
-    const int64_t t = r32 < a.M ? r32 : a.M - 1;
-    const uint8_t* pa = a.a + t * a.wide + half * 32;
     const uint8_t* pw = a.w + o * a.wide + half * 32;
-    const uint8_t* sa = a.as + t * a.pitch;
     const uint8_t* sw = a.ws + (int64_t)(o0 / kBlock) * a.pitch;
+    int64_t t = r32 % OB;
+    t = t < a.M ? t : a.M - 1;
+    const uint8_t* pa = a.a + t * a.wide + half * 32;
+    const uint8_t* sa = a.as + t * a.pitch;
     f16 acc[1][1] = {};
-    for (int kb = wave; kb < a.blocks; kb += kFewWaves) {
+    const int steps = (a.blocks + G - 1) / G;
+    for (int first = wave; first < steps; first += kFewWaves * U) {
+        i4 w[U][4], x[U][4];
+        uint32_t ew[U], ex[U];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const Z1B_GLOBAL i4* x = (const Z1B_GLOBAL i4*)(pa + (int64_t)kb * kBlock + h * 64);
-            const Z1B_GLOBAL i4* w = (const Z1B_GLOBAL i4*)(pw + (int64_t)kb * kBlock + h * 64);
-            const i8 fx[1] = {__builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7)};
-            const i8 fw[1] = {__builtin_shufflevector(w[0], w[1], 0, 1, 2, 3, 4, 5, 6, 7)};
-            const uint32_t sx[1] = {sa[kb]};
-            if constexpr (PRECISE) multiply_precise(acc, fw, fx, sw[kb], sx);
-            else acc[0][0] = multiply(acc[0][0], fw[0], fx[0], sw[kb], sx[0]);
+        for (int u = 0; u < U; ++u) {
+            if (first + u * kFewWaves >= steps) continue;
+            int kb = (first + u * kFewWaves) * G + g;
+            kb = kb < a.blocks ? kb : a.blocks - 1;    // past K's end: the last block, times nothing
+            ew[u] = sw[kb];
+            ex[u] = sa[kb];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int64_t at = (int64_t)kb * kBlock + (q >> 1) * 64 + (q & 1) * 16;
+                w[u][q] = *(const Z1B_GLOBAL i4*)(pw + at);
+                x[u][q] = *(const Z1B_GLOBAL i4*)(pa + at);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);             // the compiler would load each step when it comes to it
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (first + u * kFewWaves >= steps) continue;
+            const bool in = (first + u * kFewWaves) * G + g < a.blocks;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const i8 fw[1] = {__builtin_shufflevector(w[u][2 * h], w[u][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7)};
+                i8 fx[1] = {__builtin_shufflevector(x[u][2 * h], x[u][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7)};
+                fx[0] = in ? fx[0] : i8{};
+                const uint32_t sx[1] = {ex[u]};
+                if constexpr (PRECISE) multiply_precise(acc, fw, fx, ew[u], sx);
+                else acc[0][0] = multiply(acc[0][0], fw[0], fx[0], ew[u], ex[u]);
+            }
         }
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sums[wave][r32 * 33 + half * 16 + i] = acc[0][0][i];
+    for (int i = 0; i < 16; ++i) sums[wave][r32 * 33 + 8 * (i >> 2) + 4 * half + (i & 3)] = acc[0][0][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < 32 * 32; e += kFewWaves * 64) {
-        const int row = e >> 5, col = e & 31;
-        if (row >= a.M || o0 + col >= a.N) continue;
-        float v = sums[0][row * 33 + col];
+    for (int e = threadIdx.x; e < OB * OB; e += kFewWaves * 64) {
+        const int row = e / OB, c = e % OB;
+        if (row >= a.M || o0 + c >= a.N) continue;
+        float v = 0.0f;
 #pragma unroll
-        for (int i = 1; i < kFewWaves; ++i) v += sums[i][row * 33 + col];
-        T::put(a.y, (int64_t)row * a.N + o0 + col, v);
+        for (int k = 0; k < G; ++k)
+#pragma unroll
+            for (int i = 0; i < kFewWaves; ++i) v += sums[i][(k * OB + row) * 33 + k * OB + c];
+        T::put(a.y, (int64_t)row * a.N + o0 + c, v);
     }
 }
 
@@ -321,7 +359,8 @@ struct Gradient {
     int64_t stride;
     const uint8_t* q;                                  // [T, wide]
     const uint8_t* s;                                  // [T, pitch]
-    void* dw;                                          // [N, K]
+    void* dw;                                          // [N, K], or [parts, N, K] fp32
+    int64_t per;                                       // tokens to a part: all, or a multiple of the step
     int64_t T;
     int N, K, wide, pitch;
 };
@@ -523,6 +562,11 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
     const int tiles_k = (a.K + BK - 1) / BK;
     const int n0 = (int)(blockIdx.x / tiles_k) * BN, k0 = (int)(blockIdx.x % tiles_k) * BK;
     const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
+    const int64_t t_first = blockIdx.y * a.per;        // this part's tokens
+    a.dy += t_first * a.stride;
+    a.q += t_first * a.wide;
+    a.s += t_first * a.pitch;
+    a.T = a.T - t_first < a.per ? a.T - t_first : a.per;
     const int64_t steps = (a.T + TS - 1) / TS;
 
     // direct loads: a lane's row and piece of 16 bytes within a load's rows
@@ -631,57 +675,127 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
     for (int m = 0; m < kProducts; ++m) product(1, m);
     meet();                                            // the staging buffers are free
     constexpr int kRoom = (int)sizeof(lds) / kWaves & ~15;
+    void* dw = (typename T::elem*)a.dw + (int64_t)blockIdx.y * a.N * a.K;
 #pragma unroll
     for (int i = 0; i < NN; ++i)
-        Flush<T, WK, kRoom>::run(lds + wave * kRoom, lane, acc[i], a.dw, n0 + wn + i * 32, a.N, k0 + wk, a.K);
+        Flush<T, WK, kRoom>::run(lds + wave * kRoom, lane, acc[i], dw, n0 + wn + i * 32, a.N, k0 + wk, a.K);
 }
 
 constexpr int64_t kMaxRows = 1ll << 40;
 constexpr int64_t kMaxDim = 1 << 24;
+constexpr int kMaxParts = 16;
 constexpr int64_t kMaxTiles = 1ll << 22;               // of a launch: its threads count in 32 bits
 
 bool bad_dtype(int d) { return d != Z1_F32 && d != Z1_BF16 && d != Z1_F16; }
 
 constexpr int kCus = 256;
 
+// The sum of `parts` partial results, in order.
+constexpr int kJoinThreads = 256;
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* part, int parts, int64_t count, void* out) {
+    const int64_t i = ((int64_t)blockIdx.x * kJoinThreads + threadIdx.x) * kLane;
+    if (i >= count) return;
+    const int n = count - i < kLane ? (int)(count - i) : kLane;
+    float s[kLane] = {};
+    for (int p = 0; p < parts; ++p) {
+        float v[kLane];
+        load_row<F32>(part, p * count + i, n, v);
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) s[j] += v[j];
+    }
+    store_row<T>(out, i, n, s);
+}
+template <typename T>
+int join(const float* part, int parts, int64_t count, void* out, hipStream_t st) {
+    const int64_t per = kJoinThreads * kLane;
+    join_kernel<T><<<dim3((unsigned)((count + per - 1) / per)), kJoinThreads, 0, st>>>(part, parts, count, out);
+    return (int)hipGetLastError();
+}
+
+// The number of parts into which the long axis of a product in small tiles is cut, `steps` of it in multiples of `unit`:
+// the one with the least estimate of the time in ns.  A step takes `alone` where a CU has one tile, `shared` where it has
+// two; the joining launch takes 4.5 us (its own and the launch's) and the partial results' way out and back at 4 bytes/ps.
+int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int alone, int shared) {
+    if (tiles > kCus) return 1;
+    int best = 1;
+    int64_t least = 0;
+    for (int p = 1; p <= kMaxParts; ++p) {
+        const int64_t per = (steps + p * unit - 1) / (p * unit) * unit;
+        if (p > 1 && (per * (p - 1) >= steps || tiles * p > 2 * kCus)) continue;       // a part without steps; no room
+        const int64_t time = per * (tiles * p <= kCus ? alone : shared) + (p > 1 ? 4500 + p * results * 8 / 4000 : 0);
+        if (p == 1 || time < least) best = p, least = time;
+    }
+    return best;
+}
+
+// How a product runs.  Large tiles move fewer bytes per product (8192 x 8192 x 8192: 422 us against 553), small ones leave
+// fewer CUs without work; a CU takes one large tile at a time, or two small ones in 0.65 of its time, and the fewer rounds
+// win.  Where even small tiles leave CUs idle, a long K is cut into parts, joined by a second launch (8192 -> 3072, 128
+// rows: 44 us whole, 20 in parts; 3072 -> 8192: 19 and 19).
+struct Way {
+    bool few, large;
+    int parts, per;                                    // of K's blocks
+};
+Way product_way(int64_t M, int64_t N, int blocks, bool precise) {
+    if (M <= 32) return {true, false, 1, blocks};
+    const int64_t large = (M + 255) / 256 * ((N + 255) / 256), small = (M + 127) / 128 * ((N + 127) / 128);
+    const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
+    if (!precise && 100 * large_rounds <= 65 * small_rounds) return {false, true, 1, blocks};
+    const int parts = parts_of(small, blocks, 4, M * N, 700, 850);
+    return {false, false, parts, parts == 1 ? blocks : (blocks + 4 * parts - 1) / (4 * parts) * 4};
+}
+
 template <typename T, bool PRECISE, int BT, int BO, int WT, int WO>
-int launch_tiles(const Product& a, hipStream_t st) {
+int launch_tiles(const Product& a, int parts, hipStream_t st) {
     const int64_t tiles = (a.M + BT - 1) / BT * ((a.N + BO - 1) / BO);
     if (tiles > kMaxTiles) return Z1_E_SIZE;
-    product_kernel<T, PRECISE, BT, BO, WT, WO><<<dim3((unsigned)tiles), BT / WT * (BO / WO) * 64, 0, st>>>(a);
+    product_kernel<T, PRECISE, BT, BO, WT, WO><<<dim3((unsigned)tiles, parts), BT / WT * (BO / WO) * 64, 0, st>>>(a);
+    return (int)hipGetLastError();
+}
+
+// As many steps together as a wave has, up to four: more registers than that leave a CU fewer waves than loads.
+template <typename T, bool PRECISE, int OB>
+int launch_few(const Product& a, hipStream_t st) {
+    const int groups = 32 / OB, steps = (a.blocks + groups - 1) / groups, each = (steps + kFewWaves - 1) / kFewWaves;
+    const dim3 grid((unsigned)((a.N + OB - 1) / OB));
+    if (each == 1) product_few_kernel<T, PRECISE, OB, 1><<<grid, kFewWaves * 64, 0, st>>>(a);
+    else if (each == 2) product_few_kernel<T, PRECISE, OB, 2><<<grid, kFewWaves * 64, 0, st>>>(a);
+    else product_few_kernel<T, PRECISE, OB, 4><<<grid, kFewWaves * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 
 template <typename T, bool PRECISE>
-int launch_product(const Product& a, hipStream_t st) {
-    if (a.M <= 32) {
-        product_few_kernel<T, PRECISE><<<dim3((unsigned)((a.N + 31) / 32)), kFewWaves * 64, 0, st>>>(a);
-        return (int)hipGetLastError();
+int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) {
+    if (a.M <= 8) return launch_few<T, PRECISE, 8>(a, st);
+    if (a.M <= 16) return launch_few<T, PRECISE, 16>(a, st);
+    if (way.few) return launch_few<T, PRECISE, 32>(a, st);
+    a.per = way.per;
+    if constexpr (!PRECISE) {
+        if (way.large) return launch_tiles<T, PRECISE, 256, 256, 64, 128>(a, 1, st);
     }
-    if (PRECISE) return launch_tiles<T, PRECISE, 128, 128, 64, 64>(a, st);
-    // Large tiles move fewer bytes per product (8192 x 8192 x 8192: 422 us against 553), small ones leave fewer CUs without
-    // work.  A CU takes one large tile at a time, or two small ones in 0.65 of its time; the fewer rounds win.
-    const int64_t large = (a.M + 255) / 256 * ((a.N + 255) / 256), small = (a.M + 127) / 128 * ((a.N + 127) / 128);
-    const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
-    if (100 * large_rounds <= 65 * small_rounds) return launch_tiles<T, PRECISE, 256, 256, 64, 128>(a, st);
-    return launch_tiles<T, PRECISE, 128, 128, 64, 64>(a, st);
+    if (way.parts == 1) return launch_tiles<T, PRECISE, 128, 128, 64, 64>(a, 1, st);
+    void* y = a.y;
+    a.y = workspace;
+    if (const int rc = launch_tiles<F32, PRECISE, 128, 128, 64, 64>(a, way.parts, st)) return rc;
+    return join<T>(workspace, way.parts, a.M * a.N, y, st);
 }
 
 // fp32 results are always precise; 16-bit ones where K is short, since a short sum has few groups over which the cuts
 // average out, and its time goes into the result's writes anyway.
 constexpr int kPreciseBlocks = 3;
+bool is_precise(int dtype, int blocks) { return dtype == Z1_F32 || blocks <= kPreciseBlocks; }
+
 template <typename T>
-int product(const Product& a, hipStream_t st) {
-    return a.blocks <= kPreciseBlocks ? launch_product<T, true>(a, st) : launch_product<T, false>(a, st);
+int product(const Product& a, const Way& way, float* workspace, hipStream_t st) {
+    return a.blocks <= kPreciseBlocks ? launch_product<T, true>(a, way, workspace, st)
+                                      : launch_product<T, false>(a, way, workspace, st);
 }
 template <>
-int product<F32>(const Product& a, hipStream_t st) {
-    return launch_product<F32, true>(a, st);
+int product<F32>(const Product& a, const Way& way, float* workspace, hipStream_t st) {
+    return launch_product<F32, true>(a, way, workspace, st);
 }
 
-#ifndef WG
-#define WG 128, 128, 64, 64, 32
-#endif
 template <typename T, Edge EDGE, int BN, int BK, int WN, int WK, int TS>
 int launch_gradient(const Gradient& a, hipStream_t st) {
     const int64_t tiles = (int64_t)((a.N + BN - 1) / BN) * ((a.K + BK - 1) / BK);
@@ -689,19 +803,43 @@ int launch_gradient(const Gradient& a, hipStream_t st) {
     weight_grad_kernel<T, EDGE, BN, BK, WN, WK, TS><<<dim3((unsigned)tiles), BN / WN * (BK / WK) * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
-#ifndef WD
-#define WD 256, 256, 128, 64, 64
-#endif
-template <typename T, int BN, int BK, int WN, int WK, int TS>
-int launch_direct(const Gradient& a, hipStream_t st) {
+// How a weight gradient runs: by direct loads where dy's rows are whole dwords, in large tiles, or in small ones with the
+// tokens cut into parts where those leave CUs idle (16384 tokens, 512 x 512: 166 us whole, 28 in parts).
+struct GradientWay {
+    bool direct, large;
+    int parts;
+    int64_t per;
+};
+constexpr int kStep = 64;
+GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
+    if (!direct) return {false, false, 1, T};
+    const int64_t large = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);
+    const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
+    if (100 * large_rounds <= 62 * small_rounds) return {true, true, 1, T};
+    const int64_t steps = (T + kStep - 1) / kStep;
+    const int parts = parts_of(small, steps, 1, N * K, 650, 1100);
+    return {true, false, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
+}
+bool is_direct(const void* dy, int64_t stride) { return stride % 2 == 0 && reinterpret_cast<uintptr_t>(dy) % 4 == 0; }
+
+template <typename T, int BN, int BK, int WN, int WK>
+int launch_direct(const Gradient& a, int parts, hipStream_t st) {
     const int64_t tiles = (int64_t)((a.N + BN - 1) / BN) * ((a.K + BK - 1) / BK);
     if (tiles > kMaxTiles) return Z1_E_SIZE;
-    weight_grad_direct_kernel<T, BN, BK, WN, WK, TS><<<dim3((unsigned)tiles), BN / WN * (BK / WK) * 64, 0, st>>>(a);
+    weight_grad_direct_kernel<T, BN, BK, WN, WK, kStep><<<dim3((unsigned)tiles, parts), BN / WN * (BK / WK) * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 template <typename T>
-int gradient(const Gradient& a, hipStream_t st) {
-    if (a.stride % 2 == 0 && reinterpret_cast<uintptr_t>(a.dy) % 4 == 0) return launch_direct<T, WD>(a, st);
+int gradient(Gradient a, const GradientWay& way, float* workspace, hipStream_t st) {
+    a.per = way.per;
+    if (way.large) return launch_direct<T, 256, 256, 128, 64>(a, 1, st);
+    if (way.direct && way.parts == 1) return launch_direct<T, 128, 128, 64, 64>(a, 1, st);
+    if (way.direct) {
+        void* dw = a.dw;
+        a.dw = workspace;
+        if (const int rc = launch_direct<F32, 128, 128, 64, 64>(a, way.parts, st)) return rc;
+        return join<T>(workspace, way.parts, (int64_t)a.N * a.K, dw, st);
+    }
     if (a.N < 8) return launch_gradient<T, kFew, 128, 128, 64, 64, 32>(a, st);
     return launch_gradient<T, kCut, 128, 128, 64, 64, 32>(a, st);
 }
@@ -710,34 +848,59 @@ int gradient(const Gradient& a, hipStream_t st) {
 
 extern "C" {
 
-int z1_product8(const void* a, const void* as, int64_t M, const void* w, const void* ws, int64_t N, int64_t K, void* y,
-                int dtype, void* stream) {
+int64_t z1_product8_workspace(int64_t M, int64_t N, int64_t K, int dtype) {
     if (M < 0 || M > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim) return Z1_E_SIZE;
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
+    if (M == 0 || N == 0) return 0;
+    const int blocks = wide_of(K) / kBlock;
+    const Way way = product_way(M, N, blocks, is_precise(dtype, blocks));
+    return way.parts > 1 ? way.parts * M * N : 0;
+}
+
+int z1_product8(const void* a, const void* as, int64_t M, const void* w, const void* ws, int64_t N, int64_t K, void* y,
+                int dtype, float* workspace, int64_t workspace_floats, void* stream) {
+    const int64_t need = z1_product8_workspace(M, N, K, dtype);
+    if (need < 0) return (int)need;
     if (M == 0 || N == 0) return Z1_OK;
-    if (!a || !as || !w || !ws || !y) return Z1_E_NULL;
-    const Product p{(const uint8_t*)a, (const uint8_t*)as, (const uint8_t*)w, (const uint8_t*)ws, y, M, (int)N,
-                    wide_of(K) / kBlock, pitch_of(K), wide_of(K)};
+    if (!a || !as || !w || !ws || !y || (need && !workspace)) return Z1_E_NULL;
+    if (workspace_floats < need) return Z1_E_WORKSPACE;
+    const int blocks = wide_of(K) / kBlock;
+    const Product p{(const uint8_t*)a, (const uint8_t*)as, (const uint8_t*)w, (const uint8_t*)ws, y, blocks, M, (int)N,
+                    blocks, pitch_of(K), wide_of(K)};
+    const Way way = product_way(M, N, blocks, is_precise(dtype, blocks));
     const hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-        case Z1_F32: return product<F32>(p, st);
-        case Z1_BF16: return product<BF16>(p, st);
-        default: return product<F16>(p, st);
+        case Z1_F32: return product<F32>(p, way, workspace, st);
+        case Z1_BF16: return product<BF16>(p, way, workspace, st);
+        default: return product<F16>(p, way, workspace, st);
     }
 }
 
+int64_t z1_weight_grad8_workspace(int64_t T, int64_t N, int64_t K) {
+    if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim) return Z1_E_SIZE;
+    if (N == 0) return 0;
+    const GradientWay way = gradient_way(T, N, K, true);
+    return way.parts > 1 ? way.parts * N * K : 0;
+}
+
 int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const void* s, int64_t T, int64_t N, int64_t K,
-                    void* dw, int dtype, void* stream) {
-    if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim || stride < 0) return Z1_E_SIZE;
+                    void* dw, int dtype, float* workspace, int64_t workspace_floats, void* stream) {
+    // a step's rows lie within 32 bits of its first
+    if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim || stride < 0 || stride > kMaxDim) return Z1_E_SIZE;
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (N == 0) return Z1_OK;
     if (!dw || (T > 0 && (!dy || !q || !s))) return Z1_E_NULL;
-    const Gradient g{dy, stride, (const uint8_t*)q, (const uint8_t*)s, dw, T, (int)N, (int)K, wide_of(K), pitch_of(K)};
+    const GradientWay way = gradient_way(T, N, K, is_direct(dy, stride));
+    if (way.parts > 1) {
+        if (!workspace) return Z1_E_NULL;
+        if (workspace_floats < way.parts * N * K) return Z1_E_WORKSPACE;
+    }
+    const Gradient g{dy, stride, (const uint8_t*)q, (const uint8_t*)s, dw, T, T, (int)N, (int)K, wide_of(K), pitch_of(K)};
     const hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-        case Z1_F32: return gradient<F32>(g, st);
-        case Z1_BF16: return gradient<BF16>(g, st);
-        default: return gradient<F16>(g, st);
+        case Z1_F32: return gradient<F32>(g, way, workspace, st);
+        case Z1_BF16: return gradient<BF16>(g, way, workspace, st);
+        default: return gradient<F16>(g, way, workspace, st);
     }
 }
 

@@ -35,7 +35,9 @@ struct Api {
     decltype(&::z1_act8_unpack) act8_unpack;
     decltype(&::z1_weight8_pack) weight8_pack;
     decltype(&::z1_product8) product8;
+    decltype(&::z1_product8_workspace) product8_workspace;
     decltype(&::z1_weight_grad8) weight_grad8;
+    decltype(&::z1_weight_grad8_workspace) weight_grad8_workspace;
     decltype(&::z1_strerror) strerror;
 };
 
@@ -136,6 +138,20 @@ Tensor fresh(at::IntArrayRef size, at::ScalarType dtype) {
     return Tensor(at::detail::empty_cuda(size, dtype, c10::Device(c10::DeviceType::CUDA), std::nullopt));
 }
 
+// Scratch floats of one call.  Freed when the call returns, which torch's allocator orders behind the call's launches.
+struct Workspace {
+    Tensor t;
+    float* p = nullptr;
+    int64_t floats;
+    Workspace(int64_t n, const char* what) : floats(n) {
+        if (n < 0) check_rc(n, what);
+        if (n > 0) {
+            t = fresh({n}, at::kFloat);
+            p = static_cast<float*>(t.data_ptr());
+        }
+    }
+};
+
 struct Pair {
     Tensor q, s;
 };
@@ -235,19 +251,13 @@ std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const Op
     out.push_back(fresh({r.rows, r.dim}, dy.scalar_type()));
     if (need_dw) out.push_back(fresh({r.dim}, gt));
     if (need_db) out.push_back(fresh({r.dim}, gt));
-    Tensor ws;
-    int64_t floats = 0;
-    if (need_dw || need_db) {
-        floats = api().norm_backward_workspace(r.rows, r.dim);
-        if (floats < 0) check_rc(floats, "z1_norm_backward_workspace");
-        ws = fresh({floats}, at::kFloat);
-    }
+    const Workspace parts(need_dw || need_db ? api().norm_backward_workspace(r.rows, r.dim) : 0,
+                          "z1_norm_backward_workspace");
     check_rc(api().norm_backward(r.p, r.stride, plain ? xr.p : nullptr, xr.stride, packed ? q->const_data_ptr() : nullptr,
                                  packed ? s->const_data_ptr() : nullptr, r.rows, r.dim, r.dtype, mp, rp, w,
                                  w ? dtype_code(gt, what) : Z1_F32, center, out[0].data_ptr(),
                                  need_dw ? out[1].data_ptr() : nullptr, need_db ? out.back().data_ptr() : nullptr,
-                                 dtype_code(gt, what), ws.defined() ? static_cast<float*>(ws.data_ptr()) : nullptr, floats,
-                                 on.stream), "z1_norm_backward");
+                                 dtype_code(gt, what), parts.p, parts.floats, on.stream), "z1_norm_backward");
     return out;
 }
 
@@ -308,14 +318,17 @@ Tensor product8(const Tensor& q, const Tensor& s, const Tensor& wq, const Tensor
     const int code = dtype_code(dtype, what);
     OnDevice on(q);
     Tensor y = fresh({M, N}, dtype);
+    const Workspace parts(api().product8_workspace(M, N, inner, code), "z1_product8_workspace");
     check_rc(api().product8(q.const_data_ptr(), s.const_data_ptr(), M, wq.const_data_ptr(), ws.const_data_ptr(), N, inner,
-                            y.data_ptr(), code, on.stream), "z1_product8");
+                            y.data_ptr(), code, parts.p, parts.floats, on.stream), "z1_product8");
     return y;
 }
 
-Tensor weight_grad8(const Tensor& dy, const Tensor& q, const Tensor& s, int64_t inner, at::ScalarType dtype) {
+Tensor weight_grad8(const Tensor& dy_given, const Tensor& q, const Tensor& s, int64_t inner, at::ScalarType dtype) {
     const char* what = "linear8.weight_grad";
-    require_gpu(dy, what, "dy");
+    require_gpu(dy_given, what, "dy");
+    // a step's rows lie within 32 bits of its first
+    const Tensor dy = dy_given.dim() == 2 && dy_given.stride(0) > (1 << 24) ? dy_given.contiguous() : dy_given;
     const Rows r = rows_of(dy, what, "dy");
     TORCH_CHECK(r.dtype == Z1_BF16, what, ": expected bf16 gradient rows");
     require_on(q, dy, what, "a");
@@ -323,8 +336,10 @@ Tensor weight_grad8(const Tensor& dy, const Tensor& q, const Tensor& s, int64_t 
     const int code = dtype_code(dtype, what);
     OnDevice on(dy);
     Tensor dw = fresh({r.dim, inner}, dtype);
-    check_rc(api().weight_grad8(static_cast<const uint16_t*>(r.p), r.stride, q.const_data_ptr(), s.const_data_ptr(),
-                                r.rows, r.dim, inner, dw.data_ptr(), code, on.stream), "z1_weight_grad8");
+    const Workspace parts(api().weight_grad8_workspace(r.rows, r.dim, inner), "z1_weight_grad8_workspace");
+    check_rc(api().weight_grad8(static_cast<const uint16_t*>(r.p), r.rows > 1 ? r.stride : r.dim, q.const_data_ptr(),
+                                s.const_data_ptr(), r.rows, r.dim, inner, dw.data_ptr(), code, parts.p, parts.floats,
+                                on.stream), "z1_weight_grad8");
     return dw;
 }
 
@@ -384,7 +399,9 @@ int z1t_init_block(const char* path) {
     Z1T_RESOLVE(act8_unpack)
     Z1T_RESOLVE(weight8_pack)
     Z1T_RESOLVE(product8)
+    Z1T_RESOLVE(product8_workspace)
     Z1T_RESOLVE(weight_grad8)
+    Z1T_RESOLVE(weight_grad8_workspace)
     Z1T_RESOLVE(strerror)
 #undef Z1T_RESOLVE
     g_api = a;

@@ -298,13 +298,17 @@ int z1_weight8_pack(const void* w, int64_t N, int64_t K, int64_t stride, int dty
                     void* stream);
 
 /* y[M][N] (dtype) = 8-bit rows a, as [M][K] times the transpose of 8-bit weight w, ws [N][K].  The input gradient is the
- * same product with the rows of dy and the weight's other order. */
+ * same product with the rows of dy and the weight's other order.  workspace: device floats,
+ * z1_product8_workspace(M, N, K, dtype) of them (none for most shapes; NULL then). */
 int z1_product8(const void* a, const void* as, int64_t M, const void* w, const void* ws, int64_t N, int64_t K, void* y,
-                int dtype, void* stream);
+                int dtype, float* workspace, int64_t workspace_floats, void* stream);
+int64_t z1_product8_workspace(int64_t M, int64_t N, int64_t K, int dtype);
 
-/* dw[N][K] (dtype) = sum over T tokens of dy[t][n] (bf16) times the 8-bit rows q, s [T][K]; zeros for T = 0. */
+/* dw[N][K] (dtype) = sum over T tokens of dy[t][n] (bf16) times the 8-bit rows q, s [T][K]; zeros for T = 0.  stride at
+ * most 2^24.  workspace: device floats, z1_weight_grad8_workspace(T, N, K) of them (none for most shapes; NULL then). */
 int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const void* s, int64_t T, int64_t N, int64_t K,
-                    void* dw, int dtype, void* stream);
+                    void* dw, int dtype, float* workspace, int64_t workspace_floats, void* stream);
+int64_t z1_weight_grad8_workspace(int64_t T, int64_t N, int64_t K);
 
 /* Text for a return code (negative: argument errors; positive: hipError_t). */
 const char* z1_strerror(int code);

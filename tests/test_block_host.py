@@ -52,13 +52,21 @@ def test_argument_errors_without_device_work(pkg):
     assert L.z1_weight8_pack(a, -1, 8, 8, 0, a, a, a, a, None) == SIZE
     assert L.z1_weight8_pack(a, 8, 8, 8, 5, a, a, a, a, None) == DTYPE
     assert L.z1_weight8_pack(a, 8, 8, 8, 0, a, a, a, None, None) == NULL
-    assert L.z1_product8(a, a, -1, a, a, 8, 8, a, 0, None) == SIZE and L.z1_product8(a, a, 4, a, a, 8, 0, a, 0, None) == SIZE
-    assert L.z1_product8(a, a, 4, a, a, 8, 8, a, 4, None) == DTYPE
-    assert L.z1_product8(a, a, 4, a, None, 8, 8, a, 0, None) == NULL
-    assert L.z1_product8(None, None, 0, None, None, 8, 8, None, 0, None) == 0
-    assert L.z1_weight_grad8(a, -1, a, a, 4, 8, 8, a, 0, None) == SIZE
-    assert L.z1_weight_grad8(a, 8, a, a, 4, 8, 8, a, 4, None) == DTYPE
-    assert L.z1_weight_grad8(None, 8, a, a, 4, 8, 8, a, 0, None) == NULL
+    mul = lambda M, N, K, dtype, ws=None, n=0, p=a: L.z1_product8(p, p, M, a, a, N, K, a, dtype, ws, n, None)  # noqa: E731
+    assert mul(-1, 8, 8, 0) == SIZE and mul(4, 8, 0, 0) == SIZE and mul(4, 8, 8, 4) == DTYPE and mul(4, 8, 8, 0, p=None) == NULL
+    assert L.z1_product8(None, None, 0, None, None, 8, 8, None, 0, None, 0, None) == 0
+    need = L.z1_product8_workspace(100, 256, 8192, 1)              # few tiles, a long K: partial results
+    assert need >= 2 * 100 * 256 and need % (100 * 256) == 0
+    assert mul(100, 256, 8192, 1) == NULL and mul(100, 256, 8192, 1, a, need - 1) == WS
+    assert L.z1_product8_workspace(8, 8192, 8192, 1) == 0 and L.z1_product8_workspace(0, 8, 8, 1) == 0
+    assert L.z1_product8_workspace(4, 8, -1, 1) == SIZE and L.z1_product8_workspace(4, 8, 8, 9) == DTYPE
+    grad = lambda T, N, K, stride, dtype, ws=None, n=0, p=a: L.z1_weight_grad8(p, stride, a, a, T, N, K, a, dtype, ws, n, None)  # noqa: E731
+    assert grad(4, 8, 8, -1, 0) == SIZE and grad(4, 8, 8, (1 << 24) + 1, 0) == SIZE and grad(4, 8, 8, 8, 4) == DTYPE
+    assert grad(4, 8, 8, 8, 0, p=None) == NULL
+    need = L.z1_weight_grad8_workspace(8192, 256, 256)
+    assert need >= 2 * 256 * 256 and need % (256 * 256) == 0
+    assert grad(8192, 256, 256, 256, 1) == NULL and grad(8192, 256, 256, 256, 1, a, need - 1) == WS
+    assert L.z1_weight_grad8_workspace(8, 8, 0) == SIZE and L.z1_weight_grad8_workspace(0, 8, 8) == 0
 
 
 def test_python_surfaces_refuse_cpu_tensors(pkg):

@@ -42,6 +42,40 @@ def test_product(pkg, dev, M, N, K, dtype):
     near(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), K, dtype)
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('M,N,K', [(100, 256, 8192), (40, 70, 2300), (33, 1, 1030), (257, 300, 4100), (130, 129, 1025)])
+def test_product_in_parts_of_k(pkg, dev, M, N, K, dtype):
+    """Few tiles and a long K: partial results, joined."""
+    from faster_yoco_amd import _lib, act8, linear8
+    assert _lib.lib().z1_product8_workspace(M, N, K, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]) > 0
+    x, w, xv, wv = operands(M, N, K, 30)
+    p = linear8.pack_weight(w.to(dev))
+    y = linear8.matmul(act8.pack(x.to(dev)), p, dtype)
+    near(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), K, dtype)
+    assert torch.equal(y, linear8.matmul(act8.pack(x.to(dev)), p, dtype))
+
+
+@pytest.mark.parametrize('M,N,K', [(300, 2500, 600), (2100, 4000, 520)])
+def test_product_in_large_tiles(pkg, dev, M, N, K):
+    from faster_yoco_amd import act8, linear8
+    x, w, xv, wv = operands(M, N, K, 31)
+    y = linear8.matmul(act8.pack(x.to(dev)), linear8.pack_weight(w.to(dev)))
+    near(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), K, torch.bfloat16)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize('T,N,K', [(8192, 256, 256), (1100, 130, 70), (3001, 2, 3), (1024, 600, 300), (200, 4000, 2100)])
+def test_weight_gradient_in_parts_and_large_tiles(pkg, dev, T, N, K, dtype):
+    from faster_yoco_amd import _lib, act8, linear8
+    assert (_lib.lib().z1_weight_grad8_workspace(T, N, K) > 0) == (T > 1000)
+    x, dy = rows(T, K, 32), rows(T, N, 33) * 1e-3
+    xv, d = ref.values(*ref.pack(x), K), dy.double()
+    a = act8.pack(x.to(dev))
+    dw = linear8.weight_grad(dy.to(dev), a, dtype)
+    near(dw, d.t() @ xv, d.abs().t() @ xv.abs(), T, dtype)
+    assert torch.equal(dw, linear8.weight_grad(dy.to(dev), a, dtype))
+
+
 @pytest.mark.parametrize('M,N,K', SHAPES)
 def test_product_with_the_other_order(pkg, dev, M, N, K):
     """dy @ w: the input's gradient."""
