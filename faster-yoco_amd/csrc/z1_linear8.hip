@@ -77,7 +77,7 @@ template <typename T, int C, int ROOM>
 struct Flush {
     static constexpr int kElem = (int)sizeof(typename T::elem);
     static constexpr int pitch(int c) { return c * kElem + 16; }               // 16 neighbouring rows in different banks
-    static constexpr int kC = 32 * pitch(C) <= ROOM ? C : 32 * pitch(C / 2) <= ROOM ? C / 2 : 32;      // at a time
+    static constexpr int kC = C & (C - 1) ? 32 : 32 * pitch(C) <= ROOM ? C : 32 * pitch(C / 2) <= ROOM ? C / 2 : 32;
     static constexpr int kPitch = pitch(kC);
     static_assert(32 * kPitch <= ROOM, "room for a wave's rows");
     static __device__ __forceinline__ void run(uint8_t* own, int lane, const f16 (&acc)[C / 32], void* out, int64_t row0,
@@ -536,9 +536,17 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     }
 }
 
+// A token's 64-byte run in LDS rows of R runs: rows of whole 256 bytes start in the same banks, ones of 384 bytes in two
+// places in turn.
+template <int R>
+__device__ __forceinline__ int placed(int run, int token) {
+    static_assert(R % 2 == 0, "rows of 128 bytes or more");
+    return run ^ (R % 4 == 0 ? token & 3 : token >> 1 & 1);
+}
+
 // The same where dy's rows start at whole dwords: dy goes straight into LDS, and both operands are staged the way the
 // product's are.  Rows of both lie whole in LDS; a transposing read takes 64 bytes of four tokens at a time, so a row's
-// 64-byte runs are placed at run ^ (token & 3), which puts the four in different banks.  What lies past the last token or
+// 64-byte runs are placed (`placed`) so that the four lie in different banks.  What lies past the last token or
 // past a tensor's end is zero (the buffers' ranges).
 //
 // A step of TS tokens is TS / 16 parts.  Each part's operands are read a part ahead, and the workgroup meets before the
@@ -553,7 +561,9 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
     constexpr int kRowN = BN * 2, kRowK = BK * 2;                              // bytes of a row in LDS
     constexpr int kLoadRows = 1024 / kRowN;                                    // rows of a wave's direct load
     constexpr int kLoads = TS / kLoadRows / kWaves;
-    constexpr int kX = TS * BK / 16 / kThreads, kXRows = kThreads / (BK / 16); // 16-column pieces of a thread
+    constexpr int P = BK == 192 ? 8 : 16;              // columns of a thread's piece of a's rows
+    constexpr int kX = TS * BK / P / kThreads;
+    static_assert(kX * kThreads * P == TS * BK, "every thread has as many");
     static_assert(kLoadRows == 2 || kLoadRows == 4, "rows of 256 or 512 bytes");
     __shared__ __align__(1024) uint8_t lds[2 * TS * (kRowN + kRowK)];
     auto lds_n = [&](int64_t step) { return lds + (step & 1) * TS * kRowN; };
@@ -583,25 +593,40 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
         const __amdgpu_buffer_rsrc_t rows = buffer_of(a.dy + t0 * a.stride + n0, bytes_n - t0 * row_bytes);
         load_lds(rows, to + g * 1024, from[kLoadRows == 2 ? g & 1 : 0], g * kLoadRows * row_bytes);
     };
-    u4 x[kX];
-    uint32_t xs[kX];
-    const int row_x = threadIdx.x / (BK / 16), col_x = threadIdx.x % (BK / 16) * 16;
-    const int from_q = row_x * a.wide + k0 + col_x, from_s = row_x * a.pitch + (k0 + col_x) / kBlock;
+    uint32_t x[kX][P / 4], xs[kX];
+    int at_q[kX], at_s[kX], at_k[kX];                  // of the pieces: offsets in a step's rows, and in LDS
+#pragma unroll
+    for (int i = 0; i < kX; ++i) {
+        const int e = i * kThreads + threadIdx.x, t = e / (BK / P), c = e % (BK / P) * P;
+        at_q[i] = t * a.wide + k0 + c;
+        at_s[i] = t * a.pitch + (k0 + c) / kBlock;
+        at_k[i] = t * kRowK + (placed<BK / 32>(c >> 5, t) << 6) + (c & 31) * 2;
+    }
     auto fetch = [&](int64_t step, int i) {
         const int64_t t0 = step * TS, left = a.T - t0;
-        x[i] = __builtin_amdgcn_raw_buffer_load_b128(buffer_of(a.q + t0 * a.wide, left * a.wide), from_q,
-                                                     i * kXRows * a.wide, 0);
-        xs[i] = __builtin_amdgcn_raw_buffer_load_b8(buffer_of(a.s + t0 * a.pitch, left * a.pitch), from_s,
-                                                    i * kXRows * a.pitch, 0);
+        const __amdgpu_buffer_rsrc_t rows = buffer_of(a.q + t0 * a.wide, left * a.wide);
+        if constexpr (P == 16) {
+            const u4 v = __builtin_amdgcn_raw_buffer_load_b128(rows, at_q[i], 0, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i][j] = v[j];
+        } else {
+            const u2 v = __builtin_amdgcn_raw_buffer_load_b64(rows, at_q[i], 0, 0);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) x[i][j] = v[j];
+        }
+        xs[i] = __builtin_amdgcn_raw_buffer_load_b8(buffer_of(a.s + t0 * a.pitch, left * a.pitch), at_s[i], 0, 0);
     };
     auto keep = [&](int i, uint8_t* rows) {
-        const int t = row_x + i * kXRows;
         const float f = scale_value(xs[i]);
-        // half of the lanes write their second half first: neighbours' pieces, 32 bytes apart, then differ in their banks
-        const bool flip = (threadIdx.x >> 2 ^ threadIdx.x >> 3) & 1;
-        u4* to = (u4*)(rows + t * kRowK + (((col_x >> 3) ^ ((t & 3) << 2)) << 4));
-        to[flip ? 1 : 0] = open_bf16(flip ? u2{x[i][2], x[i][3]} : u2{x[i][0], x[i][1]}, f);
-        to[flip ? 0 : 1] = open_bf16(flip ? u2{x[i][0], x[i][1]} : u2{x[i][2], x[i][3]}, f);
+        u4* to = (u4*)(rows + at_k[i]);
+        if constexpr (P == 16) {
+            // half of the lanes write their second half first: neighbours' pieces, 32 bytes apart, then differ in banks
+            const bool flip = (threadIdx.x >> 2 ^ threadIdx.x >> 3) & 1;
+            to[flip ? 1 : 0] = open_bf16(flip ? u2{x[i][2], x[i][3]} : u2{x[i][0], x[i][1]}, f);
+            to[flip ? 0 : 1] = open_bf16(flip ? u2{x[i][0], x[i][1]} : u2{x[i][2], x[i][3]}, f);
+        } else {
+            to[0] = open_bf16(u2{x[i][0], x[i][1]}, f);
+        }
     };
 
     // lane -> the token and the four columns whose address it gives to a transposing read
@@ -636,8 +661,8 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
                     if (q * kProducts / kReads != m) continue;
                     const int i = q >> 1, t = token + (kk + 1) * 16 + (q & 1) * 4;
                     const int run = i < NK ? wk / 32 + i : wn / 32 + i - NK;
-                    const uint8_t* at = (i < NK ? from_k + t * kRowK : from_n + t * kRowN) + ((run ^ (p >> 2)) << 6) +
-                                        (i < NK ? col_k : col_n) * 2;
+                    const uint8_t* at = i < NK ? from_k + t * kRowK + (placed<BK / 32>(run, p >> 2) << 6) + col_k * 2
+                                               : from_n + t * kRowN + (placed<BN / 32>(run, p >> 2) << 6) + col_n * 2;
                     f[(kk + 1) & 1][i][q & 1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Z1B_LDS s4*)at);
                 }
                 if (kk < 0) {
@@ -803,22 +828,26 @@ int launch_gradient(const Gradient& a, hipStream_t st) {
     weight_grad_kernel<T, EDGE, BN, BK, WN, WK, TS><<<dim3((unsigned)tiles), BN / WN * (BK / WK) * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
-// How a weight gradient runs: by direct loads where dy's rows are whole dwords, in large tiles, or in small ones with the
+// How a weight gradient runs: by direct loads where dy's rows are whole dwords, in large tiles of 256 x 256 or 256 x 192 (a
+// round of which takes 0.77 of the time: 3072 columns in 12 or 16 tiles, 2048 tokens: 113 or 88 us), or in small ones with the
 // tokens cut into parts where those leave CUs idle (16384 tokens, 512 x 512: 166 us whole, 28 in parts).
 struct GradientWay {
-    bool direct, large;
+    bool direct;
+    int columns;                                       // of a tile
     int parts;
     int64_t per;
 };
 constexpr int kStep = 64;
 GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
-    if (!direct) return {false, false, 1, T};
+    if (!direct) return {false, 128, 1, T};
     const int64_t large = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);
     const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
-    if (100 * large_rounds <= 62 * small_rounds) return {true, true, 1, T};
+    const int64_t middle_rounds = ((N + 255) / 256 * ((K + 191) / 192) + kCus - 1) / kCus;
+    const bool middle = 77 * middle_rounds < 100 * large_rounds;
+    if ((middle ? 77 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds) return {true, middle ? 192 : 256, 1, T};
     const int64_t steps = (T + kStep - 1) / kStep;
     const int parts = parts_of(small, steps, 1, N * K, 650, 1100);
-    return {true, false, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
+    return {true, 128, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
 }
 bool is_direct(const void* dy, int64_t stride) { return stride % 2 == 0 && reinterpret_cast<uintptr_t>(dy) % 4 == 0; }
 
@@ -832,7 +861,8 @@ int launch_direct(const Gradient& a, int parts, hipStream_t st) {
 template <typename T>
 int gradient(Gradient a, const GradientWay& way, float* workspace, hipStream_t st) {
     a.per = way.per;
-    if (way.large) return launch_direct<T, 256, 256, 128, 64>(a, 1, st);
+    if (way.columns == 256) return launch_direct<T, 256, 256, 128, 64>(a, 1, st);
+    if (way.columns == 192) return launch_direct<T, 256, 192, 64, 96>(a, 1, st);
     if (way.direct && way.parts == 1) return launch_direct<T, 128, 128, 64, 64>(a, 1, st);
     if (way.direct) {
         void* dw = a.dw;
