@@ -829,7 +829,7 @@ int launch_gradient(const Gradient& a, hipStream_t st) {
     return (int)hipGetLastError();
 }
 // How a weight gradient runs: by direct loads where dy's rows are whole dwords, in large tiles of 256 x 256 or 256 x 192 (a
-// round of which takes 0.77 of the time: 3072 columns in 12 or 16 tiles, 2048 tokens: 113 or 88 us), or in small ones with the
+// round of which takes 0.87 of the time: 3072 columns in 12 or 16 tiles, 2048 tokens: 112 or 98 us), or in small ones with the
 // tokens cut into parts where those leave CUs idle (16384 tokens, 512 x 512: 166 us whole, 28 in parts).
 struct GradientWay {
     bool direct;
@@ -843,8 +843,8 @@ GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
     const int64_t large = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);
     const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
     const int64_t middle_rounds = ((N + 255) / 256 * ((K + 191) / 192) + kCus - 1) / kCus;
-    const bool middle = 77 * middle_rounds < 100 * large_rounds;
-    if ((middle ? 77 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds) return {true, middle ? 192 : 256, 1, T};
+    const bool middle = 87 * middle_rounds < 100 * large_rounds;
+    if ((middle ? 87 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds) return {true, middle ? 192 : 256, 1, T};
     const int64_t steps = (T + kStep - 1) / kStep;
     const int parts = parts_of(small, steps, 1, N * K, 650, 1100);
     return {true, 128, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
