@@ -9,13 +9,16 @@ namespace {
 using namespace z1blk;
 
 constexpr int kThreads = 256;
-constexpr int kPer = 4;                                // groups of 8 columns to a thread
+constexpr int kPer = 4;                                // most groups of 8 columns to a thread
 constexpr int64_t kMaxRows = 1ll << 40;
 constexpr int64_t kMaxDim = 1 << 24;
+constexpr int64_t kFewBlocks = 1024;                   // of kPer groups a thread
 constexpr int64_t kMaxBlocks = 1ll << 24;              // of a launch: its threads count in 32 bits
 
-// The rows are one run of groups of 8 columns, wide / 8 to a row: a workgroup takes kThreads * kPer of them in turn, and
-// 16 neighbouring lanes always hold one block, since a row is whole blocks.
+// The rows are one run of groups of 8 columns, wide / 8 to a row: a workgroup takes kThreads of them, or kThreads *
+// PER in turn, and 16 neighbouring lanes always hold one block, since a row is whole blocks.  Packing takes one a thread
+// at every size (16384 x 8192 BF16: 75 us, 5.4 TB/s, the same with four; 4099 x 1001: 4.8 us against 6.7), unpacking four
+// for large ones (72 us against 82, and 69, 5.8 TB/s, with stores past the caches; the norms' stores gain nothing by it).
 struct Place {
     int64_t row;
     int c;
@@ -30,40 +33,32 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void act8_pack_kernel(const void* x, int64_t stride, uint8_t* q, uint8_t* s,
                                                              int64_t rows, int dim, int wide, int pitch) {
     const uint32_t per_row = wide / kLane;
-    const int64_t first = (int64_t)blockIdx.x * (kThreads * kPer);
+    const int64_t first = (int64_t)blockIdx.x * kThreads;
     const int64_t row0 = first / per_row;
-    const uint32_t rest = (uint32_t)(first - row0 * per_row);
-    float v[kPer][kLane];
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const Place p = place(row0, rest, k * kThreads + threadIdx.x, per_row);
-        load_row<T>(x, p.row * stride + p.c, p.row < rows ? dim - p.c : 0, v[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const Place p = place(row0, rest, k * kThreads + threadIdx.x, per_row);
-        uint32_t byte;
-        const u2 w = quantize8(v[k], byte);            // every lane
-        if (p.row >= rows) continue;
-        *(Z1B_GLOBAL u2*)(q + p.row * wide + p.c) = w;
-        uint8_t* sr = s + p.row * pitch + p.c / kBlock;
-        if ((p.c & (kBlock - 1)) == 0) *sr = (uint8_t)byte;
-        if (p.c + kLane == wide)
-            for (int j = wide / kBlock; j < pitch; ++j) sr[j - wide / kBlock + 1] = 127;
-    }
+    const Place p = place(row0, (uint32_t)(first - row0 * per_row), threadIdx.x, per_row);
+    float v[kLane];
+    load_row<T>(x, p.row * stride + p.c, p.row < rows ? dim - p.c : 0, v);
+    uint32_t byte;
+    const u2 w = quantize8(v, byte);                   // every lane
+    if (p.row >= rows) return;
+    *(Z1B_GLOBAL u2*)(q + p.row * wide + p.c) = w;
+    uint8_t* sr = s + p.row * pitch + p.c / kBlock;
+    if ((p.c & (kBlock - 1)) == 0) *sr = (uint8_t)byte;
+    if (p.c + kLane == wide)
+        for (int j = wide / kBlock; j < pitch; ++j) sr[j - wide / kBlock + 1] = 127;
 }
 
-template <typename T>
+template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void act8_unpack_kernel(const uint8_t* q, const uint8_t* s, void* out,
                                                                int64_t rows, int dim, int wide, int pitch) {
     const uint32_t per_row = wide / kLane;
-    const int64_t first = (int64_t)blockIdx.x * (kThreads * kPer);
+    const int64_t first = (int64_t)blockIdx.x * (kThreads * PER);
     const int64_t row0 = first / per_row;
     const uint32_t rest = (uint32_t)(first - row0 * per_row);
-    u2 w[kPer];
-    uint32_t byte[kPer];
+    u2 w[PER];
+    uint32_t byte[PER];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
         const Place p = place(row0, rest, k * kThreads + threadIdx.x, per_row);
         if (p.row < rows) {
             w[k] = *(const Z1B_GLOBAL u2*)(q + p.row * wide + p.c);
@@ -71,7 +66,7 @@ __global__ __launch_bounds__(kThreads) void act8_unpack_kernel(const uint8_t* q,
         }
     }
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 0; k < PER; ++k) {
         const Place p = place(row0, rest, k * kThreads + threadIdx.x, per_row);
         if (p.row >= rows || p.c >= dim) continue;
         float v[kLane];
@@ -83,7 +78,8 @@ __global__ __launch_bounds__(kThreads) void act8_unpack_kernel(const uint8_t* q,
             const float x = v[j] * f;
             v[j] = x != x ? x : fminf(fmaxf(x, -T::kMax), T::kMax);
         }
-        store_row<T>(out, p.row * dim + p.c, dim - p.c, v);
+        if (dim - p.c >= kLane) T::stream(out, p.row * dim + p.c, v);
+        else store_row<T>(out, p.row * dim + p.c, dim - p.c, v);
     }
 }
 
@@ -158,11 +154,26 @@ __global__ __launch_bounds__(kThreads) void weight8_pack_kernel(const void* w, i
 
 bool bad_dtype(int d) { return d != Z1_F32 && d != Z1_BF16 && d != Z1_F16; }
 
-int shape(int64_t rows, int64_t dim, int64_t stride, int64_t* blocks) {
+int shape(int64_t rows, int64_t dim, int64_t stride, int64_t* groups) {
     if (rows < 0 || rows > kMaxRows || dim < 1 || dim > kMaxDim || stride < 0) return Z1_E_SIZE;
-    const int64_t per = kThreads * kPer;
-    *blocks = (rows * (wide_of(dim) / kLane) + per - 1) / per;
-    return *blocks > kMaxBlocks ? Z1_E_SIZE : Z1_OK;
+    *groups = rows * (wide_of(dim) / kLane);
+    return *groups > kMaxBlocks * kThreads ? Z1_E_SIZE : Z1_OK;
+}
+
+template <typename T>
+int pack(const void* x, int64_t rows, int64_t dim, int64_t stride, uint8_t* q, uint8_t* s, int64_t groups, hipStream_t st) {
+    const dim3 grid((unsigned)((groups + kThreads - 1) / kThreads));
+    act8_pack_kernel<T><<<grid, kThreads, 0, st>>>(x, stride, q, s, rows, (int)dim, wide_of(dim), pitch_of(dim));
+    return (int)hipGetLastError();
+}
+template <typename T>
+int unpack(const uint8_t* q, const uint8_t* s, int64_t rows, int64_t dim, void* out, int64_t groups, hipStream_t st) {
+    const int d = (int)dim, wide = wide_of(dim), pitch = pitch_of(dim);
+    const int64_t per = groups <= kFewBlocks * kThreads * kPer ? kThreads : kThreads * kPer;
+    const dim3 blocks((unsigned)((groups + per - 1) / per));
+    if (per == kThreads) act8_unpack_kernel<T, 1><<<blocks, kThreads, 0, st>>>(q, s, out, rows, d, wide, pitch);
+    else act8_unpack_kernel<T, kPer><<<blocks, kThreads, 0, st>>>(q, s, out, rows, d, wide, pitch);
+    return (int)hipGetLastError();
 }
 
 }  // namespace
@@ -173,39 +184,33 @@ int64_t z1_act8_columns(int64_t dim) { return dim < 1 || dim > kMaxDim ? Z1_E_SI
 int64_t z1_act8_scales(int64_t dim) { return dim < 1 || dim > kMaxDim ? Z1_E_SIZE : pitch_of(dim); }
 
 int z1_act8_pack(const void* x, int64_t rows, int64_t dim, int64_t stride, int dtype, void* q, void* s, void* stream) {
-    int64_t blocks;
-    if (const int rc = shape(rows, dim, stride, &blocks)) return rc;
+    int64_t groups;
+    if (const int rc = shape(rows, dim, stride, &groups)) return rc;
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (rows == 0) return Z1_OK;
     if (!x || !q || !s) return Z1_E_NULL;
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)blocks);
-    const int wide = wide_of(dim), pitch = pitch_of(dim);
     uint8_t *qb = (uint8_t*)q, *sb = (uint8_t*)s;
     switch (dtype) {
-        case Z1_F32: act8_pack_kernel<F32><<<grid, kThreads, 0, st>>>(x, stride, qb, sb, rows, (int)dim, wide, pitch); break;
-        case Z1_BF16: act8_pack_kernel<BF16><<<grid, kThreads, 0, st>>>(x, stride, qb, sb, rows, (int)dim, wide, pitch); break;
-        default: act8_pack_kernel<F16><<<grid, kThreads, 0, st>>>(x, stride, qb, sb, rows, (int)dim, wide, pitch); break;
+        case Z1_F32: return pack<F32>(x, rows, dim, stride, qb, sb, groups, st);
+        case Z1_BF16: return pack<BF16>(x, rows, dim, stride, qb, sb, groups, st);
+        default: return pack<F16>(x, rows, dim, stride, qb, sb, groups, st);
     }
-    return (int)hipGetLastError();
 }
 
 int z1_act8_unpack(const void* q, const void* s, int64_t rows, int64_t dim, void* out, int dtype, void* stream) {
-    int64_t blocks;
-    if (const int rc = shape(rows, dim, 0, &blocks)) return rc;
+    int64_t groups;
+    if (const int rc = shape(rows, dim, 0, &groups)) return rc;
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (rows == 0) return Z1_OK;
     if (!q || !s || !out) return Z1_E_NULL;
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)blocks);
-    const int wide = wide_of(dim), pitch = pitch_of(dim);
     const uint8_t *qb = (const uint8_t*)q, *sb = (const uint8_t*)s;
     switch (dtype) {
-        case Z1_F32: act8_unpack_kernel<F32><<<grid, kThreads, 0, st>>>(qb, sb, out, rows, (int)dim, wide, pitch); break;
-        case Z1_BF16: act8_unpack_kernel<BF16><<<grid, kThreads, 0, st>>>(qb, sb, out, rows, (int)dim, wide, pitch); break;
-        default: act8_unpack_kernel<F16><<<grid, kThreads, 0, st>>>(qb, sb, out, rows, (int)dim, wide, pitch); break;
+        case Z1_F32: return unpack<F32>(qb, sb, rows, dim, out, groups, st);
+        case Z1_BF16: return unpack<BF16>(qb, sb, rows, dim, out, groups, st);
+        default: return unpack<F16>(qb, sb, rows, dim, out, groups, st);
     }
-    return (int)hipGetLastError();
 }
 
 int z1_weight8_pack(const void* w, int64_t N, int64_t K, int64_t stride, int dtype, void* q, void* s, void* qt, void* st,

@@ -54,6 +54,12 @@ struct F32 {
         q[0] = a;
         q[1] = b;
     }
+    // past the caches
+    static __device__ __forceinline__ void stream(void* p, int64_t i, const float* v) {
+        Z1B_GLOBAL f4_any4* q = (Z1B_GLOBAL f4_any4*)((float*)p + i);
+        __builtin_nontemporal_store((f4_any4)f4{v[0], v[1], v[2], v[3]}, q);
+        __builtin_nontemporal_store((f4_any4)f4{v[4], v[5], v[6], v[7]}, q + 1);
+    }
     static __device__ __forceinline__ void put(void* p, int64_t i, float v) { ((Z1B_GLOBAL float*)p)[i] = v; }
     // eight elements to a row in LDS from element i (a multiple of 8) on, and from there to memory
     static __device__ __forceinline__ void store_local(uint8_t* row, int i, const float* v) {
@@ -95,6 +101,9 @@ struct BF16 {
     static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
         *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + i) = close(v);
     }
+    static __device__ __forceinline__ void stream(void* p, int64_t i, const float* v) {
+        __builtin_nontemporal_store((u4_any2)close(v), (Z1B_GLOBAL u4_any2*)((uint16_t*)p + i));
+    }
     static __device__ __forceinline__ void store_local(uint8_t* row, int i, const float* v) { *(u4*)(row + i * 2) = close(v); }
     static __device__ __forceinline__ void copy_local(void* p, int64_t at, const uint8_t* row, int i) {
         *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + at) = *(const u4*)(row + i * 2);
@@ -129,6 +138,9 @@ struct F16 {
     }
     static __device__ __forceinline__ void store(void* p, int64_t i, const float* v) {
         *(Z1B_GLOBAL u4_any2*)((uint16_t*)p + i) = close(v);
+    }
+    static __device__ __forceinline__ void stream(void* p, int64_t i, const float* v) {
+        __builtin_nontemporal_store((u4_any2)close(v), (Z1B_GLOBAL u4_any2*)((uint16_t*)p + i));
     }
     static __device__ __forceinline__ void store_local(uint8_t* row, int i, const float* v) { *(u4*)(row + i * 2) = close(v); }
     static __device__ __forceinline__ void copy_local(void* p, int64_t at, const uint8_t* row, int i) {

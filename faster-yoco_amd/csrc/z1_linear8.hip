@@ -117,9 +117,12 @@ struct Flush {
     }
 };
 
-// All waves of the workgroup are here, their direct loads into LDS have arrived and their reads from it are done.
+// All waves of the workgroup are here, their reads from LDS are done, and of their loads all but the LATER last ones have
+// arrived, direct loads into LDS among them.
+template <int LATER = 0>
 __device__ __forceinline__ void meet() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    static_assert(LATER < 64, "the counter's range");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LATER) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
@@ -155,13 +158,15 @@ struct Product {
 __device__ __forceinline__ int key_plain(int row) { return row >> 1 & 7; }
 __device__ __forceinline__ int key_spread(int row) { return (row >> 1 & 3) | (row >> 4 & 1) << 2; }
 
-// BT x BO outputs (tokens x outputs) of a workgroup, WT x WO of a wave.
-template <typename T, bool PRECISE, int BT, int BO, int WT, int WO>
+// BT x BO outputs (tokens x outputs) of a workgroup, WT x WO of a wave, S blocks of K staged: two leave room for a second
+// workgroup on a CU, four cover the loads' way where there is no second one.
+template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
 __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Product a) {
     constexpr int kWaves = BT / WT * (BO / WO);
     constexpr int kPT = BT / 8 / kWaves, kPO = BO / 8 / kWaves;                // direct loads of a wave: 8 rows each
     constexpr int NT = WT / 32, NO = WO / 32;
-    __shared__ __align__(1024) uint8_t lds[2][(BT + BO) * kBlock];
+    static_assert(S == 2 || S == 4, "a block's buffer is kb & (S - 1)");
+    __shared__ __align__(1024) uint8_t lds[S][(BT + BO) * kBlock];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_o = (a.N + BO - 1) / BO;
     const int64_t t0 = (int64_t)(blockIdx.x / tiles_o) * BT;
@@ -182,7 +187,7 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     const int sub = lane >> 3, piece = lane & 7;
     const int from = sub * wide + ((piece ^ (sub >> 1)) << 4);                 // in 8 rows whose keys' third bit is 0
     auto stage = [&](int kb, int i) {                  // the i-th direct load of this wave's part of a block
-        uint8_t* buf = lds[kb & 1];
+        uint8_t* buf = lds[kb & (S - 1)];
         const int g = i < kPT ? wave * kPT + i : wave * kPO + i - kPT;
         const int at = g * 8 * wide + kb * kBlock;
         if (i < kPT) load_lds(buf_t, buf + g * 8 * kBlock, g & 1 ? from ^ 64 : from, at);
@@ -210,15 +215,15 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
 
     // A block's two halves of 64 columns are read ahead by one half, and the workgroup meets between them: what follows
     // the meeting -- the next block's first reads, the direct loads into the buffer that has just been read -- runs beside
-    // the second half's products, one read or load after each, and what it waits for was issued a whole block before.
+    // the second half's products, one read or load after each, and what it waits for was issued S - 1 blocks before.
     // (All loads at once after the meeting hold up the products until the address unit has taken them: 64 loads of 16
     // cycles.)  Past the last block the reads and loads are of no use, and in bounds.
     constexpr int kReads = 2 * (NT + NO), kLoads = kPT + kPO, kProducts = NT * NO;
     i4 f[2][NT + NO][2];
     auto read = [&](int kb, int h, int q) {
         const int i = q >> 1, p = 4 * h + 2 * half + (q & 1);
-        const uint8_t* row = i < NT ? lds[kb & 1] + (wt + i * 32 + r32) * kBlock
-                                    : lds[kb & 1] + (BT + wo + (i - NT) * 32 + rs) * kBlock;
+        const uint8_t* row = i < NT ? lds[kb & (S - 1)] + (wt + i * 32 + r32) * kBlock
+                                    : lds[kb & (S - 1)] + (BT + wo + (i - NT) * 32 + rs) * kBlock;
         f[h][i][q & 1] = *(const i4*)(row + ((p ^ (i < NT ? key_plain(r32) : key_spread(rs))) << 4));
     };
     // products of half h; beside them, the reads of half 1 - h of block kb_read and the loads of block kb_load (< 0: none)
@@ -251,10 +256,12 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
         }
     };
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) stage(0, i);
-    meet();
+    for (int kb = 0; kb < S - 1; ++kb)
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) stage(1, i);
+        for (int i = 0; i < kLoads; ++i) stage(kb, i);
+    meet<(S - 2) * kLoads>();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) stage(S - 1, i);
 #pragma unroll
     for (int q = 0; q < kReads; ++q) read(0, 0, q);
     for (int kb = 0; kb < blocks; ++kb) {
@@ -265,8 +272,8 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
             scales(kb + 4 < blocks ? kb + 4 : 0);
         }
         products(0, kb, -1);
-        meet();                                        // block kb has been read, block kb + 1 has arrived
-        products(1, kb + 1, kb + 2);
+        meet<(S - 2) * kLoads>();                      // block kb has been read, block kb + 1 has arrived
+        products(1, kb + 1, kb + S);
 #pragma unroll
         for (int j = 0; j < NT; ++j) now[j] >>= 8;
         now_w >>= 8;
@@ -771,11 +778,11 @@ Way product_way(int64_t M, int64_t N, int blocks, bool precise) {
     return {false, false, parts, parts == 1 ? blocks : (blocks + 4 * parts - 1) / (4 * parts) * 4};
 }
 
-template <typename T, bool PRECISE, int BT, int BO, int WT, int WO>
+template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
 int launch_tiles(const Product& a, int parts, hipStream_t st) {
     const int64_t tiles = (a.M + BT - 1) / BT * ((a.N + BO - 1) / BO);
     if (tiles > kMaxTiles) return Z1_E_SIZE;
-    product_kernel<T, PRECISE, BT, BO, WT, WO><<<dim3((unsigned)tiles, parts), BT / WT * (BO / WO) * 64, 0, st>>>(a);
+    product_kernel<T, PRECISE, BT, BO, WT, WO, S><<<dim3((unsigned)tiles, parts), BT / WT * (BO / WO) * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 
@@ -791,18 +798,25 @@ int launch_few(const Product& a, hipStream_t st) {
 }
 
 template <typename T, bool PRECISE>
+int launch_small(const Product& a, int parts, hipStream_t st) {
+    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 127) / 128) * parts;
+    return tiles <= kCus ? launch_tiles<T, PRECISE, 128, 128, 64, 64, 4>(a, parts, st)
+                         : launch_tiles<T, PRECISE, 128, 128, 64, 64, 2>(a, parts, st);
+}
+
+template <typename T, bool PRECISE>
 int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) {
     if (a.M <= 8) return launch_few<T, PRECISE, 8>(a, st);
     if (a.M <= 16) return launch_few<T, PRECISE, 16>(a, st);
     if (way.few) return launch_few<T, PRECISE, 32>(a, st);
     a.per = way.per;
     if constexpr (!PRECISE) {
-        if (way.large) return launch_tiles<T, PRECISE, 256, 256, 64, 128>(a, 1, st);
+        if (way.large) return launch_tiles<T, PRECISE, 256, 256, 64, 128, 2>(a, 1, st);
     }
-    if (way.parts == 1) return launch_tiles<T, PRECISE, 128, 128, 64, 64>(a, 1, st);
+    if (way.parts == 1) return launch_small<T, PRECISE>(a, 1, st);
     void* y = a.y;
     a.y = workspace;
-    if (const int rc = launch_tiles<F32, PRECISE, 128, 128, 64, 64>(a, way.parts, st)) return rc;
+    if (const int rc = launch_small<F32, PRECISE>(a, way.parts, st)) return rc;
     return join<T>(workspace, way.parts, a.M * a.N, y, st);
 }
 
