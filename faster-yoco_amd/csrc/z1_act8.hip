@@ -13,7 +13,7 @@ constexpr int kPer = 4;                                // most groups of 8 colum
 constexpr int64_t kMaxRows = 1ll << 40;
 constexpr int64_t kMaxDim = 1 << 24;
 constexpr int64_t kFewBlocks = 1024;                   // of kPer groups a thread
-constexpr int64_t kMaxBlocks = 1ll << 24;              // of a launch: its threads count in 32 bits
+constexpr int64_t kMaxBlocks = (1ll << 24) - 1;        // of a launch: its threads count in 32 bits
 
 // The rows are one run of groups of 8 columns, wide / 8 to a row: a workgroup takes kThreads of them, or kThreads *
 // PER in turn, and 16 neighbouring lanes always hold one block, since a row is whole blocks.  Packing takes one a thread

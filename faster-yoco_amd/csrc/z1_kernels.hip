@@ -1683,9 +1683,9 @@ const char* z1_strerror(int code) {
         case Z1_OK: return "ok";
         case Z1_E_NULL: return "a required pointer is NULL";
         case Z1_E_SIZE: return "invalid element count";
-        case Z1_E_DTYPE: return "unknown gradient dtype";
+        case Z1_E_DTYPE: return "unknown dtype";
         case Z1_E_WORLD: return "world outside 1..Z1_MAX_WORLD";
-        case Z1_E_MODE: return "Adam mode must be 0 or 1";
+        case Z1_E_MODE: return "a mode must be 0 or 1";
         case Z1_E_WORKSPACE: return "workspace too small";
         case Z1_E_DEVICE: return "table used on another device than it was created on";
         case Z1_E_NOALLOC_MAX: return "more than Z1_NOALLOC_MAX_N elements for the no-allocation entry point";

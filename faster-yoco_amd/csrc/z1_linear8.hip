@@ -392,7 +392,7 @@ __device__ __forceinline__ u4 shift_pieces(u4 v, int n) {
 // into those registers: a load has a whole step to arrive, and neither staging nor opening stands between two steps.  The
 // loop has no branch (a branch around a load makes the waits for all of them complete): the first step has the rows that
 // do not fill one, every other is full, and past the last one the same rows are loaded again and not used.
-enum Edge { kWhole, kCut, kFew };                      // N a multiple of 8; not, but at least 8; less than 8
+enum Edge { kCut, kFew };                              // N is at least 8, or less
 template <typename T, Edge EDGE, int BN, int BK, int WN, int WK, int TS>
 __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(Gradient a) {
     constexpr int kThreads = BN / WN * (BK / WK) * 64;
@@ -593,7 +593,8 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(from) / sizeof(int)); ++i)
         from[i] = sub * row_bytes + ((piece ^ (((i * kLoadRows + sub) & 3) << 2)) << 4);
-    const int64_t bytes_n = (a.T - 1) * row_bytes + (a.N - n0) * 2;            // from the tile's first column to dy's end
+    // from the tile's first column to dy's end, in whole dwords (an odd N's last one holds nothing that is used)
+    const int64_t bytes_n = a.T > 0 ? (a.T - 1) * row_bytes + ((a.N - n0 + 1) & ~1) * 2 : 0;
     auto stage = [&](int64_t step, int i, uint8_t* to) {
         const int64_t t0 = step * TS;
         const int g = wave * kLoads + i;
@@ -863,7 +864,10 @@ GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
     const int parts = parts_of(small, steps, 1, N * K, 650, 1100);
     return {true, 128, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
 }
-bool is_direct(const void* dy, int64_t stride) { return stride % 2 == 0 && reinterpret_cast<uintptr_t>(dy) % 4 == 0; }
+// Rows of whole dwords that do not overlap: a row past the last then lies past the buffer's range.
+bool is_direct(const void* dy, int64_t stride, int64_t N) {
+    return stride % 2 == 0 && stride >= N && reinterpret_cast<uintptr_t>(dy) % 4 == 0;
+}
 
 template <typename T, int BN, int BK, int WN, int WK>
 int launch_direct(const Gradient& a, int parts, hipStream_t st) {
@@ -934,7 +938,7 @@ int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const voi
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (N == 0) return Z1_OK;
     if (!dw || (T > 0 && (!dy || !q || !s))) return Z1_E_NULL;
-    const GradientWay way = gradient_way(T, N, K, is_direct(dy, stride));
+    const GradientWay way = gradient_way(T, N, K, is_direct(dy, stride, N));
     if (way.parts > 1) {
         if (!workspace) return Z1_E_NULL;
         if (workspace_floats < way.parts * N * K) return Z1_E_WORKSPACE;

@@ -30,7 +30,7 @@ enum {
     Z1_OK = 0,
     Z1_E_NULL = -1,        /* a required pointer is NULL */
     Z1_E_SIZE = -2,        /* a negative or inconsistent element count */
-    Z1_E_DTYPE = -3,       /* unknown gradient dtype code */
+    Z1_E_DTYPE = -3,       /* unknown dtype code */
     Z1_E_WORLD = -4,       /* world outside 1..Z1_MAX_WORLD */
     Z1_E_MODE = -5,        /* Adam mode other than 0 or 1 */
     Z1_E_WORKSPACE = -6,   /* workspace too small */

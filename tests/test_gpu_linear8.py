@@ -159,6 +159,36 @@ def test_gradient_rows_of_any_stride(pkg, dev):
     assert torch.equal(linear8.weight_grad(base[:, :640].reshape(9, 10, 640), a), linear8.weight_grad(base[:, :640].contiguous(), a))
 
 
+@pytest.mark.parametrize('T', [1, 63, 130])
+def test_gradient_rows_of_whole_dwords_and_odd_width(pkg, dev, T):
+    """The last row's last element shares its dword with what lies behind the tensor."""
+    from faster_yoco_amd import act8, linear8
+    a, base = act8.pack(rows(T, 200, 41).to(dev)), rows(T, 800, 42).to(dev)
+    for n in (1, 7, 129, 333, 799):
+        dy = base[:, :n]
+        assert torch.equal(linear8.weight_grad(dy, a), linear8.weight_grad(dy.contiguous(), a))
+        assert linear8.weight_grad(dy, a)[-1].any()
+
+
+def test_gradient_of_one_row_for_all_tokens(pkg, dev):
+    """Rows a stride of zero apart, not finite in places: only what they enter is."""
+    from faster_yoco_amd import act8, linear8
+    x = rows(70, 200, 43).abs().to(dev) + 1
+    row = rows(1, 300, 44).to(dev)
+    row[0, 5] = float('inf')
+    dw = linear8.weight_grad(row.expand(70, 300), act8.pack(x), torch.float32)
+    assert torch.equal(dw, linear8.weight_grad(row.repeat(70, 1), act8.pack(x), torch.float32))
+    assert (dw[5] == float('inf')).all() and dw[:5].isfinite().all() and dw[6:].isfinite().all()
+
+
+def test_gradient_of_no_tokens(pkg, dev):
+    from faster_yoco_amd import act8, linear8
+    a = act8.pack(rows(4, 200, 45).to(dev))
+    none = act8.Act8(a.q[:0], a.s[:0], 200)
+    for dy in (torch.empty(0, 300), torch.empty(0, 301), torch.empty(1, 300).expand(1, 300)[:0]):
+        assert torch.equal(linear8.weight_grad(dy.bfloat16().to(dev), none), torch.zeros(dy.shape[1], 200, dtype=torch.bfloat16, device=dev))
+
+
 def test_linear_is_its_three_products(pkg, dev):
     from faster_yoco_amd import act8, linear8
     x = rows(96, 384, 13).to(dev).view(4, 24, 384).requires_grad_()
