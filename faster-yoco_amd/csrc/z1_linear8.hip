@@ -50,9 +50,9 @@ __device__ __forceinline__ f16 multiply(f16 acc, i8 fo, i8 ft, uint32_t so, uint
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fo, ft, acc, kE4M3, kE4M3, 0, (int)so, 0, (int)st);
 }
 template <int NO, int NT>
-__device__ __forceinline__ void multiply_precise(f16 (&acc)[NO][NT], const i8 (&fo)[NO], const i8 (&ft)[NT], uint32_t so,
-                                                 const uint32_t (&st)[NT]) {
-    const float go = scale_value(so & 0xffu);
+__device__ __forceinline__ void multiply_precise(f16 (&acc)[NO][NT], const i8 (&fo)[NO], const i8 (&ft)[NT],
+                                                 const uint32_t (&so)[1], const uint32_t (&st)[NT]) {
+    const float go = scale_value(so[0] & 0xffu);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {                      // 8 bytes of a lane: 16 columns of the wave
         u4 bo[NO], bt[NT];
@@ -196,14 +196,21 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     // scales: four blocks' bytes at a time, the next four loaded ahead
     const __amdgpu_buffer_rsrc_t buf_s = buffer_of(a.as + t0 * a.pitch, (a.M - t0) * a.pitch - kb0);
     const int r32 = lane & 31, half = lane >> 5, rs = spread(r32);
-    const int ob = (o0 + wo) / kBlock, ob_last = (a.N - 1) / kBlock;
-    const uint32_t* sw = (const uint32_t*)(a.ws + (int64_t)(ob < ob_last ? ob : ob_last) * a.pitch);
-    uint32_t now[NT] = {}, next[NT], now_w = 0, next_w;
+    // a wave of 64 or 128 outputs lies in one block of the weight, one of 96 in two
+    constexpr int NB = WO == 96 ? NO : 1;
+    __amdgpu_buffer_rsrc_t sw[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int ob = (o0 + wo + i * 32) / kBlock, last = (a.N - 1) / kBlock;
+        sw[i] = buffer_of(a.ws + (int64_t)(ob < last ? ob : last) * a.pitch, a.pitch - kb0);
+    }
+    uint32_t now[NT] = {}, next[NT], now_w[NB] = {}, next_w[NB];
     auto scales = [&](int kb) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
             next[j] = __builtin_amdgcn_raw_buffer_load_b32(buf_s, r32 * a.pitch, (wt + j * 32) * a.pitch + kb, 0);
-        next_w = sw[kb / 4];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) next_w[i] = __builtin_amdgcn_raw_buffer_load_b32(sw[i], 0, kb, 0);
     };
     scales(0);
 
@@ -249,7 +256,7 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
 #pragma unroll
             for (int m = 0; m < kProducts; ++m) {
                 const int i = m / NT, j = m % NT;
-                acc[i][j] = multiply(acc[i][j], pair(NT + i), pair(j), now_w, now[j]);
+                acc[i][j] = multiply(acc[i][j], pair(NT + i), pair(j), now_w[NB == 1 ? 0 : i], now[j]);
                 beside(m, kProducts);
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -264,19 +271,23 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     for (int i = 0; i < kLoads; ++i) stage(S - 1, i);
 #pragma unroll
     for (int q = 0; q < kReads; ++q) read(0, 0, q);
-    for (int kb = 0; kb < blocks; ++kb) {
-        if ((kb & 3) == 0) {
+    for (int kb4 = 0; kb4 < blocks; kb4 += 4) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) now[j] = next[j];
-            now_w = next_w;
-            scales(kb + 4 < blocks ? kb + 4 : 0);
+        for (int j = 0; j < NT; ++j) now[j] = next[j];
+#pragma unroll
+        for (int i = 0; i < NB; ++i) now_w[i] = next_w[i];
+        scales(kb4 + 4 < blocks ? kb4 + 4 : 0);
+        const int end = kb4 + 4 < blocks ? kb4 + 4 : blocks;
+#pragma unroll 1
+        for (int kb = kb4; kb < end; ++kb) {
+            products(0, kb, -1);
+            meet<(S - 2) * kLoads>();                  // block kb has been read, block kb + 1 has arrived
+            products(1, kb + 1, kb + S);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) now[j] >>= 8;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) now_w[i] >>= 8;
         }
-        products(0, kb, -1);
-        meet<(S - 2) * kLoads>();                      // block kb has been read, block kb + 1 has arrived
-        products(1, kb + 1, kb + S);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) now[j] >>= 8;
-        now_w >>= 8;
     }
     meet();                                            // the staging buffers are free
     constexpr int kRoom = (int)sizeof(lds) / kWaves;
@@ -290,72 +301,114 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     }
 }
 
-// Few rows: the weight is read once, straight into the matrix instructions' registers, by workgroups of OB outputs whose
-// waves share K and whose sums meet in LDS; OB rows at most.  With OB 8 or 16 the instruction's 32 rows and columns
-// are 32 / OB groups, each of the same outputs and rows with a block of K of its own: the results on its diagonal are that
-// many partial sums, so that an output range of 8 keeps all lanes loading and there are workgroups for all CUs (8192 x
-// 3072, one row: 1024 of 8 outputs).  A wave has the loads of U steps under way together.
-constexpr int kFewWaves = 8;
-template <typename T, bool PRECISE, int OB, int U>
-__global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(Product a) {
-    constexpr int G = 32 / OB;                         // blocks of K to an instruction
-    __shared__ float sums[kFewWaves][32 * 33];
+// Few rows: the weight is read once by workgroups of OB outputs whose waves share K and whose sums meet in LDS; R * OB rows
+// at most.  With OB 8 or 16 the instruction's 32 rows and columns are 32 / OB groups, each of the same outputs and rows with
+// a block of K of its own: the results on its diagonal are that many partial sums, so that a narrow output has workgroups for
+// all CUs.  A wave stages its own steps by direct loads, two under way: a lane's 16 bytes lie beside its neighbours', where
+// fragments loaded into registers would be pieces of 32 rows to an instruction.
+constexpr int few_waves(int R) { return R == 4 ? 3 : 4; }                      // what LDS has room for
+template <typename T, bool PRECISE, int OB, int R>
+__global__ __launch_bounds__(few_waves(R) * 64) void product_few_kernel(Product a) {
+    static_assert(R == 1 || OB == 32, "more row fragments than one are whole ones");
+    constexpr int G = 32 / OB, U = 2, W = few_waves(R);                        // blocks of K to an instruction; steps under way
+    constexpr int kRows = 32 * kBlock;                 // bytes: 32 rows of the weight, R times 32 of a, and their scales
+    constexpr int kScales = (1 + R) * kRows, kStep = kScales + (1 + R) * 256, kStepLoads = (1 + R) * 5;
+    __shared__ __align__(1024) uint8_t lds[W][U][kStep];
+    static_assert(U * kStep >= R * 32 * 33 * (int)sizeof(float), "a wave's sums take its staging's place");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int o0 = blockIdx.x * OB, r32 = lane & 31, half = lane >> 5, g = r32 / OB;
-    int o = o0 + r32 % OB;
-    o = o < a.N ? o : a.N - 1;
-    const uint8_t* pw = a.w + o * a.wide + half * 32;
-    const uint8_t* sw = a.ws + (int64_t)(o0 / kBlock) * a.pitch;
-    int64_t t = r32 % OB;
-    t = t < a.M ? t : a.M - 1;
-    const uint8_t* pa = a.a + t * a.wide + half * 32;
-    const uint8_t* sa = a.as + t * a.pitch;
-    f16 acc[1][1] = {};
-    const int steps = (a.blocks + G - 1) / G;
-    for (int first = wave; first < steps; first += kFewWaves * U) {
-        i4 w[U][4], x[U][4];
-        uint32_t ew[U], ex[U];
+    const int sub = lane >> 3, piece = lane & 7, last_row = (int)a.M - 1;
+    const int64_t wide = a.wide;
+    const uint8_t* from[1 + R][4];                     // a lane's 16 bytes of 8 rows, in the first block
+    const uint8_t* scale[1 + R];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (first + u * kFewWaves >= steps) continue;
-            int kb = (first + u * kFewWaves) * G + g;
-            kb = kb < a.blocks ? kb : a.blocks - 1;    // past K's end: the last block, times nothing
-            ew[u] = sw[kb];
-            ex[u] = sa[kb];
+    for (int j = 0; j <= R; ++j) {                     // rows past the end repeat the last one and are not used
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int64_t at = (int64_t)kb * kBlock + (q >> 1) * 64 + (q & 1) * 16;
-                w[u][q] = *(const Z1B_GLOBAL i4*)(pw + at);
-                x[u][q] = *(const Z1B_GLOBAL i4*)(pa + at);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const int row = 8 * i + sub, o = o0 + row % OB, t = (j - 1) * 32 + row % OB;
+            const uint8_t* p = j == 0 ? a.w + (o < a.N ? o : a.N - 1) * wide : a.a + (t < last_row ? t : last_row) * wide;
+            from[j][i] = p + ((piece ^ key_plain(row)) << 4);
         }
-        __builtin_amdgcn_sched_barrier(0);             // the compiler would load each step when it comes to it
+        const int t = (j - 1) * 32 + r32 % OB;
+        scale[j] = j == 0 ? a.ws + (int64_t)(o0 / kBlock) * a.pitch : a.as + (t < last_row ? t : last_row) * a.pitch;
+    }
+    const int steps = (a.blocks + G - 1) / G, last = a.blocks - 1;
+    auto stage = [&](int step, uint8_t* to) {          // past K's end: the last block, not used
+        int kb = step * G + g;
+        kb = (kb < last ? kb : last) & ~3;             // the dword that holds the lane's scale
+#pragma unroll
+        for (int j = 0; j <= R; ++j) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = step * G + i * 8 / OB;
+                __builtin_amdgcn_global_load_lds((const Z1B_GLOBAL void*)(from[j][i] + (int64_t)(k < last ? k : last) * kBlock),
+                                                 (Z1B_LDS void*)(to + j * kRows + i * 1024), 16, 0, 0);
+            }
+            __builtin_amdgcn_global_load_lds((const Z1B_GLOBAL void*)(scale[j] + kb),
+                                             (Z1B_LDS void*)(to + kScales + j * 256), 4, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);             // a step's loads stay together: the waits count them
+    };
+    f16 acc[1][R] = {};
+#pragma unroll
+    for (int u = 0; u < U; ++u) stage(wave + u * W, lds[wave][u]);
+    for (int first = wave; first < steps; first += W * U) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            if (first + u * kFewWaves >= steps) continue;
-            const bool in = (first + u * kFewWaves) * G + g < a.blocks;
+            const int step = first + u * W, kb = step * G + g;         // the lane's block
+            uint8_t* own = lds[wave][u];
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((U - 1) * kStepLoads) : "memory");
+            i4 f[1 + R][4];
+            uint32_t e[1 + R];
+#pragma unroll
+            for (int j = 0; j <= R; ++j) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    f[j][q] = *(const i4*)(own + j * kRows + r32 * kBlock +
+                                           (((q >> 1) * 4 + half * 2 + (q & 1)) ^ key_plain(r32)) * 16);
+                e[j] = ((const uint32_t*)(own + kScales + j * 256))[lane] >> (8 * (kb & 3));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                 // read, before it is overwritten
+            __builtin_amdgcn_sched_barrier(0);
+            stage(step + W * U, own);
+            const uint32_t so[1] = {e[0]};
+            uint32_t st[R];
+#pragma unroll
+            for (int j = 0; j < R; ++j) st[j] = e[1 + j];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const i8 fw[1] = {__builtin_shufflevector(w[u][2 * h], w[u][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7)};
-                i8 fx[1] = {__builtin_shufflevector(x[u][2 * h], x[u][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7)};
-                fx[0] = in ? fx[0] : i8{};
-                const uint32_t sx[1] = {ex[u]};
-                if constexpr (PRECISE) multiply_precise(acc, fw, fx, ew[u], sx);
-                else acc[0][0] = multiply(acc[0][0], fw[0], fx[0], ew[u], ex[u]);
+                auto pair = [&](int j) {
+                    const i8 v = __builtin_shufflevector(f[j][2 * h], f[j][2 * h + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                    return j == 0 || kb <= last ? v : i8{};                    // past K's end: times nothing
+                };
+                const i8 fw[1] = {pair(0)};
+                i8 fx[R];
+#pragma unroll
+                for (int j = 0; j < R; ++j) fx[j] = pair(1 + j);
+                if constexpr (PRECISE) {
+                    multiply_precise(acc, fw, fx, so, st);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < R; ++j) acc[0][j] = multiply(acc[0][j], fw[0], fx[j], so[0], st[j]);
+                }
             }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // nothing more arrives where the sums go
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sums[wave][r32 * 33 + 8 * (i >> 2) + 4 * half + (i & 3)] = acc[0][0][i];
+    for (int j = 0; j < R; ++j)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            ((float*)lds[wave])[(j * 32 + r32) * 33 + 8 * (i >> 2) + 4 * half + (i & 3)] = acc[0][j][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < OB * OB; e += kFewWaves * 64) {
-        const int row = e / OB, c = e % OB;
-        if (row >= a.M || o0 + c >= a.N) continue;
+    for (int n = threadIdx.x; n < R * OB * OB; n += W * 64) {
+        const int row = n / OB, c = n % OB;
+        if (row > last_row || o0 + c >= a.N) continue;
         float v = 0.0f;
 #pragma unroll
         for (int k = 0; k < G; ++k)
 #pragma unroll
-            for (int i = 0; i < kFewWaves; ++i) v += sums[i][(k * OB + row) * 33 + k * OB + c];
+            for (int i = 0; i < W; ++i) v += ((const float*)lds[i])[(k * OB + row) * 33 + k * OB + c];
         T::put(a.y, (int64_t)row * a.N + o0 + c, v);
     }
 }
@@ -716,14 +769,15 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
 
 constexpr int64_t kMaxRows = 1ll << 40;
 constexpr int64_t kMaxDim = 1 << 24;
-constexpr int kMaxParts = 16;
+constexpr int kMaxParts = 64;
 constexpr int64_t kMaxTiles = 1ll << 22;               // of a launch: its threads count in 32 bits
 
 bool bad_dtype(int d) { return d != Z1_F32 && d != Z1_BF16 && d != Z1_F16; }
 
 constexpr int kCus = 256;
 
-// The sum of `parts` partial results, in order.
+// The sum of `parts` partial results, in order: bound by their way through the last cache (four of 128 x 3072: 2.5 us and
+// their bytes at 5 TB/s).
 constexpr int kJoinThreads = 256;
 template <typename T>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* part, int parts, int64_t count, void* out) {
@@ -731,6 +785,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float* part, i
     if (i >= count) return;
     const int n = count - i < kLane ? (int)(count - i) : kLane;
     float s[kLane] = {};
+#pragma unroll 8
     for (int p = 0; p < parts; ++p) {
         float v[kLane];
         load_row<F32>(part, p * count + i, n, v);
@@ -747,36 +802,51 @@ int join(const float* part, int parts, int64_t count, void* out, hipStream_t st)
 }
 
 // The number of parts into which the long axis of a product in small tiles is cut, `steps` of it in multiples of `unit`:
-// the one with the least estimate of the time in ns.  A step takes `alone` where a CU has one tile, `shared` where it has
-// two; the joining launch takes 4.5 us (its own and the launch's) and the partial results' way out and back at 4 bytes/ps.
-int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int alone, int shared) {
-    if (tiles > kCus) return 1;
+// the one with the least estimate of the time, which *ns is.  A step takes `alone` where a CU has one tile, `shared` where
+// it has two; joining takes 2.5 us and 0.05 a part, and the partial results' way out and back at 5 bytes/ps.
+int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int alone, int shared, int64_t* ns) {
     int best = 1;
-    int64_t least = 0;
+    *ns = 0;
     for (int p = 1; p <= kMaxParts; ++p) {
         const int64_t per = (steps + p * unit - 1) / (p * unit) * unit;
         if (p > 1 && (per * (p - 1) >= steps || tiles * p > 2 * kCus)) continue;       // a part without steps; no room
-        const int64_t time = per * (tiles * p <= kCus ? alone : shared) + (p > 1 ? 4500 + p * results * 8 / 4000 : 0);
-        if (p == 1 || time < least) best = p, least = time;
+        const int64_t time = per * (tiles * p <= kCus ? alone : shared) + (p > 1 ? 2500 + p * (50 + results * 8 / 5000) : 0);
+        if (p == 1 || time < *ns) best = p, *ns = time;
     }
     return best;
 }
 
-// How a product runs.  Large tiles move fewer bytes per product (8192 x 8192 x 8192: 422 us against 553), small ones leave
-// fewer CUs without work; a CU takes one large tile at a time, or two small ones in 0.65 of its time, and the fewer rounds
-// win.  Where even small tiles leave CUs idle, a long K is cut into parts, joined by a second launch (8192 -> 3072, 128
-// rows: 44 us whole, 20 in parts; 3072 -> 8192: 19 and 19).
+// How a product runs.  Large tiles (256 x 256) move fewer bytes per product, smaller ones leave fewer CUs without work.  A
+// round of large ones, one to a CU, takes 100; of small ones (128 x 128), two to a CU, 63; of 128 x 192, one to a CU, 55 (a
+// block of K of 8192 -> 3072 with 2048 rows: 384 small tiles in 54.0 us, 256 of 128 x 192 in 47.4; with 4096 rows 192
+// large ones in 86, 512 of 128 x 192 in 93; 8192 x 8192 x 8192: 416 large, 553 small).  Where even small tiles leave CUs
+// idle, a long K is cut into parts, joined by a second launch (8192 -> 3072: 128 rows 26.8 us whole, 14.6 in four parts, 512
+// rows 27.2, 22.7 in two).  Up to 128 rows the few rows' kernel runs where it is faster: a block of K takes it 140 ns with 64
+// rows, 285 with 128, a workgroup to a CU (3072 -> 8192: 64 rows 8.4 us against 13.5, 128 rows 12.1 against 13.3; 8192 ->
+// 3072: 128 rows 23 against 14.6).
 struct Way {
-    bool few, large;
+    bool few;
+    int outputs;                                       // of a tile
     int parts, per;                                    // of K's blocks
 };
 Way product_way(int64_t M, int64_t N, int blocks, bool precise) {
-    if (M <= 32) return {true, false, 1, blocks};
-    const int64_t large = (M + 255) / 256 * ((N + 255) / 256), small = (M + 127) / 128 * ((N + 127) / 128);
-    const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
-    if (!precise && 100 * large_rounds <= 65 * small_rounds) return {false, true, 1, blocks};
-    const int parts = parts_of(small, blocks, 4, M * N, 700, 850);
-    return {false, false, parts, parts == 1 ? blocks : (blocks + 4 * parts - 1) / (4 * parts) * 4};
+    if (M <= 32) return {true, 0, 1, blocks};
+    auto rounds = [&](int rows, int outputs, int at_once) {
+        return ((M + rows - 1) / rows * ((N + outputs - 1) / outputs) + at_once - 1) / at_once;
+    };
+    const int64_t small = rounds(128, 128, 1);
+    if (small > kCus) {
+        const int64_t large_time = 100 * rounds(256, 256, kCus), middle_time = 55 * rounds(128, 192, kCus);
+        if (precise || 63 * rounds(128, 128, 2 * kCus) <= (large_time < middle_time ? large_time : middle_time))
+            return {false, 128, 1, blocks};
+        return {false, large_time <= middle_time ? 256 : 192, 1, blocks};
+    }
+    int64_t ns;
+    const int parts = parts_of(small, blocks, 4, M * N, 300, 620, &ns);
+    const int64_t groups = (N + 31) / 32;              // workgroups of few rows; with less than 64, the parts read K sooner
+    if (M <= 128 && groups >= 64 && (groups + kCus - 1) / kCus * blocks * (M <= 64 ? 140 : 285) <= ns)
+        return {true, 0, 1, blocks};
+    return {false, 128, parts, parts == 1 ? blocks : (blocks + 4 * parts - 1) / (4 * parts) * 4};
 }
 
 template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
@@ -787,14 +857,9 @@ int launch_tiles(const Product& a, int parts, hipStream_t st) {
     return (int)hipGetLastError();
 }
 
-// As many steps together as a wave has, up to four: more registers than that leave a CU fewer waves than loads.
-template <typename T, bool PRECISE, int OB>
+template <typename T, bool PRECISE, int OB, int R>
 int launch_few(const Product& a, hipStream_t st) {
-    const int groups = 32 / OB, steps = (a.blocks + groups - 1) / groups, each = (steps + kFewWaves - 1) / kFewWaves;
-    const dim3 grid((unsigned)((a.N + OB - 1) / OB));
-    if (each == 1) product_few_kernel<T, PRECISE, OB, 1><<<grid, kFewWaves * 64, 0, st>>>(a);
-    else if (each == 2) product_few_kernel<T, PRECISE, OB, 2><<<grid, kFewWaves * 64, 0, st>>>(a);
-    else product_few_kernel<T, PRECISE, OB, 4><<<grid, kFewWaves * 64, 0, st>>>(a);
+    product_few_kernel<T, PRECISE, OB, R><<<dim3((unsigned)((a.N + OB - 1) / OB)), few_waves(R) * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 
@@ -807,12 +872,21 @@ int launch_small(const Product& a, int parts, hipStream_t st) {
 
 template <typename T, bool PRECISE>
 int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) {
-    if (a.M <= 8) return launch_few<T, PRECISE, 8>(a, st);
-    if (a.M <= 16) return launch_few<T, PRECISE, 16>(a, st);
-    if (way.few) return launch_few<T, PRECISE, 32>(a, st);
+    if (way.few) {
+        if (a.M > 64) return launch_few<T, PRECISE, 32, 4>(a, st);
+        if (a.M > 32) return launch_few<T, PRECISE, 32, 2>(a, st);
+        // the fewest outputs that hold the rows, or more while there are 192 workgroups: one row of 3072 -> 8192 takes 8.4 us
+        // with 8 outputs, 6.9 with 16, 6.0 with 32; 8192 -> 3072 takes 7.2 with 8, 6.4 with 16, 9.2 with 32
+        int outputs = a.M <= 8 ? 8 : a.M <= 16 ? 16 : 32;
+        while (outputs < 32 && a.N >= 2 * outputs * 192) outputs *= 2;
+        if (outputs == 8) return launch_few<T, PRECISE, 8, 1>(a, st);
+        if (outputs == 16) return launch_few<T, PRECISE, 16, 1>(a, st);
+        return launch_few<T, PRECISE, 32, 1>(a, st);
+    }
     a.per = way.per;
     if constexpr (!PRECISE) {
-        if (way.large) return launch_tiles<T, PRECISE, 256, 256, 64, 128, 2>(a, 1, st);
+        if (way.outputs == 256) return launch_tiles<T, PRECISE, 256, 256, 64, 128, 2>(a, 1, st);
+        if (way.outputs == 192) return launch_tiles<T, PRECISE, 128, 192, 64, 96, 4>(a, 1, st);
     }
     if (way.parts == 1) return launch_small<T, PRECISE>(a, 1, st);
     void* y = a.y;
@@ -845,7 +919,8 @@ int launch_gradient(const Gradient& a, hipStream_t st) {
 }
 // How a weight gradient runs: by direct loads where dy's rows are whole dwords, in large tiles of 256 x 256 or 256 x 192 (a
 // round of which takes 0.87 of the time: 3072 columns in 12 or 16 tiles, 2048 tokens: 112 or 98 us), or in small ones with the
-// tokens cut into parts where those leave CUs idle (16384 tokens, 512 x 512: 166 us whole, 28 in parts).
+// tokens cut into parts where those leave CUs idle (512 x 512 over 16384 tokens: 160 us whole, 17 in 16 parts; 128 x 128
+// over 65536: 619 us whole, 31 in 16 parts, 15 in 64).
 struct GradientWay {
     bool direct;
     int columns;                                       // of a tile
@@ -861,7 +936,8 @@ GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
     const bool middle = 87 * middle_rounds < 100 * large_rounds;
     if ((middle ? 87 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds) return {true, middle ? 192 : 256, 1, T};
     const int64_t steps = (T + kStep - 1) / kStep;
-    const int parts = parts_of(small, steps, 1, N * K, 650, 1100);
+    int64_t ns;
+    const int parts = small > kCus ? 1 : parts_of(small, steps, 1, N * K, 600, 1100, &ns);
     return {true, 128, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
 }
 // Rows of whole dwords that do not overlap: a row past the last then lies past the buffer's range.

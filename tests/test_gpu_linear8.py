@@ -47,7 +47,8 @@ def test_product(pkg, dev, M, N, K, dtype):
 def test_product_in_parts_of_k(pkg, dev, M, N, K, dtype):
     """Few tiles and a long K: partial results, joined."""
     from faster_yoco_amd import _lib, act8, linear8
-    assert _lib.lib().z1_product8_workspace(M, N, K, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]) > 0
+    parts = _lib.lib().z1_product8_workspace(M, N, K, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}[dtype]) > 0
+    assert parts or K < 2000                           # nine blocks of K are done before a second launch would begin
     x, w, xv, wv = operands(M, N, K, 30)
     p = linear8.pack_weight(w.to(dev))
     y = linear8.matmul(act8.pack(x.to(dev)), p, dtype)
@@ -61,6 +62,26 @@ def test_product_in_large_tiles(pkg, dev, M, N, K):
     x, w, xv, wv = operands(M, N, K, 31)
     y = linear8.matmul(act8.pack(x.to(dev)), linear8.pack_weight(w.to(dev)))
     near(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), K, torch.bfloat16)
+
+
+@pytest.mark.parametrize('M,N,K', [(1900, 2900, 1300), (2048, 3072, 520), (4000, 1500, 600)])
+def test_product_in_tiles_of_128_by_192(pkg, dev, M, N, K):
+    from faster_yoco_amd import act8, linear8
+    x, w, xv, wv = operands(M, N, K, 36)
+    y = linear8.matmul(act8.pack(x.to(dev)), linear8.pack_weight(w.to(dev)))
+    near(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), K, torch.bfloat16)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('M,N,K', [(1, 12300, 300), (5, 6200, 1111), (16, 9000, 700), (33, 2100, 700), (64, 4096, 384),
+                                   (50, 2049, 1500), (65, 8190, 2000), (100, 8185, 2304), (128, 8192, 1900)])
+def test_few_rows_of_many_outputs(pkg, dev, M, N, K, dtype):
+    from faster_yoco_amd import act8, linear8
+    x, w, xv, wv = operands(M, N, K, 35)
+    a, p = act8.pack(x.to(dev)), linear8.pack_weight(w.to(dev), transposed=False)
+    y = linear8.matmul(a, p, dtype)
+    near(y, xv @ wv.t(), xv.abs() @ wv.abs().t(), K, dtype)
+    assert torch.equal(y, linear8.matmul(a, p, dtype))
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=str)
