@@ -9,6 +9,8 @@
 // Statistics and sums are fp32.
 #include "z1_block.h"
 
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace {
@@ -453,6 +455,153 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) 
     }
 }
 
+// The same in one launch, for few rows: the first workgroups sum dw and db over all rows, kStrip columns each, straight from
+// dy and x, and the others give a row's dx to each group of wpr waves.  The rows are read twice, the second time from a
+// cache, instead of partial sums written, read and added by a second launch.  What bounds it is the 50 GB/s that one CU gets
+// from beyond its XCD's L2: hence narrow strips, and eight neighbours, which share lines of 128 bytes, on one XCD (layer
+// norm of 2048 x 3072 BF16: 13.3 us; in two launches 17.5; strips of 32 columns 14.7, of 8 15.0, in launch order 17.1).
+constexpr int kStrip = 16, kStripLanes = kStrip / kLane, kStripRows = kRowThreads / kStripLanes;
+template <typename T, bool Q, bool CENTER>
+__device__ __forceinline__ void strip_sums(const Backward& a, int strip, float (*sums)[2][kStrip]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = strip * kStrip + lane % kStripLanes * kLane, last = a.dim - kLane;
+    const int from = c < last ? c : last, by = c - from;
+    const int first = threadIdx.x / kStripLanes;
+    constexpr int kTurns = 4;                          // of kStripRows rows under way
+    float dw[kLane] = {}, db[kLane] = {};
+    // kTurns turns from row0 on; `left` rows where those are fewer: past them the last, times nothing
+    auto turns = [&](int64_t row0, int left, auto whole) {
+        typename T::raw dy[kTurns];
+        Input<T, Q> x[kTurns];
+        float r[kTurns], mu[kTurns];
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+            int t = first + i * kStripRows;
+            if (!whole) t = t < left ? t : left - 1;
+            const int64_t row = row0 + t;
+            dy[i] = T::load((const typename T::elem*)a.dy + row * a.dy_stride, from);
+            x[i] = Input<T, Q>::load(a, row, c, from);
+            r[i] = a.rstd[row];
+            mu[i] = CENTER ? a.mean[row] : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kTurns; ++i) {
+            float g[kLane], xh[kLane];
+            T::open(dy[i], g);
+            x[i].open(xh, !whole && by > 0, by);
+            if (!whole) {
+                if (by > 0) settle<T>(g, by);
+            }
+            const bool in = whole || first + i * kStripRows < left;
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) {
+                float h = (CENTER ? xh[j] - mu[i] : xh[j]) * r[i];
+                if (!whole) {
+                    g[j] = in ? g[j] : 0.0f;
+                    h = in ? h : 0.0f;
+                }
+                dw[j] = __builtin_fmaf(g[j], h, dw[j]);
+                if (CENTER) db[j] += g[j];
+            }
+        }
+    };
+    constexpr int kAll = kStripRows * kTurns;
+    int64_t row0 = 0;
+    if (by == 0)
+        for (; row0 + kAll <= a.rows; row0 += kAll) turns(row0, kAll, std::true_type{});
+    for (; row0 < a.rows; row0 += kAll) turns(row0, (int)(a.rows - row0 < kAll ? a.rows - row0 : kAll), std::false_type{});
+    // the wave's rows of one column lie kStripLanes lanes apart
+#pragma unroll
+    for (int d = kStripLanes; d < 64; d *= 2) {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            dw[j] += __shfl_xor(dw[j], d);
+            if (CENTER) db[j] += __shfl_xor(db[j], d);
+        }
+    }
+    if (lane < kStripLanes) {
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            sums[wave][0][lane * kLane + j] = dw[j];
+            if (CENTER) sums[wave][1][lane * kLane + j] = db[j];
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, int NV, bool Q, bool CENTER>
+__global__ __launch_bounds__(kRowThreads) void norm_backward_once_kernel(Backward a, int strips, void* out_w, void* out_b,
+                                                                         int grad) {
+    __shared__ float red[kRowThreads / 64][2];
+    __shared__ float sums[kRowThreads / 64][2][kStrip];
+    if ((int)blockIdx.x < strips) {
+        const int strip = (int)(blockIdx.x & 7) * (strips >> 3) + (int)(blockIdx.x >> 3);
+        if (strip * kStrip >= a.dim) return;
+        strip_sums<T, Q, CENTER>(a, strip, sums);
+        const int which = threadIdx.x / kStrip, c = threadIdx.x % kStrip, at = strip * kStrip + c;
+        void* out = which ? out_b : out_w;
+        if (which >= (CENTER ? 2 : 1) || at >= a.dim || !out) return;
+        float t = sums[0][which][c];
+#pragma unroll
+        for (int i = 1; i < kRowThreads / 64; ++i) t += sums[i][which][c];
+        if (grad == Z1_F32) F32::put(out, at, t);
+        else if (grad == Z1_BF16) BF16::put(out, at, t);
+        else F16::put(out, at, t);
+        return;
+    }
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wpr = a.wpr, groups = kRowThreads / 64 / wpr, group = wave / wpr, wi = wave - group * wpr;
+    int64_t row = (int64_t)(blockIdx.x - strips) * groups + group;
+    const bool live = row < a.rows;                    // every wave stays for the barrier
+    if (!live) row = a.rows - 1;
+    const int c0 = (wi * 64 + lane) * kLane, step = wpr * kUnit, last = a.dim - kLane;
+    auto edge = [&](int k) { return (wi + 1) * kUnit + k * step > a.dim; };
+    auto from = [&](int k) { return c0 + k * step < last ? c0 + k * step : last; };
+    typename T::raw dy[NV];
+    Input<T, Q> x[NV];
+    const void* d = (const typename T::elem*)a.dy + row * a.dy_stride;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        dy[k] = T::load(d, from(k));
+        x[k] = Input<T, Q>::load(a, row, c0 + k * step, from(k));
+    }
+    const float r = a.rstd[row], mu = CENTER ? a.mean[row] : 0.0f;
+    float xh[NV][kLane], g[NV][kLane], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const int by = c0 + k * step - from(k);
+        T::open(dy[k], g[k]);
+        if (edge(k)) settle<T>(g[k], by);
+        x[k].open(xh[k], edge(k), by);
+        if (a.w) {
+            float w[kLane];
+            if (a.w32) F32::open(F32::load(a.w, from(k)), w);
+            else T::open(T::load(a.w, from(k)), w);
+            if (edge(k)) settle<T>(w, by);
+#pragma unroll
+            for (int j = 0; j < kLane; ++j) g[k][j] *= w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) {
+            xh[k][j] = (CENTER ? xh[k][j] - mu : xh[k][j]) * r;
+            if (CENTER) s1 += g[k][j];
+            s2 = __builtin_fmaf(g[k][j], xh[k][j], s2);
+        }
+    }
+    row_sums(s1, s2, red, wave, wpr);
+    if (!live) return;
+    const float inv = 1.0f / (float)a.dim, m1 = s1 * inv, m2 = s2 * inv;
+    void* out = (typename T::elem*)a.dx + row * a.dim;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        float dx[kLane];
+#pragma unroll
+        for (int j = 0; j < kLane; ++j) dx[j] = __builtin_fmaf(-xh[k][j], m2, CENTER ? g[k][j] - m1 : g[k][j]) * r;
+        if (edge(k)) store_row<T>(out, c0 + k * step, a.dim - c0 - k * step, dx);
+        else T::store(out, c0 + k * step, dx);
+    }
+}
+
 // Longer rows: dx by one workgroup a row, which reads it twice; the columns' sums apart (norm_columns_kernel).
 template <typename T, bool Q, bool CENTER>
 __global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(Backward a) {
@@ -630,6 +779,37 @@ int backward(Backward& a, const Shape& s, hipStream_t st) {
     return (int)hipGetLastError();
 }
 
+// Whether one launch takes it: few rows, since a strip has them all, and few enough in all for the second reading to come
+// from a cache.  Layer norm, one launch against two, BF16: 777 x 1537 7.7 us, 12.4; 1024 x 8192 17.2, 19.6; 2560 x 3072
+// 15.4, 18.3; but 1536 x 8192 23.3, 22.0; 4096 x 3072 22.3, 21.5; 4096 x 256 14.3, 11.5.
+constexpr int64_t kOnceRows = 2560, kOnceElements = 1 << 23;
+bool is_once(int64_t rows, int64_t dim) {
+    return rows <= kOnceRows && rows * dim <= kOnceElements && dim >= kLane && (dim + kUnit - 1) / kUnit <= 8 * kMaxVectors;
+}
+
+template <typename T, bool Q, bool CENTER>
+int backward_once(Backward& a, const Shape& s, void* dw, void* db, int grad, hipStream_t st) {
+    a.wpr = s.wpr;
+    const int strips = dw || db ? (a.dim + 8 * kStrip - 1) / (8 * kStrip) * 8 : 0;       // as many to each XCD
+    const int groups = kRowThreads / 64 / s.wpr;
+    const dim3 grid((unsigned)(strips + (a.rows + groups - 1) / groups));
+    switch (s.nv) {
+        case 1: norm_backward_once_kernel<T, 1, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+        case 2: norm_backward_once_kernel<T, 2, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+        case 3: norm_backward_once_kernel<T, 3, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+        default: norm_backward_once_kernel<T, 4, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+    }
+    return (int)hipGetLastError();
+}
+template <typename T>
+int once_of(Backward& a, bool center, const Shape& s, void* dw, void* db, int grad, hipStream_t st) {
+    if (a.q)
+        return center ? backward_once<T, true, true>(a, s, dw, db, grad, st)
+                      : backward_once<T, true, false>(a, s, dw, db, grad, st);
+    return center ? backward_once<T, false, true>(a, s, dw, db, grad, st)
+                  : backward_once<T, false, false>(a, s, dw, db, grad, st);
+}
+
 template <typename T>
 int backward_of(Backward& a, bool center, const Shape& s, hipStream_t st) {
     if (a.q) return center ? backward<T, true, true>(a, s, st) : backward<T, true, false>(a, s, st);
@@ -670,6 +850,7 @@ int z1_norm_forward(const void* x, int64_t rows, int64_t dim, int64_t stride, in
 
 int64_t z1_norm_backward_workspace(int64_t rows, int64_t dim) {
     if (bad_shape(rows, dim, 0)) return Z1_E_SIZE;
+    if (is_once(rows, dim)) return 0;
     return (int64_t)backward_shape(rows, (int)dim).blocks * 2 * dim;
 }
 
@@ -686,12 +867,20 @@ int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x
     const Shape sh = backward_shape(rows, (int)dim);
     if (rows > 0) {
         if (!dy || !x == !q || !q != !s || !rstd || (center && !mean) || !dx) return Z1_E_NULL;
-        if (dw || db) {
+        const bool once = is_once(rows, dim);
+        if (!once && (dw || db)) {
             if (!workspace) return Z1_E_NULL;
             if (workspace_floats < (int64_t)sh.blocks * 2 * dim) return Z1_E_WORKSPACE;
         }
         Backward a{dy, dy_stride, x, x_stride, (const uint8_t*)q, (const uint8_t*)s, mean, rstd, w, dx,
                    dw || db ? workspace : nullptr, 0, rows, (int)dim, wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32};
+        if (once) {
+            switch (dtype) {
+                case Z1_F32: return once_of<F32>(a, center, sh, dw, db, grad_dtype, st);
+                case Z1_BF16: return once_of<BF16>(a, center, sh, dw, db, grad_dtype, st);
+                default: return once_of<F16>(a, center, sh, dw, db, grad_dtype, st);
+            }
+        }
         int rc;
         switch (dtype) {
             case Z1_F32: rc = backward_of<F32>(a, center, sh, st); break;

@@ -280,7 +280,7 @@ int z1_norm_forward(const void* x, int64_t rows, int64_t dim, int64_t stride, in
 
 /* Its gradients, from dy and x (dtype) or x's 8-bit rows q, s: dx (dtype), dw = sum over rows of dy (x - mean) rstd, db =
  * sum over rows of dy (grad_dtype; NULL: not wanted, db only with center 1).  workspace: device floats,
- * z1_norm_backward_workspace(rows, dim) of them; NULL where neither dw nor db is wanted. */
+ * z1_norm_backward_workspace(rows, dim) of them (none for few rows); NULL where neither dw nor db is wanted. */
 int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const void* q, const void* s,
                      int64_t rows, int64_t dim, int dtype, const float* mean, const float* rstd, const void* w,
                      int w_dtype, int center, void* dx, void* dw, void* db, int grad_dtype, float* workspace,

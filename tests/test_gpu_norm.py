@@ -158,6 +158,37 @@ def test_backward(pkg, dev, n, dim, dtype, center, packed):
     check_backward(pkg, dev, x, dy, w, center, packed)
 
 
+@pytest.mark.parametrize('packed', [False, True], ids=['x', 'checkpoint'])
+@pytest.mark.parametrize('center', [True, False], ids=['layer', 'rms'])
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('n,dim', [(2561, 9), (2600, 513), (2570, 1537), (2900, 2560), (1030, 8200), (600, 14000)])
+def test_backward_of_many_rows(pkg, dev, n, dim, dtype, center, packed):
+    """Partial sums and a second launch."""
+    from faster_yoco_amd import _lib
+    assert _lib.lib().z1_norm_backward_workspace(n, dim) > 0
+    x, w, _, dy = inputs(n, dim, dtype, 12)
+    check_backward(pkg, dev, x, dy, w, center, packed)
+
+
+@pytest.mark.parametrize('center', [True, False], ids=['layer', 'rms'])
+@pytest.mark.parametrize('n,dim', [(511, 15), (512, 8), (513, 17), (1024, 129), (1537, 520), (2560, 31), (90, 16384)])
+def test_backward_of_few_rows(pkg, dev, n, dim, center):
+    """One launch: whole and partial turns of its rows, strips of columns that end inside."""
+    from faster_yoco_amd import _lib, norm
+    assert _lib.lib().z1_norm_backward_workspace(n, dim) == 0
+    x, w, _, dy = inputs(n, dim, torch.bfloat16, 13)
+    for packed in (False, True):
+        check_backward(pkg, dev, x, dy, w, center, packed)
+    if center:                                         # dw and db each without the other
+        g = [t.to(dev) for t in (dy, x, w)]
+        _, mean, rstd = norm.layer_norm(g[1], g[2])
+        both = norm.layer_norm_backward(g[0], g[1], mean, rstd, g[2], bias=True)
+        assert torch.equal(norm.layer_norm_backward(g[0], g[1], mean, rstd, g[2])[1], both[1])
+        op = torch.ops.yoco_z1.norm_backward
+        assert torch.equal(op(g[0], g[1], None, None, mean, rstd, g[2], True, False, True)[1], both[2])
+        assert torch.equal(op(g[0], g[1], None, None, mean, rstd, g[2], True, False, False)[0], both[0])
+
+
 @pytest.mark.parametrize('center', [True, False], ids=['layer', 'rms'])
 def test_backward_without_weight_and_with_fp32_one(pkg, dev, center):
     for dim in (300, 17000):
