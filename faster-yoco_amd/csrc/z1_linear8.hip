@@ -45,7 +45,7 @@ __device__ __forceinline__ u4 open_bf16(u2 q, float f) {
 // exponent and cut what is more than 13 bits below the largest (probed: 256 + 2^-5 arrives, 256 + 2^-6 does not, while
 // sums across groups keep 24 bits), an error of 1.5e-5 of the result on activations: far below a 16-bit result's own
 // rounding, not below an fp32 one's.  The precise form opens both operands to bf16 (exact) for the bf16 instructions, whose
-// sums are fp32 throughout, at half the rate.
+// sums are fp32 throughout, at half the rate (2048 rows of 3072 -> 8192, fp32: 91 us, 1.13 PFLOP/s; bf16: 42, 2.45).
 __device__ __forceinline__ f16 multiply(f16 acc, i8 fo, i8 ft, uint32_t so, uint32_t st) {
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fo, ft, acc, kE4M3, kE4M3, 0, (int)so, 0, (int)st);
 }
@@ -159,7 +159,12 @@ __device__ __forceinline__ int key_plain(int row) { return row >> 1 & 7; }
 __device__ __forceinline__ int key_spread(int row) { return (row >> 1 & 3) | (row >> 4 & 1) << 2; }
 
 // BT x BO outputs (tokens x outputs) of a workgroup, WT x WO of a wave, S blocks of K staged: two leave room for a second
-// workgroup on a CU, four cover the loads' way where there is no second one.
+// workgroup on a CU (of 128 x 128), four cover the loads' way where there is no second one.
+//
+// Large products are bound by the card's power: 8192 x 8192 x 8192 takes 415 us (2.65 PFLOP/s) with random operands and 297
+// with zeros.  So are bytes moved: eight waves of 64 x 128 read each operand from LDS fewer times than waves of 64 x 64,
+// and 256 x 128 tiles (654 us), four waves of 128 x 128 (428) or eight of 128 x 64 (451) all lost.  Smaller ones are bound by
+// the loads' latency and by CUs without a tile (below, where the tile is chosen).
 template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
 __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Product a) {
     constexpr int kWaves = BT / WT * (BO / WO);
@@ -305,7 +310,10 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
 // at most.  With OB 8 or 16 the instruction's 32 rows and columns are 32 / OB groups, each of the same outputs and rows with
 // a block of K of its own: the results on its diagonal are that many partial sums, so that a narrow output has workgroups for
 // all CUs.  A wave stages its own steps by direct loads, two under way: a lane's 16 bytes lie beside its neighbours', where
-// fragments loaded into registers would be pieces of 32 rows to an instruction.
+// fragments loaded into registers would be pieces of 32 rows to an instruction, and the address unit the bound (32 rows of
+// 8192 -> 3072: 18 us, 10.0 this way).  Bound by the weight's bytes where they are many (one row of 3072 -> 100288: 54 us, 5.7
+// TB/s), else by the launch and the loads' latency (3072 -> 8192: 6.0 us, 4.2 TB/s, from the last cache).  Three or four steps
+// under way, or eight waves, leave room for fewer workgroups and lost (one row: 9 to 14 us).
 constexpr int few_waves(int R) { return R == 4 ? 3 : 4; }                      // what LDS has room for
 template <typename T, bool PRECISE, int OB, int R>
 __global__ __launch_bounds__(few_waves(R) * 64) void product_few_kernel(Product a) {
@@ -425,6 +433,15 @@ struct Gradient {
     int N, K, wide, pitch;
 };
 
+// The workgroup's part of the tokens.
+__device__ __forceinline__ void take_part(Gradient& a) {
+    const int64_t first = blockIdx.y * a.per;
+    a.dy += first * a.stride;
+    a.q += first * a.wide;
+    a.s += first * a.pitch;
+    a.T = a.T - first < a.per ? a.T - first : a.per;
+}
+
 // Four rows (tokens) of 16 columns by 16 lanes, transposed on the way out of LDS: each lane a column's four.
 __device__ __forceinline__ s8 column_pair(const uint16_t* lo, const uint16_t* hi) {
     const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Z1B_LDS s4*)lo);
@@ -440,6 +457,8 @@ __device__ __forceinline__ u4 shift_pieces(u4 v, int n) {
     return n & 1 ? w : v;
 }
 
+// Where dy's rows do not start at whole dwords, as with an odd N, both operands are staged through registers (8191 x 3072 over
+// 2048 tokens: 143 us, where 8192 x 3072 takes 98 by the direct loads below; 7 x 3072 over 16384 tokens 57, in parts).
 // BN x BK of dw to a workgroup, WN x WK to a wave, TS tokens staged at a time, twice buffered.  While a step's products
 // run, the next step's pieces go from registers into the other buffer, and the pieces of the step after that are loaded
 // into those registers: a load has a whole step to arrive, and neither staging nor opening stands between two steps.  The
@@ -460,6 +479,7 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     const int tiles_k = (a.K + BK - 1) / BK;
     const int n0 = (int)(blockIdx.x / tiles_k) * BN, k0 = (int)(blockIdx.x % tiles_k) * BK;
     const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
+    take_part(a);
 
     // Loads ask nothing: rows past the end repeat the last one (zeroed when kept), columns past it repeat columns whose
     // results are dropped.  A piece that the row's end cuts starts 8 columns before the end and is shifted when kept.
@@ -587,12 +607,13 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     }
     __syncthreads();                                   // the staging buffers are free
     constexpr int kRoom = (int)sizeof(lds_n) / (kThreads / 64) & ~15;
+    void* dw = (typename T::elem*)a.dw + (int64_t)blockIdx.y * a.N * a.K;
 #pragma unroll
     for (int j = 0; j < NN; ++j) {
         f16 part[NK];
 #pragma unroll
         for (int i = 0; i < NK; ++i) part[i] = acc[i][j];
-        Flush<T, WK, kRoom>::run((uint8_t*)lds_n + wave * kRoom, lane, part, a.dw, n0 + wn + j * 32, a.N, k0 + wk, a.K);
+        Flush<T, WK, kRoom>::run((uint8_t*)lds_n + wave * kRoom, lane, part, dw, n0 + wn + j * 32, a.N, k0 + wk, a.K);
     }
 }
 
@@ -605,7 +626,9 @@ __device__ __forceinline__ int placed(int run, int token) {
 }
 
 // The same where dy's rows start at whole dwords: dy goes straight into LDS, and both operands are staged the way the
-// product's are.  Rows of both lie whole in LDS; a transposing read takes 64 bytes of four tokens at a time, so a row's
+// product's are.  8192 x 8192 over 8192 tokens: 880 us, 1.25 PFLOP/s (715 with zeros: power again; without opening a's values
+// 746), 8192 x 3072 over 2048: 97 us, over 16384: 736.  a's values opened once more beside the products instead of on the way
+// into LDS: 1058 us; four waves of 128 x 128 924, 128 x 128 tiles 1117.  Rows of both lie whole in LDS; a transposing read takes 64 bytes of four tokens at a time, so a row's
 // 64-byte runs are placed (`placed`) so that the four lie in different banks.  What lies past the last token or
 // past a tensor's end is zero (the buffers' ranges).
 //
@@ -632,11 +655,7 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
     const int tiles_k = (a.K + BK - 1) / BK;
     const int n0 = (int)(blockIdx.x / tiles_k) * BN, k0 = (int)(blockIdx.x % tiles_k) * BK;
     const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
-    const int64_t t_first = blockIdx.y * a.per;        // this part's tokens
-    a.dy += t_first * a.stride;
-    a.q += t_first * a.wide;
-    a.s += t_first * a.pitch;
-    a.T = a.T - t_first < a.per ? a.T - t_first : a.per;
+    take_part(a);
     const int64_t steps = (a.T + TS - 1) / TS;
 
     // direct loads: a lane's row and piece of 16 bytes within a load's rows
@@ -911,10 +930,10 @@ int product<F32>(const Product& a, const Way& way, float* workspace, hipStream_t
 }
 
 template <typename T, Edge EDGE, int BN, int BK, int WN, int WK, int TS>
-int launch_gradient(const Gradient& a, hipStream_t st) {
+int launch_gradient(const Gradient& a, int parts, hipStream_t st) {
     const int64_t tiles = (int64_t)((a.N + BN - 1) / BN) * ((a.K + BK - 1) / BK);
     if (tiles > kMaxTiles) return Z1_E_SIZE;
-    weight_grad_kernel<T, EDGE, BN, BK, WN, WK, TS><<<dim3((unsigned)tiles), BN / WN * (BK / WK) * 64, 0, st>>>(a);
+    weight_grad_kernel<T, EDGE, BN, BK, WN, WK, TS><<<dim3((unsigned)tiles, parts), BN / WN * (BK / WK) * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 // How a weight gradient runs: by direct loads where dy's rows are whole dwords, in large tiles of 256 x 256 or 256 x 192 (a
@@ -929,16 +948,18 @@ struct GradientWay {
 };
 constexpr int kStep = 64;
 GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
-    if (!direct) return {false, 128, 1, T};
-    const int64_t large = (N + 255) / 256 * ((K + 255) / 256), small = (N + 127) / 128 * ((K + 127) / 128);
-    const int64_t large_rounds = (large + kCus - 1) / kCus, small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
-    const int64_t middle_rounds = ((N + 255) / 256 * ((K + 191) / 192) + kCus - 1) / kCus;
-    const bool middle = 87 * middle_rounds < 100 * large_rounds;
-    if ((middle ? 87 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds) return {true, middle ? 192 : 256, 1, T};
+    const int64_t small = (N + 127) / 128 * ((K + 127) / 128);
+    if (direct) {
+        const int64_t large_rounds = ((N + 255) / 256 * ((K + 255) / 256) + kCus - 1) / kCus;
+        const int64_t middle_rounds = ((N + 255) / 256 * ((K + 191) / 192) + kCus - 1) / kCus;
+        const int64_t small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
+        const bool middle = 87 * middle_rounds < 100 * large_rounds;
+        if ((middle ? 87 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds) return {true, middle ? 192 : 256, 1, T};
+    }
     const int64_t steps = (T + kStep - 1) / kStep;
     int64_t ns;
-    const int parts = small > kCus ? 1 : parts_of(small, steps, 1, N * K, 600, 1100, &ns);
-    return {true, 128, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
+    const int parts = small > kCus ? 1 : parts_of(small, steps, 1, N * K, direct ? 600 : 1400, direct ? 1100 : 1500, &ns);
+    return {direct, 128, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
 }
 // Rows of whole dwords that do not overlap: a row past the last then lies past the buffer's range.
 bool is_direct(const void* dy, int64_t stride, int64_t N) {
@@ -953,19 +974,21 @@ int launch_direct(const Gradient& a, int parts, hipStream_t st) {
     return (int)hipGetLastError();
 }
 template <typename T>
+int small_gradient(const Gradient& a, const GradientWay& way, hipStream_t st) {
+    if (way.direct) return launch_direct<T, 128, 128, 64, 64>(a, way.parts, st);
+    if (a.N < 8) return launch_gradient<T, kFew, 128, 128, 64, 64, 32>(a, way.parts, st);
+    return launch_gradient<T, kCut, 128, 128, 64, 64, 32>(a, way.parts, st);
+}
+template <typename T>
 int gradient(Gradient a, const GradientWay& way, float* workspace, hipStream_t st) {
     a.per = way.per;
     if (way.columns == 256) return launch_direct<T, 256, 256, 128, 64>(a, 1, st);
     if (way.columns == 192) return launch_direct<T, 256, 192, 64, 96>(a, 1, st);
-    if (way.direct && way.parts == 1) return launch_direct<T, 128, 128, 64, 64>(a, 1, st);
-    if (way.direct) {
-        void* dw = a.dw;
-        a.dw = workspace;
-        if (const int rc = launch_direct<F32, 128, 128, 64, 64>(a, way.parts, st)) return rc;
-        return join<T>(workspace, way.parts, (int64_t)a.N * a.K, dw, st);
-    }
-    if (a.N < 8) return launch_gradient<T, kFew, 128, 128, 64, 64, 32>(a, st);
-    return launch_gradient<T, kCut, 128, 128, 64, 64, 32>(a, st);
+    if (way.parts == 1) return small_gradient<T>(a, way, st);
+    void* dw = a.dw;
+    a.dw = workspace;
+    if (const int rc = small_gradient<F32>(a, way, st)) return rc;
+    return join<T>(workspace, way.parts, (int64_t)a.N * a.K, dw, st);
 }
 
 }  // namespace
@@ -1003,8 +1026,9 @@ int z1_product8(const void* a, const void* as, int64_t M, const void* w, const v
 int64_t z1_weight_grad8_workspace(int64_t T, int64_t N, int64_t K) {
     if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim) return Z1_E_SIZE;
     if (N == 0) return 0;
-    const GradientWay way = gradient_way(T, N, K, true);
-    return way.parts > 1 ? way.parts * N * K : 0;
+    const int direct = gradient_way(T, N, K, true).parts, staged = gradient_way(T, N, K, false).parts;
+    const int64_t parts = direct > staged ? direct : staged;                   // dy's rows may be either
+    return parts > 1 ? parts * N * K : 0;
 }
 
 int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const void* s, int64_t T, int64_t N, int64_t K,
@@ -1014,11 +1038,10 @@ int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const voi
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (N == 0) return Z1_OK;
     if (!dw || (T > 0 && (!dy || !q || !s))) return Z1_E_NULL;
+    const int64_t need = z1_weight_grad8_workspace(T, N, K);
+    if (need && !workspace) return Z1_E_NULL;
+    if (workspace_floats < need) return Z1_E_WORKSPACE;
     const GradientWay way = gradient_way(T, N, K, is_direct(dy, stride, N));
-    if (way.parts > 1) {
-        if (!workspace) return Z1_E_NULL;
-        if (workspace_floats < way.parts * N * K) return Z1_E_WORKSPACE;
-    }
     const Gradient g{dy, stride, (const uint8_t*)q, (const uint8_t*)s, dw, T, T, (int)N, (int)K, wide_of(K), pitch_of(K)};
     const hipStream_t st = (hipStream_t)stream;
     switch (dtype) {

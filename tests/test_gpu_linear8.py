@@ -180,6 +180,16 @@ def test_gradient_rows_of_any_stride(pkg, dev):
     assert torch.equal(linear8.weight_grad(base[:, :640].reshape(9, 10, 640), a), linear8.weight_grad(base[:, :640].contiguous(), a))
 
 
+@pytest.mark.parametrize('T,N,K', [(3001, 65, 300), (2050, 7, 260), (5000, 1, 40), (1000, 1001, 130), (64, 9, 9)])
+def test_gradient_of_odd_rows_in_parts(pkg, dev, T, N, K):
+    from faster_yoco_amd import act8, linear8
+    x, dy = rows(T, K, 37), rows(T, N, 38) * 1e-3
+    xv, d = ref.values(*ref.pack(x), K), dy.double()
+    for dtype in DTYPES:
+        dw = linear8.weight_grad(dy.to(dev), act8.pack(x.to(dev)), dtype)
+        near(dw, d.t() @ xv, d.abs().t() @ xv.abs(), T, dtype)
+
+
 @pytest.mark.parametrize('T', [1, 63, 130])
 def test_gradient_rows_of_whole_dwords_and_odd_width(pkg, dev, T):
     """The last row's last element shares its dword with what lies behind the tensor."""
