@@ -314,11 +314,11 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
 // 8192 -> 3072: 18 us, 10.0 this way).  Bound by the weight's bytes where they are many (one row of 3072 -> 100288: 54 us, 5.7
 // TB/s), else by the launch and the loads' latency (3072 -> 8192: 6.0 us, 4.2 TB/s, from the last cache).  Three or four steps
 // under way, or eight waves, leave room for fewer workgroups and lost (one row: 9 to 14 us).
-constexpr int few_waves(int R) { return R == 4 ? 3 : 4; }                      // what LDS has room for
+constexpr int kFewWaves = 4;
 template <typename T, bool PRECISE, int OB, int R>
-__global__ __launch_bounds__(few_waves(R) * 64) void product_few_kernel(Product a) {
+__global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(Product a) {
     static_assert(R == 1 || OB == 32, "more row fragments than one are whole ones");
-    constexpr int G = 32 / OB, U = 2, W = few_waves(R);                        // blocks of K to an instruction; steps under way
+    constexpr int G = 32 / OB, U = 2, W = kFewWaves;   // blocks of K to an instruction; steps under way
     constexpr int kRows = 32 * kBlock;                 // bytes: 32 rows of the weight, R times 32 of a, and their scales
     constexpr int kScales = (1 + R) * kRows, kStep = kScales + (1 + R) * 256, kStepLoads = (1 + R) * 5;
     __shared__ __align__(1024) uint8_t lds[W][U][kStep];
@@ -822,50 +822,72 @@ int join(const float* part, int parts, int64_t count, void* out, hipStream_t st)
 
 // The number of parts into which the long axis of a product in small tiles is cut, `steps` of it in multiples of `unit`:
 // the one with the least estimate of the time, which *ns is.  A step takes `alone` where a CU has one tile, `shared` where
-// it has two; joining takes 2.5 us and 0.05 a part, and the partial results' way out and back at 5 bytes/ps.
+// it has two (0: it has no room for two); joining takes 3.3 us and 0.05 a part, and the partial results' way out and back at
+// 5 bytes/ps.
 int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int alone, int shared, int64_t* ns) {
     int best = 1;
     *ns = 0;
     for (int p = 1; p <= kMaxParts; ++p) {
         const int64_t per = (steps + p * unit - 1) / (p * unit) * unit;
-        if (p > 1 && (per * (p - 1) >= steps || tiles * p > 2 * kCus)) continue;       // a part without steps; no room
-        const int64_t time = per * (tiles * p <= kCus ? alone : shared) + (p > 1 ? 2500 + p * (50 + results * 8 / 5000) : 0);
+        if (p > 1 && (per * (p - 1) >= steps || tiles * p > (shared ? 2 * kCus : kCus))) continue;     // no steps; no room
+        const int64_t time = per * (tiles * p <= kCus ? alone : shared) + (p > 1 ? 3300 + p * (50 + results * 8 / 5000) : 0);
         if (p == 1 || time < *ns) best = p, *ns = time;
     }
     return best;
 }
 
-// How a product runs.  Large tiles (256 x 256) move fewer bytes per product, smaller ones leave fewer CUs without work.  A
-// round of large ones, one to a CU, takes 100; of small ones (128 x 128), two to a CU, 63; of 128 x 192, one to a CU, 55 (a
-// block of K of 8192 -> 3072 with 2048 rows: 384 small tiles in 54.0 us, 256 of 128 x 192 in 47.4; with 4096 rows 192
-// large ones in 86, 512 of 128 x 192 in 93; 8192 x 8192 x 8192: 416 large, 553 small).  Where even small tiles leave CUs
-// idle, a long K is cut into parts, joined by a second launch (8192 -> 3072: 128 rows 26.8 us whole, 14.6 in four parts, 512
-// rows 27.2, 22.7 in two).  Up to 128 rows the few rows' kernel runs where it is faster: a block of K takes it 140 ns with 64
-// rows, 285 with 128, a workgroup to a CU (3072 -> 8192: 64 rows 8.4 us against 13.5, 128 rows 12.1 against 13.3; 8192 ->
-// 3072: 128 rows 23 against 14.6).
+// How a product runs.
+//
+// Many tiles: large ones (256 x 256) move fewer bytes per product, smaller ones leave fewer CUs without work.  A round of
+// large ones, one to a CU, takes 100; of 128 x 128, two to a CU, 63; of 128 x 192, one to a CU, 55 (8192 -> 3072 with 2048
+// rows: 384 of 128 x 128 in 54.0 us, 256 of 128 x 192 in 47.4; with 4096 rows 192 large ones in 86, 512 of 128 x 192 in 93;
+// 8192 x 8192 x 8192: 415 large, 553 of 128 x 128).
+//
+// Up to one of 128 x 128 to a CU: what bounds a tile is how fast its one CU gets the operands, so smaller tiles on more CUs
+// win while there are CUs (kSmall: a start and a block of K, in ns, as measured), and where even they leave CUs idle, a long
+// K is cut into parts, joined by a second launch.  1000 -> 1501, 333 rows: 5.7 us in 64 x 64, 8.0 in 128 x 128; 3072 -> 8192,
+// 256 rows: 11.4 in 64 x 128, 13.8 in 128 x 128; 8192 -> 3072, 512 rows: 21.6 in 64 x 128, 22.7 in 128 x 128 of two parts;
+// 128 rows: 26.8 in 128 x 128, 14.6 of four parts.
+//
+// Up to 64 rows the few rows' kernel runs where it is faster, a workgroup to a CU, at 2.5 us and 0.1 to 0.23 us a block of K,
+// more with more of them and more rows (33 rows, 3072 -> 3072: 6.2 us against 8.4, 3072 -> 8192: 7.3 against 8.6; 64 rows, 8192
+// -> 3072: 14.0 against 12.3).
 struct Way {
     bool few;
-    int outputs;                                       // of a tile
+    int rows, outputs;                                 // of a tile
     int parts, per;                                    // of K's blocks
 };
+struct Small {
+    int rows, outputs, start, alone, shared;
+} constexpr kSmall[] = {{128, 128, 4200, 330, 620}, {64, 128, 2700, 300, 0}, {64, 64, 2900, 230, 400}};
 Way product_way(int64_t M, int64_t N, int blocks, bool precise) {
-    if (M <= 32) return {true, 0, 1, blocks};
-    auto rounds = [&](int rows, int outputs, int at_once) {
-        return ((M + rows - 1) / rows * ((N + outputs - 1) / outputs) + at_once - 1) / at_once;
-    };
-    const int64_t small = rounds(128, 128, 1);
-    if (small > kCus) {
+    if (M <= 32) return {true, 0, 0, 1, blocks};
+    auto tiles = [&](int rows, int outputs) { return (M + rows - 1) / rows * ((N + outputs - 1) / outputs); };
+    auto rounds = [&](int rows, int outputs, int at_once) { return (tiles(rows, outputs) + at_once - 1) / at_once; };
+    if (tiles(128, 128) > kCus) {
         const int64_t large_time = 100 * rounds(256, 256, kCus), middle_time = 55 * rounds(128, 192, kCus);
         if (precise || 63 * rounds(128, 128, 2 * kCus) <= (large_time < middle_time ? large_time : middle_time))
-            return {false, 128, 1, blocks};
-        return {false, large_time <= middle_time ? 256 : 192, 1, blocks};
+            return {false, 128, 128, 1, blocks};
+        if (large_time <= middle_time) return {false, 256, 256, 1, blocks};
+        return {false, 128, 192, 1, blocks};
     }
-    int64_t ns;
-    const int parts = parts_of(small, blocks, 4, M * N, 300, 620, &ns);
+    Way way{false, 0, 0, 0, 0};
+    int64_t least = 0;
+    for (const Small& t : kSmall) {
+        const int64_t n = tiles(t.rows, t.outputs);
+        if (n > (t.shared ? 2 * kCus : kCus)) continue;
+        int64_t ns;
+        const int parts = parts_of(n, blocks, 4, M * N, t.alone, t.shared, &ns);
+        if (way.parts == 0 || t.start + ns < least) {
+            least = t.start + ns;
+            way = {false, t.rows, t.outputs, parts, parts == 1 ? blocks : (blocks + 4 * parts - 1) / (4 * parts) * 4};
+        }
+    }
     const int64_t groups = (N + 31) / 32;              // workgroups of few rows; with less than 64, the parts read K sooner
-    if (M <= 128 && groups >= 64 && (groups + kCus - 1) / kCus * blocks * (M <= 64 ? 140 : 285) <= ns)
-        return {true, 0, 1, blocks};
-    return {false, 128, parts, parts == 1 ? blocks : (blocks + 4 * parts - 1) / (4 * parts) * 4};
+    const int64_t few_rounds = (groups + kCus - 1) / kCus, at_once = groups < kCus ? groups : kCus;
+    if (M <= 64 && groups >= 64 && 2500 + few_rounds * blocks * (100 + at_once * M / 128) <= least)
+        return {true, 0, 0, 1, blocks};
+    return way;
 }
 
 template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
@@ -878,21 +900,22 @@ int launch_tiles(const Product& a, int parts, hipStream_t st) {
 
 template <typename T, bool PRECISE, int OB, int R>
 int launch_few(const Product& a, hipStream_t st) {
-    product_few_kernel<T, PRECISE, OB, R><<<dim3((unsigned)((a.N + OB - 1) / OB)), few_waves(R) * 64, 0, st>>>(a);
+    product_few_kernel<T, PRECISE, OB, R><<<dim3((unsigned)((a.N + OB - 1) / OB)), kFewWaves * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 
 template <typename T, bool PRECISE>
-int launch_small(const Product& a, int parts, hipStream_t st) {
-    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 127) / 128) * parts;
-    return tiles <= kCus ? launch_tiles<T, PRECISE, 128, 128, 64, 64, 4>(a, parts, st)
-                         : launch_tiles<T, PRECISE, 128, 128, 64, 64, 2>(a, parts, st);
+int launch_small(const Product& a, const Way& way, hipStream_t st) {
+    if (way.rows == 64 && way.outputs == 64) return launch_tiles<T, PRECISE, 64, 64, 32, 32, 4>(a, way.parts, st);
+    if (way.rows == 64) return launch_tiles<T, PRECISE, 64, 128, 32, 64, 4>(a, way.parts, st);
+    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 127) / 128) * way.parts;
+    return tiles <= kCus ? launch_tiles<T, PRECISE, 128, 128, 64, 64, 4>(a, way.parts, st)
+                         : launch_tiles<T, PRECISE, 128, 128, 64, 64, 2>(a, way.parts, st);
 }
 
 template <typename T, bool PRECISE>
 int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) {
     if (way.few) {
-        if (a.M > 64) return launch_few<T, PRECISE, 32, 4>(a, st);
         if (a.M > 32) return launch_few<T, PRECISE, 32, 2>(a, st);
         // the fewest outputs that hold the rows, or more while there are 192 workgroups: one row of 3072 -> 8192 takes 8.4 us
         // with 8 outputs, 6.9 with 16, 6.0 with 32; 8192 -> 3072 takes 7.2 with 8, 6.4 with 16, 9.2 with 32
@@ -907,10 +930,10 @@ int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) 
         if (way.outputs == 256) return launch_tiles<T, PRECISE, 256, 256, 64, 128, 2>(a, 1, st);
         if (way.outputs == 192) return launch_tiles<T, PRECISE, 128, 192, 64, 96, 4>(a, 1, st);
     }
-    if (way.parts == 1) return launch_small<T, PRECISE>(a, 1, st);
+    if (way.parts == 1) return launch_small<T, PRECISE>(a, way, st);
     void* y = a.y;
     a.y = workspace;
-    if (const int rc = launch_small<F32, PRECISE>(a, way.parts, st)) return rc;
+    if (const int rc = launch_small<F32, PRECISE>(a, way, st)) return rc;
     return join<T>(workspace, way.parts, a.M * a.N, y, st);
 }
 
