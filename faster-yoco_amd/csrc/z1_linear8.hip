@@ -473,8 +473,9 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     constexpr int kDyRows = kThreads / (BN / 8), kXRows = kThreads / (BK / 8); // rows between a thread's pieces
     constexpr int NN = WN / 32, NK = WK / 32, KK = TS / 16;
     static_assert(kThreads % (BN / 8) == 0 && kThreads % (BK / 8) == 0, "a thread keeps its columns");
-    __shared__ __align__(16) uint16_t lds_n[2][TS * kPitchN];
-    __shared__ __align__(16) uint16_t lds_k[2][TS * kPitchK];
+    __shared__ __align__(16) uint16_t lds[2 * TS * (kPitchN + kPitchK)];
+    auto lds_n = [&](int buf) { return lds + buf * TS * kPitchN; };
+    auto lds_k = [&](int buf) { return lds + (2 * kPitchN + buf * kPitchK) * TS; };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_k = (a.K + BK - 1) / BK;
     const int n0 = (int)(blockIdx.x / tiles_k) * BN, k0 = (int)(blockIdx.x % tiles_k) * BK;
@@ -537,7 +538,7 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
             u4 v = dy[i];
             if (EDGE == kCut) v = shift_pieces(v, shifted ? 8 - cut : 0);
             if (rows < TS && t >= rows) v = u4{};
-            *(u4*)(lds_n[buf] + t * kPitchN + my_n) = v;
+            *(u4*)(lds_n(buf) + t * kPitchN + my_n) = v;
         }
 #pragma unroll
         for (int i = 0; i < kX; ++i) {
@@ -545,7 +546,7 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
             const int t = row_k + i * kXRows;
             u4 v = open_bf16(x[i], scale_value(xs[i]));
             if (rows < TS && t >= rows) v = u4{};
-            *(u4*)(lds_k[buf] + t * kPitchK + my_k) = v;
+            *(u4*)(lds_k(buf) + t * kPitchK + my_k) = v;
         }
     };
 
@@ -576,8 +577,8 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     for (int64_t step = 0; step < steps; ++step) {
         const int buf = (int)(step & 1);
         __syncthreads();
-        const uint16_t* bn = lds_n[buf] + row * kPitchN + wn + col_n;
-        const uint16_t* bk = lds_k[buf] + row * kPitchK + wk + col_k;
+        const uint16_t* bn = lds_n(buf) + row * kPitchN + wn + col_n;
+        const uint16_t* bk = lds_k(buf) + row * kPitchK + wk + col_k;
         s8 fn[2][NN], fk[2][NK];
         auto read = [&](int kk) {
 #pragma unroll
@@ -606,14 +607,14 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
         next = next + TS < end ? next + TS : end;
     }
     __syncthreads();                                   // the staging buffers are free
-    constexpr int kRoom = (int)sizeof(lds_n) / (kThreads / 64) & ~15;
+    constexpr int kRoom = (int)sizeof(lds) / (kThreads / 64) & ~15;
     void* dw = (typename T::elem*)a.dw + (int64_t)blockIdx.y * a.N * a.K;
 #pragma unroll
     for (int j = 0; j < NN; ++j) {
         f16 part[NK];
 #pragma unroll
         for (int i = 0; i < NK; ++i) part[i] = acc[i][j];
-        Flush<T, WK, kRoom>::run((uint8_t*)lds_n + wave * kRoom, lane, part, dw, n0 + wn + j * 32, a.N, k0 + wk, a.K);
+        Flush<T, WK, kRoom>::run((uint8_t*)lds + wave * kRoom, lane, part, dw, n0 + wn + j * 32, a.N, k0 + wk, a.K);
     }
 }
 
@@ -647,7 +648,7 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
     constexpr int P = BK == 192 ? 8 : 16;              // columns of a thread's piece of a's rows
     constexpr int kX = TS * BK / P / kThreads;
     static_assert(kX * kThreads * P == TS * BK, "every thread has as many");
-    static_assert(kLoadRows == 2 || kLoadRows == 4, "rows of 256 or 512 bytes");
+    static_assert(kLoadRows == 2 || kLoadRows == 4 || kLoadRows == 8, "rows of 128, 256 or 512 bytes");
     __shared__ __align__(1024) uint8_t lds[2 * TS * (kRowN + kRowK)];
     auto lds_n = [&](int64_t step) { return lds + (step & 1) * TS * kRowN; };
     auto lds_k = [&](int64_t step) { return lds + (2 * kRowN + (step & 1) * kRowK) * TS; };
@@ -664,7 +665,7 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
     int from[kLoadRows == 2 ? 2 : 1];                  // by the parity of the load: two rows are half of four
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(from) / sizeof(int)); ++i)
-        from[i] = sub * row_bytes + ((piece ^ (((i * kLoadRows + sub) & 3) << 2)) << 4);
+        from[i] = sub * row_bytes + (placed<BN / 32>(piece >> 2, i * kLoadRows + sub) << 2 | (piece & 3)) * 16;
     // from the tile's first column to dy's end, in whole dwords (an odd N's last one holds nothing that is used)
     const int64_t bytes_n = a.T > 0 ? (a.T - 1) * row_bytes + ((a.N - n0 + 1) & ~1) * 2 : 0;
     auto stage = [&](int64_t step, int i, uint8_t* to) {
@@ -859,7 +860,26 @@ struct Way {
 };
 struct Small {
     int rows, outputs, start, alone, shared;
-} constexpr kSmall[] = {{128, 128, 4200, 330, 620}, {64, 128, 2700, 300, 0}, {64, 64, 2900, 230, 400}};
+};
+constexpr Small kSmall[] = {{128, 128, 4200, 330, 620}, {64, 128, 2700, 300, 0}, {64, 64, 2900, 230, 400}};
+// The best of them for M x N results (M x N 128 x 128 tiles at most one to a CU, or the first is taken).
+struct Cut {
+    const Small* tile;
+    int parts;
+    int64_t ns;
+};
+template <int COUNT>
+Cut best_of(const Small (&small)[COUNT], int64_t M, int64_t N, int64_t steps, int unit) {
+    Cut best{nullptr, 1, 0};
+    for (const Small& t : small) {
+        const int64_t n = (M + t.rows - 1) / t.rows * ((N + t.outputs - 1) / t.outputs);
+        if (best.tile && n > (t.shared ? 2 * kCus : kCus)) continue;
+        int64_t ns;
+        const int parts = parts_of(n, steps, unit, M * N, t.alone, t.shared, &ns);
+        if (!best.tile || t.start + ns < best.ns) best = {&t, parts, t.start + ns};
+    }
+    return best;
+}
 Way product_way(int64_t M, int64_t N, int blocks, bool precise) {
     if (M <= 32) return {true, 0, 0, 1, blocks};
     auto tiles = [&](int rows, int outputs) { return (M + rows - 1) / rows * ((N + outputs - 1) / outputs); };
@@ -871,23 +891,13 @@ Way product_way(int64_t M, int64_t N, int blocks, bool precise) {
         if (large_time <= middle_time) return {false, 256, 256, 1, blocks};
         return {false, 128, 192, 1, blocks};
     }
-    Way way{false, 0, 0, 0, 0};
-    int64_t least = 0;
-    for (const Small& t : kSmall) {
-        const int64_t n = tiles(t.rows, t.outputs);
-        if (n > (t.shared ? 2 * kCus : kCus)) continue;
-        int64_t ns;
-        const int parts = parts_of(n, blocks, 4, M * N, t.alone, t.shared, &ns);
-        if (way.parts == 0 || t.start + ns < least) {
-            least = t.start + ns;
-            way = {false, t.rows, t.outputs, parts, parts == 1 ? blocks : (blocks + 4 * parts - 1) / (4 * parts) * 4};
-        }
-    }
+    const Cut cut = best_of(kSmall, M, N, blocks, 4);
     const int64_t groups = (N + 31) / 32;              // workgroups of few rows; with less than 64, the parts read K sooner
     const int64_t few_rounds = (groups + kCus - 1) / kCus, at_once = groups < kCus ? groups : kCus;
-    if (M <= 64 && groups >= 64 && 2500 + few_rounds * blocks * (100 + at_once * M / 128) <= least)
+    if (M <= 64 && groups >= 64 && 2500 + few_rounds * blocks * (100 + at_once * M / 128) <= cut.ns)
         return {true, 0, 0, 1, blocks};
-    return way;
+    return {false, cut.tile->rows, cut.tile->outputs, cut.parts,
+            cut.parts == 1 ? blocks : (blocks + 4 * cut.parts - 1) / (4 * cut.parts) * 4};
 }
 
 template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
@@ -960,16 +970,20 @@ int launch_gradient(const Gradient& a, int parts, hipStream_t st) {
     return (int)hipGetLastError();
 }
 // How a weight gradient runs: by direct loads where dy's rows are whole dwords, in large tiles of 256 x 256 or 256 x 192 (a
-// round of which takes 0.87 of the time: 3072 columns in 12 or 16 tiles, 2048 tokens: 112 or 98 us), or in small ones with the
-// tokens cut into parts where those leave CUs idle (512 x 512 over 16384 tokens: 160 us whole, 17 in 16 parts; 128 x 128
-// over 65536: 619 us whole, 31 in 16 parts, 15 in 64).
+// round of which takes 0.87 of the time: 3072 columns in 12 or 16 tiles, 2048 tokens: 112 or 98 us), or in small ones (their
+// start and 64 tokens in ns, as for the products) with the tokens cut into parts where those leave CUs idle (512 x 512 over
+// 16384 tokens: 106 us in 128 x 128, 17 of 16 parts; 128 x 128 over 65536: 409 us, 15 of 64 parts; 2048 x 1024 over 2048: 16.0
+// in 128 x 128, 13.3 in 64 x 64; odd rows, 2047 x 1024 over 2048: 19.2 in 128 x 128 of four parts, 16.1 in 64 x 64).
 struct GradientWay {
     bool direct;
-    int columns;                                       // of a tile
+    int rows, columns;                                 // of a tile
     int parts;
     int64_t per;
 };
 constexpr int kStep = 64;
+constexpr Small kSmallDirect[] = {{128, 128, 2900, 420, 800}, {64, 64, 2700, 280, 420}};
+constexpr Small kSmallStaged[] = {{128, 128, 2900, 1300, 1480}, {64, 64, 2700, 550, 630}};
+constexpr Small kSmallFew[] = {kSmallStaged[1]};
 GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
     const int64_t small = (N + 127) / 128 * ((K + 127) / 128);
     if (direct) {
@@ -977,12 +991,17 @@ GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
         const int64_t middle_rounds = ((N + 255) / 256 * ((K + 191) / 192) + kCus - 1) / kCus;
         const int64_t small_rounds = (small + 2 * kCus - 1) / (2 * kCus);
         const bool middle = 87 * middle_rounds < 100 * large_rounds;
-        if ((middle ? 87 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds) return {true, middle ? 192 : 256, 1, T};
+        if ((middle ? 87 * middle_rounds : 100 * large_rounds) <= 62 * small_rounds)
+            return {true, 256, middle ? 192 : 256, 1, T};
     }
+    const bool few = !direct && N < 8;
+    if (small > kCus && !few) return {direct, 128, 128, 1, T};
     const int64_t steps = (T + kStep - 1) / kStep;
-    int64_t ns;
-    const int parts = small > kCus ? 1 : parts_of(small, steps, 1, N * K, direct ? 600 : 1400, direct ? 1100 : 1500, &ns);
-    return {direct, 128, parts, parts == 1 ? T : (steps + parts - 1) / parts * kStep};
+    const Cut cut = direct ? best_of(kSmallDirect, N, K, steps, 1)
+                    : few  ? best_of(kSmallFew, N, K, steps, 1)
+                           : best_of(kSmallStaged, N, K, steps, 1);
+    return {direct, cut.tile->rows, cut.tile->outputs, cut.parts,
+            cut.parts == 1 ? T : (steps + cut.parts - 1) / cut.parts * kStep};
 }
 // Rows of whole dwords that do not overlap: a row past the last then lies past the buffer's range.
 bool is_direct(const void* dy, int64_t stride, int64_t N) {
@@ -998,9 +1017,12 @@ int launch_direct(const Gradient& a, int parts, hipStream_t st) {
 }
 template <typename T>
 int small_gradient(const Gradient& a, const GradientWay& way, hipStream_t st) {
-    if (way.direct) return launch_direct<T, 128, 128, 64, 64>(a, way.parts, st);
-    if (a.N < 8) return launch_gradient<T, kFew, 128, 128, 64, 64, 32>(a, way.parts, st);
-    return launch_gradient<T, kCut, 128, 128, 64, 64, 32>(a, way.parts, st);
+    const bool tiny = way.rows == 64;
+    if (way.direct)
+        return tiny ? launch_direct<T, 64, 64, 32, 32>(a, way.parts, st) : launch_direct<T, 128, 128, 64, 64>(a, way.parts, st);
+    if (a.N < 8) return launch_gradient<T, kFew, 64, 64, 32, 32, 64>(a, way.parts, st);
+    return tiny ? launch_gradient<T, kCut, 64, 64, 32, 32, 64>(a, way.parts, st)
+                : launch_gradient<T, kCut, 128, 128, 64, 64, 32>(a, way.parts, st);
 }
 template <typename T>
 int gradient(Gradient a, const GradientWay& way, float* workspace, hipStream_t st) {
