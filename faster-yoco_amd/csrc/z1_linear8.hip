@@ -629,9 +629,9 @@ __device__ __forceinline__ int placed(int run, int token) {
 // The same where dy's rows start at whole dwords: dy goes straight into LDS, and both operands are staged the way the
 // product's are.  8192 x 8192 over 8192 tokens: 880 us, 1.25 PFLOP/s (715 with zeros: power again; without opening a's values
 // 746), 8192 x 3072 over 2048: 97 us, over 16384: 736.  a's values opened once more beside the products instead of on the way
-// into LDS: 1058 us; four waves of 128 x 128 924, 128 x 128 tiles 1117.  Rows of both lie whole in LDS; a transposing read takes 64 bytes of four tokens at a time, so a row's
-// 64-byte runs are placed (`placed`) so that the four lie in different banks.  What lies past the last token or
-// past a tensor's end is zero (the buffers' ranges).
+// into LDS: 1058 us; four waves of 128 x 128 924, 128 x 128 tiles 1117.  Rows of both lie whole in LDS; a transposing read
+// takes 64 bytes of four tokens at a time, so a row's 64-byte runs are placed (`placed`) so that the four lie in different
+// banks.  What lies past the last token or past a tensor's end is zero (the buffers' ranges).
 //
 // A step of TS tokens is TS / 16 parts.  Each part's operands are read a part ahead, and the workgroup meets before the
 // last part: all of the step has been read by then.  From one meeting to the next (`between`) everything is read from one
@@ -788,7 +788,8 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
 }
 
 constexpr int64_t kMaxRows = 1ll << 40;
-constexpr int64_t kMaxDim = 1 << 24;
+constexpr int64_t kMaxDim = 1 << 24;                   // outputs, and elements between rows of dy
+constexpr int64_t kMaxInner = 1 << 22;                 // columns: 256 rows of them lie within 31 bits
 constexpr int kMaxParts = 64;
 constexpr int64_t kMaxTiles = 1ll << 22;               // of a launch: its threads count in 32 bits
 
@@ -1041,7 +1042,7 @@ int gradient(Gradient a, const GradientWay& way, float* workspace, hipStream_t s
 extern "C" {
 
 int64_t z1_product8_workspace(int64_t M, int64_t N, int64_t K, int dtype) {
-    if (M < 0 || M > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim) return Z1_E_SIZE;
+    if (M < 0 || M > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxInner) return Z1_E_SIZE;
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (M == 0 || N == 0) return 0;
     const int blocks = wide_of(K) / kBlock;
@@ -1069,7 +1070,7 @@ int z1_product8(const void* a, const void* as, int64_t M, const void* w, const v
 }
 
 int64_t z1_weight_grad8_workspace(int64_t T, int64_t N, int64_t K) {
-    if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim) return Z1_E_SIZE;
+    if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxInner) return Z1_E_SIZE;
     if (N == 0) return 0;
     const int direct = gradient_way(T, N, K, true).parts, staged = gradient_way(T, N, K, false).parts;
     const int64_t parts = direct > staged ? direct : staged;                   // dy's rows may be either
@@ -1079,7 +1080,7 @@ int64_t z1_weight_grad8_workspace(int64_t T, int64_t N, int64_t K) {
 int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const void* s, int64_t T, int64_t N, int64_t K,
                     void* dw, int dtype, float* workspace, int64_t workspace_floats, void* stream) {
     // a step's rows lie within 32 bits of its first
-    if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxDim || stride < 0 || stride > kMaxDim) return Z1_E_SIZE;
+    if (T < 0 || T > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxInner || stride < 0 || stride > kMaxDim) return Z1_E_SIZE;
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (N == 0) return Z1_OK;
     if (!dw || (T > 0 && (!dy || !q || !s))) return Z1_E_NULL;

@@ -298,7 +298,7 @@ int z1_weight8_pack(const void* w, int64_t N, int64_t K, int64_t stride, int dty
                     void* stream);
 
 /* y[M][N] (dtype) = 8-bit rows a, as [M][K] times the transpose of 8-bit weight w, ws [N][K].  The input gradient is the
- * same product with the rows of dy and the weight's other order.  workspace: device floats,
+ * same product with the rows of dy and the weight's other order.  K at most 2^22, here and below.  workspace: device floats,
  * z1_product8_workspace(M, N, K, dtype) of them (none for most shapes; NULL then). */
 int z1_product8(const void* a, const void* as, int64_t M, const void* w, const void* ws, int64_t N, int64_t K, void* y,
                 int dtype, float* workspace, int64_t workspace_floats, void* stream);
