@@ -152,24 +152,12 @@ struct Workspace {
     }
 };
 
-// A tensor of whole elements in `of`'s storage, `offset` of them from its start.
-Tensor within(const Tensor& of, at::IntArrayRef size, at::ScalarType dtype, int64_t offset) {
-    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(of.storage()), of.key_set(),
-                                                      c10::scalarTypeToTypeMeta(dtype));
-    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
-    t.unsafeGetTensorImpl()->set_storage_offset(offset);
-    return t;
-}
-
 struct Pair {
     Tensor q, s;
 };
-// Values and scales in one allocation (0.4 us of host time each): they are made, kept and freed together.
 Pair empty8(int64_t rows, int64_t dim, int64_t scale_rows, const char* what) {
-    const int64_t wide = wide_of(dim, what), pitch = api().act8_scales(dim);
-    const Tensor both = fresh({rows * wide + scale_rows * pitch}, at::kByte);
-    return {within(both, {rows, wide}, at::kFloat8_e4m3fn, 0),
-            within(both, {scale_rows, pitch}, at::kFloat8_e8m0fnu, rows * wide)};
+    const int64_t wide = wide_of(dim, what);
+    return {fresh({rows, wide}, at::kFloat8_e4m3fn), fresh({scale_rows, api().act8_scales(dim)}, at::kFloat8_e8m0fnu)};
 }
 
 struct OnDevice {
@@ -209,16 +197,12 @@ std::vector<Tensor> norm_forward(const Tensor& x, const OptTensor& weight, const
         out.push_back(fresh({r.rows, r.dim}, x.scalar_type()));
         y = out.back().data_ptr();
     }
-    const Tensor stats = fresh({center ? 2 * r.rows : r.rows}, at::kFloat);
-    float* rstd = static_cast<float*>(stats.data_ptr());
     if (center) {
-        mean = rstd;
-        rstd += r.rows;
-        out.push_back(within(stats, {r.rows}, at::kFloat, 0));
-        out.push_back(within(stats, {r.rows}, at::kFloat, r.rows));
-    } else {
-        out.push_back(stats);
+        out.push_back(fresh({r.rows}, at::kFloat));
+        mean = static_cast<float*>(out.back().data_ptr());
     }
+    out.push_back(fresh({r.rows}, at::kFloat));
+    float* rstd = static_cast<float*>(out.back().data_ptr());
     if (checkpoint) {
         Pair p = empty8(r.rows, r.dim, r.rows, what);
         cq = p.q.data_ptr();
