@@ -10,6 +10,7 @@
 fp32; the weight's gradient reads dy in bf16 and the checkpoint's values, which bf16 holds exactly.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import act8, library  # noqa: F401  (library registers the operators)
 from .act8 import Act8
@@ -67,6 +68,7 @@ class _Linear(torch.autograd.Function):
         return matmul(a, w8, x.dtype).view(*x.shape[:-1], w8.shape[0])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dx = dw = None
         if ctx.needs_input_grad[0]:

@@ -5,6 +5,7 @@ The forward pass reads x once and can write, in that pass, y in 8 bits (``y8``: 
 Statistics are fp32, taken about the mean.
 """
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import act8, library  # noqa: F401  (library registers the operators)
 from .act8 import Act8
@@ -17,13 +18,10 @@ def _forward(x, weight, bias, eps, center, y8, checkpoint):
     r = act8.rows_of(x)
     out = _norm_forward(r, weight, bias, eps, center, y8, checkpoint)
     d = x.shape[-1]
-    if y8:
-        out[0:2] = [Act8(out[0], out[1], d)]
-    elif x.dim() != 2:
-        out[0] = out[0].view(x.shape)
+    y, stats = (Act8(out[0], out[1], d), out[2:]) if y8 else (out[0] if x.dim() == 2 else out[0].view(x.shape), out[1:])
     if checkpoint:
-        out[-2:] = [Act8(out[-2], out[-1], d)]
-    return tuple(out)
+        return (y, *stats[:-2], Act8(stats[-2], stats[-1], d))
+    return (y, *stats)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, y8=False, checkpoint=False):
@@ -48,7 +46,7 @@ def _backward(dy, x, mean, rstd, weight, center, need_weight, need_bias):
     else:
         out = _norm_backward(r, act8.rows_of(x), None, None, mean, rstd, weight, center, need_weight, need_bias)
     if dy.dim() != 2:
-        out[0] = out[0].view(dy.shape)
+        return (out[0].view(dy.shape), *out[1:])
     return tuple(out)
 
 
@@ -74,6 +72,7 @@ class _Norm(torch.autograd.Function):
         return out[0]
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         kept, s, mean, rstd, weight = ctx.saved_tensors
         x = Act8(kept, s, dy.shape[-1]) if ctx.checkpoint else kept
