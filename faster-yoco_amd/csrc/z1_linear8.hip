@@ -476,7 +476,7 @@ __device__ __forceinline__ u4 shift_pieces(u4 v, int n) {
 }
 
 // Where dy's rows do not start at whole dwords, as with an odd N, both operands are staged through registers (8191 x 3072 over
-// 2048 tokens: 143 us, where 8192 x 3072 takes 98 by the direct loads below; 7 x 3072 over 16384 tokens 57, in parts).
+// 2048 tokens: 143 us, where 8192 x 3072 takes 95 by the direct loads below; 7 x 3072 over 16384 tokens 47, in parts).
 // BN x BK of dw to a workgroup, WN x WK to a wave, TS tokens staged at a time, twice buffered.  While a step's products
 // run, the next step's pieces go from registers into the other buffer, and the pieces of the step after that are loaded
 // into those registers: a load has a whole step to arrive, and neither staging nor opening stands between two steps.  The
@@ -496,7 +496,8 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     auto lds_k = [&](int buf) { return lds + (2 * kPitchN + buf * kPitchK) * TS; };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_k = (a.K + BK - 1) / BK;
-    const int n0 = (int)(blockIdx.x / tiles_k) * BN, k0 = (int)(blockIdx.x % tiles_k) * BK;
+    const At tile = in_panels(tiles_k, 4);             // 7 x 3072 over 16384 tokens: 52 us in order, 47
+    const int n0 = tile.down * BN, k0 = tile.across * BK;
     const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
     take_part(a);
 
@@ -646,7 +647,7 @@ __device__ __forceinline__ int placed(int run, int token) {
 
 // The same where dy's rows start at whole dwords: dy goes straight into LDS, and both operands are staged the way the
 // product's are.  8192 x 8192 over 8192 tokens: 880 us, 1.25 PFLOP/s (715 with zeros: power again; without opening a's values
-// 746), 8192 x 3072 over 2048: 97 us, over 16384: 736.  a's values opened once more beside the products instead of on the way
+// 746), 8192 x 3072 over 2048: 95 us, over 16384: 736.  a's values opened once more beside the products instead of on the way
 // into LDS: 1058 us; four waves of 128 x 128 924, 128 x 128 tiles 1117.  Rows of both lie whole in LDS; a transposing read
 // takes 64 bytes of four tokens at a time, so a row's 64-byte runs are placed (`placed`) so that the four lie in different
 // banks.  What lies past the last token or past a tensor's end is zero (the buffers' ranges).
