@@ -127,7 +127,8 @@ __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
 }
 
-// A raw buffer of `bytes` (none where negative) from p: loads past it give zeros (word 3: the raw 32-bit data format).
+// A raw buffer of `bytes` (none where negative) from p: loads whose lane offset lies past it give zeros (word 3: the raw
+// 32-bit data format).  The scalar offset of a load need not count in that check: it only moves within a row's own bytes.
 // Without a branch: a loop around it keeps its loads on their way.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64_t bytes) {
     const uint32_t low = (uint32_t)bytes, high = (uint32_t)(bytes >> 32);
@@ -203,18 +204,19 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     a.as += kb0;
     a.ws += kb0;
     const int64_t before = (int64_t)kb0 * kBlock;
-    // Rows past the end lie past their buffer's range, which a load turns to zeros.
+    // A row goes into a load's lane offset, which the buffer's range checks: rows past the end become zeros.  The block of K
+    // goes into the scalar offset, which stays in the row: past the last block the last one is loaded again, not used.
     const __amdgpu_buffer_rsrc_t buf_t = buffer_of(a.a + t0 * a.wide, (a.M - t0) * a.wide - before);
     const __amdgpu_buffer_rsrc_t buf_o = buffer_of(a.w + o0 * a.wide, (a.N - o0) * a.wide - before);
-    const int wide = (int)a.wide;
+    const int wide = (int)a.wide, last = blocks - 1;
     const int sub = lane >> 3, piece = lane & 7;
     const int from = sub * wide + ((piece ^ (sub >> 1)) << 4);                 // in 8 rows whose keys' third bit is 0
     auto stage = [&](int kb, int i) {                  // the i-th direct load of this wave's part of a block
         uint8_t* buf = lds[kb & (S - 1)];
         const int g = i < kPT ? wave * kPT + i : wave * kPO + i - kPT;
-        const int at = g * 8 * wide + kb * kBlock;
-        if (i < kPT) load_lds(buf_t, buf + g * 8 * kBlock, g & 1 ? from ^ 64 : from, at);
-        else load_lds(buf_o, buf + (BT + g * 8) * kBlock, g & 2 ? from ^ 64 : from, at);
+        const int at = (kb < last ? kb : last) * kBlock, row = g * 8 * wide;
+        if (i < kPT) load_lds(buf_t, buf + g * 8 * kBlock, row + (g & 1 ? from ^ 64 : from), at);
+        else load_lds(buf_o, buf + (BT + g * 8) * kBlock, row + (g & 2 ? from ^ 64 : from), at);
     };
     // scales: four blocks' bytes at a time, the next four loaded ahead
     const __amdgpu_buffer_rsrc_t buf_s = buffer_of(a.as + t0 * a.pitch, (a.M - t0) * a.pitch - kb0);
@@ -224,14 +226,14 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     __amdgpu_buffer_rsrc_t sw[NB];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-        const int ob = (o0 + wo + i * 32) / kBlock, last = (a.N - 1) / kBlock;
-        sw[i] = buffer_of(a.ws + (int64_t)(ob < last ? ob : last) * a.pitch, a.pitch - kb0);
+        const int ob = (o0 + wo + i * 32) / kBlock, end = (a.N - 1) / kBlock;
+        sw[i] = buffer_of(a.ws + (int64_t)(ob < end ? ob : end) * a.pitch, a.pitch - kb0);
     }
     uint32_t now[NT] = {}, next[NT], now_w[NB] = {}, next_w[NB];
     auto scales = [&](int kb) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
-            next[j] = __builtin_amdgcn_raw_buffer_load_b32(buf_s, r32 * a.pitch, (wt + j * 32) * a.pitch + kb, 0);
+            next[j] = __builtin_amdgcn_raw_buffer_load_b32(buf_s, (wt + j * 32 + r32) * a.pitch, kb, 0);
 #pragma unroll
         for (int i = 0; i < NB; ++i) next_w[i] = __builtin_amdgcn_raw_buffer_load_b32(sw[i], 0, kb, 0);
     };
@@ -686,13 +688,14 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(from) / sizeof(int)); ++i)
         from[i] = sub * row_bytes + (placed<BN / 32>(piece >> 2, i * kLoadRows + sub) << 2 | (piece & 3)) * 16;
-    // from the tile's first column to dy's end, in whole dwords (an odd N's last one holds nothing that is used)
+    // from the tile's first column to dy's end, in whole dwords (an odd N's last one holds nothing that is used); a load's
+    // token goes into its lane offset, which this range checks
     const int64_t bytes_n = a.T > 0 ? (a.T - 1) * row_bytes + ((a.N - n0 + 1) & ~1) * 2 : 0;
     auto stage = [&](int64_t step, int i, uint8_t* to) {
         const int64_t t0 = step * TS;
         const int g = wave * kLoads + i;
         const __amdgpu_buffer_rsrc_t rows = buffer_of(a.dy + t0 * a.stride + n0, bytes_n - t0 * row_bytes);
-        load_lds(rows, to + g * 1024, from[kLoadRows == 2 ? g & 1 : 0], g * kLoadRows * row_bytes);
+        load_lds(rows, to + g * 1024, from[kLoadRows == 2 ? g & 1 : 0] + g * kLoadRows * row_bytes, 0);
     };
     uint32_t x[kX][P / 4], xs[kX];
     int at_q[kX], at_s[kX], at_k[kX];                  // of the pieces: offsets in a step's rows, and in LDS
