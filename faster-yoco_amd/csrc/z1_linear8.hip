@@ -4,10 +4,9 @@
 //   product    y[t, o] = sum over blocks j of 2^(e[t, j] + f[o / 128, j]) * sum over k in j of a[t, k] w[o, k]
 //   gradient   dw[o, k] = sum over t of dy[t, o] * a[t, k] 2^e[t, k / 128]
 //
-// The matrix instructions apply the powers of two themselves (v_mfma_scale_f32_32x32x64_f8f6f4 takes one E8M0 byte for
-// each lane's 32 values), so a product accumulates over all of K in its fp32 accumulators without a pass of its own for
-// the scales.  The gradient's sum runs over tokens, each with a scale of its own: its rows are opened to bf16, which
-// holds them exactly, while they are staged, and multiplied by the bf16 instructions.
+// Both open their 8-bit operands to bf16, which holds values and scales exactly, and multiply by the bf16 instructions, whose
+// products and sums are fp32: a product on the way from LDS into the instructions, so that 8 bits are moved and staged; the
+// gradient, whose sum runs over tokens, on the way into LDS.
 #include "z1_block.h"
 
 #pragma clang fp contract(off)
@@ -25,13 +24,12 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 #define Z1B_LDS __attribute__((address_space(3)))
 
-constexpr int kE4M3 = 0;                               // the matrix instructions' code of the format
-
 // The 32 x 32 result of a matrix instruction gives lane l column l % 32 and rows 8 (i/4) + 4 (l/32) + i%4, i = 0..15.
 // Reading its first operand's rows in this order makes those 16 consecutive: 16 (l/32) + i.
 __device__ __forceinline__ int spread(int row) { return 16 * ((row >> 2) & 1) + 4 * (row >> 3) + (row & 3); }
 
-// Eight bytes of a row and its scale, opened to bf16 (exact: 4 significant bits, and bf16 has fp32's exponents).
+// Eight bytes of a row and its scale, opened to bf16 (exact: 4 significant bits, and bf16 has fp32's exponents; what is below
+// its least value, 2^-133, rounds to a multiple of that).
 __device__ __forceinline__ u4 open_bf16(u2 q, float f) {
     u4 r;
     r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[0], f, false));
@@ -41,32 +39,27 @@ __device__ __forceinline__ u4 open_bf16(u2 q, float f) {
     return r;
 }
 
-// Adds the products of two 32-row fragments of 64 columns.  The 8-bit instructions sum 8 products at a time on a common
-// exponent and cut what is more than 13 bits below the largest (probed: 256 + 2^-5 arrives, 256 + 2^-6 does not, while
-// sums across groups keep 24 bits), an error of 1.5e-5 of the result on activations: far below a 16-bit result's own
-// rounding, not below an fp32 one's.  The precise form opens both operands to bf16 (exact) for the bf16 instructions, whose
-// sums are fp32 throughout, at half the rate (2048 rows of 3072 -> 8192, fp32: 91 us, 1.13 PFLOP/s; bf16: 42, 2.45).
-__device__ __forceinline__ f16 multiply(f16 acc, i8 fo, i8 ft, uint32_t so, uint32_t st) {
-    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fo, ft, acc, kE4M3, kE4M3, 0, (int)so, 0, (int)st);
-}
-template <int NO, int NT>
-__device__ __forceinline__ void multiply_precise(f16 (&acc)[NO][NT], const i8 (&fo)[NO], const i8 (&ft)[NT],
-                                                 const uint32_t (&so)[1], const uint32_t (&st)[NT]) {
-    const float go = scale_value(so[0] & 0xffu);
+// Adds the products of NO by NT fragments of 32 rows, the s-th 16 of their 64 columns (8 bytes of a lane): both operands are
+// opened to bf16 with their scales (exact) for the bf16 instructions, whose products and sums are fp32.  The 8-bit
+// instructions have twice the rate but sum 8 products at a time on a common exponent and cut what lies more than 13 bits
+// below the largest (probed: 256 + 2^-5 arrives, 256 + 2^-6 does not): up to 7 * 2^-13 of it is lost, a sum in fewer bits
+// than 32.  after(m): what is issued beside the m-th product.
+template <int NO, int NT, int NB, typename After>
+__device__ __forceinline__ void multiply(f16 (&acc)[NO][NT], int s, const i8 (&fo)[NO], const i8 (&ft)[NT],
+                                         const uint32_t (&so)[NB], const uint32_t (&st)[NT], After after) {
+    auto open = [&](const i8& f, uint32_t scale) {
+        return __builtin_bit_cast(b8, open_bf16(u2{(uint32_t)f[2 * s], (uint32_t)f[2 * s + 1]}, scale_value(scale & 0xffu)));
+    };
+    b8 bo[NO], bt[NT];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {                      // 8 bytes of a lane: 16 columns of the wave
-        u4 bo[NO], bt[NT];
+    for (int i = 0; i < NO; ++i) bo[i] = open(fo[i], so[NB == 1 ? 0 : i]);
 #pragma unroll
-        for (int i = 0; i < NO; ++i) bo[i] = open_bf16(u2{(uint32_t)fo[i][2 * s], (uint32_t)fo[i][2 * s + 1]}, go);
+    for (int j = 0; j < NT; ++j) bt[j] = open(ft[j], st[j]);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-            bt[j] = open_bf16(u2{(uint32_t)ft[j][2 * s], (uint32_t)ft[j][2 * s + 1]}, scale_value(st[j] & 0xffu));
-#pragma unroll
-        for (int i = 0; i < NO; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, bo[i]),
-                                                                    __builtin_bit_cast(b8, bt[j]), acc[i][j], 0, 0, 0);
+    for (int m = 0; m < NO * NT; ++m) {
+        const int i = m / NT, j = m % NT;
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bo[i], bt[j], acc[i][j], 0, 0, 0);
+        after(m);
     }
 }
 
@@ -177,11 +170,11 @@ __device__ __forceinline__ int key_spread(int row) { return (row >> 1 & 3) | (ro
 // BT x BO outputs (tokens x outputs) of a workgroup, WT x WO of a wave, S blocks of K staged: two leave room for a second
 // workgroup on a CU (of 128 x 128), four cover the loads' way where there is no second one.
 //
-// Large products are bound by the card's power: 8192 x 8192 x 8192 takes 415 us (2.65 PFLOP/s) with random operands and 297
-// with zeros.  So are bytes moved: eight waves of 64 x 128 read each operand from LDS fewer times than waves of 64 x 64,
-// and 256 x 128 tiles (654 us), four waves of 128 x 128 (428) or eight of 128 x 64 (451) all lost.  Smaller ones are bound by
-// the loads' latency and by CUs without a tile (below, where the tile is chosen).
-template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
+// Large products are bound by the card's power: 8192 x 8192 x 8192 takes 739 us (1.49 PFLOP/s) with random operands and 582
+// with zeros; what counts there is products to an opened value, hence eight waves of 64 x 128 (128 x 128 tiles: 869 to 892).
+// Smaller ones are bound by the opening, which a wave does for itself (32 x 32 of a wave: 8 conversions to a product, 64 x 64:
+// 4), and by CUs without a tile (below, where the tile is chosen).
+template <typename T, int BT, int BO, int WT, int WO, int S>
 __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Product a) {
     constexpr int kWaves = BT / WT * (BO / WO);
     constexpr int kPT = BT / 8 / kWaves, kPO = BO / 8 / kWaves;                // direct loads of a wave: 8 rows each
@@ -190,9 +183,9 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     __shared__ __align__(1024) uint8_t lds[S][(BT + BO) * kBlock];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_o = (a.N + BO - 1) / BO;
-    // Every eighth of a multiple of eight columns of tiles is a few whole columns: a good share already (3072 -> 8192, 16384
-    // rows: 354 us, in panels of 8 374; 8192 -> 3072, where it is not one: 342 in order, 320 in panels of 8, 325 of 4).
-    const At tile = tiles_o & 7 ? in_panels(tiles_o, 8) : in_order(tiles_o);
+    // 16384 rows, in order against panels of 8 (panels of 4): 8192 -> 3072 566 us, 551 (556); 4096 -> 4096 384, 380 (381);
+    // 2048 -> 5120 255, 251 (250); 1536 -> 6144 242, 239 (236); 3072 -> 8192 577, 578 (576).
+    const At tile = in_panels(tiles_o, 8);
     const int64_t t0 = (int64_t)tile.down * BT;
     const int o0 = tile.across * BO;
     const int wt = wave / (BO / WO) * WT, wo = wave % (BO / WO) * WO;          // the wave's part of the tile
@@ -247,10 +240,10 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
 
     // A block's two halves of 64 columns are read ahead by one half, and the workgroup meets between them: what follows
     // the meeting -- the next block's first reads, the direct loads into the buffer that has just been read -- runs beside
-    // the second half's products, one read or load after each, and what it waits for was issued S - 1 blocks before.
-    // (All loads at once after the meeting hold up the products until the address unit has taken them: 64 loads of 16
-    // cycles.)  Past the last block the reads and loads are of no use, and in bounds.
-    constexpr int kReads = 2 * (NT + NO), kLoads = kPT + kPO, kProducts = NT * NO;
+    // the second half's products, spread over them, and what it waits for was issued S - 1 blocks before.  Past the last
+    // block the reads and loads are of no use, and in bounds.  (2048 rows of 8192 -> 3072: 88 us, with all reads and loads
+    // before the products 92.)
+    constexpr int kReads = 2 * (NT + NO), kLoads = kPT + kPO, kProducts = 4 * NT * NO;
     i4 f[2][NT + NO][2];
     auto read = [&](int kb, int h, int q) {
         const int i = q >> 1, p = 4 * h + 2 * half + (q & 1);
@@ -260,31 +253,24 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
     };
     // products of half h; beside them, the reads of half 1 - h of block kb_read and the loads of block kb_load (< 0: none)
     auto products = [&](int h, int kb_read, int kb_load) {
-        auto beside = [&](int m, int of) {
+        auto beside = [&](int m) {
 #pragma unroll
             for (int q = 0; q < kReads; ++q)
-                if (q * of / kReads == m) read(kb_read, 1 - h, q);
+                if (q * kProducts / kReads == m) read(kb_read, 1 - h, q);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
-                if (kb_load >= 0 && i * of / kLoads == m) stage(kb_load, i);
+                if (kb_load >= 0 && i * kProducts / kLoads == m) stage(kb_load, i);
         };
         auto pair = [&](int i) { return __builtin_shufflevector(f[h][i][0], f[h][i][1], 0, 1, 2, 3, 4, 5, 6, 7); };
-        if constexpr (PRECISE) {
-            beside(0, 1);
-            i8 ft[NT], fo[NO];
+        i8 ft[NT], fo[NO];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) ft[j] = pair(j);
+        for (int j = 0; j < NT; ++j) ft[j] = pair(j);
 #pragma unroll
-            for (int i = 0; i < NO; ++i) fo[i] = pair(NT + i);
-            multiply_precise(acc, fo, ft, now_w, now);
-        } else {
+        for (int i = 0; i < NO; ++i) fo[i] = pair(NT + i);
 #pragma unroll
-            for (int m = 0; m < kProducts; ++m) {
-                const int i = m / NT, j = m % NT;
-                acc[i][j] = multiply(acc[i][j], pair(NT + i), pair(j), now_w[NB == 1 ? 0 : i], now[j]);
-                beside(m, kProducts);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int s = 0; s < 4; ++s) {
+            multiply(acc, s, fo, ft, now_w, now, [&](int m) { beside(s * NO * NT + m); });
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 #pragma unroll
@@ -331,11 +317,11 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void product_kernel(Produ
 // a block of K of its own: the results on its diagonal are that many partial sums, so that a narrow output has workgroups for
 // all CUs.  A wave stages its own steps by direct loads, two under way: a lane's 16 bytes lie beside its neighbours', where
 // fragments loaded into registers would be pieces of 32 rows to an instruction, and the address unit the bound (32 rows of
-// 8192 -> 3072: 18 us, 10.0 this way).  Bound by the weight's bytes where they are many (one row of 3072 -> 100288: 54 us, 5.7
-// TB/s), else by the launch and the loads' latency (3072 -> 8192: 6.0 us, 4.2 TB/s, from the last cache).  Three or four steps
-// under way, or eight waves, leave room for fewer workgroups and lost (one row: 9 to 14 us).
+// 8192 -> 3072: 18 us, 9.8 this way).  Bound by the weight's bytes where they are many (one row of 3072 -> 100288: 56 us, 5.5
+// TB/s), else by the launch and the loads' latency (3072 -> 8192: 6.6 us, 3.8 TB/s, from the last cache).  Three or four steps
+// under way, or eight waves, leave room for fewer workgroups and lost.
 constexpr int kFewWaves = 4;
-template <typename T, bool PRECISE, int OB, int R>
+template <typename T, int OB, int R>
 __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(Product a) {
     static_assert(R == 1 || OB == 32, "more row fragments than one are whole ones");
     constexpr int G = 32 / OB, U = 2, W = kFewWaves;   // blocks of K to an instruction; steps under way
@@ -413,12 +399,8 @@ __global__ __launch_bounds__(kFewWaves * 64) void product_few_kernel(Product a) 
                 i8 fx[R];
 #pragma unroll
                 for (int j = 0; j < R; ++j) fx[j] = pair(1 + j);
-                if constexpr (PRECISE) {
-                    multiply_precise(acc, fw, fx, so, st);
-                } else {
 #pragma unroll
-                    for (int j = 0; j < R; ++j) acc[0][j] = multiply(acc[0][j], fw[0], fx[j], so[0], st[j]);
-                }
+                for (int s = 0; s < 4; ++s) multiply(acc, s, fw, fx, so, st, [](int) {});
             }
         }
     }
@@ -847,15 +829,16 @@ int join(const float* part, int parts, int64_t count, void* out, hipStream_t st)
 
 // The number of parts into which the long axis of a product in small tiles is cut, `steps` of it in multiples of `unit`:
 // the one with the least estimate of the time, which *ns is.  A step takes `alone` where a CU has one tile, `shared` where
-// it has two (0: it has no room for two); joining takes 3.3 us and 0.05 a part, and the partial results' way out and back at
-// 5 bytes/ps.
-int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int alone, int shared, int64_t* ns) {
+// it has two (0: it has no room for two); joining takes 3.3 us and 0.05 a part, and the partial results' way out and back, at
+// `rate` bytes/ns.
+constexpr int kProductRate = 16000, kGradientRate = 5000;          // as the shapes that these rules decide measured
+int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int rate, int alone, int shared, int64_t* ns) {
     int best = 1;
     *ns = 0;
     for (int p = 1; p <= kMaxParts; ++p) {
         const int64_t per = (steps + p * unit - 1) / (p * unit) * unit;
         if (p > 1 && (per * (p - 1) >= steps || tiles * p > (shared ? 2 * kCus : kCus))) continue;     // no steps; no room
-        const int64_t time = per * (tiles * p <= kCus ? alone : shared) + (p > 1 ? 3300 + p * (50 + results * 8 / 5000) : 0);
+        const int64_t time = per * (tiles * p <= kCus ? alone : shared) + (p > 1 ? 3300 + p * (50 + results * 8 / rate) : 0);
         if (p == 1 || time < *ns) best = p, *ns = time;
     }
     return best;
@@ -863,20 +846,20 @@ int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int alone,
 
 // How a product runs.
 //
-// Many tiles: large ones (256 x 256) move fewer bytes per product, smaller ones leave fewer CUs without work.  A round of
-// large ones, one to a CU, takes 100; of 128 x 128, two to a CU, 63; of 128 x 192, one to a CU, 55 (8192 -> 3072 with 2048
-// rows: 384 of 128 x 128 in 54.0 us, 256 of 128 x 192 in 47.4; with 4096 rows 192 large ones in 86, 512 of 128 x 192 in 93;
-// 8192 x 8192 x 8192: 415 large, 553 of 128 x 128).
+// Many tiles: large ones (256 x 256) open fewer values per product, smaller ones leave fewer CUs without work.  A round of
+// large ones, one to a CU, takes 100; of 128 x 128, two to a CU, 59; of 128 x 192, one to a CU, 51 (us: 3072 -> 8192 with 2048
+// rows 76 in 256 x 256, 86 in 128 x 128, 98 in 128 x 192; 8192 -> 3072 142, 94, 87, and with 4096 rows 157, 169, 179; 1536 ->
+// 6144 with 2048 rows 36, 36, 41).
 //
-// Up to one of 128 x 128 to a CU: what bounds a tile is how fast its one CU gets the operands, so smaller tiles on more CUs
-// win while there are CUs (kSmall: a start and a block of K, in ns, as measured), and where even they leave CUs idle, a long
-// K is cut into parts, joined by a second launch.  1000 -> 1501, 333 rows: 5.7 us in 64 x 64, 8.0 in 128 x 128; 3072 -> 8192,
-// 256 rows: 11.4 in 64 x 128, 13.8 in 128 x 128; 8192 -> 3072, 512 rows: 21.6 in 64 x 128, 22.7 in 128 x 128 of two parts;
-// 128 rows: 26.8 in 128 x 128, 14.6 of four parts.
+// Up to one of 128 x 128 to a CU: smaller tiles on more CUs win while there are CUs (kSmall: a start and a block of K, in ns,
+// as measured), and where even they leave CUs idle, a long K is cut into parts, joined by a second launch.  1000 -> 1501, 333
+// rows: 6.4 us in 64 x 64, 11.6 in 128 x 128; 4096 -> 4096, 512 rows: 23.9 in 64 x 128, 24.6 in 64 x 64, 27.3 in 128 x 128 of
+// two parts, 1024 rows: 34.9 in 128 x 128, 45 in either other; 8192 -> 3072, 512 rows: 34.6 in 128 x 128 of four parts, 39.6
+// in 64 x 64; 128 rows: 31 in 64 x 64, 17.9 of four parts.
 //
-// Up to 64 rows the few rows' kernel runs where it is faster, a workgroup to a CU, at 2.5 us and 0.1 to 0.23 us a block of K,
-// more with more of them and more rows (33 rows, 3072 -> 3072: 6.2 us against 8.4, 3072 -> 8192: 7.3 against 8.6; 64 rows, 8192
-// -> 3072: 14.0 against 12.3).
+// Up to 64 rows the few rows' kernel runs where it is faster, a workgroup to a CU, at 3.3 us and 0.12 to 0.25 us a block of K,
+// more with more of them and more rows (33 rows, 3072 -> 3072: 6.9 us against 13.4, 3072 -> 8192: 8.3 against 13.5; 64 rows,
+// 8192 -> 3072: 14.4 against 14.3 in 64 x 64 of eight parts).
 struct Way {
     bool few;
     int rows, outputs;                                 // of a tile
@@ -885,7 +868,7 @@ struct Way {
 struct Small {
     int rows, outputs, start, alone, shared;
 };
-constexpr Small kSmall[] = {{128, 128, 4200, 330, 620}, {64, 128, 2700, 300, 0}, {64, 64, 2900, 230, 400}};
+constexpr Small kSmall[] = {{128, 128, 5400, 940, 1590}, {64, 128, 4000, 600, 0}, {64, 64, 3100, 450, 630}};
 // The best of them for M x N results (M x N 128 x 128 tiles at most one to a CU, or the first is taken).
 struct Cut {
     const Small* tile;
@@ -893,97 +876,80 @@ struct Cut {
     int64_t ns;
 };
 template <int COUNT>
-Cut best_of(const Small (&small)[COUNT], int64_t M, int64_t N, int64_t steps, int unit) {
+Cut best_of(const Small (&small)[COUNT], int64_t M, int64_t N, int64_t steps, int unit, int rate) {
     Cut best{nullptr, 1, 0};
     for (const Small& t : small) {
         const int64_t n = (M + t.rows - 1) / t.rows * ((N + t.outputs - 1) / t.outputs);
         if (best.tile && n > (t.shared ? 2 * kCus : kCus)) continue;
         int64_t ns;
-        const int parts = parts_of(n, steps, unit, M * N, t.alone, t.shared, &ns);
+        const int parts = parts_of(n, steps, unit, M * N, rate, t.alone, t.shared, &ns);
         if (!best.tile || t.start + ns < best.ns) best = {&t, parts, t.start + ns};
     }
     return best;
 }
-Way product_way(int64_t M, int64_t N, int blocks, bool precise) {
+Way product_way(int64_t M, int64_t N, int blocks) {
     if (M <= 32) return {true, 0, 0, 1, blocks};
     auto tiles = [&](int rows, int outputs) { return (M + rows - 1) / rows * ((N + outputs - 1) / outputs); };
     auto rounds = [&](int rows, int outputs, int at_once) { return (tiles(rows, outputs) + at_once - 1) / at_once; };
     if (tiles(128, 128) > kCus) {
-        const int64_t large_time = 100 * rounds(256, 256, kCus), middle_time = 55 * rounds(128, 192, kCus);
-        if (precise || 63 * rounds(128, 128, 2 * kCus) <= (large_time < middle_time ? large_time : middle_time))
+        const int64_t large_time = 100 * rounds(256, 256, kCus), middle_time = 51 * rounds(128, 192, kCus);
+        if (59 * rounds(128, 128, 2 * kCus) <= (large_time < middle_time ? large_time : middle_time))
             return {false, 128, 128, 1, blocks};
         if (large_time <= middle_time) return {false, 256, 256, 1, blocks};
         return {false, 128, 192, 1, blocks};
     }
-    const Cut cut = best_of(kSmall, M, N, blocks, 4);
+    const Cut cut = best_of(kSmall, M, N, blocks, 4, kProductRate);
     const int64_t groups = (N + 31) / 32;              // workgroups of few rows; with less than 64, the parts read K sooner
     const int64_t few_rounds = (groups + kCus - 1) / kCus, at_once = groups < kCus ? groups : kCus;
-    if (M <= 64 && groups >= 64 && 2500 + few_rounds * blocks * (100 + at_once * M / 128) <= cut.ns)
+    if (M <= 64 && groups >= 64 && 3300 + few_rounds * blocks * (120 + at_once * M / 128) <= cut.ns)
         return {true, 0, 0, 1, blocks};
     return {false, cut.tile->rows, cut.tile->outputs, cut.parts,
             cut.parts == 1 ? blocks : (blocks + 4 * cut.parts - 1) / (4 * cut.parts) * 4};
 }
 
-template <typename T, bool PRECISE, int BT, int BO, int WT, int WO, int S>
+template <typename T, int BT, int BO, int WT, int WO, int S>
 int launch_tiles(const Product& a, int parts, hipStream_t st) {
     const int64_t tiles = (a.M + BT - 1) / BT * ((a.N + BO - 1) / BO);
     if (tiles > kMaxTiles) return Z1_E_SIZE;
-    product_kernel<T, PRECISE, BT, BO, WT, WO, S><<<dim3((unsigned)tiles, parts), BT / WT * (BO / WO) * 64, 0, st>>>(a);
+    product_kernel<T, BT, BO, WT, WO, S><<<dim3((unsigned)tiles, parts), BT / WT * (BO / WO) * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 
-template <typename T, bool PRECISE, int OB, int R>
+template <typename T, int OB, int R>
 int launch_few(const Product& a, hipStream_t st) {
-    product_few_kernel<T, PRECISE, OB, R><<<dim3((unsigned)((a.N + OB - 1) / OB)), kFewWaves * 64, 0, st>>>(a);
+    product_few_kernel<T, OB, R><<<dim3((unsigned)((a.N + OB - 1) / OB)), kFewWaves * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
-
-template <typename T, bool PRECISE>
-int launch_small(const Product& a, const Way& way, hipStream_t st) {
-    if (way.rows == 64 && way.outputs == 64) return launch_tiles<T, PRECISE, 64, 64, 32, 32, 4>(a, way.parts, st);
-    if (way.rows == 64) return launch_tiles<T, PRECISE, 64, 128, 32, 64, 4>(a, way.parts, st);
-    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 127) / 128) * way.parts;
-    return tiles <= kCus ? launch_tiles<T, PRECISE, 128, 128, 64, 64, 4>(a, way.parts, st)
-                         : launch_tiles<T, PRECISE, 128, 128, 64, 64, 2>(a, way.parts, st);
-}
-
-template <typename T, bool PRECISE>
-int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) {
-    if (way.few) {
-        if (a.M > 32) return launch_few<T, PRECISE, 32, 2>(a, st);
-        // the fewest outputs that hold the rows, or more while there are 192 workgroups: one row of 3072 -> 8192 takes 8.4 us
-        // with 8 outputs, 6.9 with 16, 6.0 with 32; 8192 -> 3072 takes 7.2 with 8, 6.4 with 16, 9.2 with 32
-        int outputs = a.M <= 8 ? 8 : a.M <= 16 ? 16 : 32;
-        while (outputs < 32 && a.N >= 2 * outputs * 192) outputs *= 2;
-        if (outputs == 8) return launch_few<T, PRECISE, 8, 1>(a, st);
-        if (outputs == 16) return launch_few<T, PRECISE, 16, 1>(a, st);
-        return launch_few<T, PRECISE, 32, 1>(a, st);
-    }
-    a.per = way.per;
-    if constexpr (!PRECISE) {
-        if (way.outputs == 256) return launch_tiles<T, PRECISE, 256, 256, 64, 128, 2>(a, 1, st);
-        if (way.outputs == 192) return launch_tiles<T, PRECISE, 128, 192, 64, 96, 4>(a, 1, st);
-    }
-    if (way.parts == 1) return launch_small<T, PRECISE>(a, way, st);
-    void* y = a.y;
-    a.y = workspace;
-    if (const int rc = launch_small<F32, PRECISE>(a, way, st)) return rc;
-    return join<T>(workspace, way.parts, a.M * a.N, y, st);
-}
-
-// fp32 results are always precise; 16-bit ones where K is short, since a short sum has few groups over which the cuts
-// average out, and its time goes into the result's writes anyway.
-constexpr int kPreciseBlocks = 3;
-bool is_precise(int dtype, int blocks) { return dtype == Z1_F32 || blocks <= kPreciseBlocks; }
 
 template <typename T>
-int product(const Product& a, const Way& way, float* workspace, hipStream_t st) {
-    return a.blocks <= kPreciseBlocks ? launch_product<T, true>(a, way, workspace, st)
-                                      : launch_product<T, false>(a, way, workspace, st);
+int launch_small(const Product& a, const Way& way, hipStream_t st) {
+    if (way.rows == 64 && way.outputs == 64) return launch_tiles<T, 64, 64, 32, 32, 4>(a, way.parts, st);
+    if (way.rows == 64) return launch_tiles<T, 64, 128, 32, 64, 4>(a, way.parts, st);
+    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 127) / 128) * way.parts;
+    return tiles <= kCus ? launch_tiles<T, 128, 128, 64, 64, 4>(a, way.parts, st)
+                         : launch_tiles<T, 128, 128, 64, 64, 2>(a, way.parts, st);
 }
-template <>
-int product<F32>(const Product& a, const Way& way, float* workspace, hipStream_t st) {
-    return launch_product<F32, true>(a, way, workspace, st);
+
+template <typename T>
+int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) {
+    if (way.few) {
+        if (a.M > 32) return launch_few<T, 32, 2>(a, st);
+        // the fewest outputs that hold the rows, or more while there are 192 workgroups: one row of 3072 -> 8192 takes 9.8 us
+        // with 8 outputs, 8.1 with 16, 6.6 with 32; 8192 -> 3072 8.2, 7.3, 9.2; 4096 -> 4096 6.1, 6.1, 6.2; 5120 -> 1280 4.1, 4.9, 6.0
+        int outputs = a.M <= 8 ? 8 : a.M <= 16 ? 16 : 32;
+        while (outputs < 32 && a.N >= 2 * outputs * 192) outputs *= 2;
+        if (outputs == 8) return launch_few<T, 8, 1>(a, st);
+        if (outputs == 16) return launch_few<T, 16, 1>(a, st);
+        return launch_few<T, 32, 1>(a, st);
+    }
+    a.per = way.per;
+    if (way.outputs == 256) return launch_tiles<T, 256, 256, 64, 128, 2>(a, 1, st);
+    if (way.outputs == 192) return launch_tiles<T, 128, 192, 64, 96, 4>(a, 1, st);
+    if (way.parts == 1) return launch_small<T>(a, way, st);
+    void* y = a.y;
+    a.y = workspace;
+    if (const int rc = launch_small<F32>(a, way, st)) return rc;
+    return join<T>(workspace, way.parts, a.M * a.N, y, st);
 }
 
 template <typename T, Edge EDGE, int BN, int BK, int WN, int WK, int TS>
@@ -1021,9 +987,9 @@ GradientWay gradient_way(int64_t T, int64_t N, int64_t K, bool direct) {
     const bool few = !direct && N < 8;
     if (small > kCus && !few) return {direct, 128, 128, 1, T};
     const int64_t steps = (T + kStep - 1) / kStep;
-    const Cut cut = direct ? best_of(kSmallDirect, N, K, steps, 1)
-                    : few  ? best_of(kSmallFew, N, K, steps, 1)
-                           : best_of(kSmallStaged, N, K, steps, 1);
+    const Cut cut = direct ? best_of(kSmallDirect, N, K, steps, 1, kGradientRate)
+                    : few  ? best_of(kSmallFew, N, K, steps, 1, kGradientRate)
+                           : best_of(kSmallStaged, N, K, steps, 1, kGradientRate);
     return {direct, cut.tile->rows, cut.tile->outputs, cut.parts,
             cut.parts == 1 ? T : (steps + cut.parts - 1) / cut.parts * kStep};
 }
@@ -1069,7 +1035,7 @@ int64_t z1_product8_workspace(int64_t M, int64_t N, int64_t K, int dtype) {
     if (bad_dtype(dtype)) return Z1_E_DTYPE;
     if (M == 0 || N == 0) return 0;
     const int blocks = wide_of(K) / kBlock;
-    const Way way = product_way(M, N, blocks, is_precise(dtype, blocks));
+    const Way way = product_way(M, N, blocks);
     return way.parts > 1 ? way.parts * M * N : 0;
 }
 
@@ -1083,12 +1049,12 @@ int z1_product8(const void* a, const void* as, int64_t M, const void* w, const v
     const int blocks = wide_of(K) / kBlock;
     const Product p{(const uint8_t*)a, (const uint8_t*)as, (const uint8_t*)w, (const uint8_t*)ws, y, blocks, M, (int)N,
                     blocks, pitch_of(K), wide_of(K)};
-    const Way way = product_way(M, N, blocks, is_precise(dtype, blocks));
+    const Way way = product_way(M, N, blocks);
     const hipStream_t st = (hipStream_t)stream;
     switch (dtype) {
-        case Z1_F32: return product<F32>(p, way, workspace, st);
-        case Z1_BF16: return product<BF16>(p, way, workspace, st);
-        default: return product<F16>(p, way, workspace, st);
+        case Z1_F32: return launch_product<F32>(p, way, workspace, st);
+        case Z1_BF16: return launch_product<BF16>(p, way, workspace, st);
+        default: return launch_product<F16>(p, way, workspace, st);
     }
 }
 
