@@ -178,17 +178,17 @@ __device__ __forceinline__ void store_row(void* p, int64_t i, int n, const float
 }
 
 // A lane's eight elements of a row of `dim` >= 8 from column c on without a branch: it loads eight that are there, from
-// column min(c, dim - 8) on, and what the row's end cuts off is moved down and filled with zeros (`settle`) afterwards.
+// column min(c, dim - 8) on, and what the row's end cuts off is moved down and filled up (`settle`) afterwards.
 // `by`: c - (dim - 8) where positive; 8 and more: no element is the lane's.
 template <typename T>
-__device__ __forceinline__ void settle(float* v, int by) {
+__device__ __forceinline__ void settle(float* v, int by, float fill = 0.0f) {
 #pragma unroll
     for (int s = 4; s; s >>= 1) {
 #pragma unroll
-        for (int j = 0; j < kLane; ++j) v[j] = by & s ? (j + s < kLane ? v[j + s] : 0.0f) : v[j];
+        for (int j = 0; j < kLane; ++j) v[j] = by & s ? (j + s < kLane ? v[j + s] : fill) : v[j];
     }
 #pragma unroll
-    for (int j = 0; j < kLane; ++j) v[j] = by >= kLane ? 0.0f : v[j];
+    for (int j = 0; j < kLane; ++j) v[j] = by >= kLane ? fill : v[j];
 }
 
 // The largest of 16 neighbouring lanes (one DPP row), in every lane of them.

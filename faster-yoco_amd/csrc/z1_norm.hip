@@ -309,16 +309,17 @@ __device__ __forceinline__ void row_sums(float& s1, float& s2, float (*red)[2], 
     for (int i = 1; i < wpr; ++i) s1 += red[first + i][0], s2 += red[first + i][1];
 }
 
-// Eight columns of a row as they are loaded: x in T, or its 8-bit rows' bytes and scale.
+// Eight columns of a row as they are loaded: x in T, or its 8-bit rows' bytes and scale.  open: their values, and `fill` past
+// the row's end.
 template <typename T, bool Q>
 struct Input {
     typename T::raw r;
     static __device__ __forceinline__ Input load(const Backward& a, int64_t row, int c, int from) {
         return {T::load((const typename T::elem*)a.x + row * a.x_stride, from)};
     }
-    __device__ __forceinline__ void open(float* v, bool edge, int by) const {
+    __device__ __forceinline__ void open(float* v, bool edge, int by, float fill) const {
         T::open(r, v);
-        if (edge) settle<T>(v, by);
+        if (edge) settle<T>(v, by, fill);
     }
 };
 template <typename T>
@@ -331,11 +332,11 @@ struct Input<T, true> {
         const uint8_t* s = a.s + row * a.pitch;
         return {*(const Z1B_GLOBAL u2*)(q + (uint32_t)c), ((const Z1B_GLOBAL uint8_t*)s)[(uint32_t)c / kBlock]};
     }
-    __device__ __forceinline__ void open(float* v, bool edge, int by) const {
+    __device__ __forceinline__ void open(float* v, bool edge, int by, float fill) const {
         const float f = scale_value(s);
         open8(q, v);
 #pragma unroll
-        for (int j = 0; j < kLane; ++j) v[j] = edge && j + by >= kLane ? 0.0f : v[j] * f;
+        for (int j = 0; j < kLane; ++j) v[j] = edge && j + by >= kLane ? fill : v[j] * f;
     }
 };
 
@@ -400,7 +401,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) 
         for (int k = 0; k < NV; ++k) {
             T::open(dy[k], g[k]);
             if (edge[k]) settle<T>(g[k], by[k]);
-            x[k].open(xh[k], edge[k], by[k]);
+            x[k].open(xh[k], edge[k], by[k], mu);
         }
         fetch(row + stride);
         if (!live) {
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) 
         for (int k = 0; k < NV; ++k) {
 #pragma unroll
             for (int j = 0; j < kLane; ++j) {
-                // past the row's end dy and w are zeros, and so is all that xh enters
+                // past the row's end dy and w are zeros, x is mu (mu r may be infinite), and so is all that xh enters
                 xh[k][j] = (CENTER ? xh[k][j] - mu : xh[k][j]) * r;
                 dw[k][j] = __builtin_fmaf(g[k][j], xh[k][j], dw[k][j]);
                 if (CENTER) db[k][j] += g[k][j];
@@ -489,7 +490,7 @@ __device__ __forceinline__ void strip_sums(const Backward& a, int strip, float (
         for (int i = 0; i < kTurns; ++i) {
             float g[kLane], xh[kLane];
             T::open(dy[i], g);
-            x[i].open(xh, !whole && by > 0, by);
+            x[i].open(xh, !whole && by > 0, by, mu[i]);
             if (!whole) {
                 if (by > 0) settle<T>(g, by);
             }
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_once_kernel(Backwar
         const int by = c0 + k * step - from(k);
         T::open(dy[k], g[k]);
         if (edge(k)) settle<T>(g[k], by);
-        x[k].open(xh[k], edge(k), by);
+        x[k].open(xh[k], edge(k), by, mu);
         if (a.w) {
             float w[kLane];
             if (a.w32) F32::open(F32::load(a.w, from(k)), w);

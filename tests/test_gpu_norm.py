@@ -333,3 +333,14 @@ def test_refusals(pkg, dev):
         norm.rms_norm_backward(x, act8.pack(x[:, :200]), r, w)
     with pytest.raises(RuntimeError, match='values'):
         norm.rms_norm_backward(x, act8.pack(x[:3]), r, w)
+
+
+@pytest.mark.parametrize('packed', [False, True], ids=['x', 'checkpoint'])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32], ids=str)
+@pytest.mark.parametrize('n,dim', [(3, 130), (5, 1537), (3, 4099), (2600, 137), (2600, 1030), (2, 20001)])
+def test_backward_of_rows_of_one_large_value(pkg, dev, n, dim, dtype, packed):
+    """x = mean = 2^120 and rstd = 316: (x - mean) rstd is 0 in the row, and mean * rstd, which the columns past its end would
+    bring in, beyond fp32."""
+    x, w, _, dy = inputs(n, dim, dtype, 21)
+    x[0], x[-1] = 2.0 ** 120, 2.0 ** 120
+    check_backward(pkg, dev, x, dy, w, True, packed)
