@@ -215,10 +215,10 @@ std::vector<Tensor> norm_forward(const Tensor& x, const OptTensor& weight, const
     return out;
 }
 
-// [dx, dw (need_dw), db (need_db)]; x, or its 8-bit rows q, s
+// [dx, dw (need_dw), db (need_db)]; x, or its 8-bit rows q, s; dw and db in grad_dtype, else the weight's, else dy's
 std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const OptTensor& q, const OptTensor& s,
                                   const OptTensor& mean, const Tensor& rstd, const OptTensor& weight, bool center,
-                                  bool need_dw, bool need_db) {
+                                  bool need_dw, bool need_db, std::optional<at::ScalarType> grad_dtype) {
     const char* what = "norm_backward";
     require_gpu(dy, what, "dy");
     const Rows r = rows_of(dy, what, "dy");
@@ -244,7 +244,8 @@ std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const Op
     }
     const float* rp = stat_of(rstd, dy, r.rows, what, "rstd");
     const void* w = weight_of(weight, dy, r.dim, what, "weight");
-    const at::ScalarType gt = w ? weight->scalar_type() : dy.scalar_type();
+    const at::ScalarType gt = grad_dtype.value_or((w ? *weight : dy).scalar_type());
+    const int grad_code = dtype_code(gt, what);
     OnDevice on(dy);
     std::vector<Tensor> out;
     out.reserve(3);
@@ -255,9 +256,9 @@ std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const Op
                           "z1_norm_backward_workspace");
     check_rc(api().norm_backward(r.p, r.stride, plain ? xr.p : nullptr, xr.stride, packed ? q->const_data_ptr() : nullptr,
                                  packed ? s->const_data_ptr() : nullptr, r.rows, r.dim, r.dtype, mp, rp, w,
-                                 w ? dtype_code(gt, what) : Z1_F32, center, out[0].data_ptr(),
+                                 w ? dtype_code(weight->scalar_type(), what) : Z1_F32, center, out[0].data_ptr(),
                                  need_dw ? out[1].data_ptr() : nullptr, need_db ? out.back().data_ptr() : nullptr,
-                                 dtype_code(gt, what), parts.p, parts.floats, on.stream), "z1_norm_backward");
+                                 grad_code, parts.p, parts.floats, on.stream), "z1_norm_backward");
     return out;
 }
 
@@ -357,7 +358,7 @@ TORCH_LIBRARY_FRAGMENT(yoco_z1, m) {
     m.def("norm_forward(Tensor x, Tensor? weight, Tensor? bias, float eps, bool center, bool y8, bool checkpoint) "
           "-> Tensor[]");
     m.def("norm_backward(Tensor dy, Tensor? x, Tensor? q, Tensor? s, Tensor? mean, Tensor rstd, Tensor? weight, "
-          "bool center, bool need_dw, bool need_db) -> Tensor[]");
+          "bool center, bool need_dw, bool need_db, ScalarType? grad_dtype=None) -> Tensor[]");
     m.def("act8_pack(Tensor x) -> (Tensor, Tensor)");
     m.def("act8_unpack(Tensor q, Tensor s, int dim, ScalarType dtype) -> Tensor");
     m.def("weight8_pack(Tensor w, bool transposed) -> Tensor[]");

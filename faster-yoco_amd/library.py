@@ -99,8 +99,9 @@ def _norm_forward_fake(x, weight, bias, eps, center, y8, checkpoint):
     return out + (_empty8(x, n, d, n) if checkpoint else [])
 
 
-def _norm_backward_fake(dy, x, q, s, mean, rstd, weight, center, need_dw, need_db):
-    gt = dy.dtype if weight is None else weight.dtype
+def _norm_backward_fake(dy, x, q, s, mean, rstd, weight, center, need_dw, need_db,
+                        grad_dtype=None):
+    gt = grad_dtype or (dy if weight is None else weight).dtype
     return [dy.new_empty(dy.shape)] + [dy.new_empty((dy.shape[1],), dtype=gt) for _ in range(need_dw + need_db)]
 
 

@@ -37,23 +37,26 @@ def rms_norm(x, weight=None, eps=1e-5, *, y8=False, checkpoint=False):
     return _forward(x, weight, None, eps, False, y8, checkpoint)
 
 
-def _backward(dy, x, mean, rstd, weight, center, need_weight, need_bias):
+def _backward(dy, x, mean, rstd, weight, center, need_weight, need_bias, grad_dtype=None):
     r = act8.rows_of(dy)
     if isinstance(x, Act8):
         if x.dim != dy.shape[-1]:
             raise RuntimeError(f'norm_backward: a checkpoint of {x.dim} columns, gradient rows of {dy.shape[-1]}')
-        out = _norm_backward(r, None, x.q, x.s, mean, rstd, weight, center, need_weight, need_bias)
+        out = _norm_backward(r, None, x.q, x.s, mean, rstd, weight, center, need_weight, need_bias,
+                             grad_dtype)
     else:
-        out = _norm_backward(r, act8.rows_of(x), None, None, mean, rstd, weight, center, need_weight, need_bias)
+        out = _norm_backward(r, act8.rows_of(x), None, None, mean, rstd, weight, center, need_weight, need_bias,
+                             grad_dtype)
     if dy.dim() != 2:
         return (out[0].view(dy.shape), *out[1:])
     return tuple(out)
 
 
-def layer_norm_backward(dy, x, mean, rstd, weight=None, *, bias=False):
+def layer_norm_backward(dy, x, mean, rstd, weight=None, *, bias=False, grad_dtype=None):
     """The gradients of layer_norm from dy, its input x (dy's type, or the Act8 of its rows) and the forward's mean and
-    rstd: (dx, dw) where weight is given, with db where bias is True; dw and db in the weight's type (dy's without one)."""
-    return _backward(dy, x, mean, rstd, weight, True, weight is not None, bias)
+    rstd: (dx, dw) where weight is given, with db where bias is True; dw and db in grad_dtype, else in the weight's type, else
+    in dy's (fp32 for an fp32 bias without a weight)."""
+    return _backward(dy, x, mean, rstd, weight, True, weight is not None, bias, grad_dtype)
 
 
 def rms_norm_backward(dy, x, rstd, weight=None):
@@ -68,7 +71,7 @@ class _Norm(torch.autograd.Function):
         mean, rstd = (out[1], out[2]) if center else (None, out[1])
         kept = (out[-1].q, out[-1].s) if checkpoint else (x, None)
         ctx.save_for_backward(*kept, mean, rstd, weight)
-        ctx.center, ctx.checkpoint, ctx.bias = center, checkpoint, bias is not None
+        ctx.center, ctx.checkpoint, ctx.bias = center, checkpoint, None if bias is None else bias.dtype
         return out[0]
 
     @staticmethod
@@ -77,8 +80,8 @@ class _Norm(torch.autograd.Function):
         kept, s, mean, rstd, weight = ctx.saved_tensors
         x = Act8(kept, s, dy.shape[-1]) if ctx.checkpoint else kept
         need_w = weight is not None and ctx.needs_input_grad[1]
-        need_b = ctx.bias and ctx.needs_input_grad[2]
-        out = list(_backward(dy, x, mean, rstd, weight, ctx.center, need_w, need_b))
+        need_b = ctx.bias is not None and ctx.needs_input_grad[2]
+        out = list(_backward(dy, x, mean, rstd, weight, ctx.center, need_w, need_b, ctx.bias))
         dx = out.pop(0)
         dw = out.pop(0) if need_w else None
         return dx, dw, out.pop(0) if need_b else None, None, None, None

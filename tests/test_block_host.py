@@ -122,3 +122,12 @@ def test_a_block_traces_on_fake_tensors(pkg):
     called = [str(n.target) for n in gm.graph.nodes if n.op == 'call_function' and 'yoco_z1' in str(n.target)]
     assert called == [f'yoco_z1.{n}.default' for n in ('norm_forward', 'weight8_pack', 'product8', 'act8_pack', 'product8',
                                                        'weight_grad8', 'act8_unpack', 'norm_backward')]
+
+
+def test_a_given_gradient_type_on_fake_tensors(pkg):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    op = torch.ops.yoco_z1.norm_backward
+    with FakeTensorMode():
+        x, r = torch.empty(40, 300, dtype=torch.bfloat16, device='cuda'), torch.empty(40, device='cuda')
+        types = lambda *a: [t.dtype for t in op(x, x, None, None, r, r, None, True, False, True, *a)]  # noqa: E731
+        assert types() == [torch.bfloat16] * 2 and types(torch.float32) == [torch.bfloat16, torch.float32]

@@ -344,3 +344,21 @@ def test_backward_of_rows_of_one_large_value(pkg, dev, n, dim, dtype, packed):
     x, w, _, dy = inputs(n, dim, dtype, 21)
     x[0], x[-1] = 2.0 ** 120, 2.0 ** 120
     check_backward(pkg, dev, x, dy, w, True, packed)
+
+
+@pytest.mark.parametrize('n,dim', [(300, 200), (3000, 520), (40, 20001)])
+def test_gradient_of_an_fp32_bias_without_a_weight(pkg, dev, n, dim):
+    """db has the bias's type: the fp32 sum itself, not one rounded to the rows' type."""
+    from faster_yoco_amd import norm
+    x, _, b, dy = inputs(n, dim, torch.bfloat16, 23, w_dtype=torch.float32)
+    xd, dyd, bd = x.to(dev), dy.to(dev), b.to(dev).requires_grad_()
+    norm.layer_norm_train(xd, None, bd).backward(dyd)
+    want, size = dy.double().sum(0), dy.double().abs().sum(0)
+    assert bd.grad.dtype == torch.float32
+    assert ((bd.grad.cpu().double() - want).abs() <= (n + 16) * U * size + ref.rounded(want, torch.float32) * 1.001).all()
+    _, mean, rstd = norm.layer_norm(xd, None, bd.detach())
+    _, db = norm.layer_norm_backward(dyd, xd, mean, rstd, bias=True, grad_dtype=torch.float32)
+    assert db.dtype == torch.float32 and torch.equal(db, bd.grad)
+    assert torch.equal(norm.layer_norm_backward(dyd, xd, mean, rstd, bias=True)[1], db.bfloat16())
+    with pytest.raises(RuntimeError, match='expected fp32, bf16 or fp16'):
+        norm.layer_norm_backward(dyd, xd, mean, rstd, bias=True, grad_dtype=torch.float64)
