@@ -39,7 +39,8 @@ class Z1UpdateScalars(ctypes.Structure):
                 ('clip_log_out', _P)]
 
 
-# name -> (argtypes, restype); every function the header declares
+# name -> (argtypes, restype); every function the header declares.  A build of the ABI may lack BLOCK_SIGNATURES, the part
+# around the update: its update runs, and the block-side operators say that they are missing when called.
 SIGNATURES = {
     'z1_table_create': ([ctypes.POINTER(Z1Tensor), _I, _I, ctypes.POINTER(_P)], _I),
     'z1_table_destroy': ([_P], _I),
@@ -68,6 +69,9 @@ SIGNATURES = {
     'z1_cast_bf16': ([_P, _P, _I64, _P], _I),
     'z1_embedding_backward': ([_P, _P, _I64, _I64, _I64, _I64, _F, _I, _P, _P, _I64, _P], _I),
     'z1_embedding_backward_workspace': ([_I64, _I64, _I64], _I64),
+    'z1_strerror': ([_I], ctypes.c_char_p),
+}
+BLOCK_SIGNATURES = {
     'z1_norm_forward': ([_P, _I64, _I64, _I64, _I, _P, _P, _I, _F, _I, _P, _P, _P, _P, _P, _P, _P, _P], _I),
     'z1_norm_backward': ([_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I64,
                           _P], _I),
@@ -81,8 +85,8 @@ SIGNATURES = {
     'z1_product8_workspace': ([_I64, _I64, _I64, _I], _I64),
     'z1_weight_grad8': ([_P, _I64, _P, _P, _I64, _I64, _I64, _P, _I, _P, _I64, _P], _I),
     'z1_weight_grad8_workspace': ([_I64, _I64, _I64], _I64),
-    'z1_strerror': ([_I], ctypes.c_char_p),
 }
+SIGNATURES.update(BLOCK_SIGNATURES)
 
 _LIB = None
 
@@ -95,7 +99,11 @@ def lib():
             raise RuntimeError(f'yoco_z1: native library {LIB_PATH} is not built (run __graft_entry__.build())')
         L = ctypes.CDLL(LIB_PATH)
         for name, (args, res) in SIGNATURES.items():
-            fn = getattr(L, name)
+            fn = getattr(L, name, None)
+            if fn is None:
+                if name in BLOCK_SIGNATURES:
+                    continue
+                raise RuntimeError(f'yoco_z1: {LIB_PATH} has no {name}')
             fn.argtypes = args
             fn.restype = res
         _LIB = L

@@ -45,7 +45,8 @@ Api g_api{};
 bool g_api_ok = false;
 
 const Api& api() {
-    TORCH_CHECK(g_api_ok, "yoco_z1: the operators are not bound to libyoco_z1.so (import faster_yoco_amd.library)");
+    TORCH_CHECK(g_api_ok, "yoco_z1: the block-side operators are not bound: faster_yoco_amd.library is not imported, or the "
+                         "selected build of libyoco_z1.so lacks them");
     return g_api;
 }
 

@@ -2,6 +2,9 @@
 operators are registered, write none of their arguments, trace on fake tensors with the shapes they return, and refuse CPU
 tensors."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -131,3 +134,23 @@ def test_a_given_gradient_type_on_fake_tensors(pkg):
         x, r = torch.empty(40, 300, dtype=torch.bfloat16, device='cuda'), torch.empty(40, device='cuda')
         types = lambda *a: [t.dtype for t in op(x, x, None, None, r, r, None, True, False, True, *a)]  # noqa: E731
         assert types() == [torch.bfloat16] * 2 and types(torch.float32) == [torch.bfloat16, torch.float32]
+
+
+def test_a_build_without_the_block_side_functions_is_accepted(pkg, tmp_path):
+    """A library of the update's functions alone binds; one that lacks any of those is refused by name."""
+    from faster_yoco_amd import _lib
+    names = [n for n in _lib.SIGNATURES if n not in _lib.BLOCK_SIGNATURES]
+    assert len(names) > 20 and len(_lib.BLOCK_SIGNATURES) >= 12
+
+    def imported(names, code):
+        src, lib = tmp_path / 'stub.c', tmp_path / f'stub{len(names)}.so'
+        src.write_text(''.join(f'int {n}(void) {{ return 0; }}\n' for n in names))
+        subprocess.run(['gcc', '-shared', '-fPIC', '-o', str(lib), str(src)], check=True)
+        root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+        return subprocess.run([sys.executable, '-c', code], cwd=root, env=dict(os.environ, YOCO_Z1_LIB=str(lib)),
+                              capture_output=True, text=True)
+    res = imported(names, 'import faster_yoco_amd as f\nL = f._lib.lib()\nassert L.z1_owner_sum_waves(5) == 0\n'
+                          "assert not hasattr(L, 'z1_norm_forward')\nprint('bound')")
+    assert res.returncode == 0 and res.stdout.strip() == 'bound', res.stderr
+    res = imported(names[1:], 'import faster_yoco_amd')
+    assert res.returncode != 0 and f'RuntimeError: yoco_z1: {tmp_path}' in res.stderr and f'has no {names[0]}' in res.stderr
