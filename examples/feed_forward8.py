@@ -14,6 +14,7 @@ import os
 import sys
 
 import torch
+from torch.autograd.function import once_differentiable
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from faster_yoco_amd import act8, linear8, norm, shard  # noqa: E402
@@ -30,15 +31,17 @@ class Block8(torch.autograd.Function):
         h = linear8.matmul(a, up8)
         u = act8.pack(torch.nn.functional.silu(h))
         h = act8.pack(h)
-        ctx.saved = (a, c, h, u, rstd, up8, down8)
-        ctx.save_for_backward(w_norm)
+        ctx.save_for_backward(w_norm, rstd, up8.qt, up8.st, down8.qt, down8.st, *(p for t in (a, c, h, u) for p in (t.q, t.s)))
+        ctx.dims, ctx.shapes = [t.dim for t in (a, c, h, u)], (up8.shape, down8.shape)
         kept.append(sum(t.nbytes() for t in (a, c, h, u)) + rstd.numel() * 4)
         return x + linear8.matmul(u, down8)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
-        (w_norm,) = ctx.saved_tensors
-        a, c, h8, u, rstd, up8, down8 = ctx.saved
+        w_norm, rstd, *weights = ctx.saved_tensors
+        a, c, h8, u = (act8.Act8(*weights[4 + 2 * i:6 + 2 * i], d) for i, d in enumerate(ctx.dims))
+        up8, down8 = (linear8.Weight8(None, None, *weights[2 * i:2 * i + 2], s) for i, s in enumerate(ctx.shapes))
         d_down = linear8.weight_grad(dy, u)
         du = linear8.matmul(act8.pack(dy), down8, transposed=True)
         h = act8.unpack(h8).float()

@@ -63,24 +63,28 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, w8):
         a = act8.pack(x)
-        ctx.save_for_backward(a.q, a.s)
-        ctx.w8, ctx.dim, ctx.x_shape, ctx.dtype, ctx.w_dtype = w8, a.dim, x.shape, x.dtype, weight.dtype
+        need_x, need_w = ctx.needs_input_grad[:2]
+        ctx.save_for_backward(*((w8.qt, w8.st) if need_x else (None, None)), *((a.q, a.s) if need_w else (None, None)))
+        ctx.shape, ctx.dim, ctx.x_shape, ctx.dtype, ctx.w_dtype = w8.shape, a.dim, x.shape, x.dtype, weight.dtype
         return matmul(a, w8, x.dtype).view(*x.shape[:-1], w8.shape[0])
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         dx = dw = None
+        qt, st, q, s = ctx.saved_tensors
         if ctx.needs_input_grad[0]:
-            dx = matmul(act8.pack(dy), ctx.w8, ctx.dtype, transposed=True).view(ctx.x_shape)
+            w8 = Weight8(None, None, qt, st, ctx.shape)
+            dx = matmul(act8.pack(dy), w8, ctx.dtype, transposed=True).view(ctx.x_shape)
         if ctx.needs_input_grad[1]:
-            dw = weight_grad(dy, Act8(*ctx.saved_tensors, ctx.dim), ctx.w_dtype)
+            dw = weight_grad(dy, Act8(q, s, ctx.dim), ctx.w_dtype)
         return dx, dw, None
 
 
 def linear(x, weight, w8):
     """x @ weight.T for bf16 x [..., K], differentiable: w8 is pack_weight(weight), packed again whenever the weight
-    changes.  What is kept for the backward pass is the 8-bit rows of x."""
+    changes.  What is kept for the backward pass is the 8-bit rows of x and w8's other order; w8's tensors may be replaced
+    before it, not written."""
     if x.dtype != torch.bfloat16:
         raise RuntimeError('linear8.linear: expected bf16 rows')
     if tuple(weight.shape) != tuple(w8.shape):

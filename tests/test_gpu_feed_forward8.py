@@ -45,3 +45,18 @@ def test_block_gradients_against_plain_blocks(example):
     example.plain(*b).backward(dy)
     for p, q in zip(a, b):
         assert float((p.grad.float() - q.grad.float()).norm() / q.grad.float().norm()) < 0.08
+
+
+def test_a_block_keeps_what_autograd_sees(example):
+    """Saved-tensor hooks see the 8-bit rows and both weights, and nothing of the block's input in its own type."""
+    from faster_yoco_amd import linear8
+    r = lambda *s: torch.randn(*s, device='cuda').bfloat16()  # noqa: E731
+    x, wn, wu, wd = r(64, 256).requires_grad_(), r(256).requires_grad_(), r(384, 256), r(256, 384)
+    p, kept, sizes = (linear8.pack_weight(wu), linear8.pack_weight(wd)), [], []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        example.Block8.apply(x, wn, wu, wd, *p, sizes)
+    assert len(kept) == 14 and not any(t.shape == (64, 256) and t.dtype == torch.bfloat16 for t in kept)
+    y = example.Block8.apply(x, wn, wu, wd, *p, sizes)            # without hooks, which pass the version check by
+    p[1].qt.view(torch.uint8).zero_()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()

@@ -339,3 +339,32 @@ def test_refusals(pkg, dev):
         linear8.linear(x.float(), x, p)
     with pytest.raises(RuntimeError, match='8-bit blocks of'):
         linear8.linear(x, x, p)
+
+
+def test_what_linear_keeps_is_saved_for_autograd(pkg, dev):
+    """Saved-tensor hooks see all that is kept, only what a gradient needs is, and a weight written before the backward pass
+    is an error, not another weight's gradient; one replaced is not used."""
+    from faster_yoco_amd import linear8
+    x, w = rows(96, 384, 13).to(dev), (rows(260, 384, 14, 0.1) * 0.05).to(dev)
+    dy = rows(96, 260, 15).to(dev)
+    p, other = linear8.pack_weight(w), linear8.pack_weight(w * 2)
+
+    def run(need_x, need_w, p):
+        kept, xs, ws = [], x.clone().requires_grad_(need_x), w.clone().requires_grad_(need_w)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+            y = linear8.linear(xs, ws, p)
+        return y, xs, ws, sorted(tuple(t.shape) for t in kept)
+    order, packed = [(3, 4), (384, 384)], [(96, 4), (96, 384)]
+    assert run(True, False, p)[3] == order and run(False, True, p)[3] == packed
+    y, xs, ws, kept = run(True, True, p)
+    assert kept == sorted(order + packed)
+    qt, p.qt = p.qt, other.qt                          # replaced: the kept one counts
+    y.backward(dy)
+    p.qt = qt
+    y2, xs2, ws2, _ = run(True, True, p)
+    y2.backward(dy)
+    assert torch.equal(xs.grad, xs2.grad) and torch.equal(ws.grad, ws2.grad)
+    y = linear8.linear(x.clone().requires_grad_(), w, p)           # without hooks, which pass the version check by
+    p.qt.view(torch.uint8).copy_(other.qt.view(torch.uint8))
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward(dy)
