@@ -64,6 +64,8 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, weight, w8):
         a = act8.pack(x)
         need_x, need_w = ctx.needs_input_grad[:2]
+        if need_x and w8.qt is None:
+            raise RuntimeError('linear8.linear: the weight was packed without its other order, which the gradient of x needs')
         ctx.save_for_backward(*((w8.qt, w8.st) if need_x else (None, None)), *((a.q, a.s) if need_w else (None, None)))
         ctx.shape, ctx.dim, ctx.x_shape, ctx.dtype, ctx.w_dtype = w8.shape, a.dim, x.shape, x.dtype, weight.dtype
         return matmul(a, w8, x.dtype).view(*x.shape[:-1], w8.shape[0])

@@ -368,3 +368,14 @@ def test_what_linear_keeps_is_saved_for_autograd(pkg, dev):
     p.qt.view(torch.uint8).copy_(other.qt.view(torch.uint8))
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         y.backward(dy)
+
+
+def test_linear_without_the_other_order(pkg, dev):
+    from faster_yoco_amd import linear8
+    x, w = rows(8, 256, 46).to(dev), rows(128, 256, 47).to(dev)
+    p = linear8.pack_weight(w, transposed=False)
+    with pytest.raises(RuntimeError, match='without its other order'):
+        linear8.linear(x.clone().requires_grad_(), w, p)
+    ws = w.clone().requires_grad_()                    # the weight's gradient does not need it
+    linear8.linear(x, ws, p).sum().backward()
+    assert ws.grad.shape == w.shape
