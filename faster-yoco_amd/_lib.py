@@ -85,6 +85,8 @@ BLOCK_SIGNATURES = {
     'z1_product8_workspace': ([_I64, _I64, _I64, _I], _I64),
     'z1_weight_grad8': ([_P, _I64, _P, _P, _I64, _I64, _I64, _P, _I, _P, _I64, _P], _I),
     'z1_weight_grad8_workspace': ([_I64, _I64, _I64], _I64),
+    'z1_product8_way': ([_I64, _I64, _I64, ctypes.POINTER(_I)], _I),
+    'z1_weight_grad8_way': ([_I64, _I64, _I64, _I, ctypes.POINTER(_I)], _I),
 }
 SIGNATURES.update(BLOCK_SIGNATURES)
 

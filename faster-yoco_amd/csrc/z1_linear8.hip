@@ -853,16 +853,16 @@ int parts_of(int64_t tiles, int64_t steps, int unit, int64_t results, int rate, 
 //
 // Up to one of 128 x 128 to a CU: smaller tiles on more CUs win while there are CUs (kSmall: a start and a block of K, in ns,
 // as measured), and where even they leave CUs idle, a long K is cut into parts, joined by a second launch.  1000 -> 1501, 333
-// rows: 6.4 us in 64 x 64, 11.6 in 128 x 128; 4096 -> 4096, 512 rows: 23.9 in 64 x 128, 24.6 in 64 x 64, 27.3 in 128 x 128 of
-// two parts, 1024 rows: 34.9 in 128 x 128, 45 in either other; 8192 -> 3072, 512 rows: 34.6 in 128 x 128 of four parts, 39.6
-// in 64 x 64; 128 rows: 31 in 64 x 64, 17.9 of four parts.
+// rows: 6.4 us in 64 x 64, 11.6 in 128 x 128; 4100 -> 3000, 600 rows: 24.1 in 64 x 128, 27.0 without it; 4096 -> 4096, 1024
+// rows: 34.9 in 128 x 128, 45.3 in 64 x 64; 8192 -> 3072, 512 rows: 34.6 in 128 x 128 of four parts, 39.6 in 64 x 64; 128 rows:
+// 31.3 in 64 x 64, 17.9 of four parts.
 //
 // Up to 64 rows the few rows' kernel runs where it is faster, a workgroup to a CU, at 3.3 us and 0.12 to 0.25 us a block of K,
 // more with more of them and more rows (33 rows, 3072 -> 3072: 6.9 us against 13.4, 3072 -> 8192: 8.3 against 13.5; 64 rows,
 // 8192 -> 3072: 14.4 against 14.3 in 64 x 64 of eight parts).
 struct Way {
-    bool few;
     int rows, outputs;                                 // of a tile
+    int stages;                                        // blocks of K staged; 0: the few rows' kernel
     int parts, per;                                    // of K's blocks
 };
 struct Small {
@@ -887,23 +887,32 @@ Cut best_of(const Small (&small)[COUNT], int64_t M, int64_t N, int64_t steps, in
     }
     return best;
 }
+Way few_way(int64_t M, int64_t N, int blocks) {
+    if (M > 32) return {64, 32, 0, 1, blocks};
+    // the fewest outputs that hold the rows, or more while there are 192 workgroups: one row of 3072 -> 8192 takes 9.8 us with
+    // 8 outputs, 8.1 with 16, 6.6 with 32; 8192 -> 3072 8.2, 7.3, 9.2; 4096 -> 4096 6.1, 6.1, 6.2; 5120 -> 1280 4.1, 4.9, 6.0
+    int outputs = M <= 8 ? 8 : M <= 16 ? 16 : 32;
+    while (outputs < 32 && N >= 2 * outputs * 192) outputs *= 2;
+    return {outputs, outputs, 0, 1, blocks};
+}
 Way product_way(int64_t M, int64_t N, int blocks) {
-    if (M <= 32) return {true, 0, 0, 1, blocks};
+    if (M <= 32) return few_way(M, N, blocks);
     auto tiles = [&](int rows, int outputs) { return (M + rows - 1) / rows * ((N + outputs - 1) / outputs); };
     auto rounds = [&](int rows, int outputs, int at_once) { return (tiles(rows, outputs) + at_once - 1) / at_once; };
     if (tiles(128, 128) > kCus) {
         const int64_t large_time = 100 * rounds(256, 256, kCus), middle_time = 51 * rounds(128, 192, kCus);
         if (59 * rounds(128, 128, 2 * kCus) <= (large_time < middle_time ? large_time : middle_time))
-            return {false, 128, 128, 1, blocks};
-        if (large_time <= middle_time) return {false, 256, 256, 1, blocks};
-        return {false, 128, 192, 1, blocks};
+            return {128, 128, 2, 1, blocks};
+        if (large_time <= middle_time) return {256, 256, 2, 1, blocks};
+        return {128, 192, 4, 1, blocks};
     }
     const Cut cut = best_of(kSmall, M, N, blocks, 4, kProductRate);
     const int64_t groups = (N + 31) / 32;              // workgroups of few rows; with less than 64, the parts read K sooner
     const int64_t few_rounds = (groups + kCus - 1) / kCus, at_once = groups < kCus ? groups : kCus;
     if (M <= 64 && groups >= 64 && 3300 + few_rounds * blocks * (120 + at_once * M / 128) <= cut.ns)
-        return {true, 0, 0, 1, blocks};
-    return {false, cut.tile->rows, cut.tile->outputs, cut.parts,
+        return few_way(M, N, blocks);
+    const int stages = cut.tile->rows == 128 && tiles(128, 128) * cut.parts > kCus ? 2 : 4;
+    return {cut.tile->rows, cut.tile->outputs, stages, cut.parts,
             cut.parts == 1 ? blocks : (blocks + 4 * cut.parts - 1) / (4 * cut.parts) * 4};
 }
 
@@ -923,23 +932,18 @@ int launch_few(const Product& a, hipStream_t st) {
 
 template <typename T>
 int launch_small(const Product& a, const Way& way, hipStream_t st) {
-    if (way.rows == 64 && way.outputs == 64) return launch_tiles<T, 64, 64, 32, 32, 4>(a, way.parts, st);
+    if (way.outputs == 64) return launch_tiles<T, 64, 64, 32, 32, 4>(a, way.parts, st);
     if (way.rows == 64) return launch_tiles<T, 64, 128, 32, 64, 4>(a, way.parts, st);
-    const int64_t tiles = (a.M + 127) / 128 * ((a.N + 127) / 128) * way.parts;
-    return tiles <= kCus ? launch_tiles<T, 128, 128, 64, 64, 4>(a, way.parts, st)
-                         : launch_tiles<T, 128, 128, 64, 64, 2>(a, way.parts, st);
+    if (way.stages == 4) return launch_tiles<T, 128, 128, 64, 64, 4>(a, way.parts, st);
+    return launch_tiles<T, 128, 128, 64, 64, 2>(a, way.parts, st);
 }
 
 template <typename T>
 int launch_product(Product a, const Way& way, float* workspace, hipStream_t st) {
-    if (way.few) {
-        if (a.M > 32) return launch_few<T, 32, 2>(a, st);
-        // the fewest outputs that hold the rows, or more while there are 192 workgroups: one row of 3072 -> 8192 takes 9.8 us
-        // with 8 outputs, 8.1 with 16, 6.6 with 32; 8192 -> 3072 8.2, 7.3, 9.2; 4096 -> 4096 6.1, 6.1, 6.2; 5120 -> 1280 4.1, 4.9, 6.0
-        int outputs = a.M <= 8 ? 8 : a.M <= 16 ? 16 : 32;
-        while (outputs < 32 && a.N >= 2 * outputs * 192) outputs *= 2;
-        if (outputs == 8) return launch_few<T, 8, 1>(a, st);
-        if (outputs == 16) return launch_few<T, 16, 1>(a, st);
+    if (way.stages == 0) {
+        if (way.rows == 64) return launch_few<T, 32, 2>(a, st);
+        if (way.outputs == 8) return launch_few<T, 8, 1>(a, st);
+        if (way.outputs == 16) return launch_few<T, 16, 1>(a, st);
         return launch_few<T, 32, 1>(a, st);
     }
     a.per = way.per;
@@ -1029,6 +1033,22 @@ int gradient(Gradient a, const GradientWay& way, float* workspace, hipStream_t s
 }  // namespace
 
 extern "C" {
+
+int z1_product8_way(int64_t M, int64_t N, int64_t K, int* way) {
+    if (M < 1 || M > kMaxRows || N < 1 || N > kMaxDim || K < 1 || K > kMaxInner) return Z1_E_SIZE;
+    if (!way) return Z1_E_NULL;
+    const Way w = product_way(M, N, wide_of(K) / kBlock);
+    way[0] = w.rows, way[1] = w.outputs, way[2] = w.stages, way[3] = w.parts;
+    return Z1_OK;
+}
+
+int z1_weight_grad8_way(int64_t T, int64_t N, int64_t K, int whole_dwords, int* way) {
+    if (T < 0 || T > kMaxRows || N < 1 || N > kMaxDim || K < 1 || K > kMaxInner) return Z1_E_SIZE;
+    if (!way) return Z1_E_NULL;
+    const GradientWay w = gradient_way(T, N, K, whole_dwords != 0);
+    way[0] = w.rows, way[1] = w.columns, way[2] = w.direct, way[3] = w.parts;
+    return Z1_OK;
+}
 
 int64_t z1_product8_workspace(int64_t M, int64_t N, int64_t K, int dtype) {
     if (M < 0 || M > kMaxRows || N < 0 || N > kMaxDim || K < 1 || K > kMaxInner) return Z1_E_SIZE;

@@ -310,6 +310,13 @@ int z1_weight_grad8(const uint16_t* dy, int64_t stride, const void* q, const voi
                     void* dw, int dtype, float* workspace, int64_t workspace_floats, void* stream);
 int64_t z1_weight_grad8_workspace(int64_t T, int64_t N, int64_t K);
 
+/* How a product or a weight gradient of these sizes runs, of interest to timing and tests: way[0], way[1] = rows and columns of
+ * a workgroup's tile of the result, way[3] = parts of the summed axis.  way[2]: blocks of K that a product stages, 0 for
+ * the kernel of few rows; 1 where a gradient's rows go straight into LDS (whole_dwords: dy's first address is a multiple
+ * of 4 and its stride even and at least N), else 0. */
+int z1_product8_way(int64_t M, int64_t N, int64_t K, int* way);
+int z1_weight_grad8_way(int64_t T, int64_t N, int64_t K, int whole_dwords, int* way);
+
 /* Text for a return code (negative: argument errors; positive: hipError_t). */
 const char* z1_strerror(int code);
 

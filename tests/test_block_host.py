@@ -154,3 +154,28 @@ def test_a_build_without_the_block_side_functions_is_accepted(pkg, tmp_path):
     assert res.returncode == 0 and res.stdout.strip() == 'bound', res.stderr
     res = imported(names[1:], 'import faster_yoco_amd')
     assert res.returncode != 0 and f'RuntimeError: yoco_z1: {tmp_path}' in res.stderr and f'has no {names[0]}' in res.stderr
+
+
+def test_every_form_of_the_products_has_a_tested_shape(pkg):
+    """The shapes that the GPU tests run are in the forms they are listed under, and no shape takes a form that is not listed."""
+    import math
+    import random
+
+    import ways
+    from faster_yoco_amd import _lib
+    L = _lib.lib()
+    for form, shape in ways.PRODUCTS.items():
+        assert ways.product(L, *shape) == form, shape
+    for form, (T, N, K) in ways.GRADIENTS.items():
+        assert ways.gradient(L, T, N, K, N % 2 == 0) == form, (T, N, K)
+    rng = random.Random(5)
+    size = lambda hi: int(math.exp(rng.uniform(0, math.log(hi))))  # noqa: E731
+    products, gradients = set(), set()
+    for _ in range(60000):
+        M, N, K = size(20000), size(20000), size(20000)
+        products.add(ways.product(L, M, N, K))
+        gradients.add(ways.gradient(L, M, N, K, rng.random() < 0.5))
+    assert products == set(ways.PRODUCTS) and gradients == set(ways.GRADIENTS)
+    way = (ctypes.c_int * 4)()
+    assert L.z1_product8_way(0, 8, 8, way) == L.z1_weight_grad8_way(8, 8, 0, 1, way) == -2
+    assert L.z1_product8_way(8, 8, 8, None) == L.z1_weight_grad8_way(8, 8, 8, 1, None) == -1
