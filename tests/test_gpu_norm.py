@@ -362,3 +362,12 @@ def test_gradient_of_an_fp32_bias_without_a_weight(pkg, dev, n, dim):
     assert torch.equal(norm.layer_norm_backward(dyd, xd, mean, rstd, bias=True)[1], db.bfloat16())
     with pytest.raises(RuntimeError, match='expected fp32, bf16 or fp16'):
         norm.layer_norm_backward(dyd, xd, mean, rstd, bias=True, grad_dtype=torch.float64)
+
+
+@pytest.mark.parametrize('center', [True, False], ids=['layer', 'rms'])
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+@pytest.mark.parametrize('dim', [1300, 3000, 5300, 9001, 10240, 12288, 12289])
+def test_forward_of_every_width_that_registers_hold(pkg, dev, dim, dtype, center):
+    """Three to six groups of 8 columns to a lane, one to four waves to a row, and the first width beyond."""
+    x, w, b, _ = inputs(5, dim, dtype, 27)
+    check_forward(pkg, dev, x, w, b if center else None, 1e-5, center)
