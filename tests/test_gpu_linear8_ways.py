@@ -46,3 +46,24 @@ def test_weight_gradient(pkg, dev, form):
         dw = linear8.weight_grad(dy.to(dev), a, dtype)
         near(dw, want, sizes, T, dtype)
         assert torch.equal(dw, linear8.weight_grad(dy.to(dev), a, dtype))
+
+
+def test_whole_numbers_past_32_bits_of_offsets(pkg, dev):
+    """2.2e9 operand bytes in 70000 rows, whole numbers of at most 8: every sum is exact in fp32, so the last rows' products
+    and their part of the weight's gradient are too, and a block of K left out or taken twice shows."""
+    from faster_yoco_amd import act8, linear8
+    n, last, N, K = 70000, 300, 40, 31000
+    assert n * K > 2 ** 31 and 8 * 8 * K < 2 ** 24
+    g = torch.Generator().manual_seed(18)
+    whole = lambda *s: torch.randint(-8, 9, s, generator=g).bfloat16()  # noqa: E731
+    rest, w, dy_rest = whole(last, K), whole(N, K), whole(last, N)
+    x = torch.zeros(n, K, dtype=torch.bfloat16, device=dev)
+    x[-last:] = rest.to(dev)
+    a = act8.pack(x)
+    del x
+    y = linear8.matmul(a, linear8.pack_weight(w.to(dev), transposed=False), torch.float32)
+    assert torch.equal(y[-last:].cpu().double(), rest.double() @ w.double().t()) and not y[:-last].any()
+    dy = torch.zeros(n, N, dtype=torch.bfloat16, device=dev)
+    dy[-last:] = dy_rest.to(dev)
+    dw = linear8.weight_grad(dy, a, torch.float32)
+    assert torch.equal(dw.cpu().double(), dy_rest.double().t() @ rest.double())
