@@ -7,7 +7,8 @@ the operand of an 8-bit product: pack it once -- alone (``pack``) or in the pass
 
 The scale of a block is the least 2^e (e >= -127) with max |x| <= 448 * 2^e over its finite elements, so that scaling is
 exact and an element has one rounding, to the nearest e4m3 value (relative error up to 2^-4; below 2^-6 of its scale, up
-to 2^-10 of the scale).  Infinities and NaN become NaN and do not count for the scale.
+to 2^-10 of the scale).  Infinities and NaN become NaN and do not count for the scale.  No gradient
+passes through ``pack`` and ``unpack``.
 """
 import torch
 

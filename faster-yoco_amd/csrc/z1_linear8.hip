@@ -29,7 +29,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 __device__ __forceinline__ int spread(int row) { return 16 * ((row >> 2) & 1) + 4 * (row >> 3) + (row & 3); }
 
 // Eight bytes of a row and its scale, opened to bf16 (exact: 4 significant bits, and bf16 has fp32's exponents; what is below
-// its least value, 2^-133, rounds to a multiple of that).
+// its least value, 2^-133, rounds to a multiple of that, and 256 * 2^120, to which the largest fp32 values round, is infinite).
 __device__ __forceinline__ u4 open_bf16(u2 q, float f) {
     u4 r;
     r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[0], f, false));
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_kernel(G
     auto lds_k = [&](int buf) { return lds + (2 * kPitchN + buf * kPitchK) * TS; };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_k = (a.K + BK - 1) / BK;
-    const At tile = in_panels(tiles_k, 4);             // 7 x 3072 over 16384 tokens: 52 us in order, 47
+    const At tile = in_panels(tiles_k, 4);             // 7 x 3072 over 16384 tokens: 53 us in order, 47
     const int n0 = tile.down * BN, k0 = tile.across * BK;
     const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
     take_part(a);
@@ -657,7 +657,9 @@ __global__ __launch_bounds__(BN / WN * (BK / WK) * 64) void weight_grad_direct_k
     auto lds_k = [&](int64_t step) { return lds + (2 * kRowN + (step & 1) * kRowK) * TS; };
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tiles_k = (a.K + BK - 1) / BK;
-    const At tile = in_panels(tiles_k, 4);             // 8192 x 3072 over 2048 tokens: 102 us in order, 98.5; of 8 100
+    // in order against panels of 4 (of 8), 2048 tokens: 8192 x 3072 99 us, 96 (97); 4096 x 4096 63, 63 (63); 6144 x 1536 47, 44
+    // (44); 16384 tokens: 4096 x 4096 454, 441 (445); 6144 x 1536 345, 332 (334); 5120 x 2048 360, 360 (360)
+    const At tile = in_panels(tiles_k, 4);
     const int n0 = tile.down * BN, k0 = tile.across * BK;
     const int wn = wave / (BK / WK) * WN, wk = wave % (BK / WK) * WK;
     take_part(a);

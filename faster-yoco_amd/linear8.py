@@ -6,8 +6,10 @@
     dx = linear8.matmul(act8.pack(dy), w, transposed=True)        # dy @ weight
     dw = linear8.weight_grad(dy, a)           # dy.T @ x, from the checkpoint
 
-``linear`` is the three of them as one differentiable function.  Products read e4m3 values and their scales and sum in
-fp32; the weight's gradient reads dy in bf16 and the checkpoint's values, which bf16 holds exactly.
+``linear`` is the three of them as one differentiable function; the others compute values only, and no gradient passes
+through them (torch warns in a backward pass that reaches one).  Products read e4m3 values and their scales, which bf16 holds
+exactly, and sum in fp32 for every result type; the weight's gradient reads dy in bf16 and the checkpoint's values.  (A value that
+rounded up to 2^128, past fp32's largest, multiplies as an infinity.)
 """
 import torch
 from torch.autograd.function import once_differentiable

@@ -2,7 +2,11 @@
 
 The forward pass reads x once and can write, in that pass, y in 8 bits (``y8``: the operand of ``linear8.matmul``) and the
 8-bit rows of x (``checkpoint``), which the backward pass then takes in x's place, so that x itself need not be kept.
-Statistics are fp32, taken about the mean.
+Statistics are fp32, taken about the mean.  y in 8 bits is rounded from its fp32 value: one within fp32's own rounding of the
+middle between two e4m3 values, or a block's largest of where its scale steps, may go either way.
+
+``layer_norm_train`` and ``rms_norm_train`` are differentiable; the others compute values only, and no gradient passes through
+them (torch warns in a backward pass that reaches one).
 """
 import torch
 from torch.autograd.function import once_differentiable
