@@ -76,6 +76,10 @@ BLOCK_SIGNATURES = {
     'z1_norm_backward': ([_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _I64,
                           _P], _I),
     'z1_norm_backward_workspace': ([_I64, _I64], _I64),
+    'z1_add_norm_forward': ([_P, _I64, _P, _I64, _I64, _I64, _I, _P, _P, _I, _F, _I, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+                            _I),
+    'z1_add_norm_backward': ([_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P,
+                              _I64, _P], _I),
     'z1_act8_columns': ([_I64], _I64),
     'z1_act8_scales': ([_I64], _I64),
     'z1_act8_pack': ([_P, _I64, _I64, _I64, _I, _P, _P, _P], _I),

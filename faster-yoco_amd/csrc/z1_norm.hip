@@ -3,6 +3,12 @@
 //   forward   mu = mean(x) (0 for RMS), r = 1/sqrt(mean((x-mu)^2) + eps), y = (x-mu) r w + b
 //   backward  xh = (x-mu) r, g = dy w:  dx = r (g - mean(g) - xh mean(g xh)) (no mean(g) for RMS),
 //             dw = sum over rows of dy xh, db = sum over rows of dy
+//   with the residual stream's addition (ADD)
+//   forward   h = x + residual, rounded to their type, is written and takes x's place
+//   backward  dx has dh added, the gradient that reaches h past the norm; it is both x's and the residual's
+//
+// (The sum is rounded before the norm so that the backward pass, which reads the h that was written, sees the values that were
+// normalised.)
 //
 // All of it is bound by memory: a row is read once, held in registers (kLane = 8 columns of a lane at a time), and the
 // variance is taken about the mean in a second pass over the registers, so that a large common offset costs no digits.
@@ -39,7 +45,28 @@ struct Forward {
     int wpr;                                           // waves of a row: 1, 2 or 4
     int w32;                                           // w and b are fp32 (else x's type)
     float eps;
+    const void* res;                                   // ADD: the residual's rows, and where the sum goes (contiguous)
+    int64_t res_stride;
+    void* sum;
 };
+
+// v + the residual's eight elements, rounded to T.
+template <typename T>
+__device__ __forceinline__ void add_rounded(float* v, const float* e) {
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) v[j] += e[j];
+    if constexpr (sizeof(typename T::elem) == 2) T::open(T::close(v), v);
+}
+// Eight columns of a row from c on, of which n are there.
+template <typename T, bool ADD>
+__device__ __forceinline__ void load_input(const Forward& a, int64_t row, int c, int n, float* v) {
+    load_row<T>(a.x, row * a.stride + c, n, v);
+    if constexpr (ADD) {
+        float e[kLane];
+        load_row<T>(a.res, row * a.res_stride + c, n, e);
+        add_rounded<T>(v, e);
+    }
+}
 
 template <typename T>
 __device__ __forceinline__ void load_weight(const void* p, int w32, int64_t c, int n, float* v) {
@@ -111,7 +138,7 @@ __device__ __forceinline__ void finish8(const Forward& a, int64_t row, int c, in
 // hardware hands out, is faster here than one that takes rows in turn and loads ahead (layer norm of 16384 x 3072 BF16 37.6
 // us, 5.4 TB/s, against 48-65; RMS norm of 8192 x 3072 with 8-bit result and checkpoint 18.9 us, 5.3 TB/s).
 // All loads are under way before the first sum, and none stands behind a branch (settle).
-template <typename T, typename W, int NV, bool CENTER>
+template <typename T, typename W, int NV, bool CENTER, bool ADD>
 __global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
     __shared__ float red[2][kFwdThreads / 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -120,13 +147,18 @@ __global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
     const bool live = row < a.rows;                    // every wave stays for the barriers
     if (!live) row = a.rows - 1;
     const int c0 = (wi * 64 + lane) * kLane, step = wpr * kUnit, last = a.dim - kLane;
-    typename T::raw x[NV];
+    typename T::raw x[NV], e[ADD ? NV : 1];
     typename W::raw w[NV], b[NV];
     const void* p = (const typename T::elem*)a.x + row * a.stride;
     const void* pw = a.w ? a.w : a.b ? a.b : a.x;      // something to load, where there is no weight
     const void* pb = a.b ? a.b : pw;
 #pragma unroll
     for (int k = 0; k < NV; ++k) x[k] = T::load(p, c0 + k * step < last ? c0 + k * step : last);
+    if constexpr (ADD) {
+        const void* pe = (const typename T::elem*)a.res + row * a.res_stride;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) e[k] = T::load(pe, c0 + k * step < last ? c0 + k * step : last);
+    }
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int c = c0 + k * step < last ? c0 + k * step : last;
@@ -141,6 +173,11 @@ __global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         T::open(x[k], v[k]);
+        if constexpr (ADD) {
+            float f[kLane];
+            T::open(e[k], f);
+            add_rounded<T>(v[k], f);
+        }
         if (edge(k)) settle<T>(v[k], by(k));
     }
     if (CENTER) {
@@ -193,6 +230,11 @@ __global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
             put8(a.yq, a.ys, row, c, a, y);
         }
         if (a.cq) put8(a.cq, a.cs, row, c, a, v[k]);
+        if constexpr (ADD) {
+            void* out = (typename T::elem*)a.sum + row * a.dim;
+            if (edge(k)) store_row<T>(out, c, a.dim - c, v[k]);
+            else T::store(out, c, v[k]);
+        }
     }
     if (wi == 0) {
         if (lane == 0) {
@@ -215,16 +257,16 @@ __device__ __forceinline__ float block_sum(float s, float* red, int wave, int wa
 }
 
 // Longer rows: one workgroup reads its row again for each pass, from a cache (2048 x 20000 BF16: 44 us, 3.7 TB/s).
-template <typename T, bool CENTER>
+template <typename T, bool CENTER, bool ADD>
 __global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(Forward a) {
     __shared__ float red[kLongThreads / 64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int64_t row = a.row0 + blockIdx.x, at = row * a.stride;
+    const int64_t row = a.row0 + blockIdx.x;
     const int step = kLongThreads * kLane;
     float mu = 0.0f, s = 0.0f, v[kLane];
     if (CENTER) {
         for (int c = threadIdx.x * kLane; c < a.dim; c += step) {
-            load_row<T>(a.x, at + c, a.dim - c, v);
+            load_input<T, ADD>(a, row, c, a.dim - c, v);
 #pragma unroll
             for (int j = 0; j < kLane; ++j) s += v[j];
         }
@@ -232,7 +274,7 @@ __global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(Forward
     }
     s = 0.0f;
     for (int c = threadIdx.x * kLane; c < a.dim; c += step) {
-        load_row<T>(a.x, at + c, a.dim - c, v);
+        load_input<T, ADD>(a, row, c, a.dim - c, v);
 #pragma unroll
         for (int j = 0; j < kLane; ++j) {
             const float d = j < a.dim - c ? v[j] - mu : 0.0f;
@@ -243,7 +285,8 @@ __global__ __launch_bounds__(kLongThreads) void norm_forward_long_kernel(Forward
     const float r = 1.0f / sqrtf(s / (float)a.dim + a.eps);
     for (int base = wave * kUnit; base < a.wide; base += step) {        // whole waves: the 8-bit forms need 16 lanes
         const int c = base + lane * kLane;
-        load_row<T>(a.x, at + c, a.dim - c, v);
+        load_input<T, ADD>(a, row, c, a.dim - c, v);
+        if constexpr (ADD) store_row<T>(a.sum, row * a.dim + c, a.dim - c, v);
         finish8<T, CENTER>(a, row, c, a.dim - c, mu, r, v);
     }
     if (wave == 0) {
@@ -273,6 +316,8 @@ struct Backward {
     int dim, wide, pitch;
     int wpr;                                           // waves of a row: 1, 2, 4 or 8
     int w32;
+    const void* dh;                                    // ADD: what is added to dx, in dy's type
+    int64_t dh_stride;
 };
 
 // xh of eight columns (zeros past the row's end).
@@ -293,6 +338,16 @@ __device__ __forceinline__ void load_xh(const Backward& a, int64_t row, int c, i
     }
 #pragma unroll
     for (int j = 0; j < kLane; ++j) xh[j] = (CENTER ? (j < n ? xh[j] - mu : 0.0f) : xh[j]) * r;
+}
+
+// ADD: eight columns of dh, added to dx.
+template <typename T>
+__device__ __forceinline__ void add_past(float* dx, const typename T::raw& dh, bool edge, int by) {
+    float v[kLane];
+    T::open(dh, v);
+    if (edge) settle<T>(v, by);
+#pragma unroll
+    for (int j = 0; j < kLane; ++j) dx[j] += v[j];
 }
 
 // Both sums of a row over its wpr waves.
@@ -345,7 +400,7 @@ struct Input<T, true> {
 // of each, which norm_reduce_kernel adds in order.  The next rows are loaded while the present ones are computed, and no
 // load stands behind a branch.  Bound by memory (layer norm of 16384 x 3072 BF16 57 us, 5.3 TB/s; RMS norm from the checkpoint
 // 46 us, 5.5); one workgroup to a CU, as 128 of them (73 us) have too few loads under way and 512 (65) twice the partial rows.
-template <typename T, int NV, bool Q, bool CENTER>
+template <typename T, int NV, bool Q, bool CENTER, bool ADD>
 __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) {
     __shared__ float red[2][kRowThreads / 64][2];
     __shared__ float sums[kRowThreads * NV * kLane];
@@ -374,7 +429,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) 
     }
     float dw[NV][kLane] = {}, db[NV][kLane] = {};
     const float inv = 1.0f / (float)a.dim;
-    typename T::raw dy[NV];
+    typename T::raw dy[NV], dh[ADD ? NV : 1];
     Input<T, Q> x[NV];
     float r_next = 0.0f, mu_next = 0.0f;
     auto fetch = [&](int64_t row) {                    // past the last row: the last, not used
@@ -386,6 +441,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) 
         for (int k = 0; k < NV; ++k) {
             dy[k] = T::load(d, from[k]);
             x[k] = Input<T, Q>::load(a, row, c0 + k * step, from[k]);
+            if constexpr (ADD) dh[k] = T::load((const typename T::elem*)a.dh + row * a.dh_stride, from[k]);
         }
     };
     const int64_t stride = (int64_t)gridDim.x * groups;
@@ -397,11 +453,13 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) 
         const bool live = row < a.rows;
         const float r = r_next, mu = mu_next;
         float xh[NV][kLane], g[NV][kLane], s1 = 0.0f, s2 = 0.0f;
+        typename T::raw past[ADD ? NV : 1];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             T::open(dy[k], g[k]);
             if (edge[k]) settle<T>(g[k], by[k]);
             x[k].open(xh[k], edge[k], by[k], mu);
+            if constexpr (ADD) past[k] = dh[k];
         }
         fetch(row + stride);
         if (!live) {
@@ -434,6 +492,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) 
 #pragma unroll
             for (int j = 0; j < kLane; ++j)
                 dx[j] = __builtin_fmaf(-xh[k][j], m2, CENTER ? g[k][j] - m1 : g[k][j]) * r;
+            if constexpr (ADD) add_past<T>(dx, past[k], edge[k], by[k]);
             if (edge[k]) store_row<T>(out, c0 + k * step, a.dim - c0 - k * step, dx);
             else T::store(out, c0 + k * step, dx);
         }
@@ -531,7 +590,7 @@ __device__ __forceinline__ void strip_sums(const Backward& a, int strip, float (
     __syncthreads();
 }
 
-template <typename T, int NV, bool Q, bool CENTER>
+template <typename T, int NV, bool Q, bool CENTER, bool ADD>
 __global__ __launch_bounds__(kRowThreads) void norm_backward_once_kernel(Backward a, int strips, void* out_w, void* out_b,
                                                                          int grad) {
     __shared__ float red[kRowThreads / 64][2];
@@ -559,13 +618,14 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_once_kernel(Backwar
     const int c0 = (wi * 64 + lane) * kLane, step = wpr * kUnit, last = a.dim - kLane;
     auto edge = [&](int k) { return (wi + 1) * kUnit + k * step > a.dim; };
     auto from = [&](int k) { return c0 + k * step < last ? c0 + k * step : last; };
-    typename T::raw dy[NV];
+    typename T::raw dy[NV], dh[ADD ? NV : 1];
     Input<T, Q> x[NV];
     const void* d = (const typename T::elem*)a.dy + row * a.dy_stride;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         dy[k] = T::load(d, from(k));
         x[k] = Input<T, Q>::load(a, row, c0 + k * step, from(k));
+        if constexpr (ADD) dh[k] = T::load((const typename T::elem*)a.dh + row * a.dh_stride, from(k));
     }
     const float r = a.rstd[row], mu = CENTER ? a.mean[row] : 0.0f;
     float xh[NV][kLane], g[NV][kLane], s1 = 0.0f, s2 = 0.0f;
@@ -599,6 +659,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_once_kernel(Backwar
         float dx[kLane];
 #pragma unroll
         for (int j = 0; j < kLane; ++j) dx[j] = __builtin_fmaf(-xh[k][j], m2, CENTER ? g[k][j] - m1 : g[k][j]) * r;
+        if constexpr (ADD) add_past<T>(dx, dh[k], edge(k), c0 + k * step - from(k));
         if (edge(k)) store_row<T>(out, c0 + k * step, a.dim - c0 - k * step, dx);
         else T::store(out, c0 + k * step, dx);
     }
@@ -606,7 +667,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_backward_once_kernel(Backwar
 
 // Longer rows: dx by one workgroup a row, which reads it twice; the columns' sums apart (norm_columns_kernel).  2048 x 20000
 // BF16: 104 us in all, 2.4 TB/s of what the gradient has to move.
-template <typename T, bool Q, bool CENTER>
+template <typename T, bool Q, bool CENTER, bool ADD>
 __global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(Backward a) {
     __shared__ float red[kLongThreads / 64];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -633,6 +694,11 @@ __global__ __launch_bounds__(kLongThreads) void norm_backward_long_kernel(Backwa
 #pragma unroll
                 for (int j = 0; j < kLane; ++j)
                     g[j] = __builtin_fmaf(-xh[j], m2, CENTER ? g[j] - m1 : g[j]) * r;
+                if constexpr (ADD) {
+                    load_row<T>(a.dh, row * a.dh_stride + c, n, xh);
+#pragma unroll
+                    for (int j = 0; j < kLane; ++j) g[j] += xh[j];
+                }
                 store_row<T>(a.dx, row * a.dim + c, n, g);
             }
         }
@@ -719,36 +785,44 @@ unsigned launch_rows(int64_t left) { return (unsigned)(left < kLaunchRows ? left
 // Waves of a row of `units` * 512 columns: up to three 8-column groups to a lane while that is enough.
 int waves_of(int units) { return units <= 3 ? 1 : units <= 6 ? 2 : units <= 12 ? 4 : 8; }
 
-template <typename T, typename W, bool CENTER>
+template <typename T, typename W, bool CENTER, bool ADD>
 int forward_rows(Forward& a, int nv, hipStream_t st) {
     const int per = kFwdThreads / 64 / a.wpr;
     for (; a.row0 < a.rows; a.row0 += kLaunchRows) {
         const dim3 grid((launch_rows(a.rows - a.row0) + per - 1) / per);
         switch (nv) {
-            case 1: norm_forward_kernel<T, W, 1, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-            case 2: norm_forward_kernel<T, W, 2, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-            case 3: norm_forward_kernel<T, W, 3, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-            case 4: norm_forward_kernel<T, W, 4, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
-            default: norm_forward_kernel<T, W, 6, CENTER><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 1: norm_forward_kernel<T, W, 1, CENTER, ADD><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 2: norm_forward_kernel<T, W, 2, CENTER, ADD><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 3: norm_forward_kernel<T, W, 3, CENTER, ADD><<<grid, kFwdThreads, 0, st>>>(a); break;
+            case 4: norm_forward_kernel<T, W, 4, CENTER, ADD><<<grid, kFwdThreads, 0, st>>>(a); break;
+            default: norm_forward_kernel<T, W, 6, CENTER, ADD><<<grid, kFwdThreads, 0, st>>>(a); break;
         }
     }
     return (int)hipGetLastError();
 }
 
-template <typename T, bool CENTER>
+template <typename T, bool CENTER, bool ADD>
 int forward(Forward& a, hipStream_t st) {
     const int units = (a.dim + kUnit - 1) / kUnit;
     if (units > 4 * 6 || a.dim < kLane) {
         for (; a.row0 < a.rows; a.row0 += kLaunchRows)
-            norm_forward_long_kernel<T, CENTER><<<launch_rows(a.rows - a.row0), kLongThreads, 0, st>>>(a);
+            norm_forward_long_kernel<T, CENTER, ADD><<<launch_rows(a.rows - a.row0), kLongThreads, 0, st>>>(a);
         return (int)hipGetLastError();
     }
     a.wpr = units <= 3 ? 1 : units <= 6 ? 2 : 4;       // two to a lane: 43.4 us, four the same as three, six 47.3
     const int nv = (units + a.wpr - 1) / a.wpr;
     if constexpr (sizeof(typename T::elem) == 2) {
-        if (a.w32 && (a.w || a.b)) return forward_rows<T, F32, CENTER>(a, nv, st);
+        if (a.w32 && (a.w || a.b)) return forward_rows<T, F32, CENTER, ADD>(a, nv, st);
     }
-    return forward_rows<T, T, CENTER>(a, nv, st);
+    return forward_rows<T, T, CENTER, ADD>(a, nv, st);
+}
+template <bool ADD>
+int forward_of(Forward& a, int dtype, bool center, hipStream_t st) {
+    switch (dtype) {
+        case Z1_F32: return center ? forward<F32, true, ADD>(a, st) : forward<F32, false, ADD>(a, st);
+        case Z1_BF16: return center ? forward<BF16, true, ADD>(a, st) : forward<BF16, false, ADD>(a, st);
+        default: return center ? forward<F16, true, ADD>(a, st) : forward<F16, false, ADD>(a, st);
+    }
 }
 
 struct Shape { int wpr, nv, blocks; };                 // wpr 0: the long rows' kernels, `blocks` shares of the rows
@@ -762,11 +836,11 @@ Shape backward_shape(int64_t rows, int dim) {
     return {wpr, (units + wpr - 1) / wpr, (int)(need < kMaxBlocks ? need : kMaxBlocks)};
 }
 
-template <typename T, bool Q, bool CENTER>
+template <typename T, bool Q, bool CENTER, bool ADD>
 int backward(Backward& a, const Shape& s, hipStream_t st) {
     if (s.wpr == 0) {
         for (; a.row0 < a.rows; a.row0 += kLaunchRows)
-            norm_backward_long_kernel<T, Q, CENTER><<<launch_rows(a.rows - a.row0), kLongThreads, 0, st>>>(a);
+            norm_backward_long_kernel<T, Q, CENTER, ADD><<<launch_rows(a.rows - a.row0), kLongThreads, 0, st>>>(a);
         if (a.part) {
             const dim3 grid((unsigned)((a.dim + kColumnThreads * kLane - 1) / (kColumnThreads * kLane)), s.blocks);
             norm_columns_kernel<T, Q, CENTER><<<grid, kColumnThreads, 0, st>>>(a);
@@ -775,10 +849,10 @@ int backward(Backward& a, const Shape& s, hipStream_t st) {
     }
     a.wpr = s.wpr;
     switch (s.nv) {
-        case 1: norm_backward_kernel<T, 1, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
-        case 2: norm_backward_kernel<T, 2, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
-        case 3: norm_backward_kernel<T, 3, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
-        default: norm_backward_kernel<T, 4, Q, CENTER><<<s.blocks, kRowThreads, 0, st>>>(a); break;
+        case 1: norm_backward_kernel<T, 1, Q, CENTER, ADD><<<s.blocks, kRowThreads, 0, st>>>(a); break;
+        case 2: norm_backward_kernel<T, 2, Q, CENTER, ADD><<<s.blocks, kRowThreads, 0, st>>>(a); break;
+        case 3: norm_backward_kernel<T, 3, Q, CENTER, ADD><<<s.blocks, kRowThreads, 0, st>>>(a); break;
+        default: norm_backward_kernel<T, 4, Q, CENTER, ADD><<<s.blocks, kRowThreads, 0, st>>>(a); break;
     }
     return (int)hipGetLastError();
 }
@@ -791,33 +865,33 @@ bool is_once(int64_t rows, int64_t dim) {
     return rows <= kOnceRows && rows * dim <= kOnceElements && dim >= kLane && (dim + kUnit - 1) / kUnit <= 8 * kMaxVectors;
 }
 
-template <typename T, bool Q, bool CENTER>
+template <typename T, bool Q, bool CENTER, bool ADD>
 int backward_once(Backward& a, const Shape& s, void* dw, void* db, int grad, hipStream_t st) {
     a.wpr = s.wpr;
     const int strips = dw || db ? (a.dim + 8 * kStrip - 1) / (8 * kStrip) * 8 : 0;       // as many to each XCD
     const int groups = kRowThreads / 64 / s.wpr;
     const dim3 grid((unsigned)(strips + (a.rows + groups - 1) / groups));
     switch (s.nv) {
-        case 1: norm_backward_once_kernel<T, 1, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
-        case 2: norm_backward_once_kernel<T, 2, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
-        case 3: norm_backward_once_kernel<T, 3, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
-        default: norm_backward_once_kernel<T, 4, Q, CENTER><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+        case 1: norm_backward_once_kernel<T, 1, Q, CENTER, ADD><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+        case 2: norm_backward_once_kernel<T, 2, Q, CENTER, ADD><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+        case 3: norm_backward_once_kernel<T, 3, Q, CENTER, ADD><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
+        default: norm_backward_once_kernel<T, 4, Q, CENTER, ADD><<<grid, kRowThreads, 0, st>>>(a, strips, dw, db, grad); break;
     }
     return (int)hipGetLastError();
 }
-template <typename T>
+template <typename T, bool ADD>
 int once_of(Backward& a, bool center, const Shape& s, void* dw, void* db, int grad, hipStream_t st) {
     if (a.q)
-        return center ? backward_once<T, true, true>(a, s, dw, db, grad, st)
-                      : backward_once<T, true, false>(a, s, dw, db, grad, st);
-    return center ? backward_once<T, false, true>(a, s, dw, db, grad, st)
-                  : backward_once<T, false, false>(a, s, dw, db, grad, st);
+        return center ? backward_once<T, true, true, ADD>(a, s, dw, db, grad, st)
+                      : backward_once<T, true, false, ADD>(a, s, dw, db, grad, st);
+    return center ? backward_once<T, false, true, ADD>(a, s, dw, db, grad, st)
+                  : backward_once<T, false, false, ADD>(a, s, dw, db, grad, st);
 }
 
-template <typename T>
-int backward_of(Backward& a, bool center, const Shape& s, hipStream_t st) {
-    if (a.q) return center ? backward<T, true, true>(a, s, st) : backward<T, true, false>(a, s, st);
-    return center ? backward<T, false, true>(a, s, st) : backward<T, false, false>(a, s, st);
+template <typename T, bool ADD>
+int rows_of(Backward& a, bool center, const Shape& s, hipStream_t st) {
+    if (a.q) return center ? backward<T, true, true, ADD>(a, s, st) : backward<T, true, false, ADD>(a, s, st);
+    return center ? backward<T, false, true, ADD>(a, s, st) : backward<T, false, false, ADD>(a, s, st);
 }
 
 bool bad_dtype(int d) { return d != Z1_F32 && d != Z1_BF16 && d != Z1_F16; }
@@ -830,6 +904,65 @@ int bad_shape(int64_t rows, int64_t dim, int64_t stride) {
     return Z1_OK;
 }
 
+// Checks a call's arguments and launches it.
+template <bool ADD>
+int run_forward(Forward a, int64_t dim, int dtype, int w_dtype, int center, hipStream_t st) {
+    if (const int rc = bad_shape(a.rows, dim, a.stride)) return rc;
+    if (bad_dtype(dtype) || (w_dtype != dtype && w_dtype != Z1_F32)) return Z1_E_DTYPE;
+    if (center != 0 && center != 1) return Z1_E_MODE;
+    if (a.rows == 0) return Z1_OK;
+    if (!a.x || !a.rstd || (center && !a.mean) || !a.y == !a.yq || !a.yq != !a.ys || !a.cq != !a.cs || (a.b && !center))
+        return Z1_E_NULL;
+    if (ADD && (!a.res || !a.sum)) return Z1_E_NULL;
+    return forward_of<ADD>(a, dtype, center, st);
+}
+
+template <bool ADD>
+int run_backward(Backward a, int64_t dim, int dtype, int w_dtype, int center, void* dw, void* db, int grad_dtype,
+                 int64_t workspace_floats, hipStream_t st) {
+    if (const int rc = bad_shape(a.rows, dim, a.dy_stride)) return rc;
+    if (a.x && a.x_stride < 0) return Z1_E_SIZE;
+    if (bad_dtype(dtype) || (w_dtype != dtype && w_dtype != Z1_F32) || bad_dtype(grad_dtype)) return Z1_E_DTYPE;
+    if (center != 0 && center != 1) return Z1_E_MODE;
+    if (db && !center) return Z1_E_NULL;
+    const Shape sh = backward_shape(a.rows, (int)dim);
+    float* const workspace = a.part;
+    if (a.rows > 0) {
+        if (!a.dy || !a.x == !a.q || !a.q != !a.s || !a.rstd || (center && !a.mean) || !a.dx) return Z1_E_NULL;
+        if (ADD && !a.dh) return Z1_E_NULL;
+        const bool once = is_once(a.rows, dim);
+        if (!once && (dw || db)) {
+            if (!workspace) return Z1_E_NULL;
+            if (workspace_floats < (int64_t)sh.blocks * 2 * dim) return Z1_E_WORKSPACE;
+        }
+        if (!dw && !db) a.part = nullptr;
+        if (once) {
+            switch (dtype) {
+                case Z1_F32: return once_of<F32, ADD>(a, center, sh, dw, db, grad_dtype, st);
+                case Z1_BF16: return once_of<BF16, ADD>(a, center, sh, dw, db, grad_dtype, st);
+                default: return once_of<F16, ADD>(a, center, sh, dw, db, grad_dtype, st);
+            }
+        }
+        int rc;
+        switch (dtype) {
+            case Z1_F32: rc = rows_of<F32, ADD>(a, center, sh, st); break;
+            case Z1_BF16: rc = rows_of<BF16, ADD>(a, center, sh, st); break;
+            default: rc = rows_of<F16, ADD>(a, center, sh, st); break;
+        }
+        if (rc) return rc;
+    }
+    if (!dw && !db) return Z1_OK;
+    const int columns = (int)dim * (center ? 2 : 1);
+    const dim3 grid((unsigned)((columns + kReduceColumns - 1) / kReduceColumns));
+    const int parts = a.rows > 0 ? sh.blocks : 0;
+    switch (grad_dtype) {
+        case Z1_F32: norm_reduce_kernel<F32><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
+        case Z1_BF16: norm_reduce_kernel<BF16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
+        default: norm_reduce_kernel<F16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
+    }
+    return (int)hipGetLastError();
+}
+
 }  // namespace
 
 extern "C" {
@@ -837,19 +970,18 @@ extern "C" {
 int z1_norm_forward(const void* x, int64_t rows, int64_t dim, int64_t stride, int dtype, const void* w, const void* b,
                     int w_dtype, float eps, int center, void* y, void* yq, void* ys, void* cq, void* cs, float* mean,
                     float* rstd, void* stream) {
-    if (const int rc = bad_shape(rows, dim, stride)) return rc;
-    if (bad_dtype(dtype) || (w_dtype != dtype && w_dtype != Z1_F32)) return Z1_E_DTYPE;
-    if (center != 0 && center != 1) return Z1_E_MODE;
-    if (rows == 0) return Z1_OK;
-    if (!x || !rstd || (center && !mean) || !y == !yq || !yq != !ys || !cq != !cs || (b && !center)) return Z1_E_NULL;
-    Forward a{x, stride, w, b, y, (uint8_t*)yq, (uint8_t*)ys, (uint8_t*)cq, (uint8_t*)cs, mean, rstd, 0, rows, (int)dim,
-              wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32, eps};
-    const hipStream_t st = (hipStream_t)stream;
-    switch (dtype) {
-        case Z1_F32: return center ? forward<F32, true>(a, st) : forward<F32, false>(a, st);
-        case Z1_BF16: return center ? forward<BF16, true>(a, st) : forward<BF16, false>(a, st);
-        default: return center ? forward<F16, true>(a, st) : forward<F16, false>(a, st);
-    }
+    const Forward a{x, stride, w, b, y, (uint8_t*)yq, (uint8_t*)ys, (uint8_t*)cq, (uint8_t*)cs, mean, rstd, 0, rows, (int)dim,
+                    wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32, eps, nullptr, 0, nullptr};
+    return run_forward<false>(a, dim, dtype, w_dtype, center, (hipStream_t)stream);
+}
+
+int z1_add_norm_forward(const void* x, int64_t stride, const void* residual, int64_t residual_stride, int64_t rows,
+                        int64_t dim, int dtype, const void* w, const void* b, int w_dtype, float eps, int center, void* h,
+                        void* y, void* yq, void* ys, void* cq, void* cs, float* mean, float* rstd, void* stream) {
+    if (residual_stride < 0) return Z1_E_SIZE;
+    const Forward a{x, stride, w, b, y, (uint8_t*)yq, (uint8_t*)ys, (uint8_t*)cq, (uint8_t*)cs, mean, rstd, 0, rows, (int)dim,
+                    wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32, eps, residual, residual_stride, h};
+    return run_forward<true>(a, dim, dtype, w_dtype, center, (hipStream_t)stream);
 }
 
 int64_t z1_norm_backward_workspace(int64_t rows, int64_t dim) {
@@ -862,47 +994,19 @@ int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x
                      int64_t rows, int64_t dim, int dtype, const float* mean, const float* rstd, const void* w,
                      int w_dtype, int center, void* dx, void* dw, void* db, int grad_dtype, float* workspace,
                      int64_t workspace_floats, void* stream) {
-    if (const int rc = bad_shape(rows, dim, dy_stride)) return rc;
-    if (x && x_stride < 0) return Z1_E_SIZE;
-    if (bad_dtype(dtype) || (w_dtype != dtype && w_dtype != Z1_F32) || bad_dtype(grad_dtype)) return Z1_E_DTYPE;
-    if (center != 0 && center != 1) return Z1_E_MODE;
-    if (db && !center) return Z1_E_NULL;
-    const hipStream_t st = (hipStream_t)stream;
-    const Shape sh = backward_shape(rows, (int)dim);
-    if (rows > 0) {
-        if (!dy || !x == !q || !q != !s || !rstd || (center && !mean) || !dx) return Z1_E_NULL;
-        const bool once = is_once(rows, dim);
-        if (!once && (dw || db)) {
-            if (!workspace) return Z1_E_NULL;
-            if (workspace_floats < (int64_t)sh.blocks * 2 * dim) return Z1_E_WORKSPACE;
-        }
-        Backward a{dy, dy_stride, x, x_stride, (const uint8_t*)q, (const uint8_t*)s, mean, rstd, w, dx,
-                   dw || db ? workspace : nullptr, 0, rows, (int)dim, wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32};
-        if (once) {
-            switch (dtype) {
-                case Z1_F32: return once_of<F32>(a, center, sh, dw, db, grad_dtype, st);
-                case Z1_BF16: return once_of<BF16>(a, center, sh, dw, db, grad_dtype, st);
-                default: return once_of<F16>(a, center, sh, dw, db, grad_dtype, st);
-            }
-        }
-        int rc;
-        switch (dtype) {
-            case Z1_F32: rc = backward_of<F32>(a, center, sh, st); break;
-            case Z1_BF16: rc = backward_of<BF16>(a, center, sh, st); break;
-            default: rc = backward_of<F16>(a, center, sh, st); break;
-        }
-        if (rc) return rc;
-    }
-    if (!dw && !db) return Z1_OK;
-    const int columns = (int)dim * (center ? 2 : 1);
-    const dim3 grid((unsigned)((columns + kReduceColumns - 1) / kReduceColumns));
-    const int parts = rows > 0 ? sh.blocks : 0;
-    switch (grad_dtype) {
-        case Z1_F32: norm_reduce_kernel<F32><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
-        case Z1_BF16: norm_reduce_kernel<BF16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
-        default: norm_reduce_kernel<F16><<<grid, 256, 0, st>>>(workspace, parts, (int)dim, columns, dw, db); break;
-    }
-    return (int)hipGetLastError();
+    const Backward a{dy, dy_stride, x, x_stride, (const uint8_t*)q, (const uint8_t*)s, mean, rstd, w, dx, workspace, 0, rows,
+                     (int)dim, wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32, nullptr, 0};
+    return run_backward<false>(a, dim, dtype, w_dtype, center, dw, db, grad_dtype, workspace_floats, (hipStream_t)stream);
+}
+
+int z1_add_norm_backward(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
+                         int64_t h_stride, const void* q, const void* s, int64_t rows, int64_t dim, int dtype,
+                         const float* mean, const float* rstd, const void* w, int w_dtype, int center, void* dx, void* dw,
+                         void* db, int grad_dtype, float* workspace, int64_t workspace_floats, void* stream) {
+    if (dh_stride < 0) return Z1_E_SIZE;
+    const Backward a{dy, dy_stride, h, h_stride, (const uint8_t*)q, (const uint8_t*)s, mean, rstd, w, dx, workspace, 0, rows,
+                     (int)dim, wide_of(dim), pitch_of(dim), 1, w_dtype == Z1_F32, dh, dh_stride};
+    return run_backward<true>(a, dim, dtype, w_dtype, center, dw, db, grad_dtype, workspace_floats, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -29,6 +29,8 @@ struct Api {
     decltype(&::z1_norm_forward) norm_forward;
     decltype(&::z1_norm_backward) norm_backward;
     decltype(&::z1_norm_backward_workspace) norm_backward_workspace;
+    decltype(&::z1_add_norm_forward) add_norm_forward;
+    decltype(&::z1_add_norm_backward) add_norm_backward;
     decltype(&::z1_act8_columns) act8_columns;
     decltype(&::z1_act8_scales) act8_scales;
     decltype(&::z1_act8_pack) act8_pack;
@@ -171,12 +173,21 @@ struct OnDevice {
 int64_t blocks_of(int64_t n) { return (n + 127) / 128; }
 
 // ------------------------------------------------------------------------------------------ norms
-// [y or (yq, ys), mean (center), rstd, (cq, cs) (checkpoint)]
-std::vector<Tensor> norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, bool center,
-                                 bool y8, bool checkpoint) {
-    const char* what = "norm";
+// Rows of x's shape and type.
+Rows rows_like(const Tensor& t, const Tensor& x, const Rows& r, const char* what, const char* name, const char* x_name) {
+    require_on(t, x, what, name);
+    const Rows o = rows_of(t, what, name);
+    TORCH_CHECK(o.rows == r.rows && o.dim == r.dim && o.dtype == r.dtype, what, ": ", x_name, " and ", name,
+                " must have one shape and type");
+    return o;
+}
+
+// [h (residual), y or (yq, ys), mean (center), rstd, (cq, cs) (checkpoint)]
+std::vector<Tensor> forward(const char* what, const Tensor& x, const Tensor* residual, const OptTensor& weight,
+                            const OptTensor& bias, double eps, bool center, bool y8, bool checkpoint) {
     require_gpu(x, what, "x");
     const Rows r = rows_of(x, what, "x");
+    const Rows e = residual ? rows_like(*residual, x, r, what, "residual", "x") : Rows{};
     const void* w = weight_of(weight, x, r.dim, what, "weight");
     const void* b = weight_of(bias, x, r.dim, what, "bias");
     TORCH_CHECK(!b || center, what, ": the uncentred norm takes no bias");
@@ -187,7 +198,8 @@ std::vector<Tensor> norm_forward(const Tensor& x, const OptTensor& weight, const
     std::vector<Tensor> out;
     void *y = nullptr, *yq = nullptr, *ys = nullptr, *cq = nullptr, *cs = nullptr;
     float* mean = nullptr;
-    out.reserve(6);
+    out.reserve(7);
+    if (residual) out.push_back(fresh({r.rows, r.dim}, x.scalar_type()));
     if (y8) {
         Pair p = empty8(r.rows, r.dim, r.rows, what);
         yq = p.q.data_ptr();
@@ -211,31 +223,45 @@ std::vector<Tensor> norm_forward(const Tensor& x, const OptTensor& weight, const
         out.push_back(std::move(p.q));
         out.push_back(std::move(p.s));
     }
-    check_rc(api().norm_forward(r.p, r.rows, r.dim, r.stride, r.dtype, w, b, w_dtype, static_cast<float>(eps), center, y,
-                                yq, ys, cq, cs, mean, rstd, on.stream), "z1_norm_forward");
+    if (residual)
+        check_rc(api().add_norm_forward(r.p, r.stride, e.p, e.stride, r.rows, r.dim, r.dtype, w, b, w_dtype,
+                                        static_cast<float>(eps), center, out[0].data_ptr(), y, yq, ys, cq, cs, mean, rstd,
+                                        on.stream), "z1_add_norm_forward");
+    else
+        check_rc(api().norm_forward(r.p, r.rows, r.dim, r.stride, r.dtype, w, b, w_dtype, static_cast<float>(eps), center, y,
+                                    yq, ys, cq, cs, mean, rstd, on.stream), "z1_norm_forward");
     return out;
 }
 
-// [dx, dw (need_dw), db (need_db)]; x, or its 8-bit rows q, s; dw and db in grad_dtype, else the weight's, else dy's
-std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const OptTensor& q, const OptTensor& s,
-                                  const OptTensor& mean, const Tensor& rstd, const OptTensor& weight, bool center,
-                                  bool need_dw, bool need_db, std::optional<at::ScalarType> grad_dtype) {
-    const char* what = "norm_backward";
+std::vector<Tensor> norm_forward(const Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps, bool center,
+                                 bool y8, bool checkpoint) {
+    return forward("norm", x, nullptr, weight, bias, eps, center, y8, checkpoint);
+}
+
+std::vector<Tensor> add_norm_forward(const Tensor& x, const Tensor& residual, const OptTensor& weight, const OptTensor& bias,
+                                     double eps, bool center, bool y8, bool checkpoint) {
+    return forward("add_norm", x, &residual, weight, bias, eps, center, y8, checkpoint);
+}
+
+// [dx, dw (need_dw), db (need_db)]; x, or its 8-bit rows q, s; dh: added to dx, or null; dw and db in grad_dtype, else the
+// weight's, else dy's
+std::vector<Tensor> backward(const char* what, const Tensor& dy, const Tensor* dh, const OptTensor& x, const OptTensor& q,
+                             const OptTensor& s, const OptTensor& mean, const Tensor& rstd, const OptTensor& weight,
+                             bool center, bool need_dw, bool need_db, std::optional<at::ScalarType> grad_dtype) {
+    const char* x_name = dh ? "h" : "x";
     require_gpu(dy, what, "dy");
     const Rows r = rows_of(dy, what, "dy");
+    const Rows past = dh ? rows_like(*dh, dy, r, what, "dh", "dy") : Rows{};
     const bool packed = q.has_value() && q->defined();
     const bool plain = x.has_value() && x->defined();
-    TORCH_CHECK(packed != plain, what, ": expected x or its 8-bit rows");
+    TORCH_CHECK(packed != plain, what, ": expected ", x_name, " or its 8-bit rows");
     Rows xr{nullptr, r.rows, r.dim, r.dim, r.dtype};
     if (packed) {
         TORCH_CHECK(s.has_value() && s->defined(), what, ": expected the scales of the 8-bit rows");
-        require_on(*q, dy, what, "x");
-        check8(*q, *s, r.rows, r.dim, r.rows, what, "x");
+        require_on(*q, dy, what, x_name);
+        check8(*q, *s, r.rows, r.dim, r.rows, what, x_name);
     } else {
-        require_on(*x, dy, what, "x");
-        xr = rows_of(*x, what, "x");
-        TORCH_CHECK(xr.rows == r.rows && xr.dim == r.dim && xr.dtype == r.dtype, what, ": dy and x must have one shape "
-                    "and type");
+        xr = rows_like(*x, dy, r, what, x_name, "dy");
     }
     TORCH_CHECK(center || !need_db, what, ": the uncentred norm has no bias");
     const float* mp = nullptr;
@@ -255,12 +281,32 @@ std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const Op
     if (need_db) out.push_back(fresh({r.dim}, gt));
     const Workspace parts(need_dw || need_db ? api().norm_backward_workspace(r.rows, r.dim) : 0,
                           "z1_norm_backward_workspace");
-    check_rc(api().norm_backward(r.p, r.stride, plain ? xr.p : nullptr, xr.stride, packed ? q->const_data_ptr() : nullptr,
-                                 packed ? s->const_data_ptr() : nullptr, r.rows, r.dim, r.dtype, mp, rp, w,
-                                 w ? dtype_code(weight->scalar_type(), what) : Z1_F32, center, out[0].data_ptr(),
-                                 need_dw ? out[1].data_ptr() : nullptr, need_db ? out.back().data_ptr() : nullptr,
-                                 grad_code, parts.p, parts.floats, on.stream), "z1_norm_backward");
+    const int w_dtype = w ? dtype_code(weight->scalar_type(), what) : Z1_F32;
+    const void* qp = packed ? q->const_data_ptr() : nullptr;
+    const void* sp = packed ? s->const_data_ptr() : nullptr;
+    void* dw = need_dw ? out[1].data_ptr() : nullptr;
+    void* db = need_db ? out.back().data_ptr() : nullptr;
+    if (dh)
+        check_rc(api().add_norm_backward(r.p, r.stride, past.p, past.stride, xr.p, xr.stride, qp, sp, r.rows, r.dim, r.dtype,
+                                         mp, rp, w, w_dtype, center, out[0].data_ptr(), dw, db, grad_code, parts.p,
+                                         parts.floats, on.stream), "z1_add_norm_backward");
+    else
+        check_rc(api().norm_backward(r.p, r.stride, xr.p, xr.stride, qp, sp, r.rows, r.dim, r.dtype, mp, rp, w, w_dtype,
+                                     center, out[0].data_ptr(), dw, db, grad_code, parts.p, parts.floats, on.stream),
+                 "z1_norm_backward");
     return out;
+}
+
+std::vector<Tensor> norm_backward(const Tensor& dy, const OptTensor& x, const OptTensor& q, const OptTensor& s,
+                                  const OptTensor& mean, const Tensor& rstd, const OptTensor& weight, bool center,
+                                  bool need_dw, bool need_db, std::optional<at::ScalarType> grad_dtype) {
+    return backward("norm_backward", dy, nullptr, x, q, s, mean, rstd, weight, center, need_dw, need_db, grad_dtype);
+}
+
+std::vector<Tensor> add_norm_backward(const Tensor& dy, const Tensor& dh, const OptTensor& h, const OptTensor& q,
+                                      const OptTensor& s, const OptTensor& mean, const Tensor& rstd, const OptTensor& weight,
+                                      bool center, bool need_dw, bool need_db, std::optional<at::ScalarType> grad_dtype) {
+    return backward("add_norm_backward", dy, &dh, h, q, s, mean, rstd, weight, center, need_dw, need_db, grad_dtype);
 }
 
 // ------------------------------------------------------------------------------------------ 8-bit rows and weights
@@ -350,7 +396,7 @@ void refuse_cpu(const c10::OperatorHandle& op, torch::jit::Stack*) {
     TORCH_CHECK(false, op.schema().name(), ": expected GPU tensors (there is no CPU path)");
 }
 
-const char* const kOps[] = {"norm_forward", "norm_backward", "act8_pack", "act8_unpack", "weight8_pack", "product8",
+const char* const kOps[] = {"norm_forward", "norm_backward", "add_norm_forward", "add_norm_backward", "act8_pack", "act8_unpack", "weight8_pack", "product8",
                             "weight_grad8"};
 
 }  // namespace
@@ -360,6 +406,10 @@ TORCH_LIBRARY_FRAGMENT(yoco_z1, m) {
           "-> Tensor[]");
     m.def("norm_backward(Tensor dy, Tensor? x, Tensor? q, Tensor? s, Tensor? mean, Tensor rstd, Tensor? weight, "
           "bool center, bool need_dw, bool need_db, ScalarType? grad_dtype=None) -> Tensor[]");
+    m.def("add_norm_forward(Tensor x, Tensor residual, Tensor? weight, Tensor? bias, float eps, bool center, bool y8, "
+          "bool checkpoint) -> Tensor[]");
+    m.def("add_norm_backward(Tensor dy, Tensor dh, Tensor? h, Tensor? q, Tensor? s, Tensor? mean, Tensor rstd, "
+          "Tensor? weight, bool center, bool need_dw, bool need_db, ScalarType? grad_dtype=None) -> Tensor[]");
     m.def("act8_pack(Tensor x) -> (Tensor, Tensor)");
     m.def("act8_unpack(Tensor q, Tensor s, int dim, ScalarType dtype) -> Tensor");
     m.def("weight8_pack(Tensor w, bool transposed) -> Tensor[]");
@@ -370,6 +420,8 @@ TORCH_LIBRARY_FRAGMENT(yoco_z1, m) {
 TORCH_LIBRARY_IMPL(yoco_z1, CUDA, m) {
     m.impl("norm_forward", &norm_forward);
     m.impl("norm_backward", &norm_backward);
+    m.impl("add_norm_forward", &add_norm_forward);
+    m.impl("add_norm_backward", &add_norm_backward);
     m.impl("act8_pack", &act8_pack);
     m.impl("act8_unpack", &act8_unpack);
     m.impl("weight8_pack", &weight8_pack);
@@ -395,6 +447,8 @@ int z1t_init_block(const char* path) {
     Z1T_RESOLVE(norm_forward)
     Z1T_RESOLVE(norm_backward)
     Z1T_RESOLVE(norm_backward_workspace)
+    Z1T_RESOLVE(add_norm_forward)
+    Z1T_RESOLVE(add_norm_backward)
     Z1T_RESOLVE(act8_columns)
     Z1T_RESOLVE(act8_scales)
     Z1T_RESOLVE(act8_pack)

@@ -287,6 +287,19 @@ int z1_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x
                      int64_t workspace_floats, void* stream);
 int64_t z1_norm_backward_workspace(int64_t rows, int64_t dim);
 
+/* The residual stream's addition and the norm of it in one pass: h = x + residual, rounded to their dtype, is written, and the
+ * norm, its statistics and the checkpoint cq, cs are h's; all else as z1_norm_forward.  h must not overlap x or residual. */
+int z1_add_norm_forward(const void* x, int64_t stride, const void* residual, int64_t residual_stride, int64_t rows,
+                        int64_t dim, int dtype, const void* w, const void* b, int w_dtype, float eps, int center, void* h,
+                        void* y, void* yq, void* ys, void* cq, void* cs, float* mean, float* rstd, void* stream);
+
+/* Its gradients from dy and from dh, the gradient that reaches h past the norm (dtype): dx, which is x's and the residual's
+ * alike, is z1_norm_backward's at h plus dh, with one rounding; dw, db and the workspace as there. */
+int z1_add_norm_backward(const void* dy, int64_t dy_stride, const void* dh, int64_t dh_stride, const void* h,
+                         int64_t h_stride, const void* q, const void* s, int64_t rows, int64_t dim, int dtype,
+                         const float* mean, const float* rstd, const void* w, int w_dtype, int center, void* dx, void* dw,
+                         void* db, int grad_dtype, float* workspace, int64_t workspace_floats, void* stream);
+
 /* Rows to 8 bits and back.  Unpacked, a finite value stays finite: one past dtype's largest becomes the largest. */
 int64_t z1_act8_columns(int64_t dim);
 int64_t z1_act8_scales(int64_t dim);
