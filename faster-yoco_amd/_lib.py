@@ -39,8 +39,19 @@ class Z1UpdateScalars(ctypes.Structure):
                 ('clip_log_out', _P)]
 
 
+class Z1Matrix(ctypes.Structure):
+    """``z1_matrix``."""
+    _fields_ = [('g', _P), ('g_stride', _I64), ('momentum', _P), ('p', _P), ('p16', _P)]
+
+
+class Z1Muon(ctypes.Structure):
+    """``z1_muon``."""
+    _fields_ = [('factor', _P), ('lr', _F), ('keep', _F), ('momentum', _F), ('nesterov', _I), ('steps', _I),
+                ('coefficients', ctypes.POINTER(_F)), ('eps', _F), ('precise', _I)]
+
+
 # name -> (argtypes, restype); every function the header declares.  A build of the ABI may lack BLOCK_SIGNATURES, the part
-# around the update: its update runs, and the block-side operators say that they are missing when called.
+# around the update: its update runs, and the block-side and matrices' operators say that they are missing when called.
 SIGNATURES = {
     'z1_table_create': ([ctypes.POINTER(Z1Tensor), _I, _I, ctypes.POINTER(_P)], _I),
     'z1_table_destroy': ([_P], _I),
@@ -93,6 +104,13 @@ BLOCK_SIGNATURES = {
     'z1_weight_grad8_way': ([_I64, _I64, _I64, _I, ctypes.POINTER(_I)], _I),
 }
 SIGNATURES.update(BLOCK_SIGNATURES)
+MATRIX_SIGNATURES = {
+    'z1_muon_workspace': ([_I64, _I64, _I64, _I], _I64),
+    'z1_orthogonalize': ([_P, _I64, _I64, _I64, _I64, _I64, _I, _P, _I, _I, ctypes.POINTER(_F), _F, _I, _P, _I64, _P], _I),
+    'z1_muon_step': ([ctypes.POINTER(Z1Matrix), _I, _I64, _I64, _I, ctypes.POINTER(Z1Muon), _P, _I64, _P], _I),
+}
+BLOCK_SIGNATURES.update(MATRIX_SIGNATURES)
+SIGNATURES.update(MATRIX_SIGNATURES)
 
 _LIB = None
 

@@ -14,10 +14,11 @@ PKG = os.path.dirname(CSRC)
 ROOT = os.path.dirname(PKG)
 INCLUDE = os.path.join(ROOT, 'include')
 SOURCES = [os.path.join(CSRC, f) for f in ('z1_kernels.hip', 'z1_embedding.hip', 'z1_norm.hip', 'z1_act8.hip',
-                                           'z1_linear8.hip')]
+                                           'z1_linear8.hip', 'z1_muon.hip')]
 OUTPUT = os.path.join(PKG, 'libyoco_z1.so')
 ARCH = os.environ.get('YOCO_Z1_ARCH', 'gfx950')
-OPS_SOURCES = [os.path.join(CSRC, f) for f in ('z1_torch_ops.cpp', 'z1_torch_block_ops.cpp')]
+OPS_SOURCES = [os.path.join(CSRC, f) for f in ('z1_torch_ops.cpp', 'z1_torch_block_ops.cpp',
+                                               'z1_torch_matrix_ops.cpp')]
 OPS_OUTPUT = os.path.join(PKG, 'libyoco_z1_torch.so')
 
 FLAGS = [

@@ -7,26 +7,13 @@
 // Both open their 8-bit operands to bf16, which holds values and scales exactly, and multiply by the bf16 instructions, whose
 // products and sums are fp32: a product on the way from LDS into the instructions, so that 8 bits are moved and staged; the
 // gradient, whose sum runs over tokens, on the way into LDS.
-#include "z1_block.h"
+#include "z1_tiles.h"
 
 #pragma clang fp contract(off)
 
 namespace {
 
 using namespace z1blk;
-
-typedef int i8 __attribute__((ext_vector_type(8)));
-typedef int i4 __attribute__((ext_vector_type(4)));
-typedef float f16 __attribute__((ext_vector_type(16)));
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef short s8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-
-#define Z1B_LDS __attribute__((address_space(3)))
-
-// The 32 x 32 result of a matrix instruction gives lane l column l % 32 and rows 8 (i/4) + 4 (l/32) + i%4, i = 0..15.
-// Reading its first operand's rows in this order makes those 16 consecutive: 16 (l/32) + i.
-__device__ __forceinline__ int spread(int row) { return 16 * ((row >> 2) & 1) + 4 * (row >> 3) + (row & 3); }
 
 // Eight bytes of a row and its scale, opened to bf16 (exact: 4 significant bits, and bf16 has fp32's exponents; what is below
 // its least value, 2^-133, rounds to a multiple of that, and 256 * 2^120, to which the largest fp32 values round, is infinite).
@@ -110,29 +97,6 @@ struct Flush {
     }
 };
 
-// All waves of the workgroup are here, their reads from LDS are done, and of their loads all but the LATER last ones have
-// arrived, direct loads into LDS among them.
-template <int LATER = 0>
-__device__ __forceinline__ void meet() {
-    static_assert(LATER < 64, "the counter's range");
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LATER) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-}
-
-// A raw buffer of `bytes` (none where negative) from p: loads whose lane offset lies past it give zeros (word 3: the raw
-// 32-bit data format).  The scalar offset of a load need not count in that check: it only moves within a row's own bytes.
-// Without a branch: a loop around it keeps its loads on their way.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, int64_t bytes) {
-    const uint32_t low = (uint32_t)bytes, high = (uint32_t)(bytes >> 32);
-    const uint32_t n = (low | (uint32_t)-(int)(high != 0)) & ~(uint32_t)((int)high >> 31);
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n, 0x00020000);
-}
-// 16 bytes a lane, straight into LDS at `to` + 16 * lane.
-__device__ __forceinline__ void load_lds(__amdgpu_buffer_rsrc_t from, void* to, int lane_at, int at) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (Z1B_LDS void*)to, 16, lane_at, at, 0, 0);
-}
-
 // A workgroup's tile, of gridDim.x in rows of `across`.  Workgroups go to the eight XCDs in turn.  In order, an XCD has every
 // eighth tile; in panels, it has one run of them, which goes down `panel` rows of tiles, then to the next column, so that
 // those it has at a time share both operands in its L2.
@@ -159,13 +123,6 @@ struct Product {
     int N, blocks, pitch;                              // blocks of 128 along K
     int64_t wide;
 };
-
-// Staging keeps rows of 128 bytes (one block of K).  A lane of a direct load writes 16 bytes at its own place in a run of
-// 1024, so the order of a row's eight 16-byte pieces is changed at the source: piece p of a row lies at p ^ key(row).  LDS
-// has 64 banks of 4 bytes, two rows: the 16 rows that neighbouring lanes read together are eight of either parity, with
-// eight different keys.
-__device__ __forceinline__ int key_plain(int row) { return row >> 1 & 7; }
-__device__ __forceinline__ int key_spread(int row) { return (row >> 1 & 3) | (row >> 4 & 1) << 2; }
 
 // BT x BO outputs (tokens x outputs) of a workgroup, WT x WO of a wave, S blocks of K staged: two leave room for a second
 // workgroup on a CU (of 128 x 128), four cover the loads' way where there is no second one.

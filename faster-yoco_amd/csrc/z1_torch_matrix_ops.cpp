@@ -1,0 +1,261 @@
+/*
+ * The matrices' update (momentum, orthogonalisation, decay) as PyTorch operators of the namespace yoco_z1: schemas, CUDA (HIP)
+ * kernels -- argument checks and calls of the C ABI on torch's current stream -- and CPU kernels that only raise.  Host code
+ * only.  Results and workspaces come from torch's allocator, on the call's stream, so the operators may be captured in a graph
+ * and used on any stream.  z1t_init_matrix(path) resolves the C ABI, as z1t_init does for the update's operators.
+ */
+#include <ATen/core/Tensor.h>
+#include <ATen/hip/EmptyTensor.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/library.h>
+
+#include <dlfcn.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <optional>
+#include <vector>
+
+#include "yoco_z1.h"
+
+namespace {
+
+using at::Tensor;
+using OptTensor = std::optional<Tensor>;
+
+struct Api {
+    decltype(&::z1_muon_workspace) muon_workspace;
+    decltype(&::z1_orthogonalize) orthogonalize;
+    decltype(&::z1_muon_step) muon_step;
+    decltype(&::z1_strerror) strerror;
+};
+
+Api g_api{};
+bool g_api_ok = false;
+
+const Api& api() {
+    TORCH_CHECK(g_api_ok, "yoco_z1: the matrices' operators are not bound: faster_yoco_amd.library is not imported, or the "
+                         "selected build of libyoco_z1.so lacks them");
+    return g_api;
+}
+
+void check_rc(int64_t rc, const char* what) {
+    if (rc != 0) {
+        const char* s = g_api.strerror ? g_api.strerror(static_cast<int>(rc)) : nullptr;
+        TORCH_CHECK(false, "yoco_z1: ", what, " failed: ", s ? s : "?", " (code ", rc, ")");
+    }
+}
+
+int dtype_code(at::ScalarType t, const char* what, const char* name) {
+    switch (t) {
+        case at::kFloat: return Z1_F32;
+        case at::kBFloat16: return Z1_BF16;
+        case at::kHalf: return Z1_F16;
+        default: TORCH_CHECK(false, what, ": ", name, ": expected fp32, bf16 or fp16, got ", c10::toString(t));
+    }
+}
+
+void require_gpu(const Tensor& t, const char* what, const char* name) {
+    TORCH_CHECK(t.defined() && t.is_cuda(), what, ": ", name, ": expected a GPU tensor (there is no CPU path)");
+}
+
+std::vector<float> coefficients_of(at::ArrayRef<double> c, int64_t steps, const char* what) {
+    TORCH_CHECK(steps >= 1 && steps <= 64, what, ": expected 1 to 64 steps, got ", steps);
+    TORCH_CHECK(static_cast<int64_t>(c.size()) == 3 * steps, what, ": expected three coefficients a step, got ", c.size(),
+                " for ", steps);
+    std::vector<float> f(c.begin(), c.end());
+    return f;
+}
+
+// Matrices of a call at once: as many as keep the workspace near 2 GiB, `most` at most.
+constexpr int64_t kRoom = int64_t{1} << 31;
+int64_t at_once(int64_t count, int64_t m, int64_t n, bool precise, int64_t most) {
+    const int64_t one = api().muon_workspace(1, m, n, precise);
+    if (one < 0) check_rc(one, "z1_muon_workspace");
+    return std::max<int64_t>(1, std::min({count, most, kRoom / one}));
+}
+Tensor workspace_of(int64_t bytes) {
+    if (bytes < 0) check_rc(bytes, "z1_muon_workspace");
+    return Tensor(at::detail::empty_cuda({bytes}, at::kByte, c10::Device(c10::DeviceType::CUDA), std::nullopt));
+}
+
+struct OnDevice {
+    c10::DeviceGuard guard;
+    void* stream;
+    explicit OnDevice(const Tensor& t)
+        : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+};
+
+const char* const kMode = "the coefficients let the iterates leave their range (singular values of at most 1 must stay below 4), "
+                          "or eps is not positive";
+
+// x [count, m, n], rows of neighbouring elements
+Tensor orthogonalize(const Tensor& x, int64_t steps, at::ArrayRef<double> coefficients, double eps, at::ScalarType dtype,
+                     bool precise) {
+    const char* what = "muon.orthogonalize";
+    require_gpu(x, what, "x");
+    TORCH_CHECK(x.dim() == 3, what, ": expected matrices [count, m, n], got ", x.dim(), " dimensions");
+    const int64_t count = x.size(0), m = x.size(1), n = x.size(2);
+    TORCH_CHECK((n <= 1 || x.stride(2) == 1) && (m <= 1 || x.stride(1) >= 0) && (count <= 1 || x.stride(0) >= 0), what,
+                ": expected rows of neighbouring elements");
+    const int code = dtype_code(x.scalar_type(), what, "x"), out_code = dtype_code(dtype, what, "dtype");
+    const std::vector<float> c = coefficients_of(coefficients, steps, what);
+    OnDevice on(x);
+    Tensor out(at::detail::empty_cuda({count, m, n}, dtype, c10::Device(c10::DeviceType::CUDA), std::nullopt));
+    if (out.numel() == 0) return out;
+    const int64_t most = at_once(count, m, n, precise, 1 << 15);
+    const Tensor room = workspace_of(api().muon_workspace(most, m, n, precise));
+    const auto* from = static_cast<const char*>(x.const_data_ptr());
+    auto* to = static_cast<char*>(out.data_ptr());
+    for (int64_t i = 0; i < count; i += most) {
+        const int rc = api().orthogonalize(from + i * x.stride(0) * x.element_size(), x.stride(0), x.stride(1),
+                                           std::min(most, count - i), m, n, code, to + i * m * n * out.element_size(),
+                                           out_code, static_cast<int>(steps), c.data(), static_cast<float>(eps), precise,
+                                           room.data_ptr(), room.numel(), on.stream);
+        TORCH_CHECK(rc != Z1_E_MODE, what, ": ", kMode);
+        check_rc(rc, "z1_orthogonalize");
+    }
+    return out;
+}
+
+void check_matrix(const Tensor& t, const Tensor& like, at::ScalarType dtype, const char* what, const char* name, size_t i) {
+    require_gpu(t, what, name);
+    TORCH_CHECK(t.device() == like.device(), what, ": ", name, "[", i, "] is on ", t.device(), ", the launch runs on ",
+                like.device());
+    TORCH_CHECK(t.scalar_type() == dtype && t.is_contiguous() && t.sizes() == like.sizes(), what, ": ", name, "[", i,
+                "]: expected a contiguous ", c10::toString(dtype), " matrix of p's shape");
+}
+
+// p = keep p - lr X, each matrix with its own
+void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at::TensorList p16, const OptTensor& factor,
+                at::ArrayRef<double> lr, at::ArrayRef<double> keep, double mu, bool nesterov,
+                int64_t steps, at::ArrayRef<double> coefficients, double eps, bool precise) {
+    const char* what = "muon.step_";
+    const size_t count = p.size();
+    TORCH_CHECK(g.size() == count && momentum.size() == count && (p16.empty() || p16.size() == count) && lr.size() == count &&
+                    keep.size() == count,
+                what, ": expected as many gradients, momenta, copies and rates as matrices");
+    const std::vector<float> c = coefficients_of(coefficients, steps, what);
+    TORCH_CHECK(mu >= 0 && mu < 1, what, ": momentum must be in [0, 1)");
+    if (count == 0) return;
+    require_gpu(p[0], what, "p");
+    std::vector<const void*> written;
+    for (size_t i = 0; i < count; ++i) {
+        TORCH_CHECK(p[i].dim() == 2, what, ": p[", i, "]: expected a matrix, got ", p[i].dim(), " dimensions");
+        require_gpu(p[i], what, "p");
+        TORCH_CHECK(p[i].device() == p[0].device(), what, ": the matrices are on different devices");
+        check_matrix(p[i], p[i], at::kFloat, what, "p", i);
+        check_matrix(momentum[i], p[i], at::kFloat, what, "momentum", i);
+        if (!p16.empty()) check_matrix(p16[i], p[i], at::kBFloat16, what, "p16", i);
+        require_gpu(g[i], what, "g");
+        TORCH_CHECK(g[i].device() == p[0].device() && g[i].sizes() == p[i].sizes() &&
+                        (g[i].size(1) <= 1 || g[i].stride(1) == 1) && (g[i].size(0) <= 1 || g[i].stride(0) >= 0),
+                    what, ": g[", i, "]: expected rows of neighbouring elements of p's shape, on its device");
+        dtype_code(g[i].scalar_type(), what, "g");
+        if (p[i].numel() == 0) continue;
+        written.push_back(p[i].const_data_ptr());
+        written.push_back(momentum[i].const_data_ptr());
+        if (!p16.empty()) written.push_back(p16[i].const_data_ptr());
+    }
+    std::sort(written.begin(), written.end());
+    TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), what,
+                ": a tensor that is written is named twice");
+    const float* f = nullptr;
+    if (factor.has_value() && factor->defined()) {
+        require_gpu(*factor, what, "factor");
+        TORCH_CHECK(factor->scalar_type() == at::kFloat && factor->numel() == 1 && factor->device() == p[0].device(), what,
+                    ": factor: expected one fp32 value on the matrices' device");
+        f = static_cast<const float*>(factor->const_data_ptr());
+    }
+    OnDevice on(p[0]);
+
+    // calls of one shape, gradient type and rate
+    std::vector<std::vector<size_t>> groups;
+    for (size_t i = 0; i < count; ++i) {
+        if (p[i].numel() == 0) continue;
+        auto same = [&](const std::vector<size_t>& v) {
+            const size_t k = v[0];
+            return p[k].sizes() == p[i].sizes() && g[k].scalar_type() == g[i].scalar_type() && lr[k] == lr[i] &&
+                   keep[k] == keep[i];
+        };
+        auto it = std::find_if(groups.begin(), groups.end(), same);
+        if (it == groups.end()) groups.push_back({i});
+        else it->push_back(i);
+    }
+    int64_t bytes = 0;
+    for (const auto& v : groups) {
+        const int64_t m = p[v[0]].size(0), n = p[v[0]].size(1);
+        const int64_t need = api().muon_workspace(at_once(v.size(), m, n, precise, Z1_MAX_MATRICES), m, n, precise);
+        if (need < 0) check_rc(need, "z1_muon_workspace");
+        bytes = std::max(bytes, need);
+    }
+    if (groups.empty()) return;
+    const Tensor room = workspace_of(bytes);
+    for (const auto& v : groups) {
+        const int64_t m = p[v[0]].size(0), n = p[v[0]].size(1);
+        const size_t most = static_cast<size_t>(at_once(v.size(), m, n, precise, Z1_MAX_MATRICES));
+        const z1_muon how{f, static_cast<float>(lr[v[0]]), static_cast<float>(keep[v[0]]),
+                          static_cast<float>(mu), nesterov, static_cast<int>(steps), c.data(), static_cast<float>(eps), precise};
+        for (size_t i = 0; i < v.size(); i += most) {
+            z1_matrix list[Z1_MAX_MATRICES];
+            const size_t k = std::min(most, v.size() - i);
+            for (size_t j = 0; j < k; ++j) {
+                const size_t at = v[i + j];
+                list[j] = {g[at].const_data_ptr(), g[at].stride(0), static_cast<float*>(momentum[at].data_ptr()),
+                           static_cast<float*>(p[at].data_ptr()),
+                           p16.empty() ? nullptr : static_cast<uint16_t*>(p16[at].data_ptr())};
+            }
+            const int rc = api().muon_step(list, static_cast<int>(k), m, n, dtype_code(g[v[0]].scalar_type(), what, "g"), &how,
+                                           room.data_ptr(), room.numel(), on.stream);
+            TORCH_CHECK(rc != Z1_E_MODE, what, ": ", kMode);
+            check_rc(rc, "z1_muon_step");
+        }
+    }
+}
+
+void refuse_cpu(const c10::OperatorHandle& op, torch::jit::Stack*) {
+    TORCH_CHECK(false, op.schema().name(), ": expected GPU tensors (there is no CPU path)");
+}
+
+}  // namespace
+
+TORCH_LIBRARY_FRAGMENT(yoco_z1, m) {
+    m.def("orthogonalize(Tensor x, int steps, float[] coefficients, float eps, ScalarType dtype, bool precise) -> Tensor");
+    m.def("muon_step_(Tensor(a!)[] p, Tensor[] g, Tensor(b!)[] momentum, Tensor(c!)[] p16, Tensor? factor, float[] lr, "
+          "float[] keep, float mu, bool nesterov, int steps, float[] coefficients, float eps, "
+          "bool precise) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(yoco_z1, CUDA, m) {
+    m.impl("orthogonalize", &orthogonalize);
+    m.impl("muon_step_", &muon_step_);
+}
+
+TORCH_LIBRARY_IMPL(yoco_z1, CPU, m) {
+    for (const char* name : {"orthogonalize", "muon_step_"})
+        m.impl(name, torch::CppFunction::makeFromBoxedFunction<&refuse_cpu>());
+}
+
+extern "C" {
+
+/* Resolves the C ABI from the already loaded library at `path`: 0, or -1 when it is not loaded, -2 when a function is
+ * missing (an older build of the ABI: the other operators work without these). */
+int z1t_init_matrix(const char* path) {
+    void* h = dlopen(path, RTLD_NOW | RTLD_NOLOAD);
+    if (!h) return -1;
+    Api a{};
+#define Z1T_RESOLVE(field)                                                        \
+    a.field = reinterpret_cast<decltype(a.field)>(dlsym(h, "z1_" #field));        \
+    if (!a.field) return -2;
+    Z1T_RESOLVE(muon_workspace)
+    Z1T_RESOLVE(orthogonalize)
+    Z1T_RESOLVE(muon_step)
+    Z1T_RESOLVE(strerror)
+#undef Z1T_RESOLVE
+    g_api = a;
+    g_api_ok = true;
+    return 0;
+}
+
+}  // extern "C"

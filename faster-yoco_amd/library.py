@@ -56,6 +56,10 @@ def _load():
     rc = L.z1t_init_block(abi._name.encode())
     if rc not in (0, -2):                   # -2: another build of the ABI without them; the operators say so when called
         raise RuntimeError(f'yoco_z1: the block-side operators could not bind to {abi._name} (code {rc})')
+    L.z1t_init_matrix.argtypes, L.z1t_init_matrix.restype = [ctypes.c_char_p], ctypes.c_int
+    rc = L.z1t_init_matrix(abi._name.encode())
+    if rc not in (0, -2):
+        raise RuntimeError(f'yoco_z1: the matrices\' operators could not bind to {abi._name} (code {rc})')
     return L
 
 
@@ -123,4 +127,15 @@ BLOCK_OPS = {
 }
 
 for _name, _fake in BLOCK_OPS.items():
+    torch.library.register_fake(f'{NS}::{_name}', _fake)
+
+
+# ------------------------------------------------------------------------------------------------ the matrices' update
+# (csrc/z1_torch_matrix_ops.cpp)
+MATRIX_OPS = {
+    'orthogonalize': lambda x, steps, coefficients, eps, dtype, precise: x.new_empty(x.shape, dtype=dtype),
+    'muon_step_': _none,
+}
+
+for _name, _fake in MATRIX_OPS.items():
     torch.library.register_fake(f'{NS}::{_name}', _fake)

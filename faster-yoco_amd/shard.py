@@ -115,6 +115,7 @@ class Zero1ShardOptimizer:
         self._factor = torch.ones(1, dtype=torch.float32, device=dev)
         self._norm = torch.zeros(1, dtype=torch.float32, device=dev)
         self._partials_ready = False
+        self._adam_table = shard.table      # the rows that Adam updates (None: none)
         # device_step: the step counter and bias corrections live on the device and the step advances there, so
         # an update captured once in a HIP graph replays correctly at every step (step_count counts host calls)
         self.device_step = bool(device_step)
@@ -231,6 +232,16 @@ class Zero1ShardOptimizer:
         if self.device_step:
             self._step_dev.fill_(int(n))
 
+    def _step_factor(self):
+        """The gradient factor as the step's kernels read it: a device tensor, or None for 1."""
+        factor = self._multiply_factor
+        if torch.is_tensor(factor):
+            return self._as_device_factor(factor)
+        if float(factor) == 1.0:
+            return None
+        self._factor.fill_(float(factor))
+        return self._factor
+
     def step(self, closure=None, groups=None, pieces=None, on_piece=None):
         """Adam + BF16 over the shard with the gradient factor folded into the gradient load, then factor := 1.
 
@@ -246,14 +257,8 @@ class Zero1ShardOptimizer:
                 raise RuntimeError(f'yoco_z1: pieces must run from 0 to {nrows} in order')
         self.step_count += 1
         bc1, bc2 = ops.bias_corrections(self.betas[0], self.betas[1], self.step_count, self.bias_correction)
-        factor = self._multiply_factor
-        if torch.is_tensor(factor):
-            factor = self._as_device_factor(factor)
-        elif float(factor) == 1.0:
-            factor = None
-        else:
-            self._factor.fill_(float(factor))
-            factor = self._factor
+        factor = self._step_factor()
+        table = self._adam_table
         if pieces is not None:
             for a, b in zip(pieces, pieces[1:]):
                 ops.adam_cast_rows(self.shard.table, a, b, factor, self.lr, self.betas[0], self.betas[1], self.eps,
@@ -262,11 +267,12 @@ class Zero1ShardOptimizer:
                     on_piece(a, b)
         elif self.device_step:
             ops.bias_corrections_step(self._step_dev, self.betas[0], self.betas[1], self._bc, self.bias_correction)
-            ops.adam_cast_dev(self.shard.table, factor, self.lr, self.betas[0], self.betas[1], self.eps, self._bc,
-                              self.weight_decay, self.mode)
-        else:
-            ops.adam_cast(self.shard.table, factor, self.lr, self.betas[0], self.betas[1], self.eps, bc1, bc2,
-                          self.weight_decay, self.mode)
+            if table is not None:
+                ops.adam_cast_dev(table, factor, self.lr, self.betas[0], self.betas[1], self.eps, self._bc,
+                                  self.weight_decay, self.mode)
+        elif table is not None:
+            ops.adam_cast(table, factor, self.lr, self.betas[0], self.betas[1], self.eps, bc1, bc2, self.weight_decay,
+                          self.mode)
         self._multiply_factor = 1.0
         self._needs_sync = False
 
