@@ -26,6 +26,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 #pragma clang fp contract(off)
 
 namespace {
@@ -41,6 +43,9 @@ constexpr int kList = 32;                              // matrices named one by 
 
 enum Mode { GRAM, SQUARE, UPDATE, LAST };
 
+// What the last step writes: p and p16 of a list, or the result in a type.
+struct Listed {};
+
 // Where a launch's matrices lie: one by one, or `step` elements apart.
 struct Inputs {
     const void* g[kList];
@@ -52,7 +57,6 @@ struct Inputs {
 struct Batch {
     const void* x;                                     // [count][m][n], rows `stride` and matrices `step` elements apart
     int64_t step, stride;
-    void* out;                                         // contiguous
 };
 
 // The workspace of a launch's matrices, `size` bytes each.
@@ -71,9 +75,7 @@ struct Coefficients {
 
 // What becomes of the last step's X.
 struct Result {
-    Batch batch;                                       // out, or
-    int list;                                          // p and p16 of `in`
-    int dtype;                                         // of out
+    void* out;                                         // contiguous (else p and p16 of `in`)
     int tall;                                          // u has more rows than columns: its rows are c
     float lr, keep;
 };
@@ -100,49 +102,16 @@ __device__ __forceinline__ Place in_panel(int i, int down, int across) {
     return {first + rest % rows, rest / rows};
 }
 
-// 32 rows (t) of 32 N columns (o), out of the matrix instructions' layout by way of a wave's own LDS: put(row, column, v)
-// gets eight neighbours of a row.
-template <int N, typename Put>
-__device__ __forceinline__ void by_rows(float* own, int lane, const f16 (&v)[N], Put put) {
-    constexpr int C = N >= 2 ? 64 : 32, kPitch = C + 4;
-    static_assert(N % (C / 32) == 0, "whole passes");
-    const int r32 = lane & 31, half = lane >> 5, c = lane % (C / 8) * 8, r = lane / (C / 8);
-#pragma unroll
-    for (int i0 = 0; i0 < N; i0 += C / 32) {
-#pragma unroll
-        for (int i = 0; i < C / 32; ++i)
-#pragma unroll
-            for (int k = 0; k < 16; k += 4)
-                *(f4*)(own + r32 * kPitch + i * 32 + half * 16 + k) =
-                    f4{v[i0 + i][k], v[i0 + i][k + 1], v[i0 + i][k + 2], v[i0 + i][k + 3]};
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                     // a wave's own bytes: nobody to meet
-#pragma unroll
-        for (int k = 0; k < 32; k += 512 / C) {
-            float x[8];
-            F32::open({*(const f4*)(own + (k + r) * kPitch + c), *(const f4*)(own + (k + r) * kPitch + c + 4)}, x);
-            put(k + r, i0 * 32 + c, x);
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                     // before the next ones overwrite them
-    }
+// A wave's results change from the matrix instructions' layout to rows, and to columns, by way of its own LDS: up to 64 rows of
+// 64 floats, whose groups of four lie at group ^ turn(row), so that no access of 16 neighbouring lanes meets in a bank: 16 rows'
+// same group (out of the instructions' layout), two rows' groups of one parity (rows), and every eighth row's same columns
+// (columns).
+__device__ __forceinline__ int turn(int row) { return (row & 7) ^ (row & 8) ^ (row >> 3 & 6); }
+__device__ __forceinline__ f4* group_at(float* own, int row, int group) {
+    return (f4*)(own + row * 64 + ((group ^ turn(row)) << 2));
 }
-// The same turned: 32 rows (o) of 32 N columns (t).
-template <int N, typename Put>
-__device__ __forceinline__ void by_columns(float* own, int lane, const f16 (&v)[N], Put put) {
-    constexpr int C = 32 * N, kPitch = C + 4;
-    const int r32 = lane & 31, half = lane >> 5, c = lane % (C / 8) * 8, r = lane / (C / 8);
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-#pragma unroll
-        for (int k = 0; k < 16; ++k) own[(16 * half + k) * kPitch + j * 32 + r32] = v[j][k];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int k = 0; k < 32; k += 512 / C) {
-        float x[8];
-        F32::open({*(const f4*)(own + (k + r) * kPitch + c), *(const f4*)(own + (k + r) * kPitch + c + 4)}, x);
-        put(k + r, c, x);
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-}
+// A wave's own bytes: nobody to meet.
+__device__ __forceinline__ void own_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // Eight values as fp16 at `at` (16-byte aligned), and what that leaves, `plane` bytes on.
 template <bool PAIR>
@@ -157,27 +126,26 @@ __device__ __forceinline__ void put_halves(uint8_t* at, int64_t plane, const flo
         *(Z1B_GLOBAL u4*)(at + plane) = F16::close(lo);
     }
 }
-// Sixteen neighbours from a buffer, zeros past its end.
-__device__ __forceinline__ void open16(__amdgpu_buffer_rsrc_t from, int at, float* v) {
-    const u4 a = __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
-    const u4 b = __builtin_amdgcn_raw_buffer_load_b128(from, at, 16, 0);
-    F16::open(a, v);
-    F16::open(b, v + 8);
+// Eight fp16 of a buffer, and eight floats; zeros past its end.
+__device__ __forceinline__ u4 halves_of(__amdgpu_buffer_rsrc_t from, int at) {
+    return __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
 }
-__device__ __forceinline__ void floats16(__amdgpu_buffer_rsrc_t from, int at, float* v) {
+__device__ __forceinline__ void floats_of(__amdgpu_buffer_rsrc_t from, int at, float* v) {
 #pragma unroll
-    for (int k = 0; k < 16; k += 4) {
+    for (int k = 0; k < 8; k += 4) {
         const u4 a = __builtin_amdgcn_raw_buffer_load_b128(from, at, k * 4, 0);
 #pragma unroll
         for (int l = 0; l < 4; ++l) v[k + l] = as_f32(a[l]);
     }
 }
 
+// A launch's workgroups are the tiles from `first` on, or, with COARSE 2, the four quarters of tiles of twice the size.
+//
 // One launch of a step over `count` matrices: GRAM A = X X^T (operands o, o), SQUARE B from A A^T, UPDATE X from t and B, LAST
 // the same into the result.  BT x BO results (t x o) of a workgroup, WT x WO of a wave, S blocks of 64 columns staged by direct
 // loads; a block's two halves are read ahead by one half and the workgroup meets between them, as in the 8-bit products.
-template <Mode MODE, bool PRECISE, int BT, int BO, int WT, int WO, int S>
-__global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Work w, Coefficients co, Result out, Inputs in) {
+template <Mode MODE, bool PRECISE, typename Out, int COARSE, int BT, int BO, int WT, int WO, int S>
+__global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Work w, Coefficients co, Result out, Inputs in, int first) {
     constexpr bool kSymmetric = MODE == GRAM || MODE == SQUARE;
     constexpr int kWaves = BT / WT * (BO / WO);
     constexpr int kPT = BT / 8 / kWaves, kPO = BO / 8 / kWaves;                // direct loads of a wave: 8 rows each
@@ -188,11 +156,13 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Work w, 
     __shared__ __align__(1024) uint8_t lds[S][(BT + BO) * kRow];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int rows_t = kSymmetric ? w.r : w.c;
-    const int down = (rows_t + BT - 1) / BT, across = (w.r + BO - 1) / BO;
+    const int down = (rows_t + COARSE * BT - 1) / (COARSE * BT), across = (w.r + COARSE * BO - 1) / (COARSE * BO);
     const int tiles = kSymmetric ? down * (down + 1) / 2 : down * across;
-    const int index = in_runs(), z = index / tiles;
+    const int run = in_runs(), index = first + run / (COARSE * COARSE), z = index / tiles;
     const Place tile = kSymmetric ? in_triangle(index - z * tiles) : in_panel(index - z * tiles, down, across);
-    const int t0 = tile.down * BT, o0 = tile.across * BO;
+    const int part = run % (COARSE * COARSE);
+    const int t0 = (tile.down * COARSE + part / COARSE) * BT, o0 = (tile.across * COARSE + part % COARSE) * BO;
+    if (COARSE > 1 && (t0 >= rows_t || o0 >= w.r || (kSymmetric && o0 > t0))) return;          // past the end, or the upper half
     const int wt = wave / (BO / WO) * WT, wo = wave % (BO / WO) * WO;          // the wave's part of the tile
     uint8_t* const mine = w.base + z * w.size;
 
@@ -278,112 +248,127 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Work w, 
     }
     meet();                                            // the staging buffers are free
 
-    // the results in the sums' place, lane by lane: row t, 16 columns o
+    // The results, 64 columns (o) of the wave's rows (t) at a time: to LDS, back as rows of eight columns to a lane, which take
+    // what they need of A or X (whole lines, all under way before the first is used) and go out, and back once more as columns
+    // for the other order.  (Taken in the instructions' layout, 16 columns of a lane's row, the same loads are 64 requests to an
+    // instruction and one latency after the other: an UPDATE's start and end of a 256 x 256 tile took 40 us.)
+    constexpr int kRoom = (int)sizeof(lds) / kWaves, kCols = WO < 64 ? WO : 64;
+    static_assert(WT <= 64 && WT * 64 * 4 <= kRoom, "room for a wave's rows");
+    constexpr int kRowLanes = kCols / 8, kRows = 64 / kRowLanes, kRowTurns = WT / kRows;
+    constexpr int kColumnLanes = WT / 8, kColumns = 64 / kColumnLanes, kColumnTurns = kCols / kColumns;
+    constexpr bool kPlane = MODE == UPDATE || MODE == LAST || (MODE == SQUARE && PRECISE);      // the operand's second halves
+    float* const own = (float*)(&lds[0][0] + wave * kRoom);
     float* const diagonal = (float*)(mine + (MODE == GRAM ? w.d : w.e));
-    // what they need of A or X and of the diagonals: without a branch, a column past the row's end is the next row's, not stored
     const uint8_t* const px = mine + (MODE == SQUARE ? w.A : w.t[w.cur]) + (int64_t)t0 * pitch;
+    // a column past a row's end is the next row's: not stored
     const __amdgpu_buffer_rsrc_t buf_x = buffer_of(px, bytes_t);
     const __amdgpu_buffer_rsrc_t buf_y = buffer_of(px + (MODE == SQUARE ? w.s_plane : w.t_plane), bytes_t);
     const __amdgpu_buffer_rsrc_t buf_d = buffer_of(mine + (MODE == SQUARE ? w.d : w.e), (int64_t)w.ldr * 4);
+    const int m = out.tall ? w.c : w.r, n = out.tall ? w.r : w.c;              // of the result
+    auto deliver = [&](int row, int c, const float* x) {
+        const int left = n - c;
+        if (row >= m || left <= 0) return;
+        const int64_t at = (int64_t)row * n + c;
+        if constexpr (std::is_same_v<Out, Listed>) {
+            float p[8];
+            load_row<F32>(in.p[z], at, left, p);
 #pragma unroll
-    for (int i = 0; i < NO; ++i) {
-        const int o = o0 + wo + i * 32 + half * 16;
+            for (int k = 0; k < 8; ++k) p[k] = __builtin_fmaf(-out.lr, x[k], p[k] * out.keep);
+            store_row<F32>(in.p[z], at, left, p);
+            if (in.p16[z]) store_row<BF16>(in.p16[z], at, left, p);
+        } else {
+            store_row<Out>(out.out, z * ((int64_t)m * n) + at, left, x);
+        }
+    };
+    const bool columns_too = kSymmetric ? t0 != o0 : MODE == UPDATE || !out.tall;
+    const int row0 = lane / kRowLanes, c = lane % kRowLanes * 8;               // of a turn's rows
+    const int col0 = lane / kColumnLanes, r = lane % kColumnLanes * 8;         // of a turn's columns
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int t = t0 + wt + j * 32 + r32, row = (t - t0) * pitch;
-            f16& v = acc[i][j];
-            float x[16] = {}, y[16] = {}, near[16] = {}, dt = 0.0f, own = 0.0f;
-            const bool on = kSymmetric && t0 == o0 && t >= o && t < o + 16;    // the diagonal's element is here
+    for (int i0 = 0; i0 < NO; i0 += kCols / 32) {
+        __builtin_amdgcn_sched_barrier(0);             // one pass's loads at a time: no registers for more
+        const int o = o0 + wo + i0 * 32 + c;
+        u4 x[kRowTurns], y[kPlane ? kRowTurns : 1];
+        float near[8] = {}, dt[kRowTurns];
+        if constexpr (MODE != GRAM) {
+#pragma unroll
+            for (int k = 0; k < kRowTurns; ++k) {
+                const int row = wt + k * kRows + row0;
+                x[k] = halves_of(buf_x, row * pitch + o * 2);
+                if constexpr (kPlane) y[k] = halves_of(buf_y, row * pitch + o * 2);
+                if constexpr (MODE == SQUARE) dt[k] = as_f32(__builtin_amdgcn_raw_buffer_load_b32(buf_d, (t0 + row) * 4, 0, 0));
+            }
+            floats_of(buf_d, o * 4, near);
+        }
+#pragma unroll
+        for (int i = 0; i < kCols / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f16& v = acc[i0 + i][j];
+                    *group_at(own, j * 32 + r32, i * 8 + half * 4 + k) = f4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+                }
+        own_done();
+#pragma unroll
+        for (int k = 0; k < kRowTurns; ++k) {
+            const int row = k * kRows + row0, t = t0 + wt + row;
+            f4* const at[2] = {group_at(own, row, c / 4), group_at(own, row, c / 4 + 1)};
+            float v[8], a[8] = {}, b[8] = {};
+            F32::open({*at[0], *at[1]}, v);
+            const bool on = kSymmetric && t0 == o0 && t >= o && t < o + 8;     // the diagonal's element is here
+            float d = 0.0f;
             if (on) {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) own = t == o + k ? v[k] : own;
+                for (int l = 0; l < 8; ++l) d = t == o + l ? v[l] : d;
             }
-            if (MODE == GRAM) {
+            if constexpr (MODE != GRAM) F16::open(x[k], a);
+            if constexpr (kPlane) F16::open(y[k], b);
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] *= kA / (kX * kX);
-            } else if (MODE == SQUARE) {
-                open16(buf_x, row + o * 2, x);
-                if (PRECISE) open16(buf_y, row + o * 2, y);
-                dt = as_f32(__builtin_amdgcn_raw_buffer_load_b32(buf_d, t * 4, 0, 0));
-                floats16(buf_d, o * 4, near);
+            for (int l = 0; l < 8; ++l) {
+                if (MODE == GRAM) v[l] *= kA / (kX * kX);
+                else if (MODE == SQUARE)
+                    v[l] = __builtin_fmaf(v[l], co.c * (kB / (kA * kA)),
+                                          __builtin_fmaf(co.c, dt[k] + near[l], co.b) * (kB / kA) * (a[l] + b[l]));
+                else v[l] = __builtin_fmaf(near[l], a[l] + b[l], v[l] * (1.0f / kB)) * (MODE == LAST ? 1.0f / kX : 1.0f);
+            }
+            if (on) {
+                d *= MODE == GRAM ? 1.0f / (kX * kX) : 1.0f / (kA * kA);
+                if (t < w.ldr) diagonal[t] = MODE == GRAM ? d : co.a + co.b * dt[k] + co.c * (dt[k] * dt[k] + d);
 #pragma unroll
-                for (int k = 0; k < 16; ++k)
-                    v[k] = __builtin_fmaf(v[k], co.c * (kB / (kA * kA)),
-                                          __builtin_fmaf(co.c, dt + near[k], co.b) * (kB / kA) * (x[k] + y[k]));
-            } else {
-                open16(buf_x, row + o * 2, x);
-                open16(buf_y, row + o * 2, y);
-                floats16(buf_d, o * 4, near);
+                for (int l = 0; l < 8; ++l) v[l] = t == o + l ? 0.0f : v[l];
+            }
+            if (columns_too) {
+                *at[0] = f4{v[0], v[1], v[2], v[3]};
+                *at[1] = f4{v[4], v[5], v[6], v[7]};
+            }
+            if constexpr (kSymmetric) {
+                if (t < w.r && o < w.ldr)
+                    put_halves<PRECISE>(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)t * w.ldr + o) * 2, w.s_plane, v);
+            } else if constexpr (MODE == UPDATE) {
+                if (t < w.c && o < w.ldr) put_halves<true>(mine + w.t[w.cur ^ 1] + ((int64_t)t * w.ldr + o) * 2, w.t_plane, v);
+            } else if (out.tall) {
+                deliver(t, o, v);
+            }
+        }
+        own_done();
+        if (columns_too) {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    v[k] = __builtin_fmaf(near[k], x[k] + y[k], v[k] * (1.0f / kB));
-                    if (MODE == LAST) v[k] *= 1.0f / kX;
+            for (int k = 0; k < kColumnTurns; ++k) {
+                const int column = k * kColumns + col0, oc = o0 + wo + i0 * 32 + column, t = t0 + wt + r;
+                float v[8];
+#pragma unroll
+                for (int l = 0; l < 8; ++l) v[l] = ((const float*)group_at(own, r + l, column >> 2))[column & 3];
+                if constexpr (kSymmetric) {
+                    if (oc < w.r && t < w.ldr)
+                        put_halves<PRECISE>(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)oc * w.ldr + t) * 2, w.s_plane, v);
+                } else if constexpr (MODE == UPDATE) {
+                    if (oc < w.r && t < w.ldc) put_halves<PRECISE>(mine + w.o + ((int64_t)oc * w.ldc + t) * 2, w.o_plane, v);
+                } else {
+                    deliver(oc, t, v);
                 }
             }
-            if (on) {
-                own *= MODE == GRAM ? 1.0f / (kX * kX) : 1.0f / (kA * kA);
-                if (t < w.ldr) diagonal[t] = MODE == GRAM ? own : co.a + co.b * dt + co.c * (dt * dt + own);
-#pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = t == o + k ? 0.0f : v[k];
-            }
-            __builtin_amdgcn_sched_barrier(0);         // one fragment's loads at a time: no registers for more
+            own_done();
         }
-    }
-
-    constexpr int kRoom = (int)sizeof(lds) / kWaves;
-    static_assert(32 * ((WO >= 64 ? 64 : 32) + 4) * 4 <= kRoom && 32 * (WT + 4) * 4 <= kRoom, "room for a wave's rows");
-    float* const own = (float*)(&lds[0][0] + wave * kRoom);
-    auto rows = [&](auto put) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            f16 x[NO];
-#pragma unroll
-            for (int i = 0; i < NO; ++i) x[i] = acc[i][j];
-            by_rows<NO>(own, lane, x, [&](int row, int c, const float* y) { put(t0 + wt + j * 32 + row, o0 + wo + c, y); });
-        }
-    };
-    auto columns = [&](auto put) {
-#pragma unroll
-        for (int i = 0; i < NO; ++i) {
-            by_columns<NT>(own, lane, acc[i], [&](int row, int c, const float* y) { put(o0 + wo + i * 32 + row, t0 + wt + c, y); });
-        }
-    };
-    if constexpr (kSymmetric) {
-        auto put = [&](int row, int c, const float* x) {
-            if (row < w.r && c < w.ldr)
-                put_halves<PRECISE>(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)row * w.ldr + c) * 2, w.s_plane, x);
-        };
-        rows(put);
-        if (t0 != o0) columns(put);
-    } else if constexpr (MODE == UPDATE) {
-        rows([&](int row, int c, const float* x) {
-            if (row < w.c && c < w.ldr) put_halves<true>(mine + w.t[w.cur ^ 1] + ((int64_t)row * w.ldr + c) * 2, w.t_plane, x);
-        });
-        columns([&](int row, int c, const float* x) {
-            if (row < w.r && c < w.ldc) put_halves<PRECISE>(mine + w.o + ((int64_t)row * w.ldc + c) * 2, w.o_plane, x);
-        });
-    } else {
-        const int m = out.tall ? w.c : w.r, n = out.tall ? w.r : w.c;
-        auto put = [&](int row, int c, const float* x) {
-            const int left = n - c;
-            if (row >= m || left <= 0) return;
-            const int64_t at = (int64_t)row * n + c;
-            if (out.list) {
-                float p[8];
-                load_row<F32>(in.p[z], at, left, p);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) p[k] = __builtin_fmaf(-out.lr, x[k], p[k] * out.keep);
-                store_row<F32>(in.p[z], at, left, p);
-                if (in.p16[z]) store_row<BF16>(in.p16[z], at, left, p);
-            } else {
-                const int64_t to = z * ((int64_t)m * n) + at;
-                if (out.dtype == Z1_BF16) store_row<BF16>(out.batch.out, to, left, x);
-                else if (out.dtype == Z1_F16) store_row<F16>(out.batch.out, to, left, x);
-                else store_row<F32>(out.batch.out, to, left, x);
-            }
-        };
-        if (out.tall) rows(put);
-        else columns(put);
     }
 }
 
@@ -562,24 +547,33 @@ bool bounded(const float* coefficients, int steps) {
     return true;
 }
 
-template <Mode MODE, bool PRECISE, int B, int WT, int WO, int S>
-int launch(const Work& w, int64_t count, const Coefficients& co, const Result& out, const Inputs& in, hipStream_t st) {
-    const int64_t across = (w.r + B - 1) / B, down = ((MODE == GRAM || MODE == SQUARE ? w.r : w.c) + B - 1) / B;
-    const int64_t tiles = count * (MODE == GRAM || MODE == SQUARE ? down * (down + 1) / 2 : down * across);
-    if (tiles > kMaxTiles) return Z1_E_SIZE;
-    step_kernel<MODE, PRECISE, B, B, WT, WO, S><<<dim3((unsigned)tiles), B / WT * (B / WO) * 64, 0, st>>>(w, co, out, in);
+template <Mode MODE, bool PRECISE, typename Out, int COARSE, int B, int WT, int WO, int S>
+int launch(const Work& w, int64_t first, int64_t tiles, const Coefficients& co, const Result& out, const Inputs& in,
+           hipStream_t st) {
+    if (tiles * COARSE * COARSE > kMaxTiles) return Z1_E_SIZE;
+    const dim3 grid((unsigned)(tiles * COARSE * COARSE));
+    step_kernel<MODE, PRECISE, Out, COARSE, B, B, WT, WO, S><<<grid, B / WT * (B / WO) * 64, 0, st>>>(w, co, out, in, (int)first);
     return (int)hipGetLastError();
 }
 constexpr int kCus = 256;
-template <Mode MODE, bool PRECISE>
+template <Mode MODE, bool PRECISE, typename Out = Listed>
 int launch_step(const Work& w, int64_t count, const Coefficients& co, const Result& out, const Inputs& in, hipStream_t st) {
     auto tiles = [&](int64_t b) {
         const int64_t across = (w.r + b - 1) / b, down = (w.c + b - 1) / b;
         return count * (MODE == GRAM || MODE == SQUARE ? across * (across + 1) / 2 : down * across);
     };
-    if (tiles(256) >= kCus) return launch<MODE, PRECISE, 256, 64, 128, 2>(w, count, co, out, in, st);
-    if (tiles(128) >= kCus) return launch<MODE, PRECISE, 128, 64, 64, 2>(w, count, co, out, in, st);
-    return launch<MODE, PRECISE, 64, 32, 32, 4>(w, count, co, out, in, st);
+    const int64_t large = tiles(256), rounds = large / kCus, rest = large % kCus;
+    if (rounds > 0) {
+        const int64_t whole = rest * 2 > kCus ? large : large - rest;
+        if (const int rc = launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(w, 0, whole, co, out, in, st)) return rc;
+        if (whole == large) return Z1_OK;
+        if (4 * rest <= kCus) return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 4>(w, whole, rest, co, out, in, st);
+        return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 2>(w, whole, rest, co, out, in, st);
+    }
+    const int64_t middle = tiles(128);
+    if (middle > kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2>(w, 0, middle, co, out, in, st);
+    if (middle * 2 > kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4>(w, 0, middle, co, out, in, st);
+    return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4>(w, 0, tiles(64), co, out, in, st);
 }
 
 template <typename T>
@@ -595,7 +589,7 @@ int start_of(const Start& a, const Work& w, int64_t count, bool precise, hipStre
     return (int)hipGetLastError();
 }
 
-template <bool PRECISE>
+template <bool PRECISE, typename Out>
 int iterate(Work w, int64_t count, int steps, const float* coefficients, const Result& out, const Inputs& in, hipStream_t st) {
     for (int k = 0; k < steps; ++k) {
         const Coefficients co{coefficients[3 * k], coefficients[3 * k + 1], coefficients[3 * k + 2]};
@@ -603,7 +597,7 @@ int iterate(Work w, int64_t count, int steps, const float* coefficients, const R
         if (const int rc = launch_step<GRAM, PRECISE>(w, count, co, out, in, st)) return rc;
         if (const int rc = launch_step<SQUARE, PRECISE>(w, count, co, out, in, st)) return rc;
         const int rc = k + 1 < steps ? launch_step<UPDATE, PRECISE>(w, count, co, out, in, st)
-                                     : launch_step<LAST, PRECISE>(w, count, co, out, in, st);
+                                     : launch_step<LAST, PRECISE, Out>(w, count, co, out, in, st);
         if (rc) return rc;
     }
     return Z1_OK;
@@ -622,6 +616,7 @@ int check(int64_t count, int64_t m, int64_t n, int dtype, int steps, const float
     return Z1_OK;
 }
 
+template <typename Out>
 int run(Start a, int64_t count, int dtype, int steps, const float* coefficients, bool precise, Result out, void* workspace,
         int64_t bytes, hipStream_t st) {
     if (count == 0) return Z1_OK;
@@ -640,8 +635,8 @@ int run(Start a, int64_t count, int dtype, int steps, const float* coefficients,
         default: rc = start_of<F16>(a, w, count, precise, st); break;
     }
     if (rc) return rc;
-    return precise ? iterate<true>(w, count, steps, coefficients, out, a.in, st)
-                   : iterate<false>(w, count, steps, coefficients, out, a.in, st);
+    return precise ? iterate<true, Out>(w, count, steps, coefficients, out, a.in, st)
+                   : iterate<false, Out>(w, count, steps, coefficients, out, a.in, st);
 }
 
 }  // namespace
@@ -661,14 +656,18 @@ int z1_orthogonalize(const void* x, int64_t step, int64_t stride, int64_t count,
     if (out_dtype != Z1_F32 && out_dtype != Z1_BF16 && out_dtype != Z1_F16) return Z1_E_DTYPE;
     if (count > 0 && (!x || !out)) return Z1_E_NULL;
     Start a{};
-    a.batch = {x, step, stride, out};
+    a.batch = {x, step, stride};
     a.m = (int)m;
     a.n = (int)n;
     a.eps = eps;
     Result to{};
-    to.batch = a.batch;
-    to.dtype = out_dtype;
-    return run(a, count, dtype, steps, coefficients, precise != 0, to, workspace, workspace_bytes, (hipStream_t)stream);
+    to.out = out;
+    const hipStream_t st = (hipStream_t)stream;
+    switch (out_dtype) {
+        case Z1_F32: return run<F32>(a, count, dtype, steps, coefficients, precise != 0, to, workspace, workspace_bytes, st);
+        case Z1_BF16: return run<BF16>(a, count, dtype, steps, coefficients, precise != 0, to, workspace, workspace_bytes, st);
+        default: return run<F16>(a, count, dtype, steps, coefficients, precise != 0, to, workspace, workspace_bytes, st);
+    }
 }
 
 int z1_muon_step(const z1_matrix* list, int count, int64_t m, int64_t n, int dtype, const z1_muon* how, void* workspace,
@@ -695,11 +694,10 @@ int z1_muon_step(const z1_matrix* list, int count, int64_t m, int64_t n, int dty
     a.nesterov = how->nesterov;
     a.eps = how->eps;
     Result to{};
-    to.list = 1;
     to.lr = how->lr;
     to.keep = how->keep;
-    return run(a, count, dtype, how->steps, how->coefficients, how->precise != 0, to, workspace, workspace_bytes,
-               (hipStream_t)stream);
+    return run<Listed>(a, count, dtype, how->steps, how->coefficients, how->precise != 0, to, workspace, workspace_bytes,
+                       (hipStream_t)stream);
 }
 
 }  // extern "C"
