@@ -41,13 +41,14 @@ class Z1UpdateScalars(ctypes.Structure):
 
 class Z1Matrix(ctypes.Structure):
     """``z1_matrix``."""
-    _fields_ = [('g', _P), ('g_stride', _I64), ('momentum', _P), ('p', _P), ('p16', _P)]
+    _fields_ = [('g', _P), ('g_stride', _I64), ('momentum', _P), ('p', _P), ('p16', _P), ('m', _I64), ('n', _I64), ('lr', _F),
+                ('keep', _F)]
 
 
 class Z1Muon(ctypes.Structure):
     """``z1_muon``."""
-    _fields_ = [('factor', _P), ('lr', _F), ('keep', _F), ('momentum', _F), ('nesterov', _I), ('steps', _I),
-                ('coefficients', ctypes.POINTER(_F)), ('eps', _F), ('precise', _I)]
+    _fields_ = [('factor', _P), ('momentum', _F), ('nesterov', _I), ('steps', _I), ('coefficients', ctypes.POINTER(_F)),
+                ('eps', _F), ('precise', _I)]
 
 
 # name -> (argtypes, restype); every function the header declares.  A build of the ABI may lack BLOCK_SIGNATURES, the part
@@ -105,9 +106,10 @@ BLOCK_SIGNATURES = {
 }
 SIGNATURES.update(BLOCK_SIGNATURES)
 MATRIX_SIGNATURES = {
-    'z1_muon_workspace': ([_I64, _I64, _I64, _I], _I64),
     'z1_orthogonalize': ([_P, _I64, _I64, _I64, _I64, _I64, _I, _P, _I, _I, ctypes.POINTER(_F), _F, _I, _P, _I64, _P], _I),
-    'z1_muon_step': ([ctypes.POINTER(Z1Matrix), _I, _I64, _I64, _I, ctypes.POINTER(Z1Muon), _P, _I64, _P], _I),
+    'z1_orthogonalize_workspace': ([_I64, _I64, _I64, _I], _I64),
+    'z1_muon_step': ([ctypes.POINTER(Z1Matrix), _I, _I, ctypes.POINTER(Z1Muon), _P, _I64, _P], _I),
+    'z1_muon_workspace': ([ctypes.POINTER(Z1Matrix), _I, _I], _I64),
 }
 BLOCK_SIGNATURES.update(MATRIX_SIGNATURES)
 SIGNATURES.update(MATRIX_SIGNATURES)

@@ -25,9 +25,10 @@ using at::Tensor;
 using OptTensor = std::optional<Tensor>;
 
 struct Api {
-    decltype(&::z1_muon_workspace) muon_workspace;
     decltype(&::z1_orthogonalize) orthogonalize;
+    decltype(&::z1_orthogonalize_workspace) orthogonalize_workspace;
     decltype(&::z1_muon_step) muon_step;
+    decltype(&::z1_muon_workspace) muon_workspace;
     decltype(&::z1_strerror) strerror;
 };
 
@@ -68,15 +69,10 @@ std::vector<float> coefficients_of(at::ArrayRef<double> c, int64_t steps, const 
     return f;
 }
 
-// Matrices of a call at once: as many as keep the workspace near 2 GiB, `most` at most.
+// A call's matrices run in launches whose workspace stays near 2 GiB.
 constexpr int64_t kRoom = int64_t{1} << 31;
-int64_t at_once(int64_t count, int64_t m, int64_t n, bool precise, int64_t most) {
-    const int64_t one = api().muon_workspace(1, m, n, precise);
-    if (one < 0) check_rc(one, "z1_muon_workspace");
-    return std::max<int64_t>(1, std::min({count, most, kRoom / one}));
-}
 Tensor workspace_of(int64_t bytes) {
-    if (bytes < 0) check_rc(bytes, "z1_muon_workspace");
+    if (bytes < 0) check_rc(bytes, "the matrices' workspace");
     return Tensor(at::detail::empty_cuda({bytes}, at::kByte, c10::Device(c10::DeviceType::CUDA), std::nullopt));
 }
 
@@ -104,8 +100,10 @@ Tensor orthogonalize(const Tensor& x, int64_t steps, at::ArrayRef<double> coeffi
     OnDevice on(x);
     Tensor out(at::detail::empty_cuda({count, m, n}, dtype, c10::Device(c10::DeviceType::CUDA), std::nullopt));
     if (out.numel() == 0) return out;
-    const int64_t most = at_once(count, m, n, precise, 1 << 15);
-    const Tensor room = workspace_of(api().muon_workspace(most, m, n, precise));
+    const int64_t one = api().orthogonalize_workspace(1, m, n, precise);
+    if (one < 0) check_rc(one, "z1_orthogonalize_workspace");
+    const int64_t most = std::max<int64_t>(1, std::min({count, int64_t{1} << 15, kRoom / std::max<int64_t>(1, one)}));
+    const Tensor room = workspace_of(api().orthogonalize_workspace(most, m, n, precise));
     const auto* from = static_cast<const char*>(x.const_data_ptr());
     auto* to = static_cast<char*>(out.data_ptr());
     for (int64_t i = 0; i < count; i += most) {
@@ -170,47 +168,40 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
     }
     OnDevice on(p[0]);
 
-    // calls of one shape, gradient type and rate
-    std::vector<std::vector<size_t>> groups;
-    for (size_t i = 0; i < count; ++i) {
-        if (p[i].numel() == 0) continue;
-        auto same = [&](const std::vector<size_t>& v) {
-            const size_t k = v[0];
-            return p[k].sizes() == p[i].sizes() && g[k].scalar_type() == g[i].scalar_type() && lr[k] == lr[i] &&
-                   keep[k] == keep[i];
-        };
-        auto it = std::find_if(groups.begin(), groups.end(), same);
-        if (it == groups.end()) groups.push_back({i});
-        else it->push_back(i);
-    }
+    // launches of one gradient type, as many matrices as may be named and as the workspace holds
+    std::vector<std::vector<z1_matrix>> launches;
+    std::vector<int> codes;
     int64_t bytes = 0;
-    for (const auto& v : groups) {
-        const int64_t m = p[v[0]].size(0), n = p[v[0]].size(1);
-        const int64_t need = api().muon_workspace(at_once(v.size(), m, n, precise, Z1_MAX_MATRICES), m, n, precise);
-        if (need < 0) check_rc(need, "z1_muon_workspace");
-        bytes = std::max(bytes, need);
-    }
-    if (groups.empty()) return;
-    const Tensor room = workspace_of(bytes);
-    for (const auto& v : groups) {
-        const int64_t m = p[v[0]].size(0), n = p[v[0]].size(1);
-        const size_t most = static_cast<size_t>(at_once(v.size(), m, n, precise, Z1_MAX_MATRICES));
-        const z1_muon how{f, static_cast<float>(lr[v[0]]), static_cast<float>(keep[v[0]]),
-                          static_cast<float>(mu), nesterov, static_cast<int>(steps), c.data(), static_cast<float>(eps), precise};
-        for (size_t i = 0; i < v.size(); i += most) {
-            z1_matrix list[Z1_MAX_MATRICES];
-            const size_t k = std::min(most, v.size() - i);
-            for (size_t j = 0; j < k; ++j) {
-                const size_t at = v[i + j];
-                list[j] = {g[at].const_data_ptr(), g[at].stride(0), static_cast<float*>(momentum[at].data_ptr()),
-                           static_cast<float*>(p[at].data_ptr()),
-                           p16.empty() ? nullptr : static_cast<uint16_t*>(p16[at].data_ptr())};
+    for (const at::ScalarType type : {at::kFloat, at::kBFloat16, at::kHalf}) {
+        const size_t first = launches.size();
+        for (size_t i = 0; i < count; ++i) {
+            if (p[i].numel() == 0 || g[i].scalar_type() != type) continue;
+            const z1_matrix x{g[i].const_data_ptr(), g[i].stride(0), static_cast<float*>(momentum[i].data_ptr()),
+                              static_cast<float*>(p[i].data_ptr()),
+                              p16.empty() ? nullptr : static_cast<uint16_t*>(p16[i].data_ptr()), p[i].size(0), p[i].size(1),
+                              static_cast<float>(lr[i]), static_cast<float>(keep[i])};
+            if (launches.size() == first || launches.back().size() == Z1_MAX_MATRICES) {
+                launches.push_back({x});
+                codes.push_back(dtype_code(type, what, "g"));
+            } else {
+                launches.back().push_back(x);
+                if (api().muon_workspace(launches.back().data(), static_cast<int>(launches.back().size()), precise) > kRoom) {
+                    launches.back().pop_back();
+                    launches.push_back({x});
+                    codes.push_back(codes.back());
+                }
             }
-            const int rc = api().muon_step(list, static_cast<int>(k), m, n, dtype_code(g[v[0]].scalar_type(), what, "g"), &how,
-                                           room.data_ptr(), room.numel(), on.stream);
-            TORCH_CHECK(rc != Z1_E_MODE, what, ": ", kMode);
-            check_rc(rc, "z1_muon_step");
+            bytes = std::max(bytes, api().muon_workspace(launches.back().data(), static_cast<int>(launches.back().size()), precise));
         }
+    }
+    if (launches.empty()) return;
+    const Tensor room = workspace_of(bytes);
+    const z1_muon how{f, static_cast<float>(mu), nesterov, static_cast<int>(steps), c.data(), static_cast<float>(eps), precise};
+    for (size_t i = 0; i < launches.size(); ++i) {
+        const int rc = api().muon_step(launches[i].data(), static_cast<int>(launches[i].size()), codes[i], &how, room.data_ptr(),
+                                       room.numel(), on.stream);
+        TORCH_CHECK(rc != Z1_E_MODE, what, ": ", kMode);
+        check_rc(rc, "z1_muon_step");
     }
 }
 
@@ -248,9 +239,10 @@ int z1t_init_matrix(const char* path) {
 #define Z1T_RESOLVE(field)                                                        \
     a.field = reinterpret_cast<decltype(a.field)>(dlsym(h, "z1_" #field));        \
     if (!a.field) return -2;
-    Z1T_RESOLVE(muon_workspace)
     Z1T_RESOLVE(orthogonalize)
+    Z1T_RESOLVE(orthogonalize_workspace)
     Z1T_RESOLVE(muon_step)
+    Z1T_RESOLVE(muon_workspace)
     Z1T_RESOLVE(strerror)
 #undef Z1T_RESOLVE
     g_api = a;

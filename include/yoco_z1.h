@@ -338,14 +338,14 @@ int z1_weight_grad8_way(int64_t T, int64_t N, int64_t K, int whole_dwords, int* 
  * below 32 on their squares (Z1_E_MODE otherwise); eps > 0; steps 1 to 64; m and n at most 2^20.  A matrix with an infinity or
  * a NaN becomes NaN, one of zeros zeros.  precise 0: within about 1e-3 of the exact result (2-norm of the difference over
  * the result's), for bf16 results; 1: as fp32 products leave it, at three times the matrix work.
- * workspace: z1_muon_workspace(count, m, n, precise) bytes of device memory, 16-byte aligned; calls that may overlap must not
+ * workspace: as many bytes of device memory as the workspace function says, 16-byte aligned; calls that may overlap must not
  * share one. */
-int64_t z1_muon_workspace(int64_t count, int64_t m, int64_t n, int precise);
 
 /* out[count][m][n] (out_dtype, contiguous) = x's matrices (dtype), `step` elements apart, rows `stride` apart, orthogonalised. */
 int z1_orthogonalize(const void* x, int64_t step, int64_t stride, int64_t count, int64_t m, int64_t n, int dtype, void* out,
                      int out_dtype, int steps, const float* coefficients, float eps, int precise, void* workspace,
                      int64_t workspace_bytes, void* stream);
+int64_t z1_orthogonalize_workspace(int64_t count, int64_t m, int64_t n, int precise);
 
 #define Z1_MAX_MATRICES 32
 typedef struct z1_matrix {
@@ -354,11 +354,12 @@ typedef struct z1_matrix {
     float* momentum;     /* [m][n], and so are p and p16; all contiguous, and disjoint over a call's matrices */
     float* p;
     uint16_t* p16;       /* the bf16 copy, or NULL */
+    int64_t m, n;
+    float lr;            /* p = keep p - lr orthogonalised(u) */
+    float keep;          /* 1 - learning rate * weight decay */
 } z1_matrix;
 typedef struct z1_muon {
     const float* factor; /* device scalar that multiplies the gradients, or NULL */
-    float lr;            /* of this shape: p = keep p - lr orthogonalised(u) */
-    float keep;          /* 1 - lr * weight decay */
     float momentum;      /* mu: momentum = mu momentum + (1 - mu) factor g */
     int nesterov;        /* u = mu momentum + (1 - mu) factor g with the new momentum; 0: u = the new momentum */
     int steps;
@@ -366,9 +367,10 @@ typedef struct z1_muon {
     float eps;
     int precise;
 } z1_muon;
-/* One update of up to Z1_MAX_MATRICES matrices of one shape. */
-int z1_muon_step(const z1_matrix* list, int count, int64_t m, int64_t n, int dtype, const z1_muon* how, void* workspace,
-                 int64_t workspace_bytes, void* stream);
+/* One update of up to Z1_MAX_MATRICES matrices, of any shapes: their products share the launches. */
+int z1_muon_step(const z1_matrix* list, int count, int dtype, const z1_muon* how, void* workspace, int64_t workspace_bytes,
+                 void* stream);
+int64_t z1_muon_workspace(const z1_matrix* list, int count, int precise);
 
 /* Text for a return code (negative: argument errors; positive: hipError_t). */
 const char* z1_strerror(int code);

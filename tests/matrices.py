@@ -41,6 +41,20 @@ def _pair(v, scale):
     return hi, _h(v - hi, scale)
 
 
+def _product(p, q, pairs):
+    """p @ q of pairs (hi, lo) or of first halves alone.  In fp32 the sums are added as the kernels add them, 16 terms at a time
+    and hi hi before hi lo before lo hi: N additions one after another, each off by up to U32 of the sum so far, are less exact
+    than a library's blocked ones."""
+    (ph, pl), (qh, ql) = p, q
+    if not pairs:
+        return ph @ qh
+    acc = torch.zeros(ph.shape[0], qh.shape[1], dtype=ph.dtype)
+    for a, b in ((ph, qh), (ph, ql), (pl, qh)):
+        for k in range(0, a.shape[1], 16):
+            acc = acc + (a[:, k:k + 16].double() @ b[k:k + 16].double()).float()
+    return acc
+
+
 def stored(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, precise=False):
     """One matrix's steps with operands rounded as they are stored; precise: as pairs, and products and sums in fp32."""
     x = start(x, eps)
@@ -50,20 +64,16 @@ def stored(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, precise=False):
     for a, b, c in triples(coefficients, steps):
         hi, lo = _pair(x, KX)
         x = hi + lo
-        if precise:
-            A = hi @ hi.t() + (hi @ lo.t() + lo @ hi.t())
-        else:
-            A = hi @ hi.t()
+        A = _product((hi, lo), (hi.t(), lo.t()), precise)
         d = A.diagonal().clone()
         A = A - torch.diag(d)
         Ah, Al = _pair(A, KA)
         A = Ah + Al if precise else Ah
-        S = Ah @ Ah + (Ah @ Al + Al @ Ah) if precise else Ah @ Ah
+        S = _product((Ah, Al), (Ah, Al), precise)
         e = a + b * d + c * d * d + c * S.diagonal()
         B = c * S + (b + c * (d[:, None] + d)) * A
         B = B - torch.diag(B.diagonal())
-        Bh, Bl = _pair(B, KB)
-        x = e[:, None] * x + (Bh @ hi + (Bh @ lo + Bl @ hi) if precise else Bh @ hi)
+        x = e[:, None] * x + _product(_pair(B, KB), (hi, lo), precise)
     x = x.t() if tall else x
     return x.double()
 

@@ -12,7 +12,8 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 # one row or column, less than a block and a tile, their neighbours, tall and wide, every tile's size and its ends
 SHAPES = [(1, 1), (1, 9), (7, 1), (2, 2), (3, 5), (16, 16), (17, 100), (63, 64), (65, 64), (64, 65), (128, 130), (100, 37),
-          (200, 333), (257, 256), (300, 1000), (511, 129)]
+          (31, 33), (32, 2048), (2048, 20), (64, 1000), (96, 300),
+          (129, 131), (200, 333), (257, 256), (300, 1000), (511, 129), (128, 512), (127, 600), (512, 120), (130, 4000)]
 KINDS = ['noise', 'strong', 'falling', 'flat']
 
 

@@ -19,12 +19,12 @@ def test_argument_errors_without_device_work(pkg):
     L = _lib.lib()
     NULL, SIZE, DTYPE, MODE, WS = -1, -2, -3, -5, -6
     a = P(64)                                                     # never read: every call below stops before a launch
-    need = L.z1_muon_workspace(2, 30, 70, 0)
-    assert need > 0 and need % 16 == 0 and L.z1_muon_workspace(2, 30, 70, 1) > need
-    assert L.z1_muon_workspace(2, 70, 30, 0) == need and L.z1_muon_workspace(0, 30, 70, 0) == 0
+    need = L.z1_orthogonalize_workspace(2, 300, 700, 0)
+    assert need > 0 and need % 16 == 0 and L.z1_orthogonalize_workspace(2, 300, 700, 1) > need
+    assert L.z1_orthogonalize_workspace(2, 700, 300, 0) == need and L.z1_orthogonalize_workspace(0, 300, 700, 0) == 0
     for bad in ((-1, 30, 70), (2, 0, 70), (2, 30, 0), (2, 30, (1 << 20) + 1), (1 << 20, 30, 70)):
-        assert L.z1_muon_workspace(*bad, 0) == SIZE
-    call = lambda **k: L.z1_orthogonalize(*({'x': a, 'step': 2100, 'stride': 70, 'count': 2, 'm': 30, 'n': 70, 'dtype': 1,  # noqa: E731
+        assert L.z1_orthogonalize_workspace(*bad, 0) == SIZE
+    call = lambda **k: L.z1_orthogonalize(*({'x': a, 'step': 2100, 'stride': 700, 'count': 2, 'm': 300, 'n': 700, 'dtype': 1,  # noqa: E731
                                              'out': a, 'od': 1, 'steps': 1, 'c': floats(GOOD), 'eps': 1e-7, 'precise': 0,
                                              'ws': a, 'bytes': need, 'stream': None} | k).values())
     for bad, rc in (({'count': -1}, SIZE), ({'m': 0}, SIZE), ({'n': 1 << 21}, SIZE), ({'stride': -1}, SIZE), ({'step': -1}, SIZE),
@@ -34,15 +34,24 @@ def test_argument_errors_without_device_work(pkg):
                     ({'bytes': need - 1}, WS), ({'precise': 1}, WS)):
         assert call(**bad) == rc, bad
     assert call(count=0, x=None, out=None, ws=None) == 0
-    m = _lib.Z1Matrix(a, 70, a, a, None)
-    how = _lib.Z1Muon(None, 1e-3, 1.0, 0.9, 1, 1, floats(GOOD), 1e-7, 0)
-    step = lambda **k: L.z1_muon_step(*({'list': (_lib.Z1Matrix * 2)(m, m), 'count': 2, 'm': 30, 'n': 70, 'dtype': 1,  # noqa: E731
-                                         'how': ctypes.byref(how), 'ws': a, 'bytes': need, 'stream': None} | k).values())
-    none = [_lib.Z1Matrix(None, 70, a, a, None), _lib.Z1Matrix(a, 70, None, a, None), _lib.Z1Matrix(a, 70, a, None, None)]
-    for bad, rc in (({'count': -1}, SIZE), ({'count': 33}, SIZE), ({'m': 0}, SIZE), ({'dtype': 9}, DTYPE), ({'how': None}, NULL),
-                    ({'list': None}, NULL), *(({'list': (_lib.Z1Matrix * 2)(m, b)}, NULL) for b in none),
-                    ({'list': (_lib.Z1Matrix * 2)(m, _lib.Z1Matrix(a, -1, a, a, None))}, SIZE), ({'ws': None}, NULL),
-                    ({'bytes': need - 1}, WS)):
+    matrix = lambda **k: _lib.Z1Matrix(*({'g': a, 'stride': 700, 'momentum': a, 'p': a, 'p16': None, 'm': 300, 'n': 700,  # noqa: E731
+                                          'lr': 1e-3, 'keep': 1.0} | k).values())
+    two = lambda **k: (_lib.Z1Matrix * 2)(matrix(), matrix(**k))  # noqa: E731
+    need = L.z1_muon_workspace(two(), 2, 0)
+    assert need == L.z1_orthogonalize_workspace(2, 300, 700, 0) and L.z1_muon_workspace(two(), 2, 1) > need
+    assert L.z1_muon_workspace(None, 0, 0) == 0 and L.z1_muon_workspace(None, 1, 0) == NULL
+    assert L.z1_muon_workspace(two(), 33, 0) == L.z1_muon_workspace(two(), -1, 0) == SIZE
+    assert L.z1_muon_workspace(two(m=0), 2, 0) == L.z1_muon_workspace(two(n=1 << 21), 2, 0) == SIZE
+    good = _lib.Z1Muon(None, 0.9, 1, 1, floats(GOOD), 1e-7, 0)
+    how = lambda **k: ctypes.byref(_lib.Z1Muon(*({'f': None, 'mu': 0.9, 'n': 1, 'steps': 1, 'c': floats(GOOD), 'eps': 1e-7,  # noqa: E731
+                                                  'precise': 0} | k).values()))
+    step = lambda **k: L.z1_muon_step(*({'list': two(), 'count': 2, 'dtype': 1, 'how': ctypes.byref(good), 'ws': a,  # noqa: E731
+                                         'bytes': need, 'stream': None} | k).values())
+    for bad, rc in (({'count': -1}, SIZE), ({'count': 33}, SIZE), ({'list': two(m=0)}, SIZE), ({'dtype': 9}, DTYPE),
+                    ({'how': None}, NULL), ({'list': None}, NULL), ({'list': two(g=None)}, NULL), ({'list': two(p=None)}, NULL),
+                    ({'list': two(momentum=None)}, NULL), ({'list': two(stride=-1)}, SIZE), ({'how': how(steps=0)}, SIZE),
+                    ({'how': how(c=None)}, NULL), ({'how': how(eps=0.0)}, MODE), ({'how': how(c=floats([9, 0, 0]))}, MODE),
+                    ({'ws': None}, NULL), ({'bytes': need - 1}, WS), ({'how': how(precise=1)}, WS)):
         assert step(**bad) == rc, bad
     assert step(count=0, list=None, ws=None) == 0
 
@@ -59,7 +68,7 @@ def test_coefficients_are_admitted_as_the_polynomial_says(pkg):
         c = [[rng.uniform(0, 4.2), rng.uniform(-6, 1), rng.choice((0.0, rng.uniform(-1, 4)))] for _ in range(steps)]
         if k == 0:
             c = [GOOD] * 5
-        rc = L.z1_orthogonalize(P(64), 0, 8, 1, 8, 8, 0, P(64), 0, len(c), floats([v for t in c for v in t]), 1e-7, 0, None, 0, None)
+        rc = L.z1_orthogonalize(P(64), 0, 700, 1, 300, 700, 0, P(64), 0, len(c), floats([v for t in c for v in t]), 1e-7, 0, None, 0, None)
         admitted = rc == -1                                       # the missing workspace is what it stops at
         assert admitted or rc == -5
         seen[admitted] += 1
