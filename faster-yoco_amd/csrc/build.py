@@ -14,7 +14,8 @@ PKG = os.path.dirname(CSRC)
 ROOT = os.path.dirname(PKG)
 INCLUDE = os.path.join(ROOT, 'include')
 SOURCES = [os.path.join(CSRC, f) for f in ('z1_kernels.hip', 'z1_embedding.hip', 'z1_norm.hip', 'z1_act8.hip',
-                                           'z1_linear8.hip', 'z1_muon.hip')]
+                                           'z1_linear8.hip', 'z1_muon.hip', 'z1_muon_fast.hip',
+                                           'z1_muon_precise.hip', 'z1_muon_small.hip')]
 OUTPUT = os.path.join(PKG, 'libyoco_z1.so')
 ARCH = os.environ.get('YOCO_Z1_ARCH', 'gfx950')
 OPS_SOURCES = [os.path.join(CSRC, f) for f in ('z1_torch_ops.cpp', 'z1_torch_block_ops.cpp',
@@ -49,7 +50,7 @@ def build(output=OUTPUT, extra=(), verbose=False):
             print('\n'.join(noise), file=sys.stderr)
 
     tmp = output + '.tmp'
-    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(4) as pool:
+    with tempfile.TemporaryDirectory() as d, ThreadPoolExecutor(8) as pool:
         objects = [os.path.join(d, os.path.basename(s) + '.o') for s in SOURCES]
         compile_ = [f for f in FLAGS if f != '-shared'] + list(extra) + ['-I', INCLUDE, '-c']
         list(pool.map(lambda so: run([hipcc()] + compile_ + ['-o', so[1], so[0]]), zip(SOURCES, objects)))

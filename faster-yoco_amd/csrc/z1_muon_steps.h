@@ -1,0 +1,357 @@
+// A step's products over matrices of any size (the mathematics: z1_muon.h).  Included by one source for each PRECISE.
+#pragma once
+
+#include "z1_muon.h"
+
+#include <type_traits>
+
+namespace {
+
+using namespace z1muon;
+
+// ------------------------------------------------------------------------------------------------------ products
+// A launch's i-th workgroup in an order that gives each XCD one run of neighbours.
+__device__ __forceinline__ int in_runs() {
+    const int total = gridDim.x, x = blockIdx.x & 7, share = total >> 3, more = total & 7;
+    return x * share + (x < more ? x : more) + (int)(blockIdx.x >> 3);
+}
+struct Place {
+    int down, across;
+};
+// The i-th tile of a lower triangle, in rows.
+__device__ __forceinline__ Place in_triangle(int i) {
+    int d = (int)((sqrtf(8.0f * (float)i + 1.0f) - 1.0f) * 0.5f);
+    while (d * (d + 1) / 2 > i) --d;
+    while ((d + 1) * (d + 2) / 2 <= i) ++d;
+    return {d, i - d * (d + 1) / 2};
+}
+// The i-th tile of `down` x `across`, in panels of 8 rows, each down its columns.
+__device__ __forceinline__ Place in_panel(int i, int down, int across) {
+    const int first = i / (8 * across) * 8, rest = i - first * across, rows = down - first < 8 ? down - first : 8;
+    return {first + rest % rows, rest / rows};
+}
+
+// A wave's results change from the matrix instructions' layout to rows, and to columns, by way of its own LDS: up to 64 rows of
+// 64 floats, whose groups of four lie at group ^ turn(row), so that no access of 16 neighbouring lanes meets in a bank: 16 rows'
+// same group (out of the instructions' layout), two rows' groups of one parity (rows), and every eighth row's same columns
+// (columns).
+__device__ __forceinline__ int turn(int row) { return (row & 7) ^ (row & 8) ^ (row >> 3 & 6); }
+__device__ __forceinline__ f4* group_at(float* own, int row, int group) {
+    return (f4*)(own + row * 64 + ((group ^ turn(row)) << 2));
+}
+// A wave's own bytes: nobody to meet.
+__device__ __forceinline__ void own_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Eight fp16 of a buffer, and eight floats; zeros past its end.
+__device__ __forceinline__ u4 halves_of(__amdgpu_buffer_rsrc_t from, int at) {
+    return __builtin_amdgcn_raw_buffer_load_b128(from, at, 0, 0);
+}
+__device__ __forceinline__ void floats_of(__amdgpu_buffer_rsrc_t from, int at, float* v) {
+#pragma unroll
+    for (int k = 0; k < 8; k += 4) {
+        const u4 a = __builtin_amdgcn_raw_buffer_load_b128(from, at, k * 4, 0);
+#pragma unroll
+        for (int l = 0; l < 4; ++l) v[k + l] = as_f32(a[l]);
+    }
+}
+
+// A launch's workgroups are the tiles from `first` on, or, with COARSE 2, the four quarters of tiles of twice the size.
+//
+// One launch of a step over `count` matrices: GRAM A = X X^T (operands o, o), SQUARE B from A A^T, UPDATE X from t and B, LAST
+// the same into the result.  BT x BO results (t x o) of a workgroup, WT x WO of a wave, S blocks of 64 columns staged by direct
+// loads; a block's two halves are read ahead by one half and the workgroup meets between them, as in the 8-bit products.
+template <Mode MODE, bool PRECISE, typename Out, int COARSE, int BT, int BO, int WT, int WO, int S>
+__global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan plan, Coefficients co, void* out, Inputs in, int first) {
+    constexpr bool kSymmetric = MODE == GRAM || MODE == SQUARE;
+    constexpr int kWaves = BT / WT * (BO / WO);
+    constexpr int kPT = BT / 8 / kWaves, kPO = BO / 8 / kWaves;                // direct loads of a wave: 8 rows each
+    constexpr int NT = WT / 32, NO = WO / 32;
+    static_assert(!kSymmetric || BT == BO, "a triangle of square tiles");
+    static_assert(S == 2 || S == 4, "a block's buffer is kb & (S - 1)");
+    constexpr int kRow = kHalves * 2;
+    __shared__ __align__(1024) uint8_t lds[S][(BT + BO) * kRow];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int run = in_runs(), index = first + run / (COARSE * COARSE);
+    const Group& g = group_of_tile(plan, index);
+    const Layout w = layout_of(g.r, g.c, PRECISE);
+    const int64_t t_now = plan.cur ? w.t[1] : w.t[0], t_next = plan.cur ? w.t[0] : w.t[1];
+    const int rows_t = kSymmetric ? g.r : g.c;
+    const int down = (rows_t + COARSE * BT - 1) / (COARSE * BT), across = (g.r + COARSE * BO - 1) / (COARSE * BO);
+    const int tiles = kSymmetric ? down * (down + 1) / 2 : down * across;
+    const int nth = (index - g.tile0) / tiles, place = index - g.tile0 - nth * tiles, z = g.first + nth;
+    const Place tile = kSymmetric ? in_triangle(place) : in_panel(place, down, across);
+    const int part = run % (COARSE * COARSE);
+    const int t0 = (tile.down * COARSE + part / COARSE) * BT, o0 = (tile.across * COARSE + part % COARSE) * BO;
+    if (COARSE > 1 && (t0 >= rows_t || o0 >= g.r || (kSymmetric && o0 > t0))) return;          // past the end, or the upper half
+    const int wt = wave / (BO / WO) * WT, wo = wave % (BO / WO) * WO;          // the wave's part of the tile
+    uint8_t* const mine = plan.base + g.base + nth * w.size;
+
+    const int ld = MODE == GRAM ? w.ldc : w.ldr, pitch = ld * 2, blocks = ld / kHalves;
+    const uint8_t* const pt = mine + (MODE == GRAM ? w.o : MODE == SQUARE ? w.A : t_now) + (int64_t)t0 * pitch;
+    const uint8_t* const po = mine + (MODE == GRAM ? w.o : MODE == SQUARE ? w.A : w.B) + (int64_t)o0 * pitch;
+    const int64_t plane_t = MODE == GRAM ? w.o_plane : MODE == SQUARE ? w.s_plane : w.t_plane;
+    const int64_t plane_o = MODE == GRAM ? w.o_plane : w.s_plane;
+    const int64_t bytes_t = (int64_t)(rows_t - t0) * pitch, bytes_o = (int64_t)(g.r - o0) * pitch;
+    // A row goes into a load's lane offset, which the buffer's range checks: rows past the end become zeros.  The block goes
+    // into the scalar offset, which stays in the row: past the last block the last one is loaded again, not used.
+    const __amdgpu_buffer_rsrc_t hi_t = buffer_of(pt, bytes_t), hi_o = buffer_of(po, bytes_o);
+    const __amdgpu_buffer_rsrc_t lo_t = buffer_of(pt + (PRECISE ? plane_t : 0), bytes_t);
+    const __amdgpu_buffer_rsrc_t lo_o = buffer_of(po + (PRECISE ? plane_o : 0), bytes_o);
+    const int total = PRECISE ? 3 * blocks : blocks, last = total - 1;
+    const int sub = lane >> 3, piece = lane & 7;
+    const int from = sub * pitch + ((piece ^ (sub >> 1)) << 4);                // in 8 rows whose keys' third bit is 0
+    auto stage = [&](int kb, int i) {                  // the i-th direct load of this wave's part of a block
+        uint8_t* buf = lds[kb & (S - 1)];
+        const int l = i < kPT ? wave * kPT + i : wave * kPO + i - kPT;
+        int k = kb < last ? kb : last;
+        bool t_lo = false, o_lo = false;
+        if (PRECISE) {                                 // hi hi, hi lo, lo hi
+            t_lo = k >= 2 * blocks;
+            o_lo = k >= blocks && !t_lo;
+            k -= t_lo ? 2 * blocks : o_lo ? blocks : 0;
+        }
+        const int row = l * 8 * pitch;
+        if (i < kPT) load_lds(t_lo ? lo_t : hi_t, buf + l * 8 * kRow, row + (l & 1 ? from ^ 64 : from), k * kRow);
+        else load_lds(o_lo ? lo_o : hi_o, buf + (BT + l * 8) * kRow, row + (l & 2 ? from ^ 64 : from), k * kRow);
+    };
+    const int r32 = lane & 31, half = lane >> 5, rs = spread(r32);
+
+    f16 acc[NO][NT];
+#pragma unroll
+    for (int i = 0; i < NO; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f16{};
+
+    // what follows the meeting -- the next block's first reads, the direct loads into the buffer that has just been read --
+    // runs beside the second half's products; past the last block the reads and loads are of no use, and in bounds
+    constexpr int kReads = 2 * (NT + NO), kLoads = kPT + kPO, kProducts = 2 * NT * NO;
+    i4 f[2][NT + NO][2];
+    auto read = [&](int kb, int h, int q) {
+        const int i = q >> 1, p = 4 * h + 2 * (q & 1) + half;
+        const uint8_t* row = i < NT ? lds[kb & (S - 1)] + (wt + i * 32 + r32) * kRow
+                                    : lds[kb & (S - 1)] + (BT + wo + (i - NT) * 32 + rs) * kRow;
+        f[h][i][q & 1] = *(const i4*)(row + ((p ^ (i < NT ? key_plain(r32) : key_spread(rs))) << 4));
+    };
+    // products of half h; beside them, the reads of half 1 - h of block kb_read and the loads of block kb_load (< 0: none)
+    auto products = [&](int h, int kb_read, int kb_load) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+            for (int m = 0; m < NO * NT; ++m) {
+                const int i = m / NT, j = m % NT, at = s * NO * NT + m;
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, f[h][NT + i][s]),
+                                                                   __builtin_bit_cast(h8, f[h][j][s]), acc[i][j], 0, 0, 0);
+#pragma unroll
+                for (int q = 0; q < kReads; ++q)
+                    if (q * kProducts / kReads == at) read(kb_read, 1 - h, q);
+#pragma unroll
+                for (int l = 0; l < kLoads; ++l)
+                    if (kb_load >= 0 && l * kProducts / kLoads == at) stage(kb_load, l);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+#pragma unroll
+    for (int kb = 0; kb < S - 1; ++kb)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) stage(kb, i);
+    meet<(S - 2) * kLoads>();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) stage(S - 1, i);
+#pragma unroll
+    for (int q = 0; q < kReads; ++q) read(0, 0, q);
+#pragma unroll 1
+    for (int kb = 0; kb < total; ++kb) {
+        products(0, kb, -1);
+        meet<(S - 2) * kLoads>();                      // block kb has been read, block kb + 1 has arrived
+        products(1, kb + 1, kb + S);
+    }
+    meet();                                            // the staging buffers are free
+
+    // The results, 64 columns (o) of the wave's rows (t) at a time: to LDS, back as rows of eight columns to a lane, which take
+    // what they need of A or X (whole lines, all under way before the first is used) and go out, and back once more as columns
+    // for the other order.  (Taken in the instructions' layout, 16 columns of a lane's row, the same loads are 64 requests to an
+    // instruction and one latency after the other: an UPDATE's start and end of a 256 x 256 tile took 40 us.)
+    constexpr int kRoom = (int)sizeof(lds) / kWaves, kCols = WO < 64 ? WO : 64;
+    static_assert(WT <= 64 && WT * 64 * 4 <= kRoom, "room for a wave's rows");
+    constexpr int kRowLanes = kCols / 8, kRows = 64 / kRowLanes, kRowTurns = WT / kRows;
+    constexpr int kColumnLanes = WT / 8, kColumns = 64 / kColumnLanes, kColumnTurns = kCols / kColumns;
+    constexpr bool kPlane = MODE == UPDATE || MODE == LAST || (MODE == SQUARE && PRECISE);      // the operand's second halves
+    float* const own = (float*)(&lds[0][0] + wave * kRoom);
+    float* const diagonal = (float*)(mine + (MODE == GRAM ? w.d : w.e));
+    const uint8_t* const px = mine + (MODE == SQUARE ? w.A : t_now) + (int64_t)t0 * pitch;
+    // a column past a row's end is the next row's: not stored
+    const __amdgpu_buffer_rsrc_t buf_x = buffer_of(px, bytes_t);
+    const __amdgpu_buffer_rsrc_t buf_y = buffer_of(px + (MODE == SQUARE ? w.s_plane : w.t_plane), bytes_t);
+    const __amdgpu_buffer_rsrc_t buf_d = buffer_of(mine + (MODE == SQUARE ? w.d : w.e), (int64_t)w.ldr * 4);
+    const int m = g.tall ? g.c : g.r, n = g.tall ? g.r : g.c;                  // of the result
+    auto deliver = [&](int row, int c, const float* x) {
+        const int left = n - c;
+        if (row >= m || left <= 0) return;
+        const int64_t at = (int64_t)row * n + c;
+        if constexpr (std::is_same_v<Out, Listed>) {
+            float p[8];
+            load_row<F32>(in.p[z], at, left, p);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) p[k] = __builtin_fmaf(-g.lr, x[k], p[k] * g.keep);
+            store_row<F32>(in.p[z], at, left, p);
+            if (in.p16[z]) store_row<BF16>(in.p16[z], at, left, p);
+        } else {
+            store_row<Out>(out, z * ((int64_t)m * n) + at, left, x);
+        }
+    };
+    const bool columns_too = kSymmetric ? t0 != o0 : MODE == UPDATE || !g.tall;
+    const int row0 = lane / kRowLanes, c = lane % kRowLanes * 8;               // of a turn's rows
+    const int col0 = lane / kColumnLanes, r = lane % kColumnLanes * 8;         // of a turn's columns
+#pragma unroll
+    for (int i0 = 0; i0 < NO; i0 += kCols / 32) {
+        __builtin_amdgcn_sched_barrier(0);             // one pass's loads at a time: no registers for more
+        const int o = o0 + wo + i0 * 32 + c;
+        u4 x[kRowTurns], y[kPlane ? kRowTurns : 1];
+        float near[8] = {}, dt[kRowTurns];
+        if constexpr (MODE != GRAM) {
+#pragma unroll
+            for (int k = 0; k < kRowTurns; ++k) {
+                const int row = wt + k * kRows + row0;
+                x[k] = halves_of(buf_x, row * pitch + o * 2);
+                if constexpr (kPlane) y[k] = halves_of(buf_y, row * pitch + o * 2);
+                if constexpr (MODE == SQUARE) dt[k] = as_f32(__builtin_amdgcn_raw_buffer_load_b32(buf_d, (t0 + row) * 4, 0, 0));
+            }
+            floats_of(buf_d, o * 4, near);
+        }
+#pragma unroll
+        for (int i = 0; i < kCols / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f16& v = acc[i0 + i][j];
+                    *group_at(own, j * 32 + r32, i * 8 + half * 4 + k) = f4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+                }
+        own_done();
+#pragma unroll
+        for (int k = 0; k < kRowTurns; ++k) {
+            const int row = k * kRows + row0, t = t0 + wt + row;
+            f4* const at[2] = {group_at(own, row, c / 4), group_at(own, row, c / 4 + 1)};
+            float v[8], a[8] = {}, b[8] = {};
+            F32::open({*at[0], *at[1]}, v);
+            const bool on = kSymmetric && t0 == o0 && t >= o && t < o + 8;     // the diagonal's element is here
+            float d = 0.0f;
+            if (on) {
+#pragma unroll
+                for (int l = 0; l < 8; ++l) d = t == o + l ? v[l] : d;
+            }
+            if constexpr (MODE != GRAM) F16::open(x[k], a);
+            if constexpr (kPlane) F16::open(y[k], b);
+#pragma unroll
+            for (int l = 0; l < 8; ++l) {
+                if (MODE == GRAM) v[l] *= kA / (kX * kX);
+                else if (MODE == SQUARE)
+                    v[l] = __builtin_fmaf(v[l], co.c * (kB / (kA * kA)),
+                                          __builtin_fmaf(co.c, dt[k] + near[l], co.b) * (kB / kA) * (a[l] + b[l]));
+                else v[l] = __builtin_fmaf(near[l], a[l] + b[l], v[l] * (1.0f / kB)) * (MODE == LAST ? 1.0f / kX : 1.0f);
+            }
+            if (on) {
+                d *= MODE == GRAM ? 1.0f / (kX * kX) : 1.0f / (kA * kA);
+                if (t < w.ldr) diagonal[t] = MODE == GRAM ? d : co.a + co.b * dt[k] + co.c * (dt[k] * dt[k] + d);
+#pragma unroll
+                for (int l = 0; l < 8; ++l) v[l] = t == o + l ? 0.0f : v[l];
+            }
+            if (columns_too) {
+                *at[0] = f4{v[0], v[1], v[2], v[3]};
+                *at[1] = f4{v[4], v[5], v[6], v[7]};
+            }
+            if constexpr (kSymmetric) {
+                if (t < g.r && o < w.ldr)
+                    put_halves<PRECISE>(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)t * w.ldr + o) * 2, w.s_plane, v);
+            } else if constexpr (MODE == UPDATE) {
+                if (t < g.c && o < w.ldr) put_halves<true>(mine + t_next + ((int64_t)t * w.ldr + o) * 2, w.t_plane, v);
+            } else if (g.tall) {
+                deliver(t, o, v);
+            }
+        }
+        own_done();
+        if (columns_too) {
+#pragma unroll
+            for (int k = 0; k < kColumnTurns; ++k) {
+                const int column = k * kColumns + col0, oc = o0 + wo + i0 * 32 + column, t = t0 + wt + r;
+                float v[8];
+#pragma unroll
+                for (int l = 0; l < 8; ++l) v[l] = ((const float*)group_at(own, r + l, column >> 2))[column & 3];
+                if constexpr (kSymmetric) {
+                    if (oc < g.r && t < w.ldr)
+                        put_halves<PRECISE>(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)oc * w.ldr + t) * 2, w.s_plane, v);
+                } else if constexpr (MODE == UPDATE) {
+                    if (oc < g.r && t < w.ldc) put_halves<PRECISE>(mine + w.o + ((int64_t)oc * w.ldc + t) * 2, w.o_plane, v);
+                } else {
+                    deliver(oc, t, v);
+                }
+            }
+            own_done();
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------ host
+// Tiles of b x b in a launch, each group's first one noted in it.
+template <Mode MODE>
+int64_t tiles_of(Plan& w, int64_t b) {
+    int64_t n = 0;
+    for (int k = 0; k < w.groups; ++k) {
+        Group& g = w.g[k];
+        const int64_t across = (g.r + b - 1) / b, down = (g.c + b - 1) / b;
+        g.tile0 = (int)n;
+        n += g.count * (MODE == GRAM || MODE == SQUARE ? across * (across + 1) / 2 : down * across);
+        if (n > kMaxTiles) return n;
+    }
+    return n;
+}
+
+template <Mode MODE, bool PRECISE, typename Out, int COARSE, int B, int WT, int WO, int S>
+int launch(Steps& a, int64_t first, int64_t last) {
+    const int64_t all = tiles_of<MODE>(a.plan, COARSE * B), tiles = ((last < 0 ? all : last) - first) * COARSE * COARSE;
+    if (all > kMaxTiles || tiles > kMaxTiles) return Z1_E_SIZE;
+    step_kernel<MODE, PRECISE, Out, COARSE, B, B, WT, WO, S>
+        <<<dim3((unsigned)tiles), B / WT * (B / WO) * 64, 0, a.st>>>(a.plan, a.co, a.out, a.in, (int)first);
+    return (int)hipGetLastError();
+}
+template <Mode MODE, bool PRECISE, typename Out = Listed>
+int launch_step(Steps& a) {
+    const int64_t large = tiles_of<MODE>(a.plan, 256), rounds = large / kCus, rest = large % kCus;
+    if (rounds > 0) {
+        const int64_t whole = rest * 2 > kCus ? large : large - rest;
+        if (const int rc = launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(a, 0, whole)) return rc;
+        if (whole == large) return Z1_OK;
+        if (4 * rest <= kCus) return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 4>(a, whole, large);
+        return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 2>(a, whole, large);
+    }
+    const int64_t middle = tiles_of<MODE>(a.plan, 128);
+    if (middle > kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2>(a, 0, -1);
+    if (middle * 2 > kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4>(a, 0, -1);
+    return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4>(a, 0, -1);
+}
+
+template <bool PRECISE, typename Out>
+int iterate(Steps& a, int steps, const float* coefficients) {
+    for (int k = 0; k < steps; ++k) {
+        a.co = {coefficients[3 * k], coefficients[3 * k + 1], coefficients[3 * k + 2]};
+        a.plan.cur = k & 1;
+        if (const int rc = launch_step<GRAM, PRECISE>(a)) return rc;
+        if (const int rc = launch_step<SQUARE, PRECISE>(a)) return rc;
+        const int rc = k + 1 < steps ? launch_step<UPDATE, PRECISE>(a) : launch_step<LAST, PRECISE, Out>(a);
+        if (rc) return rc;
+    }
+    return Z1_OK;
+}
+
+template <bool PRECISE>
+int iterate_of(Steps& a, int steps, const float* coefficients, Kind kind) {
+    switch (kind) {
+        case OUT_F32: return iterate<PRECISE, F32>(a, steps, coefficients);
+        case OUT_BF16: return iterate<PRECISE, BF16>(a, steps, coefficients);
+        case OUT_F16: return iterate<PRECISE, F16>(a, steps, coefficients);
+        default: return iterate<PRECISE, Listed>(a, steps, coefficients);
+    }
+}
+
+}  // namespace
