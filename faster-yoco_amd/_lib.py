@@ -108,6 +108,7 @@ SIGNATURES.update(BLOCK_SIGNATURES)
 MATRIX_SIGNATURES = {
     'z1_orthogonalize': ([_P, _I64, _I64, _I64, _I64, _I64, _I, _P, _I, _I, ctypes.POINTER(_F), _F, _I, _P, _I64, _P], _I),
     'z1_orthogonalize_workspace': ([_I64, _I64, _I64, _I], _I64),
+    'z1_orthogonalize_way': ([_I64, _I64, _I64, _I, ctypes.POINTER(_I)], _I),
     'z1_muon_step': ([ctypes.POINTER(Z1Matrix), _I, _I, ctypes.POINTER(Z1Muon), _P, _I64, _P], _I),
     'z1_muon_workspace': ([ctypes.POINTER(Z1Matrix), _I, _I], _I64),
 }

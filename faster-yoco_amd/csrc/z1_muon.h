@@ -181,6 +181,8 @@ enum Kind { OUT_F32, OUT_BF16, OUT_F16, OUT_LIST };
 // The steps' products over the plan's matrices, X's start in place; out by `kind`.
 int iterate_fast(Steps& a, int steps, const float* coefficients, Kind kind);
 int iterate_precise(Steps& a, int steps, const float* coefficients, Kind kind);
+void ways_fast(Plan& w, int* way);
+void ways_precise(Plan& w, int* way);
 
 // The small matrices' kernel: fragments to a wave and bytes of LDS.  0: the matrix is too large for it.
 struct WholeWay {

@@ -213,6 +213,23 @@ int z1_orthogonalize(const void* x, int64_t step, int64_t stride, int64_t count,
     return run(a, w, count, dtype, steps, coefficients, precise != 0, out, kind, workspace, st);
 }
 
+int z1_orthogonalize_way(int64_t count, int64_t m, int64_t n, int precise, int* way) {
+    if (!way) return Z1_E_NULL;
+    if (count < 1 || count > kMaxCount || bad_side(m) || bad_side(n)) return Z1_E_SIZE;
+    for (int i = 0; i < 12; ++i) way[i] = 0;
+    const WholeWay small = whole_way(m, n, precise != 0);
+    if (small.pieces) {
+        way[1] = small.pieces;
+        return Z1_OK;
+    }
+    Plan w{};
+    w.groups = 1;
+    w.g[0] = {0, (int)(m < n ? m : n), (int)(m < n ? n : m), m > n, 0, (int)count, 0, 0.0f, 0.0f};
+    if (precise) ways_precise(w, way);
+    else ways_fast(w, way);
+    return Z1_OK;
+}
+
 int64_t z1_muon_workspace(const z1_matrix* list, int count, int precise) {
     if (count < 0 || count > kList) return Z1_E_SIZE;
     if (count > 0 && !list) return Z1_E_NULL;

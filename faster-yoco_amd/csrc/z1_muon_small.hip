@@ -26,8 +26,8 @@ struct Places {
     int x_plane, a_plane, A, B, sums, d, e, size;
     int cuts;                                          // parts of A's summed axis
 };
-__host__ __device__ inline Places places_of(int R, int C, bool precise) {
-    Places p;
+__host__ __device__ constexpr Places places_of(int R, int C, bool precise) {
+    Places p{};
     const int planes = precise ? 2 : 1;
     p.px = C * 64 + 16;
     p.pa = R * 64 + 16;
@@ -301,9 +301,16 @@ __global__ __launch_bounds__(kWholeWaves * 64) void whole_kernel(Whole a) {
 
 template <int R, bool PRECISE>
 int launch_whole(const Whole& a, const WholeWay& way, int64_t count, hipStream_t st) {
+    // what a matrix of R rows of fragments takes at least (it has as many columns of them)
+    constexpr int kLeast = places_of(R, R, PRECISE).size;
     const dim3 grid((unsigned)count);
-    if (way.pieces == 2) whole_kernel<R, PRECISE, 2, 64 << 10><<<grid, kWholeWaves * 64, 0, st>>>(a);
-    else whole_kernel<R, PRECISE, 4, 159 << 10><<<grid, kWholeWaves * 64, 0, st>>>(a);
+    if constexpr (kLeast <= 64 << 10) {
+        if (way.pieces == 2) {
+            whole_kernel<R, PRECISE, 2, 64 << 10><<<grid, kWholeWaves * 64, 0, st>>>(a);
+            return (int)hipGetLastError();
+        }
+    }
+    if constexpr (kLeast <= 159 << 10) whole_kernel<R, PRECISE, 4, 159 << 10><<<grid, kWholeWaves * 64, 0, st>>>(a);
     return (int)hipGetLastError();
 }
 template <int R>

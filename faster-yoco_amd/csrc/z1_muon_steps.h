@@ -60,8 +60,13 @@ __device__ __forceinline__ void floats_of(__amdgpu_buffer_rsrc_t from, int at, f
 // One launch of a step over `count` matrices: GRAM A = X X^T (operands o, o), SQUARE B from A A^T, UPDATE X from t and B, LAST
 // the same into the result.  BT x BO results (t x o) of a workgroup, WT x WO of a wave, S blocks of 64 columns staged by direct
 // loads; a block's two halves are read ahead by one half and the workgroup meets between them, as in the 8-bit products.
-template <Mode MODE, bool PRECISE, typename Out, int COARSE, int BT, int BO, int WT, int WO, int S>
-__global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan plan, Coefficients co, void* out, Inputs in, int first) {
+//
+// PART, JOINED: a long summed axis in parts, each a workgroup of its own, which leaves its sums as they are in its lanes (in the
+// next t's place: free then), and a launch that adds them in order and goes on from there.
+enum Phase { ALL, PART, JOINED };
+template <Mode MODE, bool PRECISE, typename Out, int COARSE, int BT, int BO, int WT, int WO, int S, Phase PHASE>
+__global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan plan, Coefficients co, void* out, Inputs in, int first,
+                                                                            int parts) {
     constexpr bool kSymmetric = MODE == GRAM || MODE == SQUARE;
     constexpr int kWaves = BT / WT * (BO / WO);
     constexpr int kPT = BT / 8 / kWaves, kPO = BO / 8 / kWaves;                // direct loads of a wave: 8 rows each
@@ -71,7 +76,10 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
     constexpr int kRow = kHalves * 2;
     __shared__ __align__(1024) uint8_t lds[S][(BT + BO) * kRow];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int run = in_runs(), index = first + run / (COARSE * COARSE);
+    // parts: one after another, so that an XCD's share is tiles of one part
+    const int among = PHASE == PART ? gridDim.x / parts : 1, run_all = in_runs();
+    const int axis = PHASE == PART ? run_all / among : 0, run = PHASE == PART ? run_all - axis * among : run_all;
+    const int index = first + run / (COARSE * COARSE);
     const Group& g = group_of_tile(plan, index);
     const Layout w = layout_of(g.r, g.c, PRECISE);
     const int64_t t_now = plan.cur ? w.t[1] : w.t[0], t_next = plan.cur ? w.t[0] : w.t[1];
@@ -97,13 +105,15 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
     const __amdgpu_buffer_rsrc_t hi_t = buffer_of(pt, bytes_t), hi_o = buffer_of(po, bytes_o);
     const __amdgpu_buffer_rsrc_t lo_t = buffer_of(pt + (PRECISE ? plane_t : 0), bytes_t);
     const __amdgpu_buffer_rsrc_t lo_o = buffer_of(po + (PRECISE ? plane_o : 0), bytes_o);
-    const int total = PRECISE ? 3 * blocks : blocks, last = total - 1;
+    const int all = PRECISE ? 3 * blocks : blocks, last = all - 1;
+    const int per = PHASE == PART ? (all + parts - 1) / parts : all, begin = axis * per;
+    const int total = all - begin < per ? all - begin : per;                   // none where not positive: zeros are left
     const int sub = lane >> 3, piece = lane & 7;
     const int from = sub * pitch + ((piece ^ (sub >> 1)) << 4);                // in 8 rows whose keys' third bit is 0
     auto stage = [&](int kb, int i) {                  // the i-th direct load of this wave's part of a block
         uint8_t* buf = lds[kb & (S - 1)];
         const int l = i < kPT ? wave * kPT + i : wave * kPO + i - kPT;
-        int k = kb < last ? kb : last;
+        int k = begin + kb < last ? begin + kb : last;
         bool t_lo = false, o_lo = false;
         if (PRECISE) {                                 // hi hi, hi lo, lo hi
             t_lo = k >= 2 * blocks;
@@ -151,22 +161,53 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
             __builtin_amdgcn_sched_barrier(0);
         }
     };
+    // a part's sums of a tile: the lanes' own, 16 bytes of neighbours beside each other
+    auto left = [&](int part, int i, int j, int k) {
+        const int64_t tile_of = ((int64_t)part * tiles + place) * kWaves + wave;
+        return (Z1B_GLOBAL f4*)(mine + t_next) + ((tile_of * NO + i) * NT + j) * 256 + k * 64 + lane;
+    };
+    if constexpr (PHASE != JOINED) {
 #pragma unroll
-    for (int kb = 0; kb < S - 1; ++kb)
+        for (int kb = 0; kb < S - 1; ++kb)
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) stage(kb, i);
-    meet<(S - 2) * kLoads>();
+            for (int i = 0; i < kLoads; ++i) stage(kb, i);
+        meet<(S - 2) * kLoads>();
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) stage(S - 1, i);
+        for (int i = 0; i < kLoads; ++i) stage(S - 1, i);
 #pragma unroll
-    for (int q = 0; q < kReads; ++q) read(0, 0, q);
+        for (int q = 0; q < kReads; ++q) read(0, 0, q);
 #pragma unroll 1
-    for (int kb = 0; kb < total; ++kb) {
-        products(0, kb, -1);
-        meet<(S - 2) * kLoads>();                      // block kb has been read, block kb + 1 has arrived
-        products(1, kb + 1, kb + S);
+        for (int kb = 0; kb < total; ++kb) {
+            products(0, kb, -1);
+            meet<(S - 2) * kLoads>();                      // block kb has been read, block kb + 1 has arrived
+            products(1, kb + 1, kb + S);
+        }
+        meet();                                            // the staging buffers are free
     }
-    meet();                                            // the staging buffers are free
+    if constexpr (PHASE == PART) {
+#pragma unroll
+        for (int i = 0; i < NO; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *left(axis, i, j, k) = f4{acc[i][j][4 * k], acc[i][j][4 * k + 1], acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+        return;
+    }
+    if constexpr (PHASE == JOINED) {
+        for (int p = 0; p < parts; ++p) {
+#pragma unroll
+            for (int i = 0; i < NO; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const f4 v = *left(p, i, j, k);
+#pragma unroll
+                        for (int l = 0; l < 4; ++l) acc[i][j][4 * k + l] += v[l];
+                    }
+        }
+    }
 
     // The results, 64 columns (o) of the wave's rows (t) at a time: to LDS, back as rows of eight columns to a lane, which take
     // what they need of A or X (whole lines, all under way before the first is used) and go out, and back once more as columns
@@ -307,28 +348,123 @@ int64_t tiles_of(Plan& w, int64_t b) {
     return n;
 }
 
-template <Mode MODE, bool PRECISE, typename Out, int COARSE, int B, int WT, int WO, int S>
-int launch(Steps& a, int64_t first, int64_t last) {
-    const int64_t all = tiles_of<MODE>(a.plan, COARSE * B), tiles = ((last < 0 ? all : last) - first) * COARSE * COARSE;
+template <Mode MODE, bool PRECISE, typename Out, int COARSE, int B, int WT, int WO, int S, Phase PHASE = ALL>
+int launch(Steps& a, int64_t first, int64_t last, int parts = 1) {
+    const int64_t all = tiles_of<MODE>(a.plan, COARSE * B);
+    const int64_t tiles = ((last < 0 ? all : last) - first) * COARSE * COARSE * (PHASE == PART ? parts : 1);
     if (all > kMaxTiles || tiles > kMaxTiles) return Z1_E_SIZE;
-    step_kernel<MODE, PRECISE, Out, COARSE, B, B, WT, WO, S>
-        <<<dim3((unsigned)tiles), B / WT * (B / WO) * 64, 0, a.st>>>(a.plan, a.co, a.out, a.in, (int)first);
+    step_kernel<MODE, PRECISE, Out, COARSE, B, B, WT, WO, S, PHASE>
+        <<<dim3((unsigned)tiles), B / WT * (B / WO) * 64, 0, a.st>>>(a.plan, a.co, a.out, a.in, (int)first, parts);
     return (int)hipGetLastError();
 }
+// How a step's tiles run: all of one size, or whole rounds of 256 and what is left in quarters.
+enum Kinds { ALL_256, WHOLE_256, ALL_128, ALL_64 };
+struct Way {
+    Kinds kind;
+    int parts;                                         // of the summed axis
+};
+
+// The tiles of b x b, their mean number of blocks of the summed axis and the largest one.
+struct Load {
+    int64_t tiles;
+    double blocks, most;
+};
+template <Mode MODE, bool PRECISE>
+Load load_of(Plan& w, int64_t b) {
+    Load l{tiles_of<MODE>(w, b), 0.0, 0.0};
+    for (int k = 0; k < w.groups; ++k) {
+        const Group& g = w.g[k];
+        const double n = (double)((k + 1 < w.groups ? w.g[k + 1].tile0 : l.tiles) - g.tile0);
+        const double blocks = (PRECISE ? 3.0 : 1.0) * (((MODE == GRAM ? g.c : g.r) + kHalves - 1) / kHalves);
+        l.blocks += n * blocks;
+        l.most = blocks > l.most ? blocks : l.most;
+    }
+    l.blocks /= (double)(l.tiles > 0 ? l.tiles : 1);
+    return l;
+}
+// Estimates in us, as measured on launches of 10 to 9216 tiles over 16 to 128 blocks.  256: one to a CU, a start and an end of 15
+// us and 1.0 us a block, which the card's power makes 1.8 when all CUs are at it (78 tiles over 48 and 128 blocks 67 and 149 us,
+// 256 tiles over 48 105); X's update moves more (117).  128: 7 us and 0.42 alone on a CU (136 over 32 and 128 blocks 20 and 61),
+// two to a CU 9 us and 1.1 (512 over 48 57 to 66).  64: 3.3 us and 0.19 alone (136 over 64 15), two to a CU 2 us and 0.56.
+double time_256(double tiles, double blocks, bool update) {
+    const double fill = tiles < kCus ? tiles / kCus : 1.0, hot = fill > 0.3 ? (fill - 0.3) / 0.7 : 0.0;
+    return 15.0 + blocks * (1.0 + 0.8 * hot) + (update ? 12.0 * fill : 0.0);
+}
+constexpr int kMostParts = 16;
+// Tiles of which a CU holds two: up to one to each, `alone`; beyond, those that share a CU take about half as long again at once.
+double shared(double tiles, double alone, double two) {
+    if (tiles <= kCus) return alone;
+    if (tiles > 2 * kCus) return (tiles / (2 * kCus) + 0.3) * two;
+    return two > alone ? alone + (two - alone) * (0.45 + 0.55 * (tiles - kCus) / kCus) : alone;
+}
+double time_128(double tiles, double blocks, double most, bool update) {
+    return shared(tiles, 7.0 + 0.42 * most, 9.0 + 1.1 * blocks + (update ? 8.0 : 0.0));
+}
+double time_64(double tiles, double blocks, double most) {
+    const double alone = 3.3 + 0.19 * most, all = shared(tiles, alone, 2.0 + 0.56 * blocks);
+    return all > alone ? all : alone;
+}
+template <Mode MODE, bool PRECISE>
+Way way_of(Plan& w) {
+    const bool update = MODE == UPDATE;
+    const Load a = load_of<MODE, PRECISE>(w, 256), b = load_of<MODE, PRECISE>(w, 128), c = load_of<MODE, PRECISE>(w, 64);
+    const int64_t rounds = a.tiles / kCus, rest = a.tiles % kCus;
+    const double full = (double)rounds * time_256(kCus, a.blocks, update);
+    double best = full + (rest ? time_256((double)rest, rounds ? a.blocks : a.most, update) : 0.0);
+    Way way{ALL_256, 1};
+    auto take = [&](Kinds kind, double time, int parts = 1) {
+        if (time < best) best = time, way = {kind, parts};
+    };
+    if (rounds && rest) take(WHOLE_256, full + time_128(4.0 * (double)rest, a.blocks, a.blocks, update));
+    take(ALL_128, time_128((double)b.tiles, b.blocks, b.most, update));
+    take(ALL_64, time_64((double)c.tiles, c.blocks, c.most));
+    if (MODE != GRAM) return way;
+    // The long axis of A in parts, where few tiles leave CUs idle: 6.5 us for a second launch, which reads what the parts leave at
+    // 80 bytes/ns a CU (400 x 8000: 23.3 us, 14.9 of 4 to 8 parts; 200 x 4000: 13.8, 11.5; 1536 x 6144: 40.8, 31.4 of 3;
+    // 2048 x 8192: 61, 54 of 3; but 1024 x 4096 15.3, 17.5 of 3, and 300 x 1000 6.5, 9.7).
+    auto fits = [&](int64_t side) {                    // parts that the next t's place holds
+        int64_t n = kMostParts;
+        for (int k = 0; k < w.groups; ++k) {
+            const Group& g = w.g[k];
+            const int64_t d = (g.r + side - 1) / side, room = 2 * layout_of(g.r, g.c, PRECISE).t_plane / (d * (d + 1) / 2 * side * side * 4);
+            n = room < n ? room : n;
+        }
+        return n;
+    };
+    auto join = [](double parts, double side) { return 6.5 + (parts + 1.0) * side * side * 4.0 / 80000.0; };
+    const int64_t most_b = fits(128), most_c = fits(64);
+    for (int p = 2; p <= most_b && b.tiles * p <= 4 * kCus; ++p)
+        take(ALL_128, time_128((double)(b.tiles * p), b.blocks / p, b.most / p, false) + join(p, 128), p);
+    for (int p = 2; p <= most_c && c.tiles * p <= 4 * kCus; ++p)
+        take(ALL_64, time_64((double)(c.tiles * p), c.blocks / p, c.most / p) + join(p, 64), p);
+    return way;
+}
+
 template <Mode MODE, bool PRECISE, typename Out = Listed>
 int launch_step(Steps& a) {
-    const int64_t large = tiles_of<MODE>(a.plan, 256), rounds = large / kCus, rest = large % kCus;
-    if (rounds > 0) {
-        const int64_t whole = rest * 2 > kCus ? large : large - rest;
-        if (const int rc = launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(a, 0, whole)) return rc;
-        if (whole == large) return Z1_OK;
-        if (4 * rest <= kCus) return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 4>(a, whole, large);
-        return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 2>(a, whole, large);
+    const auto [way, parts] = way_of<MODE, PRECISE>(a.plan);
+    if constexpr (MODE == GRAM) {
+        if (parts > 1 && way == ALL_128) {
+            const bool alone = tiles_of<MODE>(a.plan, 128) * parts <= kCus;
+            if (const int rc = alone ? launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4, PART>(a, 0, -1, parts)
+                                     : launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2, PART>(a, 0, -1, parts)) return rc;
+            return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2, JOINED>(a, 0, -1, parts);
+        }
+        if (parts > 1) {
+            if (const int rc = launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4, PART>(a, 0, -1, parts)) return rc;
+            return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4, JOINED>(a, 0, -1, parts);
+        }
     }
-    const int64_t middle = tiles_of<MODE>(a.plan, 128);
-    if (middle > kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2>(a, 0, -1);
-    if (middle * 2 > kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4>(a, 0, -1);
-    return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4>(a, 0, -1);
+    if (way == ALL_256) return launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(a, 0, -1);
+    if (way == WHOLE_256) {
+        const int64_t large = tiles_of<MODE>(a.plan, 256), rest = large % kCus;
+        if (const int rc = launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(a, 0, large - rest)) return rc;
+        if (4 * rest <= kCus) return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 4>(a, large - rest, large);
+        return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 2>(a, large - rest, large);
+    }
+    if (way == ALL_64) return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4>(a, 0, -1);
+    if (tiles_of<MODE>(a.plan, 128) <= kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4>(a, 0, -1);
+    return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2>(a, 0, -1);
 }
 
 template <bool PRECISE, typename Out>
@@ -342,6 +478,23 @@ int iterate(Steps& a, int steps, const float* coefficients) {
         if (rc) return rc;
     }
     return Z1_OK;
+}
+
+// How the three products run (z1_orthogonalize_way).
+template <bool PRECISE, Mode MODE>
+void way_into(Plan& w, int* way) {
+    const auto [kind, parts] = way_of<MODE, PRECISE>(w);
+    const int64_t rest = tiles_of<MODE>(w, 256) % kCus, middle = tiles_of<MODE>(w, 128) * parts;
+    way[0] = kind == ALL_64 ? 64 : kind == ALL_128 ? 128 : 256;
+    way[1] = kind == WHOLE_256 ? (int)rest : 0;
+    way[2] = parts;
+    way[3] = kind == ALL_64 || (kind == ALL_128 && middle <= kCus) || (kind == WHOLE_256 && 4 * rest <= kCus) ? 4 : 2;
+}
+template <bool PRECISE>
+void ways_of(Plan& w, int* way) {
+    way_into<PRECISE, GRAM>(w, way);
+    way_into<PRECISE, SQUARE>(w, way + 4);
+    way_into<PRECISE, UPDATE>(w, way + 8);
 }
 
 template <bool PRECISE>

@@ -346,6 +346,11 @@ int z1_orthogonalize(const void* x, int64_t step, int64_t stride, int64_t count,
                      int out_dtype, int steps, const float* coefficients, float eps, int precise, void* workspace,
                      int64_t workspace_bytes, void* stream);
 int64_t z1_orthogonalize_workspace(int64_t count, int64_t m, int64_t n, int precise);
+/* How matrices of these sizes run, of interest to timing and tests: for each of the three products (A, its square, B X) way[0] =
+ * rows and columns of a workgroup's tile, way[1] = tiles of 256 that are left to quarters of 128, way[2] = parts of the summed
+ * axis, way[3] = blocks of it that are staged (by the quarters where there are any).  Small matrices, a workgroup each: way[0] is
+ * 0 and way[1] the fragments of X to a wave. */
+int z1_orthogonalize_way(int64_t count, int64_t m, int64_t n, int precise, int* way);
 
 #define Z1_MAX_MATRICES 32
 typedef struct z1_matrix {

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import matrices as ref
+import ways_muon
 from matrices import HALF
 
 pytestmark = pytest.mark.gpu
@@ -99,6 +100,34 @@ def test_every_tile(pkg, dev):
         want, most = limit(x, torch.bfloat16, False)
         assert far(many[0], want) <= most
     assert torch.equal(muon.orthogonalize(x.to(dev), dtype=torch.bfloat16), one)
+
+
+@pytest.mark.parametrize('precise,size', [(0, t) for t in ways_muon.FAST] + [(1, t) for t in ways_muon.PRECISE], ids=str)
+def test_every_form(pkg, dev, precise, size):
+    """Sizes that take every form of the kernels: two matrices by turns, every copy within its bound of the 64-bit form (computed on
+    the GPU, where the largest take seconds less), and the same bits for each -- but for pairs, whose products hi lo and lo hi are
+    added in the other order above the diagonal of a tile of 256 than where its quarters are tiles, which have no such half."""
+    from faster_yoco_amd import muon
+    count, m, n = size
+    g = torch.Generator(device=dev).manual_seed(m * 31 + n)
+    x = torch.randn(2, m, n, generator=g, device=dev) * 1e-3
+    k = min(3, m, n)
+    x[1] = x[1] * 0.05 + torch.randn(m, k, generator=g, device=dev) @ torch.randn(k, n, generator=g, device=dev) * 1e-3
+    out = torch.float32 if precise else torch.bfloat16
+    got = muon.orthogonalize(x[torch.arange(count, device=dev) % 2], dtype=out, precise=bool(precise))
+    for i in range(min(count, 2)):
+        assert precise or all(torch.equal(got[j], got[i]) for j in range(i, count, 2))
+        want = ref.exact(x[i])
+        # fp16 operands: as the stored roundings leave it.  Pairs: what N = 3 K / 16 additions in fp32 leave, N^(1/2) U32 of a
+        # sum where their roundings add up at random: of X_0 (norm 1) into the small directions, 3.4^5 = 484 times by the end,
+        # twice that with the later steps', and of each step's large ones, through slopes up to 1.6, 17 times; four times both
+        if precise:
+            many = math.sqrt(3 * max(m, n) / 16 + 8) * ref.U32
+            most = 4 * (2 * 484 * many + 17 * many * float(want.norm()))
+        else:
+            most = 4 * float((ref.stored(x[i]) - want).norm()) + 2.0 ** -13 * float(want.norm())
+        for j in range(i, count, 2):
+            assert float((got[j].double() - want).norm()) <= most + HALF[out] * float(want.norm())
 
 
 def test_scales_of_the_input(pkg, dev):

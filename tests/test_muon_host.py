@@ -130,3 +130,23 @@ def test_shapes_on_fake_tensors(pkg):
         assert muon.orthogonalize(x, dtype=torch.bfloat16).dtype == torch.bfloat16
         p, m = torch.empty(30, 70, device='cuda'), torch.empty(30, 70, device='cuda')
         muon.step_([p], [x[0, 0]], [m], [p.bfloat16()], lr=1e-3)
+
+
+def test_every_form_has_a_tested_size(pkg):
+    """The sizes that the GPU tests run take every form that any size takes."""
+    import math
+
+    import ways_muon
+    from faster_yoco_amd import _lib
+    L = _lib.lib()
+    rng = random.Random(7)
+    size = lambda lo, hi: int(math.exp(rng.uniform(math.log(lo), math.log(hi))))  # noqa: E731
+    for precise, tested in ((0, ways_muon.FAST), (1, ways_muon.PRECISE)):
+        covered = set().union(*(ways_muon.forms(L, *t, precise) for t in tested))
+        seen = set()
+        for _ in range(20000):
+            seen |= ways_muon.forms(L, size(1, 300), size(1, 9000), size(1, 9000), precise)
+        assert seen <= covered, seen - covered
+    way = (ctypes.c_int * 12)()
+    assert L.z1_orthogonalize_way(0, 8, 8, 0, way) == L.z1_orthogonalize_way(1, 0, 8, 0, way) == -2
+    assert L.z1_orthogonalize_way(1, 8, 8, 0, None) == -1
