@@ -73,8 +73,12 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
     constexpr int NT = WT / 32, NO = WO / 32;
     static_assert(!kSymmetric || BT == BO, "a triangle of square tiles");
     static_assert(S == 2 || S == 4, "a block's buffer is kb & (S - 1)");
-    constexpr int kRow = kHalves * 2;
-    __shared__ __align__(1024) uint8_t lds[S][(BT + BO) * kRow];
+    // pairs: where LDS holds a block's both halves they are staged together and take three products, hi hi, hi lo and lo hi (A of
+    // three of 777 x 401 12.0 -> 9.5 us, of 2048 x 2048 52 -> 43); larger tiles go through the axis three times
+    constexpr bool kTogether = PRECISE && BT <= 128;
+    constexpr int kPlanes = kTogether ? 2 : 1;
+    constexpr int kRow = kHalves * 2, kSide = (BT + BO) * kRow;                // bytes of a block's first halves
+    __shared__ __align__(1024) uint8_t lds[S][kPlanes * kSide];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // parts: one after another, so that an XCD's share is tiles of one part
     const int among = PHASE == PART ? gridDim.x / parts : 1, run_all = in_runs();
@@ -105,23 +109,24 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
     const __amdgpu_buffer_rsrc_t hi_t = buffer_of(pt, bytes_t), hi_o = buffer_of(po, bytes_o);
     const __amdgpu_buffer_rsrc_t lo_t = buffer_of(pt + (PRECISE ? plane_t : 0), bytes_t);
     const __amdgpu_buffer_rsrc_t lo_o = buffer_of(po + (PRECISE ? plane_o : 0), bytes_o);
-    const int all = PRECISE ? 3 * blocks : blocks, last = all - 1;
+    const int all = PRECISE && !kTogether ? 3 * blocks : blocks, last = all - 1;
     const int per = PHASE == PART ? (all + parts - 1) / parts : all, begin = axis * per;
     const int total = all - begin < per ? all - begin : per;                   // none where not positive: zeros are left
     const int sub = lane >> 3, piece = lane & 7;
     const int from = sub * pitch + ((piece ^ (sub >> 1)) << 4);                // in 8 rows whose keys' third bit is 0
     auto stage = [&](int kb, int i) {                  // the i-th direct load of this wave's part of a block
-        uint8_t* buf = lds[kb & (S - 1)];
-        const int l = i < kPT ? wave * kPT + i : wave * kPO + i - kPT;
+        const int plane = i / (kPT + kPO), ip = i % (kPT + kPO);
+        uint8_t* buf = lds[kb & (S - 1)] + plane * kSide;
+        const int l = ip < kPT ? wave * kPT + ip : wave * kPO + ip - kPT;
         int k = begin + kb < last ? begin + kb : last;
-        bool t_lo = false, o_lo = false;
-        if (PRECISE) {                                 // hi hi, hi lo, lo hi
+        bool t_lo = kTogether && plane, o_lo = t_lo;
+        if (PRECISE && !kTogether) {                   // hi hi, hi lo, lo hi
             t_lo = k >= 2 * blocks;
             o_lo = k >= blocks && !t_lo;
             k -= t_lo ? 2 * blocks : o_lo ? blocks : 0;
         }
         const int row = l * 8 * pitch;
-        if (i < kPT) load_lds(t_lo ? lo_t : hi_t, buf + l * 8 * kRow, row + (l & 1 ? from ^ 64 : from), k * kRow);
+        if (ip < kPT) load_lds(t_lo ? lo_t : hi_t, buf + l * 8 * kRow, row + (l & 1 ? from ^ 64 : from), k * kRow);
         else load_lds(o_lo ? lo_o : hi_o, buf + (BT + l * 8) * kRow, row + (l & 2 ? from ^ 64 : from), k * kRow);
     };
     const int r32 = lane & 31, half = lane >> 5, rs = spread(r32);
@@ -134,23 +139,25 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
 
     // what follows the meeting -- the next block's first reads, the direct loads into the buffer that has just been read --
     // runs beside the second half's products; past the last block the reads and loads are of no use, and in bounds
-    constexpr int kReads = 2 * (NT + NO), kLoads = kPT + kPO, kProducts = 2 * NT * NO;
-    i4 f[2][NT + NO][2];
+    constexpr int kEach = NT + NO, kReads = 2 * kEach * kPlanes, kLoads = kPlanes * (kPT + kPO);
+    constexpr int kTimes = kTogether ? 3 : 1, kProducts = 2 * NT * NO * kTimes;
+    i4 f[2][kEach * kPlanes][2];
     auto read = [&](int kb, int h, int q) {
-        const int i = q >> 1, p = 4 * h + 2 * (q & 1) + half;
-        const uint8_t* row = i < NT ? lds[kb & (S - 1)] + (wt + i * 32 + r32) * kRow
-                                    : lds[kb & (S - 1)] + (BT + wo + (i - NT) * 32 + rs) * kRow;
-        f[h][i][q & 1] = *(const i4*)(row + ((p ^ (i < NT ? key_plain(r32) : key_spread(rs))) << 4));
+        const int at = q >> 1, i = at % kEach, p = 4 * h + 2 * (q & 1) + half;
+        const uint8_t* side = lds[kb & (S - 1)] + at / kEach * kSide;
+        const uint8_t* row = i < NT ? side + (wt + i * 32 + r32) * kRow : side + (BT + wo + (i - NT) * 32 + rs) * kRow;
+        f[h][at][q & 1] = *(const i4*)(row + ((p ^ (i < NT ? key_plain(r32) : key_spread(rs))) << 4));
     };
     // products of half h; beside them, the reads of half 1 - h of block kb_read and the loads of block kb_load (< 0: none)
     auto products = [&](int h, int kb_read, int kb_load) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
 #pragma unroll
-            for (int m = 0; m < NO * NT; ++m) {
-                const int i = m / NT, j = m % NT, at = s * NO * NT + m;
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, f[h][NT + i][s]),
-                                                                   __builtin_bit_cast(h8, f[h][j][s]), acc[i][j], 0, 0, 0);
+            for (int m = 0; m < NO * NT * kTimes; ++m) {
+                const int i = m % (NO * NT) / NT, j = m % NT, time = m / (NO * NT), at = s * NO * NT * kTimes + m;
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                    __builtin_bit_cast(h8, f[h][(time == 1 ? kEach : 0) + NT + i][s]),
+                    __builtin_bit_cast(h8, f[h][(time == 2 ? kEach : 0) + j][s]), acc[i][j], 0, 0, 0);
 #pragma unroll
                 for (int q = 0; q < kReads; ++q)
                     if (q * kProducts / kReads == at) read(kb_read, 1 - h, q);
@@ -375,7 +382,7 @@ Load load_of(Plan& w, int64_t b) {
     for (int k = 0; k < w.groups; ++k) {
         const Group& g = w.g[k];
         const double n = (double)((k + 1 < w.groups ? w.g[k + 1].tile0 : l.tiles) - g.tile0);
-        const double blocks = (PRECISE ? 3.0 : 1.0) * (((MODE == GRAM ? g.c : g.r) + kHalves - 1) / kHalves);
+        const double blocks = (PRECISE && b == 256 ? 3.0 : 1.0) * (((MODE == GRAM ? g.c : g.r) + kHalves - 1) / kHalves);
         l.blocks += n * blocks;
         l.most = blocks > l.most ? blocks : l.most;
     }
@@ -386,42 +393,65 @@ Load load_of(Plan& w, int64_t b) {
 // us and 1.0 us a block, which the card's power makes 1.8 when all CUs are at it (78 tiles over 48 and 128 blocks 67 and 149 us,
 // 256 tiles over 48 105); X's update moves more (117).  128: 7 us and 0.42 alone on a CU (136 over 32 and 128 blocks 20 and 61),
 // two to a CU 9 us and 1.1 (512 over 48 57 to 66).  64: 3.3 us and 0.19 alone (136 over 64 15), two to a CU 2 us and 0.56.
+// Pairs: 256 has three times the blocks.  128: a CU holds one, 8 us and 0.82 (36 over 16 and 64 blocks 22 and 64), with all CUs
+// at it 12 us and 1.27 (256 over 16 and 32 33 and 53).  64: 4.7 us and 0.36 alone (136 over 16 and 64 11 and 28), two to a CU 4.1
+// us and 0.88 (1024 over 16 and 32 36 and 65).
+template <bool PRECISE>
 double time_256(double tiles, double blocks, bool update) {
-    const double fill = tiles < kCus ? tiles / kCus : 1.0, hot = fill > 0.3 ? (fill - 0.3) / 0.7 : 0.0;
+    constexpr double kCool = PRECISE ? 0.45 : 0.3;     // of the CUs
+    const double fill = tiles < kCus ? tiles / kCus : 1.0, hot = fill > kCool ? (fill - kCool) / (1.0 - kCool) : 0.0;
     return 15.0 + blocks * (1.0 + 0.8 * hot) + (update ? 12.0 * fill : 0.0);
 }
 constexpr int kMostParts = 16;
+// Rounds of which the last is not full: it takes more than its part of one.
+double rounds_of(double tiles, double round) {
+    const double n = tiles / round;
+    return n + 0.6 * (ceil(n) - n);
+}
 // Tiles of which a CU holds two: up to one to each, `alone`; beyond, those that share a CU take about half as long again at once.
+template <bool PRECISE>
 double shared(double tiles, double alone, double two) {
     if (tiles <= kCus) return alone;
-    if (tiles > 2 * kCus) return (tiles / (2 * kCus) + 0.3) * two;
+    if (tiles > 2 * kCus) return (PRECISE ? rounds_of(tiles, 2 * kCus) : tiles / (2 * kCus) + 0.3) * two;
     return two > alone ? alone + (two - alone) * (0.45 + 0.55 * (tiles - kCus) / kCus) : alone;
 }
+template <bool PRECISE>
 double time_128(double tiles, double blocks, double most, bool update) {
-    return shared(tiles, 7.0 + 0.42 * most, 9.0 + 1.1 * blocks + (update ? 8.0 : 0.0));
+    if (!PRECISE) return shared<PRECISE>(tiles, 7.0 + 0.42 * most, 9.0 + 1.1 * blocks + (update ? 8.0 : 0.0));
+    const double fill = tiles < kCus ? tiles / kCus : 1.0;
+    const double one = 8.0 + (update ? 7.0 : 4.0) * fill + (0.82 + 0.45 * fill) * (tiles > kCus ? blocks : most);
+    return tiles > kCus ? rounds_of(tiles, kCus) * one : one;
 }
+template <bool PRECISE>
 double time_64(double tiles, double blocks, double most) {
-    const double alone = 3.3 + 0.19 * most, all = shared(tiles, alone, 2.0 + 0.56 * blocks);
+    const double alone = PRECISE ? 4.7 + 0.36 * most : 3.3 + 0.19 * most;
+    const double all = shared<PRECISE>(tiles, alone, PRECISE ? 4.1 + 0.88 * blocks : 2.0 + 0.56 * blocks);
     return all > alone ? all : alone;
 }
+// A last round of 256 tiles in quarters: triangles of pairs leave 256 to 128 tiles before it comes to that.
+template <Mode MODE, bool PRECISE>
+constexpr bool quarters = !PRECISE || MODE == UPDATE || MODE == LAST;
 template <Mode MODE, bool PRECISE>
 Way way_of(Plan& w) {
-    const bool update = MODE == UPDATE;
+    const bool update = MODE == UPDATE || (PRECISE && MODE == LAST);
     const Load a = load_of<MODE, PRECISE>(w, 256), b = load_of<MODE, PRECISE>(w, 128), c = load_of<MODE, PRECISE>(w, 64);
     const int64_t rounds = a.tiles / kCus, rest = a.tiles % kCus;
-    const double full = (double)rounds * time_256(kCus, a.blocks, update);
-    double best = full + (rest ? time_256((double)rest, rounds ? a.blocks : a.most, update) : 0.0);
+    const double full = (double)rounds * time_256<PRECISE>(kCus, a.blocks, update);
+    double best = full + (rest ? time_256<PRECISE>((double)rest, rounds ? a.blocks : a.most, update) : 0.0);
     Way way{ALL_256, 1};
     auto take = [&](Kinds kind, double time, int parts = 1) {
         if (time < best) best = time, way = {kind, parts};
     };
-    if (rounds && rest) take(WHOLE_256, full + time_128(4.0 * (double)rest, a.blocks, a.blocks, update));
-    take(ALL_128, time_128((double)b.tiles, b.blocks, b.most, update));
-    take(ALL_64, time_64((double)c.tiles, c.blocks, c.most));
+    const double axis = PRECISE ? a.blocks / 3.0 : a.blocks;
+    if (rounds && rest && quarters<MODE, PRECISE>)
+        take(WHOLE_256, full + time_128<PRECISE>(4.0 * (double)rest, axis, axis, update));
+    take(ALL_128, time_128<PRECISE>((double)b.tiles, b.blocks, b.most, update));
+    take(ALL_64, time_64<PRECISE>((double)c.tiles, c.blocks, c.most));
     if (MODE != GRAM) return way;
-    // The long axis of A in parts, where few tiles leave CUs idle: 6.5 us for a second launch, which reads what the parts leave at
-    // 80 bytes/ns a CU (400 x 8000: 23.3 us, 14.9 of 4 to 8 parts; 200 x 4000: 13.8, 11.5; 1536 x 6144: 40.8, 31.4 of 3;
-    // 2048 x 8192: 61, 54 of 3; but 1024 x 4096 15.3, 17.5 of 3, and 300 x 1000 6.5, 9.7).
+    // The long axis of A in parts, where few tiles leave CUs idle: 6.5 us for a second launch, less what the first does not do at
+    // its end (pairs: 3), and its reads of what the parts leave at 80 bytes/ns a CU (400 x 8000: 23.3 us, 14.9 of 4 to 8 parts;
+    // 200 x 4000: 13.8, 11.5; 1536 x 6144: 40.8, 31.4 of 3; 2048 x 8192: 61, 54 of 3; but 1024 x 4096 15.3, 17.5 of 3, and 300 x
+    // 1000 6.5, 9.7.  Pairs: 400 x 8000 43.0, 19.0 of 4; 1024 x 4096 28.4, 25.3 of 3; but three of 777 x 401 9.5, 11.9 of 2).
     auto fits = [&](int64_t side) {                    // parts that the next t's place holds
         int64_t n = kMostParts;
         for (int k = 0; k < w.groups; ++k) {
@@ -431,40 +461,48 @@ Way way_of(Plan& w) {
         }
         return n;
     };
-    auto join = [](double parts, double side) { return 6.5 + (parts + 1.0) * side * side * 4.0 / 80000.0; };
+    auto join = [](double parts, double side) { return (PRECISE ? 3.0 : 6.5) + (parts + 1.0) * side * side * 4.0 / 80000.0; };
     const int64_t most_b = fits(128), most_c = fits(64);
     for (int p = 2; p <= most_b && b.tiles * p <= 4 * kCus; ++p)
-        take(ALL_128, time_128((double)(b.tiles * p), b.blocks / p, b.most / p, false) + join(p, 128), p);
+        take(ALL_128, time_128<PRECISE>((double)(b.tiles * p), b.blocks / p, b.most / p, false) + join(p, 128), p);
     for (int p = 2; p <= most_c && c.tiles * p <= 4 * kCus; ++p)
-        take(ALL_64, time_64((double)(c.tiles * p), c.blocks / p, c.most / p) + join(p, 64), p);
+        take(ALL_64, time_64<PRECISE>((double)(c.tiles * p), c.blocks / p, c.most / p) + join(p, 64), p);
     return way;
 }
 
+// Tiles of 64 or 128: as many blocks staged as LDS holds where a CU has one tile, and as leave room for a second one where not.
+template <Mode MODE, bool PRECISE, typename Out, Phase PHASE>
+int launch_small(Steps& a, Kinds way, int parts) {
+    if (way == ALL_64) {
+        if constexpr (PRECISE)
+            if (tiles_of<MODE>(a.plan, 64) * parts > kCus) return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 2, PHASE>(a, 0, -1, parts);
+        return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4, PHASE>(a, 0, -1, parts);
+    }
+    if constexpr (!PRECISE)
+        if (tiles_of<MODE>(a.plan, 128) * parts <= kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4, PHASE>(a, 0, -1, parts);
+    return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2, PHASE>(a, 0, -1, parts);
+}
 template <Mode MODE, bool PRECISE, typename Out = Listed>
 int launch_step(Steps& a) {
     const auto [way, parts] = way_of<MODE, PRECISE>(a.plan);
     if constexpr (MODE == GRAM) {
-        if (parts > 1 && way == ALL_128) {
-            const bool alone = tiles_of<MODE>(a.plan, 128) * parts <= kCus;
-            if (const int rc = alone ? launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4, PART>(a, 0, -1, parts)
-                                     : launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2, PART>(a, 0, -1, parts)) return rc;
-            return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2, JOINED>(a, 0, -1, parts);
-        }
         if (parts > 1) {
-            if (const int rc = launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4, PART>(a, 0, -1, parts)) return rc;
-            return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4, JOINED>(a, 0, -1, parts);
+            if (const int rc = launch_small<MODE, PRECISE, Out, PART>(a, way, parts)) return rc;
+            return way == ALL_64 ? launch<MODE, PRECISE, Out, 1, 64, 32, 32, PRECISE ? 2 : 4, JOINED>(a, 0, -1, parts)
+                                 : launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2, JOINED>(a, 0, -1, parts);
         }
     }
     if (way == ALL_256) return launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(a, 0, -1);
-    if (way == WHOLE_256) {
-        const int64_t large = tiles_of<MODE>(a.plan, 256), rest = large % kCus;
-        if (const int rc = launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(a, 0, large - rest)) return rc;
-        if (4 * rest <= kCus) return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 4>(a, large - rest, large);
-        return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 2>(a, large - rest, large);
+    if constexpr (quarters<MODE, PRECISE>) {
+        if (way == WHOLE_256) {
+            const int64_t large = tiles_of<MODE>(a.plan, 256), rest = large % kCus;
+            if (const int rc = launch<MODE, PRECISE, Out, 1, 256, 64, 128, 2>(a, 0, large - rest)) return rc;
+            if constexpr (!PRECISE)
+                if (4 * rest <= kCus) return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 4>(a, large - rest, large);
+            return launch<MODE, PRECISE, Out, 2, 128, 64, 64, 2>(a, large - rest, large);
+        }
     }
-    if (way == ALL_64) return launch<MODE, PRECISE, Out, 1, 64, 32, 32, 4>(a, 0, -1);
-    if (tiles_of<MODE>(a.plan, 128) <= kCus) return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 4>(a, 0, -1);
-    return launch<MODE, PRECISE, Out, 1, 128, 64, 64, 2>(a, 0, -1);
+    return launch_small<MODE, PRECISE, Out, ALL>(a, way, 1);
 }
 
 template <bool PRECISE, typename Out>
@@ -484,11 +522,12 @@ int iterate(Steps& a, int steps, const float* coefficients) {
 template <bool PRECISE, Mode MODE>
 void way_into(Plan& w, int* way) {
     const auto [kind, parts] = way_of<MODE, PRECISE>(w);
-    const int64_t rest = tiles_of<MODE>(w, 256) % kCus, middle = tiles_of<MODE>(w, 128) * parts;
+    const int64_t rest = tiles_of<MODE>(w, 256) % kCus, middle = tiles_of<MODE>(w, 128) * parts, small = tiles_of<MODE>(w, 64) * parts;
     way[0] = kind == ALL_64 ? 64 : kind == ALL_128 ? 128 : 256;
     way[1] = kind == WHOLE_256 ? (int)rest : 0;
     way[2] = parts;
-    way[3] = kind == ALL_64 || (kind == ALL_128 && middle <= kCus) || (kind == WHOLE_256 && 4 * rest <= kCus) ? 4 : 2;
+    if (kind == ALL_64) way[3] = PRECISE && small > kCus ? 2 : 4;
+    else way[3] = !PRECISE && (kind == ALL_128 ? middle <= kCus : kind == WHOLE_256 && 4 * rest <= kCus) ? 4 : 2;
 }
 template <bool PRECISE>
 void ways_of(Plan& w, int* way) {

@@ -20,4 +20,5 @@ FAST = [(2, 20, 31), (2, 60, 61), (2, 72, 65), (2, 1, 428), (2, 103, 35), (2, 99
         (1, 3198, 40), (12, 1602, 1643), (3, 1263, 1033), (1, 2116, 967), (5, 1156, 1333), (18, 1109, 775), (13, 1072, 922)]
 PRECISE = [(2, 20, 31), (2, 35, 33), (2, 1, 291), (2, 33, 106), (2, 77, 69), (97, 210, 217), (59, 204, 196), (1, 3422, 1936),
            (1, 1960, 1518), (56, 418, 485), (12, 1731, 1744), (101, 467, 402), (2, 1, 897), (1, 1052, 1), (7, 390, 1166),
-           (100, 199, 67), (49, 337, 386), (57, 530, 457), (159, 479, 151)]
+           (100, 199, 67), (49, 337, 386), (57, 530, 457), (159, 479, 151),
+           (2, 526, 1294), (1, 3753, 1477), (289, 223, 206)]
