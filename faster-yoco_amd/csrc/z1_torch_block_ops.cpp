@@ -396,7 +396,8 @@ void refuse_cpu(const c10::OperatorHandle& op, torch::jit::Stack*) {
     TORCH_CHECK(false, op.schema().name(), ": expected GPU tensors (there is no CPU path)");
 }
 
-const char* const kOps[] = {"norm_forward", "norm_backward", "add_norm_forward", "add_norm_backward", "act8_pack", "act8_unpack", "weight8_pack", "product8",
+const char* const kOps[] = {"norm_forward", "norm_backward", "add_norm_forward", "add_norm_backward",
+                             "act8_pack", "act8_unpack", "weight8_pack", "product8",
                             "weight_grad8"};
 
 }  // namespace

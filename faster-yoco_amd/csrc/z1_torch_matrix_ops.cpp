@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "yoco_z1.h"
@@ -125,6 +126,14 @@ void check_matrix(const Tensor& t, const Tensor& like, at::ScalarType dtype, con
                 "]: expected a contiguous ", c10::toString(dtype), " matrix of p's shape");
 }
 
+// A matrix's bytes, from its first one to its last one's end.
+using Span = std::pair<const char*, const char*>;
+Span span_of(const Tensor& t) {
+    const auto* at = static_cast<const char*>(t.const_data_ptr());
+    const int64_t rows = t.size(0) > 1 ? (t.size(0) - 1) * t.stride(0) : 0;
+    return {at, at + (rows + t.size(1)) * t.element_size()};
+}
+
 // p = keep p - lr X, each matrix with its own
 void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at::TensorList p16, const OptTensor& factor,
                 at::ArrayRef<double> lr, at::ArrayRef<double> keep, double mu, bool nesterov,
@@ -138,7 +147,7 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
     TORCH_CHECK(mu >= 0 && mu < 1, what, ": momentum must be in [0, 1)");
     if (count == 0) return;
     require_gpu(p[0], what, "p");
-    std::vector<const void*> written;
+    std::vector<Span> written, read;
     for (size_t i = 0; i < count; ++i) {
         TORCH_CHECK(p[i].dim() == 2, what, ": p[", i, "]: expected a matrix, got ", p[i].dim(), " dimensions");
         require_gpu(p[i], what, "p");
@@ -152,13 +161,19 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
                     what, ": g[", i, "]: expected rows of neighbouring elements of p's shape, on its device");
         dtype_code(g[i].scalar_type(), what, "g");
         if (p[i].numel() == 0) continue;
-        written.push_back(p[i].const_data_ptr());
-        written.push_back(momentum[i].const_data_ptr());
-        if (!p16.empty()) written.push_back(p16[i].const_data_ptr());
+        written.push_back(span_of(p[i]));
+        written.push_back(span_of(momentum[i]));
+        if (!p16.empty()) written.push_back(span_of(p16[i]));
+        read.push_back(span_of(g[i]));
     }
     std::sort(written.begin(), written.end());
-    TORCH_CHECK(std::adjacent_find(written.begin(), written.end()) == written.end(), what,
-                ": a tensor that is written is named twice");
+    for (size_t i = 1; i < written.size(); ++i)
+        TORCH_CHECK(written[i - 1].second <= written[i].first, what, ": tensors that are written overlap, or one is named twice");
+    for (const Span& s : read) {
+        auto next = std::lower_bound(written.begin(), written.end(), s);
+        TORCH_CHECK((next == written.end() || s.second <= next->first) && (next == written.begin() || (--next)->second <= s.first),
+                    what, ": a gradient overlaps what is written");
+    }
     const float* f = nullptr;
     if (factor.has_value() && factor->defined()) {
         require_gpu(*factor, what, "factor");

@@ -18,6 +18,7 @@ import torch
 from . import library, ops, shard as shard_mod  # noqa: F401  (library registers the operators)
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+MAX_STEPS = 64
 
 _orthogonalize = torch.ops.yoco_z1.orthogonalize.default
 _step = torch.ops.yoco_z1.muon_step_.default
@@ -25,6 +26,8 @@ _step = torch.ops.yoco_z1.muon_step_.default
 
 def _coefficients(coefficients, steps):
     """[a, b, c] of each step, in a row: one triple for all of them, or a triple for each."""
+    if not 1 <= steps <= MAX_STEPS:
+        raise RuntimeError(f'muon: expected 1 to {MAX_STEPS} steps, got {steps}')
     c = list(coefficients)
     if len(c) == 3 and not any(hasattr(v, '__len__') for v in c):
         return [float(v) for v in c] * int(steps)
@@ -72,7 +75,7 @@ def step_(params, grads, momenta, copies=None, *, lr, momentum=0.95, nesterov=Tr
         p_i = p_i * (1 - lr * weight_decay) - rate(lr, p_i.shape, adjust) * orthogonalize(u_i)
 
     grads: fp32, bf16 or fp16, with rows of neighbouring elements.  factor: None or a one-element fp32 device tensor, as the
-    clip leaves it.  Matrices of one shape run together."""
+    clip leaves it.  Nothing that is written may overlap another of the call's tensors.  Matrices of one shape run together."""
     params, grads, momenta, copies = list(params), list(grads), list(momenta), [] if copies is None else list(copies)
     if not (params or grads or momenta or copies):
         return

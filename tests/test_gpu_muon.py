@@ -373,6 +373,41 @@ def test_refusals(pkg, dev):
     assert torch.equal(p, x) and torch.equal(m, x)                # nothing was written
 
 
+def test_overlapping_tensors_are_refused(pkg, dev):
+    """Views that share some bytes with what is written; gradients may share theirs with each other, and lie next to it."""
+    from faster_yoco_amd import muon
+    flat, g = torch.ones(200, device=dev), torch.ones(10, 20, device=dev)
+    at = lambda i, m=4, n=6: flat[i:i + m * n].view(m, n)  # noqa: E731
+    z = lambda m=4, n=6: torch.zeros(m, n, device=dev)  # noqa: E731
+    for args, text in ((([at(0), at(23)], [g[:4, :6]] * 2, [z(), z()]), 'overlap'), (([at(0)], [g[:4, :6]], [at(20)]), 'overlap'),
+                       (([at(0), at(100)], [g[:4, :6]] * 2, [z(), at(90)]), 'overlap'),
+                       (([at(24)], [at(0, 5)[1:]], [z()]), 'overlaps what is written'),
+                       (([at(24)], [at(47)], [z()]), 'overlaps what is written'),
+                       (([at(24)], [at(10, 2, 48)[:, :24].reshape(2, 24)[:, :6].expand(2, 6)], [z()]), "p's shape"),
+                       (([at(30, 2, 5)], [flat.as_strided((2, 5), (100, 1), 20)], [z(2, 5)]), 'overlaps what is written')):
+        with pytest.raises(RuntimeError, match=text):
+            muon.step_(*args, lr=0.1)
+    assert (flat == 1).all()
+    muon.step_([at(24), at(48)], [at(0), at(0)], [at(72), at(96)], lr=0.1)
+    assert (flat[:24] == 1).all() and (flat[120:] == 1).all() and (flat[24:72] < 1).all()
+    assert ((flat[72:120] - 1).abs() < 1e-6).all()                # 0.95 + 0.05 of ones
+
+
+def test_parameters_and_their_gradients(pkg, dev):
+    """A model's parameters as they are, outside no_grad too: the update records nothing."""
+    from faster_yoco_amd import muon
+    w = [torch.nn.Parameter(matrix(30, 20).to(dev)), torch.nn.Parameter(matrix(150, 140).to(dev))]
+    sum((p * p).sum() for p in w).backward()
+    old = [p.detach().clone() for p in w]
+    momenta = [torch.zeros_like(p, requires_grad=False) for p in w]
+    muon.step_(w, [p.grad for p in w], momenta, lr=0.01, weight_decay=0.0, nesterov=False, momentum=0.0)
+    for p, o, m in zip(w, old, momenta):
+        assert p.is_leaf and p.grad_fn is None and torch.equal(m, p.grad)
+        # the same call's launches hold other matrices: last bits, 1e-3 of the result
+        want = o - muon.rate(0.01, o.shape, 'rms') * muon.orthogonalize(2 * o, precise=False)
+        assert float((p.detach() - want).norm()) < 4e-3 * float((want - o).norm())
+
+
 def test_as_operators(pkg, dev):
     ops = torch.ops.yoco_z1
     c = [3.4445, -4.775, 2.0315] * 2

@@ -113,6 +113,8 @@ def test_cpu_tensors_and_wrong_arguments_are_refused(pkg):
     for call, text in ((lambda: muon.orthogonalize(x[0]), 'matrices'),
                        (lambda: muon.orthogonalize(x, coefficients=[1.0, 2.0, 3.0, 4.0, 5.0]), 'triple'),
                        (lambda: muon.orthogonalize(x, coefficients=[(1.0, 2.0)] * 5), 'triple'),
+                       (lambda: muon.orthogonalize(x, steps=1 << 60), '1 to 64 steps'),
+                       (lambda: muon.orthogonalize(x, steps=-1), '1 to 64 steps'),
                        (lambda: muon.step_([x], [x], [x], lr=1.0, adjust='none'), 'adjust')):
         with pytest.raises(RuntimeError, match=text):
             call()
