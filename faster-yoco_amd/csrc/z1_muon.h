@@ -39,7 +39,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr float kX = 4096.0f, kA = 2048.0f, kB = 1024.0f;
 constexpr int kHalves = 64;                            // columns of a staged block: 128 bytes
-constexpr int kParts = 256;                            // partial sums of a matrix's squares
+constexpr int kParts = 1024;                           // partial sums of a matrix's squares, at most
 constexpr int kList = Z1_MAX_MATRICES;                 // matrices named one by one in a launch, and groups of them
 constexpr int kMaxSteps = 64;
 constexpr int kWholeSide = 128;                        // shorter side of the small matrices, at most
@@ -131,23 +131,36 @@ struct Start {
     double* partials;                                  // [matrices][kParts]
 };
 
-// Eight of u, and with MOVE the momentum's step before.
-template <typename T, bool MOVE>
-__device__ __forceinline__ void load_u(const Start& a, int z, int64_t row, int n, int c, float factor, float* u) {
+// Eight of a gradient and of its momentum; zeros past a row's end.
+struct Eight {
+    float g[8], buf[8];
+};
+template <typename T>
+__device__ __forceinline__ void load_eight(const Start& a, int z, int64_t row, int n, int c, Eight& e) {
     const int left = n - c;
     const void* g = a.list ? a.in.g[z] : (const void*)((const typename T::elem*)a.batch.x + z * a.batch.step);
-    load_row<T>(g, row * (a.list ? a.in.stride[z] : a.batch.stride) + c, left, u);
+    load_row<T>(g, row * (a.list ? a.in.stride[z] : a.batch.stride) + c, left, e.g);
+    if (a.list) load_row<F32>(a.in.buf[z], row * n + c, left, e.buf);
+}
+// u of them, and with MOVE the momentum's step before.
+template <bool MOVE>
+__device__ __forceinline__ void u_of(const Start& a, int z, int64_t row, int n, int c, float factor, Eight& e, float* u) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = e.g[j];
     if (!a.list) return;
-    const int64_t at = row * n + c;
-    float buf[8];
-    load_row<F32>(a.in.buf[z], at, left, buf);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float g = (u[j] * factor) * (1.0f - a.mu);
-        if (MOVE) buf[j] = __builtin_fmaf(a.mu, buf[j], g);
-        u[j] = a.nesterov ? __builtin_fmaf(a.mu, buf[j], g) : buf[j];
+        if (MOVE) e.buf[j] = __builtin_fmaf(a.mu, e.buf[j], g);
+        u[j] = a.nesterov ? __builtin_fmaf(a.mu, e.buf[j], g) : e.buf[j];
     }
-    if (MOVE) store_row<F32>(a.in.buf[z], at, left, buf);
+    if (MOVE) store_row<F32>(a.in.buf[z], row * n + c, n - c, e.buf);
+}
+template <typename T, bool MOVE>
+__device__ __forceinline__ void load_u(const Start& a, int z, int64_t row, int n, int c, float factor, float* u) {
+    Eight e;
+    load_eight<T>(a, z, row, n, c, e);
+    u_of<MOVE>(a, z, row, n, c, factor, e, u);
 }
 
 // Eight values as fp16 at `at` (16-byte aligned), and what that leaves, `plane` bytes on.

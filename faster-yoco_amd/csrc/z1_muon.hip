@@ -11,24 +11,38 @@ namespace {
 using namespace z1muon;
 
 // ------------------------------------------------------------------------------------------------------ start
-// The momentum's step, and u's squares summed in 64 bits (an fp32 u may be as large as its type goes): a workgroup's rows in
-// turn, as many threads to a row as it has groups of eight columns.
-constexpr int kStartThreads = 256;
+// The momentum's step, and u's squares summed in 64 bits (an fp32 u may be as large as its type goes).  Bound by memory: the
+// workgroups of a matrix pass over its groups of eight columns side by side, kAhead of them on the way to a thread (8192 x 3072
+// in BF16: 16 us, 37 by 256 workgroups, 44 with one on the way as well; the matrices of two blocks, 690 MB, 130 us, 5.3 TB/s, and 148).
+constexpr int kStartThreads = 256, kAhead = 4;
 template <typename T>
 __global__ __launch_bounds__(kStartThreads) void momentum_kernel(Start a, Plan plan) {
     __shared__ double sums[kStartThreads];
     const int z = blockIdx.y;
     const Group& group = group_of_matrix(plan, z);
     const int m = group.tall ? group.c : group.r, n = group.tall ? group.r : group.c;
-    int lanes = 1;
-    while (lanes < kStartThreads && lanes * 8 < n) lanes *= 2;
-    const int per = kStartThreads / lanes, first = threadIdx.x / lanes, lane = threadIdx.x % lanes;
+    const int groups = (n + 7) / 8, step = gridDim.x * kStartThreads, begin = blockIdx.x * kStartThreads + threadIdx.x;
+    const int rows = step / groups, more = step % groups;
+    int row = begin / groups, i = begin % groups;      // rows below 2^20 and some 2^20 more
     const float factor = a.factor ? *a.factor : 1.0f;
     double s = 0.0;
-    for (int64_t row = (int64_t)blockIdx.x * per + first; row < m; row += (int64_t)gridDim.x * per) {
-        for (int c = lane * 8; c < n; c += lanes * 8) {
+    while (row < m) {
+        Eight e[kAhead];
+        int at[kAhead], c[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            at[k] = row;
+            c[k] = i * 8;
+            if (row < m) load_eight<T>(a, z, row, n, c[k], e[k]);
+            row += rows;
+            i += more;
+            if (i >= groups) i -= groups, ++row;
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (at[k] >= m) break;
             float u[8];
-            load_u<T, true>(a, z, row, n, c, factor, u);
+            u_of<true>(a, z, at[k], n, c[k], factor, e[k], u);
 #pragma unroll
             for (int j = 0; j < 8; ++j) s = __builtin_fma((double)u[j], (double)u[j], s);
         }
@@ -45,7 +59,7 @@ __global__ __launch_bounds__(kStartThreads) void momentum_kernel(Start a, Plan p
 // X in both orders from u: 64 x 64 of it to a workgroup.  parts: of each matrix's kParts sums, that are there.
 template <typename T, bool PRECISE>
 __global__ __launch_bounds__(kStartThreads) void start_kernel(Start a, Plan plan, int parts) {
-    __shared__ double sums[kParts];
+    __shared__ double sums[kStartThreads];
     __shared__ float turned[64][68];
     const Group& group = group_of_tile(plan, blockIdx.x);
     const int m = group.tall ? group.c : group.r, n = group.tall ? group.r : group.c;
@@ -53,9 +67,11 @@ __global__ __launch_bounds__(kStartThreads) void start_kernel(Start a, Plan plan
     const int across = (n + 63) / 64, down = (m + 63) / 64, nth = (blockIdx.x - group.tile0) / (across * down);
     const int index = blockIdx.x - group.tile0 - nth * across * down, i0 = index / across * 64, j0 = index % across * 64;
     const int z = group.first + nth;
-    sums[threadIdx.x] = (int)threadIdx.x < parts ? a.partials[(int64_t)z * kParts + threadIdx.x] : 0.0;
+    double s = 0.0;
+    for (int k = threadIdx.x; k < parts; k += kStartThreads) s += a.partials[(int64_t)z * kParts + k];
+    sums[threadIdx.x] = s;
     __syncthreads();
-    for (int k = kParts / 2; k; k >>= 1) {
+    for (int k = kStartThreads / 2; k; k >>= 1) {
         if ((int)threadIdx.x < k) sums[threadIdx.x] += sums[threadIdx.x + k];
         __syncthreads();
     }
@@ -129,17 +145,19 @@ bool bounded(const float* coefficients, int steps) {
 
 template <typename T>
 int start_of(const Start& a, Plan& w, int64_t count, bool precise, hipStream_t st) {
-    // enough workgroups for the largest matrix, 2048 elements or a row each
+    // enough workgroups for the largest matrix, a group of eight columns to a thread, and for the card: four of them to a CU
     int64_t parts = 1, tiles = 0;
     for (int k = 0; k < w.groups; ++k) {
         Group& g = w.g[k];
-        const int64_t m = g.tall ? g.c : g.r, n = g.tall ? g.r : g.c, rows = 2048 / (n < 8 ? 8 : n) + 1, need = (m + rows - 1) / rows;
+        const int64_t m = g.tall ? g.c : g.r, n = g.tall ? g.r : g.c;
+        const int64_t need = (m * ((n + 7) / 8) + kStartThreads - 1) / kStartThreads;
         parts = need > parts ? need : parts;
         g.tile0 = (int)tiles;
         tiles += g.count * ((n + 63) / 64) * ((m + 63) / 64);
         if (tiles > 2 * kMaxTiles) return Z1_E_SIZE;
     }
-    if (parts > kParts) parts = kParts;
+    const int64_t most = count < 4 ? kParts / count : 256;
+    if (parts > most) parts = most;
     momentum_kernel<T><<<dim3((unsigned)parts, (unsigned)count), kStartThreads, 0, st>>>(a, w);
     const dim3 grid((unsigned)tiles);
     if (precise) start_kernel<T, true><<<grid, kStartThreads, 0, st>>>(a, w, (int)parts);
