@@ -197,6 +197,12 @@ int iterate_precise(Steps& a, int steps, const float* coefficients, Kind kind);
 void ways_fast(Plan& w, int* way);
 void ways_precise(Plan& w, int* way);
 
+// Matrices of up to four fragments of 32 x 32 take pairs in any case: the fewer elements, the less their roundings average out
+// (16 x 16: up to 1.2e-3, 64 x 256 6.5e-4), and there it costs little (32 x 32: 12.7 -> 15.2 us, 64 x 64 17.1 -> 20.3; but 64 x 256
+// 26.6 -> 34.4).
+__host__ __device__ inline bool has_pairs(int64_t r, int64_t c, bool precise) {
+    return precise || ((r + 31) / 32) * ((c + 31) / 32) <= 4;
+}
 // The small matrices' kernel: fragments to a wave and bytes of LDS.  0: the matrix is too large for it.
 struct WholeWay {
     int pieces, bytes;
@@ -204,16 +210,16 @@ struct WholeWay {
 WholeWay whole_way(int64_t m, int64_t n, bool precise);
 inline bool is_whole(int64_t m, int64_t n, bool precise) { return whole_way(m, n, precise).pieces != 0; }
 
-// By rows of fragments: the largest of a launch's small matrices, or none.
+// By exactness and rows of fragments: the largest of a launch's small matrices, or none.
 struct WholeWays {
-    WholeWay of[kWholeSide / 32];
+    WholeWay of[2][kWholeSide / 32];
     void add(int64_t m, int64_t n, bool precise) {
         const WholeWay w = whole_way(m, n, precise);
-        WholeWay& own = of[((m < n ? m : n) - 1) / 32];
+        WholeWay& own = of[has_pairs(m, n, precise)][((m < n ? m : n) - 1) / 32];
         if (w.pieces > own.pieces) own = w;
     }
 };
-// `count` matrices of the plan's groups, all of them small, in one launch for each number of rows of fragments.
+// `count` matrices of the plan's groups, all of them small, in one launch for each exactness and number of rows of fragments.
 int run_whole(const Start& start, const Plan& plan, const WholeWays& ways, int64_t count, int dtype, int steps,
               const float* coefficients, bool precise, void* out, int out_dtype, hipStream_t st);
 

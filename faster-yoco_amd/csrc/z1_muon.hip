@@ -238,6 +238,7 @@ int z1_orthogonalize_way(int64_t count, int64_t m, int64_t n, int precise, int* 
     const WholeWay small = whole_way(m, n, precise != 0);
     if (small.pieces) {
         way[1] = small.pieces;
+        way[2] = has_pairs(m, n, precise != 0);
         return Z1_OK;
     }
     Plan w{};

@@ -16,7 +16,7 @@ struct Whole {
     Start start;
     void* out;                                         // or p and p16 of the list
     int dtype, out_dtype;
-    int steps;
+    int steps, precise;
     float co[3 * kMaxSteps];
 };
 constexpr int kWholeWaves = 8;
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kWholeWaves * 64) void whole_kernel(Whole a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int z = blockIdx.x, l32 = lane & 31, half = lane >> 5, rs = spread(l32);
     const Group& g = group_of_matrix(a.plan, z);
-    if ((g.r + 31) / 32 != R) return;                  // another launch's
+    if ((g.r + 31) / 32 != R || has_pairs(g.r, g.c, a.precise) != PRECISE) return;              // another launch's
     const int C = (g.c + 31) / 32, pieces = R * C;
     const Places at = places_of(R, C, PRECISE);
     const int m = g.tall ? g.c : g.r, n = g.tall ? g.r : g.c;
@@ -314,10 +314,11 @@ int launch_whole(const Whole& a, const WholeWay& way, int64_t count, hipStream_t
     return (int)hipGetLastError();
 }
 template <int R>
-int run_rows(const Whole& a, const WholeWays& ways, int64_t count, bool precise, hipStream_t st) {
-    const WholeWay& way = ways.of[R - 1];
-    if (!way.pieces) return Z1_OK;
-    return precise ? launch_whole<R, true>(a, way, count, st) : launch_whole<R, false>(a, way, count, st);
+int run_rows(const Whole& a, const WholeWays& ways, int64_t count, hipStream_t st) {
+    const WholeWay &single = ways.of[0][R - 1], &pairs = ways.of[1][R - 1];
+    if (single.pieces)
+        if (const int rc = launch_whole<R, false>(a, single, count, st)) return rc;
+    return pairs.pieces ? launch_whole<R, true>(a, pairs, count, st) : Z1_OK;
 }
 }  // namespace
 
@@ -326,7 +327,7 @@ namespace z1muon {
 WholeWay whole_way(int64_t m, int64_t n, bool precise) {
     const int64_t r = m < n ? m : n, c = m < n ? n : m;
     if (r > kWholeSide || c > 32 * 32) return {0, 0};
-    const int R = (int)(r + 31) / 32, C = (int)(c + 31) / 32, bytes = places_of(R, C, precise).size;
+    const int R = (int)(r + 31) / 32, C = (int)(c + 31) / 32, bytes = places_of(R, C, has_pairs(r, c, precise)).size;
     for (const WholeWay way : {WholeWay{2, 64 << 10}, WholeWay{4, 159 << 10}})
         if (R * C <= way.pieces * kWholeWaves && bytes <= way.bytes) return way;
     return {0, 0};
@@ -334,12 +335,12 @@ WholeWay whole_way(int64_t m, int64_t n, bool precise) {
 
 int run_whole(const Start& start, const Plan& plan, const WholeWays& ways, int64_t count, int dtype, int steps,
               const float* coefficients, bool precise, void* out, int out_dtype, hipStream_t st) {
-    Whole a{plan, start, out, dtype, out_dtype, steps, {}};
+    Whole a{plan, start, out, dtype, out_dtype, steps, precise, {}};
     for (int i = 0; i < 3 * steps; ++i) a.co[i] = coefficients[i];
-    if (const int rc = run_rows<1>(a, ways, count, precise, st)) return rc;
-    if (const int rc = run_rows<2>(a, ways, count, precise, st)) return rc;
-    if (const int rc = run_rows<3>(a, ways, count, precise, st)) return rc;
-    return run_rows<4>(a, ways, count, precise, st);
+    if (const int rc = run_rows<1>(a, ways, count, st)) return rc;
+    if (const int rc = run_rows<2>(a, ways, count, st)) return rc;
+    if (const int rc = run_rows<3>(a, ways, count, st)) return rc;
+    return run_rows<4>(a, ways, count, st);
 }
 
 }  // namespace z1muon

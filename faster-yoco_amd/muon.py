@@ -8,7 +8,7 @@ X = u / max(|u|_F, eps), then for each step's (a, b, c): X <- a X + b (X X^T) X 
 take singular values from 1e-3 of the norm up to between 0.7 and 1.2 in five steps.  The products run on fp16 operands with
 fp32 sums, X kept in 22 bits and the diagonals of both symmetric products in fp32, which leaves the result within 1e-3 of the
 exact iterate (2-norm, relative); with ``precise`` the operands are pairs of fp16, for the exactness of fp32 products at three
-times the work.  The products of a call's matrices share launches, whose tiles are chosen by how much there is in all: the same
+times the work (matrices of up to four parts of 32 x 32 have pairs in any case).  The products of a call's matrices share launches, whose tiles are chosen by how much there is in all: the same
 call gives the same bits, but the last bits of a matrix may differ with the matrices beside it.  None of it is differentiable.
 """
 import math

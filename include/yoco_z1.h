@@ -337,7 +337,8 @@ int z1_weight_grad8_way(int64_t T, int64_t N, int64_t K, int whole_dwords, int* 
  * (a, b, c), coefficients[steps][3].  Coefficients are admitted only where singular values in [0, 1] stay below 4 and b l + c l^2
  * below 32 on their squares (Z1_E_MODE otherwise); eps > 0; steps 1 to 64; m and n at most 2^20.  A matrix with an infinity or
  * a NaN becomes NaN, one of zeros zeros.  precise 0: within about 1e-3 of the exact result (2-norm of the difference over
- * the result's), for bf16 results; 1: as fp32 products leave it, at three times the matrix work.
+ * the result's), for bf16 results; 1: as fp32 products leave it, at three times the matrix work (matrices of up to four parts of
+ * 32 x 32 in any case).
  * workspace: as many bytes of device memory as the workspace function says, 16-byte aligned; calls that may overlap must not
  * share one. */
 
@@ -349,7 +350,7 @@ int64_t z1_orthogonalize_workspace(int64_t count, int64_t m, int64_t n, int prec
 /* How matrices of these sizes run, of interest to timing and tests: for each of the three products (A, its square, B X) way[0] =
  * rows and columns of a workgroup's tile, way[1] = tiles of 256 that are left to quarters of 128, way[2] = parts of the summed
  * axis, way[3] = blocks of it that are staged (by the quarters where there are any).  Small matrices, a workgroup each: way[0] is
- * 0 and way[1] the fragments of X to a wave. */
+ * 0, way[1] the fragments of X to a wave and way[2] whether pairs are the operands. */
 int z1_orthogonalize_way(int64_t count, int64_t m, int64_t n, int precise, int* way);
 
 #define Z1_MAX_MATRICES 32

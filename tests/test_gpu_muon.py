@@ -373,6 +373,22 @@ def test_refusals(pkg, dev):
     assert torch.equal(p, x) and torch.equal(m, x)                # nothing was written
 
 
+def test_small_matrices_of_a_call_side_by_side(pkg, dev):
+    """Small matrices run by themselves whatever else a call holds: in any mixture each comes out as alone, bit for bit.  Those
+    of up to four parts of 32 x 32 come out as exactly as pairs do."""
+    from faster_yoco_amd import muon
+    sizes = [(20, 31), (20, 200), (60, 61), (200, 20), (40, 100), (1, 1), (33, 90), (64, 64), (128, 32), (100, 90), (16, 16), (1, 400)]
+    u = [matrix(m, n, KINDS[i % len(KINDS)]).to(dev) for i, (m, n) in enumerate(sizes)]
+    for precise in (False, True):
+        p = [torch.zeros_like(t) for t in u]
+        muon.step_(p, u, [torch.zeros_like(t) for t in u], lr=1.0, adjust=1.0, weight_decay=0.0, momentum=0.0, precise=precise)
+        for t, q in zip(u, p):
+            assert torch.equal(-q, muon.orthogonalize(t, precise=precise)), t.shape
+            if -(-t.shape[0] // 32) * -(-t.shape[1] // 32) <= 4:
+                want, most = limit(t.cpu(), torch.float32, True)
+                assert far(-q, want) <= most, t.shape
+
+
 def test_overlapping_tensors_are_refused(pkg, dev):
     """Views that share some bytes with what is written; gradients may share theirs with each other, and lie next to it."""
     from faster_yoco_amd import muon
