@@ -13,7 +13,8 @@ using namespace z1muon;
 // ------------------------------------------------------------------------------------------------------ start
 // The momentum's step, and u's squares summed in 64 bits (an fp32 u may be as large as its type goes).  Bound by memory: the
 // workgroups of a matrix pass over its groups of eight columns side by side, kAhead of them on the way to a thread (8192 x 3072
-// in BF16: 16 us, 37 by 256 workgroups, 44 with one on the way as well; the matrices of two blocks, 690 MB, 130 us, 5.3 TB/s, and 148).
+// in BF16: 16 us, 37 by 256 workgroups, 44 with one on the way as well; the matrices of two blocks, 690 MB, 130 us, 5.3 TB/s, and
+// 148).
 constexpr int kStartThreads = 256, kAhead = 4;
 template <typename T>
 __global__ __launch_bounds__(kStartThreads) void momentum_kernel(Start a, Plan plan) {
@@ -56,7 +57,9 @@ __global__ __launch_bounds__(kStartThreads) void momentum_kernel(Start a, Plan p
     if (threadIdx.x == 0) a.partials[(int64_t)z * kParts + blockIdx.x] = sums[0];
 }
 
-// X in both orders from u: 64 x 64 of it to a workgroup.  parts: of each matrix's kParts sums, that are there.
+// X in both orders from u: 64 x 64 of it to a workgroup, turned by way of LDS.  Bound by memory (the matrices of two blocks,
+// 830 MB, 164 us, 5.1 TB/s; four of 3072 x 3072 59; u again from the gradient and the momentum is as much as a stored u).
+// parts: of each matrix's kParts sums, that are there.
 template <typename T, bool PRECISE>
 __global__ __launch_bounds__(kStartThreads) void start_kernel(Start a, Plan plan, int parts) {
     __shared__ double sums[kStartThreads];

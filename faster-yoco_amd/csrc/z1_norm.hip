@@ -136,7 +136,8 @@ __device__ __forceinline__ void finish8(const Forward& a, int64_t row, int c, in
 
 // Rows of 8 to 4 * NV * 512 columns: a row's wpr waves hold it in registers.  One row to them: a grid of rows, which the
 // hardware hands out, is faster here than one that takes rows in turn and loads ahead (layer norm of 16384 x 3072 BF16 37.6
-// us, 5.4 TB/s, against 48-65; RMS norm of 8192 x 3072 with 8-bit result and checkpoint 18.9 us, 5.3 TB/s).
+// us, 5.4 TB/s, against 48-65; RMS norm of 8192 x 3072 with 8-bit result and checkpoint 18.9 us, 5.3 TB/s; with the residual
+// added, read and h written beside them 34.5 us, 5.8 TB/s).
 // All loads are under way before the first sum, and none stands behind a branch (settle).
 template <typename T, typename W, int NV, bool CENTER, bool ADD>
 __global__ __launch_bounds__(kFwdThreads) void norm_forward_kernel(Forward a) {
@@ -399,7 +400,8 @@ struct Input<T, true> {
 // db sums in registers over all of them, the groups' sums meet in LDS at the end, and the workgroup writes one partial row
 // of each, which norm_reduce_kernel adds in order.  The next rows are loaded while the present ones are computed, and no
 // load stands behind a branch.  Bound by memory (layer norm of 16384 x 3072 BF16 57 us, 5.3 TB/s; RMS norm from the checkpoint
-// 46 us, 5.5); one workgroup to a CU, as 128 of them (73 us) have too few loads under way and 512 (65) twice the partial rows.
+// 46 us, 5.5, and with dh added 68, 5.2); one workgroup to a CU, as 128 of them (73 us) have too few loads under way and 512
+// (65) twice the partial rows.
 template <typename T, int NV, bool Q, bool CENTER, bool ADD>
 __global__ __launch_bounds__(kRowThreads) void norm_backward_kernel(Backward a) {
     __shared__ float red[2][kRowThreads / 64][2];
