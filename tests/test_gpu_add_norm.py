@@ -178,6 +178,32 @@ def test_strided_rows(pkg, dev, n, dim):
     assert three[0].shape == (1, n, dim) and torch.equal(three[0][0], h) and three[1].rows == n
 
 
+def test_rows_past_32_bits_apart(pkg, dev):
+    from faster_yoco_amd import norm
+    x, res, w, b, dy, dh = (t.to(dev) for t in inputs(3, 515, torch.bfloat16, 9))
+    flat = torch.empty((1 << 31) + 4000, dtype=torch.bfloat16, device=dev)
+    far = [flat[i * 600:].as_strided((3, 515), ((1 << 30) + 3, 1)) for i in range(4)]
+    for t, v in zip((x, res, dy, dh), far):
+        v.copy_(t)
+    want, got = norm.add_layer_norm(x, res, w, b), norm.add_layer_norm(far[0], far[1], w, b)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    h, _, mean, rstd = want
+    assert all(torch.equal(p, q) for p, q in zip(norm.add_layer_norm_backward(dy, dh, h, mean, rstd, w, bias=True),
+                                                 norm.add_layer_norm_backward(far[2], far[3], h, mean, rstd, w, bias=True)))
+
+
+def test_one_tensor_as_both(pkg, dev):
+    """h = 2 x, exactly; x's gradient is twice dx."""
+    from faster_yoco_amd import norm
+    x, _, w, _, dy, dh = (None if t is None else t.to(dev) for t in inputs(7, 300, torch.float32, 10))
+    a, r = x.clone().requires_grad_(), [t.clone().requires_grad_() for t in (x, x)]
+    for args in ((a, a), r):
+        h, y = norm.add_rms_norm_train(*args, w)
+        assert torch.equal(h, 2 * x)
+        torch.autograd.backward([h, y], [dh, dy])
+    assert torch.equal(r[0].grad, r[1].grad) and torch.equal(a.grad, 2 * r[0].grad)
+
+
 def test_no_rows(pkg, dev):
     from faster_yoco_amd import norm
     x, w = torch.empty(0, 300, device=dev, dtype=torch.bfloat16), torch.ones(300, device=dev, dtype=torch.bfloat16)

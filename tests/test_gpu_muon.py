@@ -389,6 +389,24 @@ def test_small_matrices_of_a_call_side_by_side(pkg, dev):
                 assert far(-q, want) <= most, t.shape
 
 
+def test_offsets_past_32_bits(pkg, dev):
+    """Matrices and rows that lie 2^31 elements and more apart, read by the small matrices' kernel and by the others."""
+    from faster_yoco_amd import muon
+    flat = torch.empty((1 << 31) + 300000, dtype=torch.bfloat16, device=dev)
+    for m, n in ((40, 50), (150, 140)):
+        x = flat.as_strided((2, m, n), ((1 << 31) + 77, n + 3, 1))
+        x.copy_(torch.stack([matrix(m, n), matrix(m, n, 'strong')]))
+        assert torch.equal(muon.orthogonalize(x), muon.orthogonalize(x.clone(memory_format=torch.contiguous_format)))
+    for n in (60, 2000):
+        x = flat.as_strided((3, n), ((1 << 30) + 5, 1))
+        x.copy_(matrix(3, n))
+        assert torch.equal(muon.orthogonalize(x), muon.orthogonalize(x.clone(memory_format=torch.contiguous_format)))
+        p, q = (torch.zeros(3, n, device=dev) for _ in range(2))
+        muon.step_([p], [x], [torch.zeros_like(p)], lr=0.1)
+        muon.step_([q], [x.clone(memory_format=torch.contiguous_format)], [torch.zeros_like(q)], lr=0.1)
+        assert torch.equal(p, q) and (p != 0).any()
+
+
 def test_overlapping_tensors_are_refused(pkg, dev):
     """Views that share some bytes with what is written; gradients may share theirs with each other, and lie next to it."""
     from faster_yoco_amd import muon
