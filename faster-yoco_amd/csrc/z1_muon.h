@@ -15,10 +15,12 @@
 //   - the diagonals d of A and e of a + B stay in fp32, apart from the operands:  with A = D + A', B = E + B',
 //     A^2 = D^2 + D A' + A' D + A'^2,  so B'[i][j] = c A'^2[i][j] + (b + c (d_i + d_j)) A'[i][j],
 //     e_i = a + b d_i + c d_i^2 + c A'^2[i][i],  X <- e X + B' X;
-//   - X is kept as a pair of fp16 (22 bits), of which products take the first and e X both.
-// That leaves 1e-4 to 8e-4 for any spectrum, at the same number of products: enough for a result in bf16, whose own rounding is
-// 1.7e-3.  For results that hold more, PRECISE takes pairs for A and B as well and three products for one, hi hi + hi lo +
-// lo hi: 1e-6 to 3e-5, as plain fp32 products leave.
+//   - X is kept as a pair of fp16 (22 bits), of which e X takes both, and B' X too in the first steps (both_halves): what the
+//     first half leaves out there goes into all directions, those of no size among them, and grows from step to step; what A and
+//     B lose only turns the directions that are there.
+// That leaves 4e-4 to 1.3e-3 of the result (2-norm), whatever the spectrum, with more than 64 rows: less than the rounding of a
+// result in bf16, 1.7e-3.  Fewer rows, and PRECISE for results that hold more, take pairs for A and B as well and three products
+// for one, hi hi + hi lo + lo hi: 1e-6 to 3e-5, and up to 1e-4 with few directions in the input, as plain fp32 products leave.
 //
 // Stored values are scaled by powers of two, so that fp16's range covers them: the host admits coefficients only if the
 // iterates stay below 4 and B below 32, so |X| kX <= 2^14, |A| kA <= 2^15, |B| kB <= 2^15.
@@ -62,14 +64,15 @@ struct Batch {
     int64_t step, stride;
 };
 
-// A matrix's part of the workspace: offsets of X in both orders (t twice: read and written), A, B (pairs) and the diagonals, bytes
-// from a pair's first halves to its second ones, and bytes in all.  Every array starts at a multiple of 1024 bytes.
+// A matrix's part of the workspace, with `planes` halves of X's second order, A and B (2: pairs): offsets of X in both orders (t
+// twice: read and written), A, B and the diagonals, bytes from a pair's first halves to its second ones, and bytes in all.
+// Every array starts at a multiple of 1024 bytes.
 struct Layout {
     int64_t t[2], o, A, B, d, e, size;
     int64_t t_plane, o_plane, s_plane;
     int ldr, ldc;                                      // r and c rounded up to blocks
 };
-__host__ __device__ inline Layout layout_of(int r, int c, bool precise) {
+__host__ __device__ inline Layout layout_of(int r, int c, int planes) {
     Layout w;
     w.ldr = (r + kHalves - 1) / kHalves * kHalves;
     w.ldc = (c + kHalves - 1) / kHalves * kHalves;
@@ -77,7 +80,6 @@ __host__ __device__ inline Layout layout_of(int r, int c, bool precise) {
     w.t_plane = room((int64_t)c * w.ldr * 2);
     w.o_plane = room((int64_t)r * w.ldc * 2);
     w.s_plane = room((int64_t)r * w.ldr * 2);
-    const int planes = precise ? 2 : 1;
     w.t[0] = 0;
     w.t[1] = 2 * w.t_plane;
     w.o = 4 * w.t_plane;
@@ -102,6 +104,7 @@ struct Plan {
     uint8_t* base;
     int groups;
     int cur;                                           // which t is read
+    int both;                                          // B X on single operands takes both halves of X
     Group g[kList];
 };
 // The group of a workgroup, or of a matrix.
@@ -197,12 +200,34 @@ int iterate_precise(Steps& a, int steps, const float* coefficients, Kind kind);
 void ways_fast(Plan& w, int* way);
 void ways_precise(Plan& w, int* way);
 
-// Matrices of up to four fragments of 32 x 32 take pairs in any case: the fewer elements, the less their roundings average out
-// (16 x 16: up to 1.2e-3, 64 x 256 6.5e-4), and there it costs little (32 x 32: 12.7 -> 15.2 us, 64 x 64 17.1 -> 20.3; but 64 x 256
-// 26.6 -> 34.4).
-__host__ __device__ inline bool has_pairs(int64_t r, int64_t c, bool precise) {
-    return precise || ((r + 31) / 32) * ((c + 31) / 32) <= 4;
+// Matrices of few rows take pairs in any case: the fewer rows, the less what A and B lose averages out (2 rows up to 5e-3, 3 x
+// 2000 2e-3, 16 x 16 1.6e-3, 33 x 96 1.2e-3; 65 to 128 rows 1.0e-3 at most), and there it costs least (32 x 32: 12.7 -> 15.2
+// us, 64 x 256 26.6 -> 35.0, 40 x 2000 91 -> 109).
+constexpr int kPairSide = 64;
+__host__ __device__ inline bool has_pairs(int m, int n, bool precise) { return precise || (m < n ? m : n) <= kPairSide; }
+
+// In a kernel: a number that the compiler does not take apart into a truth value, as which it leaves the scalar unit, and every
+// address that follows with it.
+template <bool PRECISE>
+__device__ __forceinline__ int planes_of(const Group& g) {
+    return PRECISE ? 2 : __builtin_amdgcn_readfirstlane(has_pairs(g.r, g.c, false) ? 2 : 1);
 }
+
+// On single operands: the steps whose B X takes both halves of X, a bit each.  A direction of no size grows by `a` a step, and
+// with it what the first half leaves out, 2^-12 of X in every element: both halves until no more than a factor of 16 is to come
+// (the first two of five steps with the default coefficients.  A rank of one or four in 65 x 4000: 6.7e-3 of the result without,
+// 9.1e-4 with two steps, 6.2e-4 with three, 5.3e-4 with all five; 65 x 65 to 1024 x 1024 of other spectra up to 1.3e-3 with two
+// and with five alike.  Each such step is a tenth more work).
+inline uint64_t both_halves(const float* coefficients, int steps) {
+    uint64_t both = 0;
+    double growth = 1.0;
+    for (int k = steps - 1; k >= 0; --k) {
+        if (growth > 16.0) both |= 1ull << k;
+        growth *= coefficients[3 * k] < 0.0f ? -coefficients[3 * k] : coefficients[3 * k];
+    }
+    return both;
+}
+
 // The small matrices' kernel: fragments to a wave and bytes of LDS.  0: the matrix is too large for it.
 struct WholeWay {
     int pieces, bytes;
@@ -210,16 +235,16 @@ struct WholeWay {
 WholeWay whole_way(int64_t m, int64_t n, bool precise);
 inline bool is_whole(int64_t m, int64_t n, bool precise) { return whole_way(m, n, precise).pieces != 0; }
 
-// By exactness and rows of fragments: the largest of a launch's small matrices, or none.
+// By rows of fragments, which with `precise` decide on pairs: the largest of a launch's small matrices, or none.
 struct WholeWays {
-    WholeWay of[2][kWholeSide / 32];
+    WholeWay of[kWholeSide / 32];
     void add(int64_t m, int64_t n, bool precise) {
         const WholeWay w = whole_way(m, n, precise);
-        WholeWay& own = of[has_pairs(m, n, precise)][((m < n ? m : n) - 1) / 32];
+        WholeWay& own = of[((m < n ? m : n) - 1) / 32];
         if (w.pieces > own.pieces) own = w;
     }
 };
-// `count` matrices of the plan's groups, all of them small, in one launch for each exactness and number of rows of fragments.
+// `count` matrices of the plan's groups, all of them small, in one launch for each number of rows of fragments.
 int run_whole(const Start& start, const Plan& plan, const WholeWays& ways, int64_t count, int dtype, int steps,
               const float* coefficients, bool precise, void* out, int out_dtype, hipStream_t st);
 

@@ -66,7 +66,9 @@ __global__ __launch_bounds__(kStartThreads) void start_kernel(Start a, Plan plan
     __shared__ float turned[64][68];
     const Group& group = group_of_tile(plan, blockIdx.x);
     const int m = group.tall ? group.c : group.r, n = group.tall ? group.r : group.c;
-    const Layout w = layout_of(group.r, group.c, PRECISE);
+    const int planes = planes_of<PRECISE>(group);
+    const bool pairs = planes == 2;
+    const Layout w = layout_of(group.r, group.c, planes);
     const int across = (n + 63) / 64, down = (m + 63) / 64, nth = (blockIdx.x - group.tile0) / (across * down);
     const int index = blockIdx.x - group.tile0 - nth * across * down, i0 = index / across * 64, j0 = index % across * 64;
     const int z = group.first + nth;
@@ -89,7 +91,7 @@ __global__ __launch_bounds__(kStartThreads) void start_kernel(Start a, Plan plan
     const int ld_plain = tall ? w.ldr : w.ldc, ld_other = tall ? w.ldc : w.ldr;
     const int c = threadIdx.x % 8 * 8;
     auto put = [&](uint8_t* at, int64_t plane, bool pair, const float* v) {
-        if (PRECISE || pair) put_halves<true>(at, plane, v);
+        if (pairs || pair) put_halves<true>(at, plane, v);
         else put_halves<false>(at, plane, v);
     };
 #pragma unroll
@@ -170,7 +172,7 @@ int start_of(const Start& a, Plan& w, int64_t count, bool precise, hipStream_t s
 
 int64_t partials_of(int64_t count) { return (count * kParts * (int64_t)sizeof(double) + 1023) / 1024 * 1024; }
 int64_t size_of(int64_t m, int64_t n, bool precise) {
-    return layout_of((int)(m < n ? m : n), (int)(m < n ? n : m), precise).size;
+    return layout_of((int)(m < n ? m : n), (int)(m < n ? n : m), has_pairs((int)m, (int)n, precise) ? 2 : 1).size;
 }
 
 bool bad_dtype(int d) { return d != Z1_F32 && d != Z1_BF16 && d != Z1_F16; }
@@ -241,7 +243,7 @@ int z1_orthogonalize_way(int64_t count, int64_t m, int64_t n, int precise, int* 
     const WholeWay small = whole_way(m, n, precise != 0);
     if (small.pieces) {
         way[1] = small.pieces;
-        way[2] = has_pairs(m, n, precise != 0);
+        way[2] = has_pairs((int)m, (int)n, precise != 0);
         return Z1_OK;
     }
     Plan w{};

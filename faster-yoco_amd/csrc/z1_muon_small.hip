@@ -17,11 +17,12 @@ struct Whole {
     Start start;
     void* out;                                         // or p and p16 of the list
     int dtype, out_dtype;
-    int steps, precise;
+    int steps;
+    uint64_t both;                                     // both_halves
     float co[3 * kMaxSteps];
 };
 constexpr int kWholeWaves = 8;
-// Bytes of a matrix of R x C fragments, and where they are.
+// Bytes of a matrix of R x C fragments, and where they are.  X is a pair in any case.
 struct Places {
     int px, pa;                                        // bytes of a row of X, and of A and B
     int x_plane, a_plane, A, B, sums, d, e, size;
@@ -37,7 +38,7 @@ __host__ __device__ constexpr Places places_of(int R, int C, bool precise) {
     const int most = R > 2 ? 1 : 8 / (R * R), half = C / 2;                    // four steps of 16 columns to a part at least
     p.cuts = 1;
     while (p.cuts < most && p.cuts < half) p.cuts *= 2;
-    p.A = planes * p.x_plane;
+    p.A = 2 * p.x_plane;
     p.B = p.A + planes * p.a_plane;
     p.d = p.B + planes * p.a_plane;
     p.e = p.d + R * 128;
@@ -71,7 +72,7 @@ __global__ __launch_bounds__(kWholeWaves * 64) void whole_kernel(Whole a) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int z = blockIdx.x, l32 = lane & 31, half = lane >> 5, rs = spread(l32);
     const Group& g = group_of_matrix(a.plan, z);
-    if ((g.r + 31) / 32 != R || has_pairs(g.r, g.c, a.precise) != PRECISE) return;              // another launch's
+    if ((g.r + 31) / 32 != R) return;                  // another launch's
     const int C = (g.c + 31) / 32, pieces = R * C;
     const Places at = places_of(R, C, PRECISE);
     const int m = g.tall ? g.c : g.r, n = g.tall ? g.r : g.c;
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(kWholeWaves * 64) void whole_kernel(Whole a) {
         float v[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) v[k] = x[q][k] * kX;
-        keep16<PRECISE>(lds + o_of(q) * at.px + t_of(q) * 2, at.x_plane, v);
+        keep16<true>(lds + o_of(q) * at.px + t_of(q) * 2, at.x_plane, v);
     };
 #pragma unroll
     for (int q = 0; q < F; ++q) {
@@ -170,6 +171,7 @@ __global__ __launch_bounds__(kWholeWaves * 64) void whole_kernel(Whole a) {
 
     for (int step = 0; step < a.steps; ++step) {
         const float ca = a.co[3 * step], cb = a.co[3 * step + 1], cc = a.co[3 * step + 2];
+        const bool both = PRECISE || (a.both >> step & 1);
         __syncthreads();                               // X is there
         // A: row j, columns i .. i + 15 of a fragment to a lane
         auto finish_a = [&](int ij, f16 v) {
@@ -243,10 +245,8 @@ __global__ __launch_bounds__(kWholeWaves * 64) void whole_kernel(Whole a) {
                 };
                 const h8 p = by_column(lds), b = by_row(lds + at.B, at.pa, o + l32, k);
                 acc = add(acc, p, b);
-                if constexpr (PRECISE) {
-                    acc = add(acc, p, by_row(lds + at.B + at.a_plane, at.pa, o + l32, k));
-                    acc = add(acc, by_column(lds + at.x_plane), b);
-                }
+                if constexpr (PRECISE) acc = add(acc, p, by_row(lds + at.B + at.a_plane, at.pa, o + l32, k));
+                if (both) acc = add(acc, by_column(lds + at.x_plane), b);
             }
 #pragma unroll
             for (int k = 0; k < 16; ++k) x[q][k] = acc[k] * (1.0f / (kX * kB));
@@ -315,12 +315,14 @@ int launch_whole(const Whole& a, const WholeWay& way, int64_t count, hipStream_t
     return (int)hipGetLastError();
 }
 template <int R>
-int run_rows(const Whole& a, const WholeWays& ways, int64_t count, hipStream_t st) {
-    const WholeWay &single = ways.of[0][R - 1], &pairs = ways.of[1][R - 1];
-    if (single.pieces)
-        if (const int rc = launch_whole<R, false>(a, single, count, st)) return rc;
-    return pairs.pieces ? launch_whole<R, true>(a, pairs, count, st) : Z1_OK;
+int run_rows(const Whole& a, const WholeWays& ways, int64_t count, bool precise, hipStream_t st) {
+    const WholeWay& way = ways.of[R - 1];
+    if (!way.pieces) return Z1_OK;
+    if constexpr (R * 32 > kPairSide)
+        if (!precise) return launch_whole<R, false>(a, way, count, st);
+    return launch_whole<R, true>(a, way, count, st);
 }
+static_assert(kPairSide % 32 == 0, "rows of fragments decide on pairs");
 }  // namespace
 
 namespace z1muon {
@@ -328,7 +330,7 @@ namespace z1muon {
 WholeWay whole_way(int64_t m, int64_t n, bool precise) {
     const int64_t r = m < n ? m : n, c = m < n ? n : m;
     if (r > kWholeSide || c > 32 * 32) return {0, 0};
-    const int R = (int)(r + 31) / 32, C = (int)(c + 31) / 32, bytes = places_of(R, C, has_pairs(r, c, precise)).size;
+    const int R = (int)(r + 31) / 32, C = (int)(c + 31) / 32, bytes = places_of(R, C, has_pairs((int)r, (int)c, precise)).size;
     for (const WholeWay way : {WholeWay{2, 64 << 10}, WholeWay{4, 159 << 10}})
         if (R * C <= way.pieces * kWholeWaves && bytes <= way.bytes) return way;
     return {0, 0};
@@ -336,12 +338,12 @@ WholeWay whole_way(int64_t m, int64_t n, bool precise) {
 
 int run_whole(const Start& start, const Plan& plan, const WholeWays& ways, int64_t count, int dtype, int steps,
               const float* coefficients, bool precise, void* out, int out_dtype, hipStream_t st) {
-    Whole a{plan, start, out, dtype, out_dtype, steps, precise, {}};
+    Whole a{plan, start, out, dtype, out_dtype, steps, both_halves(coefficients, steps), {}};
     for (int i = 0; i < 3 * steps; ++i) a.co[i] = coefficients[i];
-    if (const int rc = run_rows<1>(a, ways, count, st)) return rc;
-    if (const int rc = run_rows<2>(a, ways, count, st)) return rc;
-    if (const int rc = run_rows<3>(a, ways, count, st)) return rc;
-    return run_rows<4>(a, ways, count, st);
+    if (const int rc = run_rows<1>(a, ways, count, precise, st)) return rc;
+    if (const int rc = run_rows<2>(a, ways, count, precise, st)) return rc;
+    if (const int rc = run_rows<3>(a, ways, count, precise, st)) return rc;
+    return run_rows<4>(a, ways, count, precise, st);
 }
 
 }  // namespace z1muon

@@ -89,7 +89,9 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
     const int axis = PHASE == PART ? run_all / among : 0, run = PHASE == PART ? run_all - axis * among : run_all;
     const int index = first + run / (COARSE * COARSE);
     const Group& g = group_of_tile(plan, index);
-    const Layout w = layout_of(g.r, g.c, PRECISE);
+    const int planes = planes_of<PRECISE>(g);
+    const bool pairs = planes == 2;
+    const Layout w = layout_of(g.r, g.c, planes);
     const int64_t t_now = plan.cur ? w.t[1] : w.t[0], t_next = plan.cur ? w.t[0] : w.t[1];
     const int rows_t = kSymmetric ? g.r : g.c;
     const int down = (rows_t + COARSE * BT - 1) / (COARSE * BT), across = (g.r + COARSE * BO - 1) / (COARSE * BO);
@@ -111,9 +113,11 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
     // A row goes into a load's lane offset, which the buffer's range checks: rows past the end become zeros.  The block goes
     // into the scalar offset, which stays in the row: past the last block the last one is loaded again, not used.
     const __amdgpu_buffer_rsrc_t hi_t = buffer_of(pt, bytes_t), hi_o = buffer_of(po, bytes_o);
-    const __amdgpu_buffer_rsrc_t lo_t = buffer_of(pt + (PRECISE ? plane_t : 0), bytes_t);
-    const __amdgpu_buffer_rsrc_t lo_o = buffer_of(po + (PRECISE ? plane_o : 0), bytes_o);
-    const int all = PRECISE && !kTogether ? 3 * blocks : blocks, last = all - 1;
+    // (a matrix without pairs has no second halves to read, but for t in UPDATE)
+    const __amdgpu_buffer_rsrc_t lo_t = buffer_of(pt + plane_t, pairs || MODE == UPDATE ? bytes_t : 0);
+    const __amdgpu_buffer_rsrc_t lo_o = buffer_of(po + plane_o, pairs ? bytes_o : 0);
+    // times through the axis: pairs hi hi, hi lo and lo hi; single operands once, or X's second halves too
+    const int times = kTogether ? 1 : pairs ? 3 : MODE == UPDATE && plan.both ? 2 : 1, all = times * blocks, last = all - 1;
     const int per = PHASE == PART ? (all + parts - 1) / parts : all, begin = axis * per;
     const int total = all - begin < per ? all - begin : per;                   // none where not positive: zeros are left
     const int sub = lane >> 3, piece = lane & 7;
@@ -124,10 +128,11 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
         const int l = ip < kPT ? wave * kPT + ip : wave * kPO + ip - kPT;
         int k = begin + kb < last ? begin + kb : last;
         bool t_lo = kTogether && plane, o_lo = t_lo;
-        if (PRECISE && !kTogether) {                   // hi hi, hi lo, lo hi
-            t_lo = k >= 2 * blocks;
-            o_lo = k >= blocks && !t_lo;
-            k -= t_lo ? 2 * blocks : o_lo ? blocks : 0;
+        if (!kTogether) {
+            const bool third = k >= 2 * blocks, second = k >= blocks && !third;
+            t_lo = PRECISE ? third : second;
+            o_lo = PRECISE ? second : third;
+            k -= third ? 2 * blocks : second ? blocks : 0;
         }
         const int row = l * 8 * pitch;
         if (ip < kPT) load_lds(t_lo ? lo_t : hi_t, buf + l * 8 * kRow, row + (l & 1 ? from ^ 64 : from), k * kRow);
@@ -229,6 +234,10 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
     constexpr int kRowLanes = kCols / 8, kRows = 64 / kRowLanes, kRowTurns = WT / kRows;
     constexpr int kColumnLanes = WT / 8, kColumns = 64 / kColumnLanes, kColumnTurns = kCols / kColumns;
     constexpr bool kPlane = MODE == UPDATE || MODE == LAST || (MODE == SQUARE && PRECISE);      // the operand's second halves
+    auto put = [&](uint8_t* at, int64_t plane, const float* v) {
+        if (pairs) put_halves<true>(at, plane, v);
+        else put_halves<false>(at, plane, v);
+    };
     float* const own = (float*)(&lds[0][0] + wave * kRoom);
     float* const diagonal = (float*)(mine + (MODE == GRAM ? w.d : w.e));
     const uint8_t* const px = mine + (MODE == SQUARE ? w.A : t_now) + (int64_t)t0 * pitch;
@@ -295,6 +304,7 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
             }
             if constexpr (MODE != GRAM) F16::open(x[k], a);
             if constexpr (kPlane) F16::open(y[k], b);
+            else if (MODE == SQUARE && pairs) F16::open(halves_of(buf_y, (wt + row) * pitch + o * 2), b);      // few rows: no registers for it
 #pragma unroll
             for (int l = 0; l < 8; ++l) {
                 if (MODE == GRAM) v[l] *= kA / (kX * kX);
@@ -315,7 +325,7 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
             }
             if constexpr (kSymmetric) {
                 if (t < g.r && o < w.ldr)
-                    put_halves<PRECISE>(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)t * w.ldr + o) * 2, w.s_plane, v);
+                    put(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)t * w.ldr + o) * 2, w.s_plane, v);
             } else if constexpr (MODE == UPDATE) {
                 if (t < g.c && o < w.ldr) put_halves<true>(mine + t_next + ((int64_t)t * w.ldr + o) * 2, w.t_plane, v);
             } else if (g.tall) {
@@ -332,9 +342,9 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
                 for (int l = 0; l < 8; ++l) v[l] = ((const float*)group_at(own, r + l, column >> 2))[column & 3];
                 if constexpr (kSymmetric) {
                     if (oc < g.r && t < w.ldr)
-                        put_halves<PRECISE>(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)oc * w.ldr + t) * 2, w.s_plane, v);
+                        put(mine + (MODE == GRAM ? w.A : w.B) + ((int64_t)oc * w.ldr + t) * 2, w.s_plane, v);
                 } else if constexpr (MODE == UPDATE) {
-                    if (oc < g.r && t < w.ldc) put_halves<PRECISE>(mine + w.o + ((int64_t)oc * w.ldc + t) * 2, w.o_plane, v);
+                    if (oc < g.r && t < w.ldc) put(mine + w.o + ((int64_t)oc * w.ldc + t) * 2, w.o_plane, v);
                 } else {
                     deliver(oc, t, v);
                 }
@@ -386,7 +396,9 @@ Load load_of(Plan& w, int64_t b) {
     for (int k = 0; k < w.groups; ++k) {
         const Group& g = w.g[k];
         const double n = (double)((k + 1 < w.groups ? w.g[k + 1].tile0 : l.tiles) - g.tile0);
-        const double blocks = (PRECISE && b == 256 ? 3.0 : 1.0) * (((MODE == GRAM ? g.c : g.r) + kHalves - 1) / kHalves);
+        const bool apart = !PRECISE || b == 256;       // a time after the other
+        const double times = !apart ? 1.0 : has_pairs(g.r, g.c, PRECISE) ? 3.0 : MODE == UPDATE && w.both ? 2.0 : 1.0;
+        const double blocks = times * (((MODE == GRAM ? g.c : g.r) + kHalves - 1) / kHalves);
         l.blocks += n * blocks;
         l.most = blocks > l.most ? blocks : l.most;
     }
@@ -460,7 +472,7 @@ Way way_of(Plan& w) {
         int64_t n = kMostParts;
         for (int k = 0; k < w.groups; ++k) {
             const Group& g = w.g[k];
-            const int64_t d = (g.r + side - 1) / side, room = 2 * layout_of(g.r, g.c, PRECISE).t_plane / (d * (d + 1) / 2 * side * side * 4);
+            const int64_t d = (g.r + side - 1) / side, room = 2 * layout_of(g.r, g.c, 1).t_plane / (d * (d + 1) / 2 * side * side * 4);
             n = room < n ? room : n;
         }
         return n;
@@ -511,9 +523,11 @@ int launch_step(Steps& a) {
 
 template <bool PRECISE, typename Out>
 int iterate(Steps& a, int steps, const float* coefficients) {
+    const uint64_t both = both_halves(coefficients, steps);
     for (int k = 0; k < steps; ++k) {
         a.co = {coefficients[3 * k], coefficients[3 * k + 1], coefficients[3 * k + 2]};
         a.plan.cur = k & 1;
+        a.plan.both = both >> k & 1;
         if (const int rc = launch_step<GRAM, PRECISE>(a)) return rc;
         if (const int rc = launch_step<SQUARE, PRECISE>(a)) return rc;
         const int rc = k + 1 < steps ? launch_step<UPDATE, PRECISE>(a) : launch_step<LAST, PRECISE, Out>(a);
@@ -535,6 +549,7 @@ void way_into(Plan& w, int* way) {
 }
 template <bool PRECISE>
 void ways_of(Plan& w, int* way) {
+    w.both = 1;
     way_into<PRECISE, GRAM>(w, way);
     way_into<PRECISE, SQUARE>(w, way + 4);
     way_into<PRECISE, UPDATE>(w, way + 8);
