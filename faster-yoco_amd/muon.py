@@ -69,7 +69,7 @@ def rate(lr, shape, adjust):
 
 
 def step_(params, grads, momenta, copies=None, *, lr, momentum=0.95, nesterov=True, weight_decay=0.1, adjust='rms', factor=None,
-          steps=5, coefficients=COEFFICIENTS, eps=1e-7, precise=False):
+          steps=5, coefficients=COEFFICIENTS, eps=1e-7, precise=None):
     """One update, in place, of matrices `params` (fp32, contiguous) with `momenta` (alike) and their BF16 `copies` (or None):
 
         momentum_i = momentum * momentum_i + (1 - momentum) * factor * g_i
@@ -77,13 +77,14 @@ def step_(params, grads, momenta, copies=None, *, lr, momentum=0.95, nesterov=Tr
         p_i = p_i * (1 - lr * weight_decay) - rate(lr, p_i.shape, adjust) * orthogonalize(u_i)
 
     grads: fp32, bf16 or fp16, with rows of neighbouring elements.  factor: None or a one-element fp32 device tensor, as the
-    clip leaves it.  Nothing that is written may overlap another of the call's tensors.  Matrices of one shape run together."""
+    clip leaves it.  Nothing that is written may overlap another of the call's tensors.  precise: None for what fp32 masters hold
+    (yes); False takes half the time and leaves p off by some 1e-3 of its update."""
     params, grads, momenta, copies = list(params), list(grads), list(momenta), [] if copies is None else list(copies)
     if not (params or grads or momenta or copies):
         return
     lrs = [rate(lr, p.shape, adjust) if p.dim() == 2 else lr for p in params]
     _step(params, grads, momenta, copies, factor, lrs, [1.0 - lr * weight_decay] * len(params), float(momentum), bool(nesterov),
-          int(steps), _coefficients(coefficients, steps), float(eps), bool(precise))
+          int(steps), _coefficients(coefficients, steps), float(eps), precise is None or bool(precise))
 
 
 class MuonShardOptimizer(shard_mod.Zero1ShardOptimizer):
@@ -96,7 +97,7 @@ class MuonShardOptimizer(shard_mod.Zero1ShardOptimizer):
     step_'s.  A step in pieces is refused: the matrices of one shape run together."""
 
     def __init__(self, shard, matrices=None, matrix_lr=None, matrix_weight_decay=None, momentum=0.95, nesterov=True,
-                 adjust='rms', steps=5, coefficients=COEFFICIENTS, matrix_eps=1e-7, precise=False, **adam):
+                 adjust='rms', steps=5, coefficients=COEFFICIENTS, matrix_eps=1e-7, precise=None, **adam):
         super().__init__(shard, **adam)
         if matrices is None:
             matrices = [i for i, s in enumerate(shard.shapes) if len(s) == 2 and min(s) > 1]
