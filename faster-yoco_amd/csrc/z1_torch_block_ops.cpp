@@ -29,7 +29,7 @@ struct Api {
     decltype(&::z1_norm_forward) norm_forward;
     decltype(&::z1_norm_backward) norm_backward;
     decltype(&::z1_norm_backward_workspace) norm_backward_workspace;
-    decltype(&::z1_add_norm_forward) add_norm_forward;
+    decltype(&::z1_add_norm_forward) add_norm_forward;             // null in builds from before the addition
     decltype(&::z1_add_norm_backward) add_norm_backward;
     decltype(&::z1_act8_columns) act8_columns;
     decltype(&::z1_act8_scales) act8_scales;
@@ -186,6 +186,7 @@ Rows rows_like(const Tensor& t, const Tensor& x, const Rows& r, const char* what
 std::vector<Tensor> forward(const char* what, const Tensor& x, const Tensor* residual, const OptTensor& weight,
                             const OptTensor& bias, double eps, bool center, bool y8, bool checkpoint) {
     require_gpu(x, what, "x");
+    TORCH_CHECK(!residual || api().add_norm_forward, what, ": the selected build of libyoco_z1.so lacks it");
     const Rows r = rows_of(x, what, "x");
     const Rows e = residual ? rows_like(*residual, x, r, what, "residual", "x") : Rows{};
     const void* w = weight_of(weight, x, r.dim, what, "weight");
@@ -250,6 +251,7 @@ std::vector<Tensor> backward(const char* what, const Tensor& dy, const Tensor* d
                              bool center, bool need_dw, bool need_db, std::optional<at::ScalarType> grad_dtype) {
     const char* x_name = dh ? "h" : "x";
     require_gpu(dy, what, "dy");
+    TORCH_CHECK(!dh || api().add_norm_backward, what, ": the selected build of libyoco_z1.so lacks it");
     const Rows r = rows_of(dy, what, "dy");
     const Rows past = dh ? rows_like(*dh, dy, r, what, "dh", "dy") : Rows{};
     const bool packed = q.has_value() && q->defined();
@@ -437,7 +439,8 @@ TORCH_LIBRARY_IMPL(yoco_z1, CPU, m) {
 extern "C" {
 
 /* Resolves the C ABI from the already loaded library at `path`: 0, or -1 when it is not loaded, -2 when a function is
- * missing (an older build of the ABI: the update's operators work without these). */
+ * missing (an older build of the ABI: the update's operators work without these).  The residual stream's addition came later: a
+ * build without it binds, and its operators alone say that it is missing. */
 int z1t_init_block(const char* path) {
     void* h = dlopen(path, RTLD_NOW | RTLD_NOLOAD);
     if (!h) return -1;
@@ -448,8 +451,6 @@ int z1t_init_block(const char* path) {
     Z1T_RESOLVE(norm_forward)
     Z1T_RESOLVE(norm_backward)
     Z1T_RESOLVE(norm_backward_workspace)
-    Z1T_RESOLVE(add_norm_forward)
-    Z1T_RESOLVE(add_norm_backward)
     Z1T_RESOLVE(act8_columns)
     Z1T_RESOLVE(act8_scales)
     Z1T_RESOLVE(act8_pack)
@@ -461,6 +462,8 @@ int z1t_init_block(const char* path) {
     Z1T_RESOLVE(weight_grad8_workspace)
     Z1T_RESOLVE(strerror)
 #undef Z1T_RESOLVE
+    a.add_norm_forward = reinterpret_cast<decltype(a.add_norm_forward)>(dlsym(h, "z1_add_norm_forward"));
+    a.add_norm_backward = reinterpret_cast<decltype(a.add_norm_backward)>(dlsym(h, "z1_add_norm_backward"));
     g_api = a;
     g_api_ok = true;
     return 0;
