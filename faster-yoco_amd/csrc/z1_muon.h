@@ -179,7 +179,7 @@ __device__ __forceinline__ void put_halves(uint8_t* at, int64_t plane, const flo
         *(Z1B_GLOBAL u4*)(at + plane) = F16::close(lo);
     }
 }
-constexpr int64_t kMaxSide = 1 << 20;
+constexpr int64_t kMaxSide = Z1_MAX_SIDE;
 constexpr int64_t kMaxCount = 1 << 15;                 // of a call: a grid's second axis
 constexpr int64_t kMaxTiles = 1ll << 22;               // of a launch: its threads count in 32 bits
 constexpr int kCus = 256;

@@ -70,6 +70,11 @@ std::vector<float> coefficients_of(at::ArrayRef<double> c, int64_t steps, const 
     return f;
 }
 
+void check_sides(int64_t m, int64_t n, const char* what) {
+    TORCH_CHECK(m <= Z1_MAX_SIDE && n <= Z1_MAX_SIDE, what, ": expected matrices with sides of 1 to ", Z1_MAX_SIDE, ", got ", m,
+                " x ", n);
+}
+
 // A call's matrices run in launches whose workspace stays near 2 GiB.
 constexpr int64_t kRoom = int64_t{1} << 31;
 Tensor workspace_of(int64_t bytes) {
@@ -101,6 +106,7 @@ Tensor orthogonalize(const Tensor& x, int64_t steps, at::ArrayRef<double> coeffi
     OnDevice on(x);
     Tensor out(at::detail::empty_cuda({count, m, n}, dtype, c10::Device(c10::DeviceType::CUDA), std::nullopt));
     if (out.numel() == 0) return out;
+    check_sides(m, n, what);
     const int64_t one = api().orthogonalize_workspace(1, m, n, precise);
     if (one < 0) check_rc(one, "z1_orthogonalize_workspace");
     const int64_t most = std::max<int64_t>(1, std::min({count, int64_t{1} << 15, kRoom / std::max<int64_t>(1, one)}));
@@ -161,6 +167,7 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
                     what, ": g[", i, "]: expected rows of neighbouring elements of p's shape, on its device");
         dtype_code(g[i].scalar_type(), what, "g");
         if (p[i].numel() == 0) continue;
+        check_sides(p[i].size(0), p[i].size(1), what);
         written.push_back(span_of(p[i]));
         written.push_back(span_of(momentum[i]));
         if (!p16.empty()) written.push_back(span_of(p16[i]));
@@ -187,6 +194,11 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
     std::vector<std::vector<z1_matrix>> launches;
     std::vector<int> codes;
     int64_t bytes = 0;
+    auto room_of = [&](const std::vector<z1_matrix>& list) {
+        const int64_t n = api().muon_workspace(list.data(), static_cast<int>(list.size()), precise);
+        if (n < 0) check_rc(n, "z1_muon_workspace");
+        return n;
+    };
     for (const at::ScalarType type : {at::kFloat, at::kBFloat16, at::kHalf}) {
         const size_t first = launches.size();
         for (size_t i = 0; i < count; ++i) {
@@ -200,13 +212,13 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
                 codes.push_back(dtype_code(type, what, "g"));
             } else {
                 launches.back().push_back(x);
-                if (api().muon_workspace(launches.back().data(), static_cast<int>(launches.back().size()), precise) > kRoom) {
+                if (room_of(launches.back()) > kRoom) {
                     launches.back().pop_back();
                     launches.push_back({x});
                     codes.push_back(codes.back());
                 }
             }
-            bytes = std::max(bytes, api().muon_workspace(launches.back().data(), static_cast<int>(launches.back().size()), precise));
+            bytes = std::max(bytes, room_of(launches.back()));
         }
     }
     if (launches.empty()) return;

@@ -21,6 +21,7 @@ from . import library, ops, shard as shard_mod  # noqa: F401  (library registers
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 MAX_STEPS = 64
+MAX_SIDE = 1 << 20
 
 _orthogonalize = torch.ops.yoco_z1.orthogonalize.default
 _step = torch.ops.yoco_z1.muon_step_.default
@@ -39,7 +40,7 @@ def _coefficients(coefficients, steps):
 
 
 def orthogonalize(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7, dtype=None, precise=None):
-    """The matrices of x [..., m, n] (fp32, bf16 or fp16, m and n of at least 1), each orthogonalised by `steps` steps, in
+    """The matrices of x [..., m, n] (fp32, bf16 or fp16, m and n from 1 to 2^20), each orthogonalised by `steps` steps, in
     `dtype` (x's own where None) and contiguous.  coefficients: one (a, b, c), or one for each step; they must keep singular
     values that start in [0, 1] below 4.  A matrix of zeros stays one; an infinity or NaN makes its whole matrix NaN.  precise:
     None for what `dtype` holds (bf16: no, fp16 and fp32: yes)."""
@@ -76,6 +77,7 @@ def step_(params, grads, momenta, copies=None, *, lr, momentum=0.95, nesterov=Tr
         u_i = momentum * momentum_i + (1 - momentum) * factor * g_i  (nesterov), or momentum_i
         p_i = p_i * (1 - lr * weight_decay) - rate(lr, p_i.shape, adjust) * orthogonalize(u_i)
 
+    Sides from 1 to 2^20; a call that is refused has written nothing.
     grads: fp32, bf16 or fp16, with rows of neighbouring elements.  factor: None or a one-element fp32 device tensor, as the
     clip leaves it.  Nothing that is written may overlap another of the call's tensors.  precise: None for what fp32 masters hold
     (yes); False takes half the time and leaves p off by some 1e-3 of its update."""
@@ -105,6 +107,9 @@ class MuonShardOptimizer(shard_mod.Zero1ShardOptimizer):
         if len(set(self.matrices)) != len(self.matrices) or any(
                 not 0 <= i < len(shard.shapes) or len(shard.shapes[i]) != 2 for i in self.matrices):
             raise RuntimeError('muon: matrices must be rows of the shard with two dimensions, each once')
+        for i in self.matrices:
+            if max(shard.shapes[i]) > MAX_SIDE:
+                raise RuntimeError(f'muon: row {i} of {shard.shapes[i]}: sides of at most {MAX_SIDE}; name the other matrices')
         self.matrix_lr = None if matrix_lr is None else float(matrix_lr)
         self.matrix_weight_decay = None if matrix_weight_decay is None else float(matrix_weight_decay)
         self.how = dict(momentum=momentum, nesterov=nesterov, adjust=adjust, steps=steps, coefficients=coefficients,
