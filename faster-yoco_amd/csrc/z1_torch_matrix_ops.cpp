@@ -4,7 +4,9 @@
  * only.  Results and workspaces come from torch's allocator, on the call's stream, so the operators may be captured in a graph
  * and used on any stream.  z1t_init_matrix(path) resolves the C ABI, as z1t_init does for the update's operators.
  */
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -232,6 +234,22 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
     }
 }
 
+// The step below autograd; then what it wrote counts as written there, as after torch's own in-place operators: a backward pass
+// over values saved before it is refused.  (Tensors made in inference mode have no version.)
+void muon_step_versions_(at::TensorList p, at::TensorList g, at::TensorList momentum, at::TensorList p16, const OptTensor& factor,
+                         at::ArrayRef<double> lr, at::ArrayRef<double> keep, double mu, bool nesterov, int64_t steps,
+                         at::ArrayRef<double> coefficients, double eps, bool precise) {
+    static const auto op =
+        c10::Dispatcher::singleton().findSchemaOrThrow("yoco_z1::muon_step_", "").typed<decltype(muon_step_)>();
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        op.call(p, g, momentum, p16, factor, lr, keep, mu, nesterov, steps, coefficients, eps, precise);
+    }
+    for (const at::TensorList& list : {p, momentum, p16})
+        for (const Tensor& t : list)
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void refuse_cpu(const c10::OperatorHandle& op, torch::jit::Stack*) {
     TORCH_CHECK(false, op.schema().name(), ": expected GPU tensors (there is no CPU path)");
 }
@@ -249,6 +267,8 @@ TORCH_LIBRARY_IMPL(yoco_z1, CUDA, m) {
     m.impl("orthogonalize", &orthogonalize);
     m.impl("muon_step_", &muon_step_);
 }
+
+TORCH_LIBRARY_IMPL(yoco_z1, ADInplaceOrView, m) { m.impl("muon_step_", &muon_step_versions_); }
 
 TORCH_LIBRARY_IMPL(yoco_z1, CPU, m) {
     for (const char* name : {"orthogonalize", "muon_step_"})

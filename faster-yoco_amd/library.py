@@ -12,8 +12,9 @@ yoco/tasks/zero1_fast.py:150-160.
 
 Host cost: an operator call from Python is torch's dispatch (about 3 us) plus the C++ kernel; the table binding
 costs nanoseconds per row.  (A ``torch.library.custom_op`` with Python kernels took about 19 us per call before any
-work, plus microseconds per tensor for the checks and binding in Python.)  The operators make no version-counter
-bumps of the tensors they write, as the reference's Triton launches make none; none is ever differentiated.
+work, plus microseconds per tensor for the checks and binding in Python.)  The update's operators make no version-counter
+bumps of the tensors they write, as the reference's Triton launches make none; none is ever differentiated.  The matrices'
+step, which takes a model's parameters as they are, does make them.
 
 Tables are named by ``table`` (``kernels.Table.handle_int``; ``kernels.Table`` registers each table it creates).
 Operators over a table take the tensors it covers, one list per stream: for a flat table one buffer each (g, p, m,
