@@ -178,17 +178,19 @@ void muon_step_(at::TensorList p, at::TensorList g, at::TensorList momentum, at:
     std::sort(written.begin(), written.end());
     for (size_t i = 1; i < written.size(); ++i)
         TORCH_CHECK(written[i - 1].second <= written[i].first, what, ": tensors that are written overlap, or one is named twice");
-    for (const Span& s : read) {
+    auto apart = [&](const Span& s) {                  // of all that is written
         auto next = std::lower_bound(written.begin(), written.end(), s);
-        TORCH_CHECK((next == written.end() || s.second <= next->first) && (next == written.begin() || (--next)->second <= s.first),
-                    what, ": a gradient overlaps what is written");
-    }
+        return (next == written.end() || s.second <= next->first) && (next == written.begin() || (--next)->second <= s.first);
+    };
+    for (const Span& s : read) TORCH_CHECK(apart(s), what, ": a gradient overlaps what is written");
     const float* f = nullptr;
     if (factor.has_value() && factor->defined()) {
         require_gpu(*factor, what, "factor");
         TORCH_CHECK(factor->scalar_type() == at::kFloat && factor->numel() == 1 && factor->device() == p[0].device(), what,
                     ": factor: expected one fp32 value on the matrices' device");
         f = static_cast<const float*>(factor->const_data_ptr());
+        const auto* at = reinterpret_cast<const char*>(f);
+        TORCH_CHECK(apart({at, at + sizeof(float)}), what, ": factor overlaps what is written");
     }
     OnDevice on(p[0]);
 
