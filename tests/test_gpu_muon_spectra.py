@@ -74,3 +74,16 @@ def test_other_coefficients(pkg, dev):
                 want = ref.exact(x.float(), steps, c)
                 got = muon.orthogonalize(x.float().to(dev), steps, c, precise=False).cpu().double()
                 assert float((got - want).norm() / want.norm()) <= SINGLE, (name, steps)
+
+
+def test_matrices_of_few_rows_beside_large_ones(pkg, dev):
+    """One launch's tiles hold matrices with pairs and without (64-bit forms on the GPU: the large ones take seconds less)."""
+    from faster_yoco_amd import muon
+    shapes = [(40, 2000), (3, 5000), (9000, 64), (64, 256), (65, 600)] + [(2304, 2304)] * 3
+    u = [next(x for name, x in spectra(m, n, i) if name == 'rank 1 over noise').float().to(dev) for i, (m, n) in enumerate(shapes)]
+    p = [torch.zeros_like(t) for t in u]
+    muon.step_(p, u, [torch.zeros_like(t) for t in u], lr=1.0, adjust=1.0, weight_decay=0.0, momentum=0.0, precise=False)
+    for t, q in zip(u, p):
+        want = ref.exact(t)
+        off = float((q.double() + want).norm() / want.norm())
+        assert off <= (PAIRS if min(t.shape) <= 64 else SINGLE), (t.shape, off)
