@@ -202,7 +202,7 @@ void ways_precise(Plan& w, int* way);
 
 // Matrices of few rows take pairs in any case: the fewer rows, the less what A and B lose averages out (2 rows up to 5e-3, 3 x
 // 2000 2e-3, 16 x 16 1.6e-3, 33 x 96 1.2e-3; 65 to 128 rows 1.0e-3 at most), and there it costs least (32 x 32: 12.7 -> 15.2
-// us, 64 x 256 26.6 -> 35.0, 40 x 2000 91 -> 109).
+// us, 64 x 256 26.6 -> 35, 40 x 2000 91 -> 117).
 constexpr int kPairSide = 64;
 __host__ __device__ inline bool has_pairs(int m, int n, bool precise) { return precise || (m < n ? m : n) <= kPairSide; }
 

@@ -1,5 +1,5 @@
-// A matrix whose shorter side is at most 128 and that LDS holds: one workgroup does all of it in one launch (64 x 256: 25 us,
-// where 17 launches took 71; 16 x 16 with pairs 15).  Bound by latency: fifteen products in a row, each a few fragments to a
+// A matrix whose shorter side is at most 128 and that LDS holds: one workgroup does all of it in one launch (64 x 256: 34 us,
+// where 17 launches took 71 without pairs; 16 x 16 15).  Bound by latency: fifteen products in a row, each a few fragments to a
 // wave.  X itself stays in registers, in fp32 and in the matrix instructions' layout (so e X is what their sums begin with),
 // and its fp16 form in LDS is read by rows for A and turned, by transposing reads, for B X.
 //

@@ -62,8 +62,9 @@ __device__ __forceinline__ void floats_of(__amdgpu_buffer_rsrc_t from, int at, f
 // loads; a block's two halves are read ahead by one half and the workgroup meets between them, as in the 8-bit products.
 //
 // Bound by the matrix instructions and the card's power: of 256 x 256 tiles a full round of 256 takes 98 us over 3072 columns in
-// GRAM and LAST (1.05 PFLOP/s) and 119 in UPDATE, whose results are written in both orders and as pairs; the quarters of 56 tiles
-// 34.  The largest library product of this card reaches 1.34 PFLOP/s, one of 3072^3 0.94.
+// GRAM and LAST (1.05 PFLOP/s) and 119 in UPDATE, whose results are written in both orders and as pairs (192 with both halves of X
+// as its operand); the quarters of 56 tiles 34.  On zeros, four 3072 x 3072 take 12 % less in all.  The largest library product of
+// this card reaches 1.34 PFLOP/s, one of 3072^3 0.94.
 //
 // PART, JOINED: a long summed axis in parts, each a workgroup of its own, which leaves its sums as they are in its lanes (in the
 // next t's place: free then), and a launch that adds them in order and goes on from there.
@@ -410,8 +411,8 @@ Load load_of(Plan& w, int64_t b) {
 // 256 tiles over 48 105); X's update moves more (117).  128: 7 us and 0.42 alone on a CU (136 over 32 and 128 blocks 20 and 61),
 // two to a CU 9 us and 1.1 (512 over 48 57 to 66).  64: 3.3 us and 0.19 alone (136 over 64 15), two to a CU 2 us and 0.56.
 // Pairs: 256 has three times the blocks.  128: a CU holds one, 8 us and 0.82 (36 over 16 and 64 blocks 22 and 64), with all CUs
-// at it 12 us and 1.27 (256 over 16 and 32 33 and 53).  64: 4.7 us and 0.36 alone (136 over 16 and 64 11 and 28), two to a CU 4.1
-// us and 0.88 (1024 over 16 and 32 36 and 65).
+// at it 12 us and 1.27 (256 over 16 and 32 33 and 53; longer axes take more: 1200 over 48 to 128 895, where this says 604).  64:
+// 4.7 us and 0.36 alone (136 over 16 and 64 11 and 28), two to a CU 4.1 us and 0.88 (1024 over 16 and 32 36 and 65).
 template <bool PRECISE>
 double time_256(double tiles, double blocks, bool update) {
     constexpr double kCool = PRECISE ? 0.45 : 0.3;     // of the CUs

@@ -77,7 +77,7 @@ def step_(params, grads, momenta, copies=None, *, lr, momentum=0.95, nesterov=Tr
         u_i = momentum * momentum_i + (1 - momentum) * factor * g_i  (nesterov), or momentum_i
         p_i = p_i * (1 - lr * weight_decay) - rate(lr, p_i.shape, adjust) * orthogonalize(u_i)
 
-    Sides from 1 to 2^20; a call that is refused has written nothing.
+    Sides from 1 to 2^20; a call that is refused has written nothing.  momentum is taken in fp32, and 1 - momentum from it.
     grads: fp32, bf16 or fp16, with rows of neighbouring elements.  factor: None or a one-element fp32 device tensor, as the
     clip leaves it.  Nothing that is written may overlap another of the call's tensors.  precise: None for what fp32 masters hold
     (yes); False takes half the time and leaves p off by some 1e-3 of its update."""
@@ -96,7 +96,7 @@ class MuonShardOptimizer(shard_mod.Zero1ShardOptimizer):
     matrices: the shard's rows that are updated so (all of its two-dimensional ones with more than one row and column where
     None; embeddings and output layers are usually left to Adam).  Their momentum is kept in the shard's ``m``; their part of
     ``v`` is not used.  matrix_lr, matrix_weight_decay: lr and weight_decay where None; the other arguments are Adam's, or
-    step_'s.  A step in pieces is refused: the matrices of one shape run together."""
+    step_'s.  A step in pieces is refused: a step's matrices share launches."""
 
     def __init__(self, shard, matrices=None, matrix_lr=None, matrix_weight_decay=None, momentum=0.95, nesterov=True,
                  adjust='rms', steps=5, coefficients=COEFFICIENTS, matrix_eps=1e-7, precise=None, **adam):
@@ -125,7 +125,7 @@ class MuonShardOptimizer(shard_mod.Zero1ShardOptimizer):
     def step(self, closure=None, groups=None, pieces=None, on_piece=None):
         """The matrices' update, then Adam over the other rows, with the gradient factor in both; then factor := 1."""
         if pieces is not None:
-            raise RuntimeError('muon: a step in pieces is not available: matrices of one shape run together')
+            raise RuntimeError('muon: a step in pieces is not available: its matrices share launches')
         if self.matrices:
             lr = self.lr if self.matrix_lr is None else self.matrix_lr
             decay = self.weight_decay if self.matrix_weight_decay is None else self.matrix_weight_decay

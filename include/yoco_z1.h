@@ -368,7 +368,7 @@ typedef struct z1_matrix {
 } z1_matrix;
 typedef struct z1_muon {
     const float* factor; /* device scalar that multiplies the gradients, or NULL */
-    float momentum;      /* mu: momentum = mu momentum + (1 - mu) factor g */
+    float momentum;      /* mu: momentum = mu momentum + (1 - mu) factor g, 1 - mu in fp32 */
     int nesterov;        /* u = mu momentum + (1 - mu) factor g with the new momentum; 0: u = the new momentum */
     int steps;
     const float* coefficients;
