@@ -18,9 +18,10 @@
 //   - X is kept as a pair of fp16 (22 bits), of which e X takes both, and B' X too in the first steps (both_halves): what the
 //     first half leaves out there goes into all directions, those of no size among them, and grows from step to step; what A and
 //     B lose only turns the directions that are there.
-// That leaves 4e-4 to 1.3e-3 of the result (2-norm), whatever the spectrum, with more than 64 rows: less than the rounding of a
-// result in bf16, 1.7e-3.  Fewer rows, and PRECISE for results that hold more, take pairs for A and B as well and three products
-// for one, hi hi + hi lo + lo hi: 1e-6 to 3e-5, and up to 1e-4 with few directions in the input, as plain fp32 products leave.
+// That leaves 4e-4 to 1e-3 of the result (2-norm) mostly and up to 2e-3 whatever the spectrum (many equal singular values), with
+// more than 64 rows: about the rounding of a result in bf16, 1.7e-3, at the most.  Fewer rows, and PRECISE for results that hold
+// more, take pairs for A and B as well and three products for one, hi hi + hi lo + lo hi: 1e-6 to 3e-5, and with few directions in
+// the input 1e-4 (500 rows) to 4e-4 (3000), as plain fp32 products leave (1.8e-4 and 4.6e-4).
 //
 // Stored values are scaled by powers of two, so that fp16's range covers them: the host admits coefficients only if the
 // iterates stay below 4 and B below 32, so |X| kX <= 2^14, |A| kA <= 2^15, |B| kB <= 2^15.
@@ -214,15 +215,15 @@ __device__ __forceinline__ int planes_of(const Group& g) {
 }
 
 // On single operands: the steps whose B X takes both halves of X, a bit each.  A direction of no size grows by `a` a step, and
-// with it what the first half leaves out, 2^-12 of X in every element: both halves until no more than a factor of 16 is to come
-// (the first two of five steps with the default coefficients.  A rank of one or four in 65 x 4000: 6.7e-3 of the result without,
-// 9.1e-4 with two steps, 6.2e-4 with three, 5.3e-4 with all five; 65 x 65 to 1024 x 1024 of other spectra up to 1.3e-3 with two
-// and with five alike.  Each such step is a tenth more work).
+// with it what the first half leaves out, 2^-12 of X in every element: both halves until no more than a factor of 4 is to come
+// (the first three of five steps with the default coefficients.  Of 12,000 spectra of one to three levels, 65 to 352 rows, the
+// worst, some 60 equal singular values of 96, come out 4.2e-3 off with two such steps, 1.9e-3 with three and with all five; ranks
+// of one to four 4e-2 without.  Each such step is a tenth more work).
 inline uint64_t both_halves(const float* coefficients, int steps) {
     uint64_t both = 0;
     double growth = 1.0;
     for (int k = steps - 1; k >= 0; --k) {
-        if (growth > 16.0) both |= 1ull << k;
+        if (growth > 4.0) both |= 1ull << k;
         growth *= coefficients[3 * k] < 0.0f ? -coefficients[3 * k] : coefficients[3 * k];
     }
     return both;

@@ -7,11 +7,11 @@
 X = u / max(|u|_F, eps), then for each step's (a, b, c): X <- a X + b (X X^T) X + c (X X^T)^2 X.  The default coefficients
 take singular values from 1e-3 of the norm up to between 0.7 and 1.2 in five steps.  The products run on fp16 operands with
 fp32 sums, X kept in 22 bits and the diagonals of both symmetric products in fp32.  ``precise``: the operands are pairs of fp16,
-which leaves the result as fp32 products do, 1e-6 to 3e-5 off the exact iterate (2-norm, relative; up to 1e-4 where the input has
-few directions).  Without it, 4e-4 to 1.3e-3 whatever the spectrum, less than a bf16 result's rounding (1.7e-3), at two fifths of
-the work; matrices whose shorter side is at most 64 have pairs in any case.  The products of a call's matrices share launches,
-whose tiles are chosen by how much there is in all: the same call gives the same bits, but the last bits of a matrix may differ
-with the matrices beside it.  None of it is differentiable.
+which leaves the result as fp32 products do, 1e-6 to 3e-5 off the exact iterate (2-norm, relative; 1e-4 to 4e-4 where the input
+has few directions).  Without it, 4e-4 to 1e-3 mostly and up to 2e-3 whatever the spectrum, about a bf16 result's rounding
+(1.7e-3) at the most, at two fifths of the work; matrices whose shorter side is at most 64 have pairs in any case.  The products
+of a call's matrices share launches, whose tiles are chosen by how much there is in all: the same call gives the same bits, but
+the last bits of a matrix may differ with the matrices beside it.  None of it is differentiable.
 """
 import math
 

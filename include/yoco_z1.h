@@ -335,11 +335,11 @@ int z1_weight_grad8_way(int64_t T, int64_t N, int64_t K, int whole_dwords, int* 
  *
  * orthogonalised: X = u / max(|u|_F, eps), then `steps` times X <- a X + b (X X^T) X + c (X X^T)^2 X with that step's
  * (a, b, c), coefficients[steps][3].  Coefficients are admitted only where singular values in [0, 1] stay below 4 and b l + c l^2
- * below 32 on their squares (Z1_E_MODE otherwise); eps > 0; steps 1 to 64; m and n at most Z1_MAX_SIDE.  A matrix with an infinity or
- * a NaN becomes NaN, one of zeros zeros.  precise 1: as fp32 products leave it, within 1e-6 to 3e-5 of the exact result (2-norm
- * of the difference over the result's), and up to 1e-4 where the input has few directions; matrices whose shorter side is at most
- * 64 come out so in any case.  0: within 4e-4 to 1.3e-3 whatever the spectrum, less than the rounding of a bf16 result (1.7e-3),
- * at two fifths of the matrix work.  Elements of X are held to 2^-37, which a u far below eps falls under.
+ * below 32 on their squares (Z1_E_MODE otherwise); eps > 0; steps 1 to 64; m and n at most Z1_MAX_SIDE.  A matrix with an infinity
+ * or a NaN becomes NaN, one of zeros zeros.  precise 1: as fp32 products leave it, within 1e-6 to 3e-5 of the exact result (2-norm
+ * of the difference over the result's), 1e-4 to 4e-4 where the input has few directions; matrices whose shorter side is at most
+ * 64 come out so in any case.  0: within 4e-4 to 1e-3 mostly and 2e-3 whatever the spectrum, about the rounding of a bf16 result
+ * (1.7e-3) at the most, at two fifths of the matrix work.  Elements of X are held to 2^-37, which a u far below eps falls under.
  * workspace: as many bytes of device memory as the workspace function says, 16-byte aligned; calls that may overlap must not
  * share one. */
 
