@@ -305,7 +305,8 @@ __global__ __launch_bounds__(BT / WT * (BO / WO) * 64) void step_kernel(Plan pla
             }
             if constexpr (MODE != GRAM) F16::open(x[k], a);
             if constexpr (kPlane) F16::open(y[k], b);
-            else if (MODE == SQUARE && pairs) F16::open(halves_of(buf_y, (wt + row) * pitch + o * 2), b);      // few rows: no registers for it
+            // pairs among single operands are of few rows: loaded here, as registers for them would spill in every tile
+            else if (MODE == SQUARE && pairs) F16::open(halves_of(buf_y, (wt + row) * pitch + o * 2), b);
 #pragma unroll
             for (int l = 0; l < 8; ++l) {
                 if (MODE == GRAM) v[l] *= kA / (kX * kX);
